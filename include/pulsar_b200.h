@@ -351,6 +351,90 @@ int pb_tq_attention(int bits, const float* d_q, const uint32_t* d_kcode, const f
                     const uint32_t* d_vcode, const float* d_vscale, int nkv, int ctx, int T, float* d_atto,
                     void* d_scratch, void* stream);
 
+/* ---- paged K/V cache ------------------------------------------------------
+ * A pool of pages for K and one for V, and per sequence a table of its pages
+ * in order: row j of sequence b is row j % page_size of page
+ * d_table[b * table_ld + j / page_size]. One pool serves any number of
+ * sequences of one layer (the contiguous caches of pb_state and
+ * pb_bonsai_state hold one each). The entry points below store new rows
+ * (pb_kv_append), attend with one new token per sequence (pb_kv_decode) or
+ * with the last rows of each (pb_kv_prefill), and drop the rows of least
+ * accumulated weight (pb_kv_evict). None has a counterpart in the reference,
+ * whose caches are contiguous; their results are held to the formulas (fp32
+ * sums, one rounding at the store), not to the reference's orders.
+ *  - head_dim 64 or 128; page_size 16, 32, 64, 128 or 256; dtype (of K, V and
+ *    q) PB_DT_F16 or PB_DT_BF16; n_heads / n_kv a whole number up to 16.
+ *  - Strides are in elements, the last dimension is contiguous, rows start on
+ *    16 bytes, and no two rows overlap; [page][head][row] and
+ *    [page][row][head] orders and interleaved K and V pools all do.
+ *  - A table entry outside [0, n_pages) names no page: rows there are not
+ *    seen, stored or moved. Entries that no seen row needs are not used.
+ *  - Lengths live on the device and are read there, so a captured graph
+ *    replays with each step's lengths. max_len bounds them (0: the table's
+ *    rows); a length above it counts as max_len, one below 0 as 0.
+ *  - A row that is not seen may hold anything, infinities and NaN among it.
+ *    In pb_kv_prefill that goes for rows that no query of the chunk sees; a
+ *    row that one query of a chunk sees is finite.
+ *  - scratch: *_scratch bytes (0: none) of device memory, 16-byte aligned, with no contents kept between
+ *    calls; calls that may run at the same time take different scratch.
+ * Everything is asynchronous on `stream`; tables, lengths and rows must stay
+ * as they are until the call has run.                                        */
+typedef struct {
+  void* k;                /* row (page 0, head 0, row 0) of the K pool, and of the V pool */
+  void* v;
+  float* weight;          /* accumulated weights fp32 [page][kv head][row], or NULL */
+  int dtype, n_pages, page_size, n_kv, head_dim;
+  long long page_stride, head_stride, row_stride;
+} pb_kv_pages;
+/* n_tok rows d_qkv [n_tok][ldx] (bf16, fp16 or fp32; q heads | k heads | v
+ * heads, anything behind them ignored: the gate values of a q|k|v|gate
+ * projection): RMS norm of every query and key head (weights d_qnorm,
+ * d_knorm fp32 [head_dim]; NULL: no norm), rotation of the pairs (i, i +
+ * head_dim/2), i < half, by row d_pos[i] (NULL: d_slot[i]) of d_cos / d_sin
+ * (fp32 [n_rope][half]; half 0: none), the query heads to d_q [n_tok][ldq],
+ * the K and V rows to row d_slot[i] of sequence d_seq[i], whose weight
+ * becomes 0. A row whose sequence, slot, page or position is out of range is
+ * padding: nothing is written for it. Two rows of a call with the same
+ * sequence and slot leave that cache row undefined. q must not overlap qkv. */
+int pb_kv_append(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const void* d_qkv, int x_dtype,
+                 long long ldx, int n_tok, int n_heads, const int* d_seq, const int* d_slot, const int* d_pos,
+                 const float* d_qnorm, const float* d_knorm, float eps, const float* d_cos, const float* d_sin, int half,
+                 int n_rope, void* d_q, long long ldq, void* stream);
+/* attention of one token per sequence: row b of q (heads [n_heads][head_dim],
+ * row stride ldq) is the token at row t = d_len[b] - 1 of sequence b, whose
+ * K and V are stored. It sees row j <= t, and with a window > 0 only
+ * j > t - window or j < sinks. out[b] = sum_j p_j v_j, p = softmax(scale
+ * q.k_j); 0 where nothing is seen. out_dtype PB_DT_BF16 or PB_DT_F16.
+ * accumulate: the cache's weight of every seen row and K/V head grows by the
+ * sum of p_j over the query heads of its group; two sequences of one call
+ * then share no page. out must not overlap q.                                */
+long long pb_kv_decode_scratch(const pb_kv_pages* c, int n_seq, int max_len, int n_heads, int accumulate);
+int pb_kv_decode(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const int* d_len, int max_len,
+                 int n_heads, const void* d_q, long long ldq, float scale, int window, int sinks, int accumulate,
+                 void* d_out, int out_dtype, long long ldo, void* d_scratch, long long scratch_bytes, void* stream);
+/* attention of the last rows of each sequence (prompt chunks, whole prompts,
+ * a ragged batch of them): rows d_start[b] .. d_start[b+1]-1 of q (d_start
+ * int32 [n_seq + 1], ascending, within [0, n_tok]) are the tokens at the
+ * last rows of sequence b, each with the masks of pb_kv_decode. Rows of out
+ * outside every sequence are left as they were.                              */
+long long pb_kv_prefill_scratch(const pb_kv_pages* c, int n_seq, int max_len, int n_tok, int n_heads);
+int pb_kv_prefill(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const int* d_start, const int* d_len,
+                  int max_len, int n_tok, int n_heads, const void* d_q, long long ldq, float scale, int window, int sinks,
+                  void* d_out, int out_dtype, long long ldo, void* d_scratch, long long scratch_bytes, void* stream);
+/* per sequence and K/V head, keep the first `sinks` rows, the last `recent`
+ * rows and, up to `budget` rows in all, those of the largest weight (equal
+ * weights: the lowest row first; a weight that is not above 0 counts as 0).
+ * The kept rows move in order, with their weights, to rows 0.. of the pages
+ * of d_dst_table (row stride dst_ld), which must share no page with the
+ * sequences' own; d_new_len[b] = min(d_len[b], budget) (may be d_len). A
+ * sequence within the budget moves whole. The old pages are left as they are.
+ * Kept rows stay rotated by their own positions, so later tokens go to slot
+ * new_len.. with their true positions in pb_kv_append's d_pos.               */
+long long pb_kv_evict_scratch(const pb_kv_pages* c, int n_seq, int max_len, int budget);
+int pb_kv_evict(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const int* d_len, int max_len,
+                const int* d_dst_table, int dst_ld, int* d_new_len, int budget, int sinks, int recent, void* d_scratch,
+                long long scratch_bytes, void* stream);
+
 /* ---- sampler: sample_topkpp + frand01 (pulsar_arm/bonsai2/fwd8.c:465-521) ----
  * for each of B rows of fp32 logits (row b at d_logits + b*ld, n values):
  * top-k (topk <= 0 or > 1024 means 1024; ties in the reference's order,

@@ -1,0 +1,471 @@
+// pb_kv.cu -- the paged K/V cache: append (head norms, rotation and store in
+// one pass) and evict (the rows of largest accumulated weight to fresh pages).
+#include "pb_kv.cuh"
+#include <climits>
+
+namespace {
+
+// ------------------------------------------------------------------ append
+// Per token and head of D values: y = x w / sqrt(mean(x^2) + eps), then for
+// i < half the pair (y_i, y_{i+D/2}) turned by the token's angle. All of it in
+// fp32 with one rounding at the store. V heads are only rounded.
+//
+// D / 8 lanes hold a head, 8 consecutive values each (16-byte loads and
+// stores); the partner of a lane's values is D / 16 lanes away, so the
+// rotation is one exchange by shuffle. A warp takes one token and every
+// parts-th group of heads, so the angles and the norm weights are read once
+// per warp.
+struct AppendArgs {
+  KvPool p;
+  const char* x;
+  long long ldx, ldq;      // bytes
+  char* q;
+  const int* seq;
+  const int* slot;
+  const int* pos;          // null: the slot
+  const float *qn, *kn, *cs, *sn;
+  int n_tok, nh, half, n_rope, rows, parts;
+  float eps;
+};
+
+template <int XT>
+struct KvRaw {
+  uint4 a, b;
+};
+
+template <int XT>
+PB_DEV void ap_load(KvRaw<XT>& r, const char* p) {
+  r.a = pb_ldg_stream(p);
+  if (XT == PB_DT_F32) r.b = pb_ldg_stream(p + 16);
+}
+template <int XT>
+PB_DEV void ap_up(const KvRaw<XT>& r, float (&x)[8]) {
+  if (XT == PB_DT_F32) {
+    const unsigned u[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = __uint_as_float(u[i]);
+  } else {
+    const unsigned u[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float2 f = kv_up<XT>(u[i]);
+      x[2 * i] = f.x; x[2 * i + 1] = f.y;
+    }
+  }
+}
+
+constexpr int AP_W = 8;    // warps per CTA
+constexpr int AP_U = 4;    // head groups whose loads are in flight together
+
+template <int D, int XT, int CT>
+__global__ void __launch_bounds__(32 * AP_W) k_kv_append(AppendArgs a) {
+  constexpr int LPH = D / 8, HPW = 32 / LPH, XB = XT == PB_DT_F32 ? 4 : 2;
+  const int lane = threadIdx.x & 31, l = lane % LPH, sub = lane / LPH;
+  const long long unit = (long long)blockIdx.x * AP_W + (threadIdx.x >> 5);
+  const int t = (int)(unit / a.parts), part = (int)(unit % a.parts);
+  if (t >= a.n_tok) return;
+  const int seq = __ldg(a.seq + t), slot = __ldg(a.slot + t), pos = a.pos ? __ldg(a.pos + t) : slot;
+  if ((unsigned)seq >= (unsigned)a.p.n_seq || (unsigned)slot >= (unsigned)a.rows) return;
+  if (a.half > 0 && (unsigned)pos >= (unsigned)a.n_rope) return;
+  const int page = kv_page(a.p, a.p.table + (size_t)seq * a.p.table_ld, slot);
+  if (page < 0) return;
+  const int row = slot & ((1 << a.p.shift) - 1);
+  const long long at = (long long)page * a.p.ps + (long long)row * a.p.rs + l * 16;
+
+  // this lane's angles (both lanes of a pair hold the same ones): index
+  // i = 8l mod D/2; past `half` the angle is zero
+  float c[8], s[8];
+  const int i0 = (8 * l) % (D / 2);
+  const float *cp = a.cs + (size_t)pos * a.half + i0, *sp = a.sn + (size_t)pos * a.half + i0;
+  if (a.half == D / 2 && (reinterpret_cast<size_t>(a.cs) & 15) == 0 && (reinterpret_cast<size_t>(a.sn) & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 4) {
+      const float4 x = __ldg(reinterpret_cast<const float4*>(cp + i)), y = __ldg(reinterpret_cast<const float4*>(sp + i));
+      c[i] = x.x; c[i + 1] = x.y; c[i + 2] = x.z; c[i + 3] = x.w;
+      s[i] = y.x; s[i + 1] = y.y; s[i + 2] = y.z; s[i + 3] = y.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const bool in = i0 + i < a.half;
+      c[i] = in ? __ldg(cp + i) : 1.0f;
+      s[i] = in ? __ldg(sp + i) : 0.0f;
+    }
+  }
+  const bool upper = 8 * l >= D / 2;   // the second of each pair: y' = y c + partner s; the first: y c - partner s
+#pragma unroll
+  for (int i = 0; i < 8; i++) s[i] = upper ? s[i] : -s[i];
+  float qw[8], kw[8];
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    qw[i] = a.qn ? __ldg(a.qn + 8 * l + i) : 1.0f;
+    kw[i] = a.kn ? __ldg(a.kn + 8 * l + i) : 1.0f;
+  }
+
+  const int nk = a.p.n_kv, all = a.nh + 2 * nk, step = a.parts * HPW;
+  const char* x0 = a.x + (long long)t * a.ldx + (size_t)(l * 8 * XB);
+  for (int h0 = part * HPW; h0 < all; h0 += AP_U * step) {
+    KvRaw<XT> raw[AP_U];
+#pragma unroll
+    for (int u = 0; u < AP_U; u++) {
+      const int h = h0 + u * step + sub;
+      if (h < all) ap_load<XT>(raw[u], x0 + (size_t)h * (D * XB));
+      else raw[u].a = raw[u].b = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < AP_U; u++) {
+      if (h0 + u * step >= all) break;   // warp-uniform
+      const int h = h0 + u * step + sub;
+      const bool isq = h < a.nh, isv = h >= a.nh + nk;
+      float x[8];
+      ap_up<XT>(raw[u], x);
+      float ss = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; i++) ss = __fmaf_rn(x[i], x[i], ss);
+#pragma unroll
+      for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const bool norm = isq ? a.qn != nullptr : (!isv && a.kn != nullptr);
+      const float r = norm ? __fdiv_rn(1.0f, __fsqrt_rn(ss * (1.0f / D) + a.eps)) : 1.0f;
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) y[i] = isv ? x[i] : x[i] * r * (isq ? qw[i] : kw[i]);
+      if (a.half > 0) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float o = __shfl_xor_sync(0xffffffffu, y[i], LPH / 2);
+          if (!isv && i0 + i < a.half) y[i] = __fmaf_rn(o, s[i], y[i] * c[i]);
+        }
+      }
+      if (h >= all) continue;
+      const uint4 w = make_uint4(kv_down<CT>(y[0], y[1]), kv_down<CT>(y[2], y[3]), kv_down<CT>(y[4], y[5]),
+                                 kv_down<CT>(y[6], y[7]));
+      if (isq) {
+        *reinterpret_cast<uint4*>(a.q + (long long)t * a.ldq + (size_t)h * (D * 2) + l * 16) = w;
+      } else {
+        const int kh = isv ? h - a.nh - nk : h - a.nh;
+        *reinterpret_cast<uint4*>((isv ? a.p.v : a.p.k) + at + (long long)kh * a.p.hs) = w;
+        if (isv && a.p.w && l == 0) a.p.w[((size_t)page * nk + kh) * (1 << a.p.shift) + row] = 0.0f;
+      }
+    }
+  }
+}
+
+template <int D, int XT>
+void ap_launch(const AppendArgs& a, int ct, dim3 grid, cudaStream_t st) {
+  if (ct == PB_DT_F16) k_kv_append<D, XT, PB_DT_F16><<<grid, 32 * AP_W, 0, st>>>(a);
+  else k_kv_append<D, XT, PB_DT_BF16><<<grid, 32 * AP_W, 0, st>>>(a);
+}
+
+// ------------------------------------------------------------------- evict
+// One CTA per sequence and K/V head finds the rows that stay: the first
+// `sinks`, the last `recent`, and of the others the `need` of largest weight
+// (equal weights: the lowest row first), by a radix select on the weights'
+// bits (non-negative floats order as integers; anything not above zero counts
+// as zero), then lists them in order with ballots.
+struct EvictArgs {
+  KvPool p;
+  const int* len;
+  int* new_len;
+  const int* dst;       // table of the fresh pages
+  int dst_ld, max_len, budget, sinks, recent;
+  int lcap;             // rows of a list: min(budget, max_len)
+  int* list;            // [sequence][kv head][lcap]
+  int staged;           // rows whose keys fit in shared memory
+};
+
+constexpr int EV_T = 1024;
+
+PB_DEV unsigned ev_key(const EvictArgs& a, const int* trow, int h, int j) {
+  const int page = kv_page(a.p, trow, j);
+  if (page < 0) return 0u;
+  const float w = a.p.w[((size_t)page * a.p.n_kv + h) * (1 << a.p.shift) + (j & ((1 << a.p.shift) - 1))];
+  return w > 0.0f ? __float_as_uint(w) : 0u;
+}
+
+__global__ void __launch_bounds__(EV_T) k_kv_select(EvictArgs a) {
+  extern __shared__ unsigned keys[];
+  __shared__ int hist[2048];
+  __shared__ int wsum[EV_T / 32], wsum2[EV_T / 32];
+  __shared__ int s_bin, s_need;
+  const int b = blockIdx.x / a.p.n_kv, h = blockIdx.x % a.p.n_kv;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int len = kv_len(a.len[b], a.max_len);
+  if (len <= a.budget) return;   // every row stays: the gather needs no list
+  const int* trow = a.p.table + (size_t)b * a.p.table_ld;
+  const int lo = min(a.sinks, len), hi = max(lo, len - a.recent);   // [lo, hi) competes
+  int need = a.budget - (len - (hi - lo));                          // how many of it stay (>= 0: sinks + recent <= budget)
+  const int m = min(hi, a.staged);
+  for (int j = lo + t; j < m; j += EV_T) keys[j] = ev_key(a, trow, h, j);
+  __syncthreads();
+  auto key = [&](int j) { return j < a.staged ? keys[j] : ev_key(a, trow, h, j); };
+
+  unsigned prefix = 0, mask = 0;
+  if (need > 0) {
+    for (int pass = 0; pass < 3; pass++) {
+      const int sh = pass == 0 ? 20 : (pass == 1 ? 10 : 0), nb = pass == 0 ? 2048 : 1024;
+      for (int i = t; i < nb; i += EV_T) hist[i] = 0;
+      __syncthreads();
+      for (int j = lo + t; j < hi; j += EV_T) {
+        const unsigned k = key(j);
+        if ((k & mask) == prefix) atomicAdd(&hist[(k >> sh) & (nb - 1)], 1);
+      }
+      __syncthreads();
+      // the bin, counted from the top, in which the need-th largest key lies
+      const int per = nb / EV_T;   // 2 or 1 bins per thread, from the top
+      int own = 0;
+      for (int i = 0; i < per; i++) own += hist[nb - 1 - (t * per + i)];
+      int inc = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      if (lane == 31) wsum[warp] = inc;
+      __syncthreads();
+      if (warp == 0) {
+        int v = wsum[lane], x = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        wsum[lane] = x - v;
+      }
+      __syncthreads();
+      int before = wsum[warp] + inc - own;   // keys in the bins above this thread's
+      for (int i = 0; i < per; i++) {
+        const int bin = nb - 1 - (t * per + i), n = hist[bin];
+        if (before < need && before + n >= need) { s_bin = bin; s_need = need - before; }
+        before += n;
+      }
+      __syncthreads();
+      prefix |= (unsigned)s_bin << sh;
+      mask |= (unsigned)(nb - 1) << sh;
+      need = s_need;
+      __syncthreads();
+    }
+  }
+  // kept: outside [lo, hi), a key above prefix, or one of the first `need`
+  // keys equal to it. (need == 0 here only when nothing of [lo, hi) stays.)
+  const bool none = need == 0;
+  int* out = a.list + ((size_t)b * a.p.n_kv + h) * a.lcap;
+  const int seg = (len + EV_T - 1) / EV_T * 32, j0 = warp * seg, j1 = min(len, j0 + seg);
+  int ngt = 0, neq = 0;
+  for (int j = j0 + lane; j - lane < j1; j += 32) {
+    bool gt = false, eq = false;
+    if (j < j1) {
+      const bool in = j >= lo && j < hi;
+      const unsigned k = in && !none ? key(j) : 0u;
+      gt = !in || (!none && k > prefix);
+      eq = in && !none && k == prefix;
+    }
+    ngt += __popc(__ballot_sync(0xffffffffu, gt));
+    neq += __popc(__ballot_sync(0xffffffffu, eq));
+  }
+  if (lane == 0) { wsum[warp] = ngt; wsum2[warp] = neq; }
+  __syncthreads();
+  int pgt = 0, peq = 0;
+  for (int w = 0; w < warp; w++) { pgt += wsum[w]; peq += wsum2[w]; }
+  const unsigned lt = (1u << lane) - 1u;
+  for (int j = j0 + lane; j - lane < j1; j += 32) {
+    bool gt = false, eq = false;
+    if (j < j1) {
+      const bool in = j >= lo && j < hi;
+      const unsigned k = in && !none ? key(j) : 0u;
+      gt = !in || (!none && k > prefix);
+      eq = in && !none && k == prefix;
+    }
+    const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
+    const int e = peq + __popc(be & lt);
+    const int d = pgt + __popc(bg & lt) + min(e, need);
+    if ((gt || (eq && e < need)) && d < a.lcap) out[d] = j;
+    pgt += __popc(bg);
+    peq += __popc(be);
+  }
+}
+
+// The kept rows to the fresh pages: D / 8 lanes per row, K and V and the
+// weight, EV_R rows per lane group with all their loads in flight.
+constexpr int EV_R = 4, EV_GT = 256;
+
+template <int D>
+__global__ void __launch_bounds__(EV_GT) k_kv_gather(EvictArgs a, int chunks) {
+  constexpr int LPH = D / 8, G = EV_GT / LPH;   // lane groups per CTA
+  const int bh = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+  const int b = bh / a.p.n_kv, h = bh % a.p.n_kv;
+  const int l = threadIdx.x % LPH, g = threadIdx.x / LPH;
+  const int len = kv_len(a.len[b], a.max_len), n = min(len, a.budget);
+  const int ps = 1 << a.p.shift;
+  if (chunk == 0 && h == 0 && threadIdx.x == 0) a.new_len[b] = n;   // may be len[b]: min(n, budget) = n either way
+  const int* trow = a.p.table + (size_t)b * a.p.table_ld;
+  const int* drow = a.dst + (size_t)b * a.dst_ld;
+  const int* list = a.list + ((size_t)b * a.p.n_kv + h) * a.lcap;
+  const int i0 = chunk * (G * EV_R) + g;
+  uint4 kk[EV_R], vv[EV_R];
+  float w[EV_R];
+  long long to[EV_R];
+  size_t wto[EV_R];
+#pragma unroll
+  for (int r = 0; r < EV_R; r++) {
+    const int i = i0 + r * G;
+    to[r] = -1;
+    if (i >= n) continue;
+    const int j = len > a.budget ? list[i] : i;
+    const int sp = kv_page(a.p, trow, j), dp = kv_page(a.p, drow, i);
+    if (sp < 0 || dp < 0) continue;
+    const long long from = (long long)sp * a.p.ps + (long long)h * a.p.hs + (long long)(j & (ps - 1)) * a.p.rs + l * 16;
+    to[r] = (long long)dp * a.p.ps + (long long)h * a.p.hs + (long long)(i & (ps - 1)) * a.p.rs + l * 16;
+    wto[r] = ((size_t)dp * a.p.n_kv + h) * ps + (i & (ps - 1));
+    kk[r] = *reinterpret_cast<const uint4*>(a.p.k + from);
+    vv[r] = *reinterpret_cast<const uint4*>(a.p.v + from);
+    w[r] = a.p.w[((size_t)sp * a.p.n_kv + h) * ps + (j & (ps - 1))];
+  }
+#pragma unroll
+  for (int r = 0; r < EV_R; r++) {
+    if (to[r] < 0) continue;
+    *reinterpret_cast<uint4*>(a.p.k + to[r]) = kk[r];
+    *reinterpret_cast<uint4*>(a.p.v + to[r]) = vv[r];
+    if (l == 0) a.p.w[wto[r]] = w[r];
+  }
+}
+
+}  // namespace
+
+int kv_pool(const char* who, const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, KvPool* p) {
+  if (!c || !c->k || !c->v || !d_table) return pb_set_error(PB_EINVAL, "%s: null argument", who);
+  if (c->dtype != PB_DT_F16 && c->dtype != PB_DT_BF16)
+    return pb_set_error(PB_ENOTSUP, "%s: cache dtype %d (fp16 or bf16)", who, c->dtype);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return pb_set_error(PB_ENOTSUP, "%s: head_dim %d (64 or 128)", who, c->head_dim);
+  if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
+    return pb_set_error(PB_ENOTSUP, "%s: page_size %d (16, 32, 64, 128 or 256)", who, c->page_size);
+  if (c->n_pages <= 0 || c->n_kv <= 0 || c->n_kv > 1024 || n_seq < 0 || n_seq > (1 << 20) || table_ld <= 0 ||
+      table_ld > (1 << 30) / c->page_size)
+    return pb_set_error(PB_EINVAL, "%s: %d pages, %d K/V heads, %d sequences, table of %d pages", who, c->n_pages, c->n_kv,
+                        n_seq, table_ld);
+  if (((reinterpret_cast<size_t>(c->k) | reinterpret_cast<size_t>(c->v)) & 15) ||
+      ((c->page_stride | c->head_stride | c->row_stride) & 7))
+    return pb_set_error(PB_EINVAL, "%s: rows are 16-byte aligned (strides are multiples of 8 elements)", who);
+  // the strides, smallest first, must each step over everything below it:
+  // no two rows of the pool share memory
+  struct { long long st; int n; } d[3] = {{c->page_stride, c->n_pages}, {c->head_stride, c->n_kv}, {c->row_stride, c->page_size}};
+  for (int i = 0; i < 2; i++)
+    for (int j = 0; j < 2 - i; j++)
+      if (d[j].st > d[j + 1].st) { const auto x = d[j]; d[j] = d[j + 1]; d[j + 1] = x; }
+  long long span = c->head_dim;
+  for (int i = 0; i < 3; i++) {
+    if (d[i].n == 1) continue;
+    if (d[i].st < span || d[i].st > (1ll << 52) / d[i].n)
+      return pb_set_error(PB_EINVAL, "%s: strides %lld (page), %lld (head), %lld (row) make rows overlap", who, c->page_stride,
+                          c->head_stride, c->row_stride);
+    span += d[i].st * (d[i].n - 1);
+  }
+  p->k = static_cast<char*>(c->k);
+  p->v = static_cast<char*>(c->v);
+  p->w = c->weight;
+  p->table = d_table;
+  p->ps = c->page_stride * 2;
+  p->hs = c->head_stride * 2;
+  p->rs = c->row_stride * 2;
+  p->table_ld = table_ld;
+  p->n_pages = c->n_pages;
+  p->n_kv = c->n_kv;
+  p->n_seq = n_seq;
+  p->shift = 31 - __builtin_clz((unsigned)c->page_size);
+  return PB_OK;
+}
+
+extern "C" int pb_kv_append(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const void* d_qkv, int x_dtype,
+                            long long ldx, int n_tok, int n_heads, const int* d_seq, const int* d_slot, const int* d_pos,
+                            const float* d_qnorm, const float* d_knorm, float eps, const float* d_cos, const float* d_sin,
+                            int half, int n_rope, void* d_q, long long ldq, void* stream) {
+  AppendArgs a{};
+  if (int rc = kv_pool("pb_kv_append", c, n_seq, d_table, table_ld, &a.p)) return rc;
+  const int D = c->head_dim;
+  if (!d_qkv || !d_seq || !d_slot || !d_q) return pb_set_error(PB_EINVAL, "pb_kv_append: null argument");
+  if (x_dtype != PB_DT_BF16 && x_dtype != PB_DT_F32 && x_dtype != PB_DT_F16)
+    return pb_set_error(PB_EINVAL, "pb_kv_append: x_dtype %d", x_dtype);
+  if (n_tok < 0 || n_heads <= 0 || n_heads > 65536) return pb_set_error(PB_EINVAL, "pb_kv_append: %d tokens, %d heads", n_tok, n_heads);
+  if (half < 0 || half > D / 2 || (half > 0 && (!d_cos || !d_sin || n_rope <= 0)))
+    return pb_set_error(PB_EINVAL, "pb_kv_append: half %d of head_dim %d, %d positions", half, D, n_rope);
+  const long long wide = (long long)(n_heads + 2 * c->n_kv) * D;
+  const int xb = x_dtype == PB_DT_F32 ? 4 : 2;
+  if (ldx < wide || ldq < (long long)n_heads * D) return pb_set_error(PB_EINVAL, "pb_kv_append: row strides %lld, %lld", ldx, ldq);
+  if (((reinterpret_cast<size_t>(d_qkv) | reinterpret_cast<size_t>(d_q) | (size_t)(ldx * xb) | (size_t)(ldq * 2)) & 15))
+    return pb_set_error(PB_EINVAL, "pb_kv_append: qkv and q rows must be 16-byte aligned");
+  if (n_tok == 0) return PB_OK;
+  if (kv_overlap(d_qkv, ((size_t)(n_tok - 1) * ldx + wide) * xb, d_q, ((size_t)(n_tok - 1) * ldq + (size_t)n_heads * D) * 2))
+    return pb_set_error(PB_EINVAL, "pb_kv_append: q overlaps qkv");
+  a.x = static_cast<const char*>(d_qkv);
+  a.ldx = ldx * xb;
+  a.q = static_cast<char*>(d_q);
+  a.ldq = ldq * 2;
+  a.seq = d_seq; a.slot = d_slot; a.pos = d_pos;
+  a.qn = d_qnorm; a.kn = d_knorm; a.cs = d_cos; a.sn = d_sin;
+  a.n_tok = n_tok; a.nh = n_heads; a.half = half; a.n_rope = n_rope;
+  a.rows = table_ld * c->page_size;
+  a.eps = eps;
+  // few tokens: a warp per group of heads; many: a warp per token
+  const int groups = (int)((n_heads + 2 * c->n_kv + 256 / D - 1) / (256 / D));
+  const long long per = (long long)n_tok * groups / ((long long)pb_num_sms() * 48);
+  const int iters = per < 1 ? 1 : (per > groups ? groups : (int)per);
+  a.parts = (groups + iters - 1) / iters;
+  const long long blocks = ((long long)n_tok * a.parts + AP_W - 1) / AP_W;
+  if (blocks > INT_MAX) return pb_set_error(PB_EINVAL, "pb_kv_append: %d tokens", n_tok);
+  const dim3 grid((unsigned)blocks);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (D == 64) {
+    if (x_dtype == PB_DT_BF16) ap_launch<64, PB_DT_BF16>(a, c->dtype, grid, st);
+    else if (x_dtype == PB_DT_F16) ap_launch<64, PB_DT_F16>(a, c->dtype, grid, st);
+    else ap_launch<64, PB_DT_F32>(a, c->dtype, grid, st);
+  } else {
+    if (x_dtype == PB_DT_BF16) ap_launch<128, PB_DT_BF16>(a, c->dtype, grid, st);
+    else if (x_dtype == PB_DT_F16) ap_launch<128, PB_DT_F16>(a, c->dtype, grid, st);
+    else ap_launch<128, PB_DT_F32>(a, c->dtype, grid, st);
+  }
+  PB_LAUNCHED("k_kv_append");
+  return PB_OK;
+}
+
+extern "C" long long pb_kv_evict_scratch(const pb_kv_pages* c, int n_seq, int max_len, int budget) {
+  if (!c || n_seq < 0 || c->n_kv <= 0 || max_len < 0 || budget <= 0) return -1;
+  const long long cap = max_len > budget ? budget : 0;   // no list when nothing can pass the budget
+  return (long long)n_seq * c->n_kv * cap * 4;
+}
+
+extern "C" int pb_kv_evict(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const int* d_len, int max_len,
+                           const int* d_dst_table, int dst_ld, int* d_new_len, int budget, int sinks, int recent,
+                           void* d_scratch, long long scratch_bytes, void* stream) {
+  EvictArgs a{};
+  if (int rc = kv_pool("pb_kv_evict", c, n_seq, d_table, table_ld, &a.p)) return rc;
+  if (!c->weight || !d_len || !d_dst_table || !d_new_len) return pb_set_error(PB_EINVAL, "pb_kv_evict: null argument");
+  if (d_dst_table == d_table) return pb_set_error(PB_EINVAL, "pb_kv_evict: the fresh pages must not be the old ones");
+  if (max_len <= 0 || max_len > table_ld * c->page_size) max_len = table_ld * c->page_size;
+  if (budget <= 0 || sinks < 0 || recent < 0 || sinks > budget || recent > budget - sinks)
+    return pb_set_error(PB_EINVAL, "pb_kv_evict: budget %d, %d first and %d last rows", budget, sinks, recent);
+  const int cap = budget < max_len ? budget : max_len;
+  if (dst_ld <= 0 || dst_ld < (cap + c->page_size - 1) / c->page_size)
+    return pb_set_error(PB_EINVAL, "pb_kv_evict: %d rows need more than %d pages", cap, dst_ld);
+  const long long need = pb_kv_evict_scratch(c, n_seq, max_len, budget);
+  if (need > 0 && (!d_scratch || scratch_bytes < need))
+    return pb_set_error(PB_EINVAL, "pb_kv_evict: scratch of %lld bytes, %lld needed", scratch_bytes, need);
+  if (n_seq == 0) return PB_OK;
+  a.len = d_len; a.new_len = d_new_len; a.dst = d_dst_table; a.dst_ld = dst_ld;
+  a.max_len = max_len; a.budget = budget; a.sinks = sinks; a.recent = recent;
+  a.lcap = cap;
+  a.list = static_cast<int*>(d_scratch);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (max_len > budget) {
+    // keys in shared memory up to 40 KB (no opt-in needed), the rest re-read
+    a.staged = max_len < 8192 ? max_len : 8192;
+    k_kv_select<<<n_seq * c->n_kv, EV_T, (size_t)a.staged * 4, st>>>(a);
+    PB_LAUNCHED("k_kv_select");
+  }
+  const int per = EV_GT / (c->head_dim / 8) * EV_R, chunks = (cap + per - 1) / per;
+  const long long blocks = (long long)n_seq * c->n_kv * chunks;
+  if (blocks > INT_MAX) return pb_set_error(PB_EINVAL, "pb_kv_evict: %d sequences of %d rows", n_seq, cap);
+  if (c->head_dim == 64) k_kv_gather<64><<<(unsigned)blocks, EV_GT, 0, st>>>(a, chunks);
+  else k_kv_gather<128><<<(unsigned)blocks, EV_GT, 0, st>>>(a, chunks);
+  PB_LAUNCHED("k_kv_gather");
+  return PB_OK;
+}

@@ -91,6 +91,16 @@ def lib():
     L.pb_tq_store.argtypes = [i, vp, i, vp, vp, vp, vp, i, i, vp]
     L.pb_tq_attention.argtypes = [i, vp, vp, vp, vp, vp, i, i, i, vp, vp, vp]
     L.pb_sample_topkpp.argtypes = [vp, i, i, C.c_longlong, C.c_float, C.c_float, i, C.c_float, vp, vp, vp]
+    ll, f, kvp = C.c_longlong, C.c_float, C.POINTER(_KVPages)
+    L.pb_kv_append.argtypes = [kvp, i, vp, i, vp, i, ll, i, i, vp, vp, vp, vp, vp, f, vp, vp, i, i, vp, ll, vp]
+    L.pb_kv_decode.argtypes = [kvp, i, vp, i, vp, i, i, vp, ll, f, i, i, i, vp, i, ll, vp, ll, vp]
+    L.pb_kv_prefill.argtypes = [kvp, i, vp, i, vp, vp, i, i, i, vp, ll, f, i, i, vp, i, ll, vp, ll, vp]
+    L.pb_kv_evict.argtypes = [kvp, i, vp, i, vp, i, vp, i, vp, i, i, i, vp, ll, vp]
+    L.pb_kv_decode_scratch.argtypes = [kvp, i, i, i, i]
+    L.pb_kv_prefill_scratch.argtypes = [kvp, i, i, i, i]
+    L.pb_kv_evict_scratch.argtypes = [kvp, i, i, i]
+    for fn in (L.pb_kv_decode_scratch, L.pb_kv_prefill_scratch, L.pb_kv_evict_scratch):
+        fn.restype = ll
     L.pb_q1_gemv.argtypes = [vp, vp, vp, vp, vp]
     L.pq1_pq1_compat_gemv.restype = None
     L.pq1_pq1_compat_gemv.argtypes = [i, i, vp, vp, vp, vp]
@@ -133,6 +143,13 @@ def lib():
     L.pb_bonsai_decode_greedy.argtypes = [vp, vp, i, i, i, vp, vp]
     _lib = L
     return L
+
+
+class _KVPages(C.Structure):
+    """pb_kv_pages (include/pulsar_b200.h)"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("weight", C.c_void_p)] + \
+               [(n, C.c_int) for n in ("dtype", "n_pages", "page_size", "n_kv", "head_dim")] + \
+               [(n, C.c_longlong) for n in ("page_stride", "head_stride", "row_stride")]
 
 
 class BonsaiCfg(C.Structure):
@@ -318,6 +335,181 @@ def sample_topkpp(logits, temp, topp, topk, minp, rng, ids, stream=None):
     check(lib().pb_sample_topkpp(_ptr(lg), lg.shape[0], lg.shape[1], lg.stride(0), float(temp), float(topp),
                                  int(topk), float(minp), _ptr(rng) if rng is not None else None, _ptr(ids),
                                  _stream(stream)))
+
+
+def _dtype_code(t):
+    """PB_DT_* of a torch tensor's dtype (int16 tensors hold bf16 bits, as elsewhere in this module)"""
+    import torch
+    if not _DTYPES:
+        _DTYPES.update({torch.bfloat16: PB_DT_BF16, torch.int16: PB_DT_BF16, torch.float32: PB_DT_F32,
+                        torch.float16: PB_DT_F16})
+    try:
+        return _DTYPES[t.dtype]
+    except KeyError:
+        raise PBError(-1, "dtype %s" % t.dtype) from None
+
+
+_DTYPES = {}
+
+
+class KVPages:
+    """A paged K/V cache (pb_kv_pages): k and v are CUDA tensors [page][kv
+    head][row][dim] (fp16 or bf16, any strides with a contiguous last
+    dimension, the same for both), weight an optional contiguous fp32 tensor
+    [page][kv head][row]. The object keeps them alive; it holds no other
+    state, so one may be used from several streams. Tables, lengths, slots and
+    positions are int32 CUDA tensors on the pools' device. stream: the torch
+    stream to run on (default: the device's current one); scratch, where a
+    call needs some and none is given, is allocated on that stream."""
+
+    def __init__(self, k, v, weight=None):
+        import torch
+        if k.dim() != 4 or not k.is_cuda or k.dtype not in (torch.float16, torch.bfloat16):
+            raise PBError(-1, "KVPages: k is a CUDA tensor [page][kv head][row][dim] of fp16 or bf16")
+        if v.shape != k.shape or v.stride() != k.stride() or v.dtype != k.dtype or v.device != k.device or k.stride(3) != 1:
+            raise PBError(-1, "KVPages: v needs k's shape, strides, dtype and device, and contiguous rows")
+        if weight is not None and (weight.shape != k.shape[:3] or weight.dtype != torch.float32 or
+                                   weight.device != k.device or not weight.is_contiguous()):
+            raise PBError(-1, "KVPages: weight is a contiguous fp32 tensor [page][kv head][row] beside k")
+        self.k, self.v, self.weight = k, v, weight
+        self.device, self.dtype = k.device, k.dtype
+        n, h, r, d = k.shape
+        self._c = _KVPages(k.data_ptr(), v.data_ptr(), weight.data_ptr() if weight is not None else None, _dtype_code(k),
+                           n, r, h, d, k.stride(0), k.stride(1), k.stride(2))
+        self._r = C.byref(self._c)
+        self.n_kv, self.page_size, self.head_dim = h, r, d
+
+    @classmethod
+    def alloc(cls, n_pages, page_size, n_kv, head_dim, dtype=None, weights=False, device="cuda"):
+        """zeroed pools of n_pages pages (fp16 by default)"""
+        import torch
+        shape = (n_pages, n_kv, page_size, head_dim)
+        k = torch.zeros(shape, dtype=dtype or torch.float16, device=device)
+        return cls(k, torch.zeros_like(k),
+                   torch.zeros(shape[:3], dtype=torch.float32, device=device) if weights else None)
+
+    def _ints(self, what, t, dim=1, n=None):
+        if t.dtype != self._int32 or t.device != self.device or t.dim() != dim or not t.is_contiguous() or \
+                (n is not None and t.shape[0] != n):
+            raise PBError(-1, "%s: an int32 tensor on %s of %d dimension%s%s, contiguous" % (
+                what, self.device, dim, "" if dim == 1 else "s", "" if n is None else " and length %d" % n))
+        return t.data_ptr()
+
+    def _heads(self, what, t, dtype=None):
+        """a tensor [row][head][dim] whose rows are contiguous"""
+        if t.dim() != 3 or t.device != self.device or t.shape[2] != self.head_dim or (dtype and t.dtype != dtype) or \
+                (t.numel() and (t.stride(2) != 1 or t.stride(1) != self.head_dim)):
+            raise PBError(-1, "%s: a tensor [row][head][%d]%s on %s with contiguous rows" % (
+                what, self.head_dim, " of %s" % dtype if dtype else "", self.device))
+        return t.data_ptr()
+
+    def _floats(self, what, t, shape):
+        if t is None:
+            return None
+        if t.dtype != self._float32 or t.device != self.device or tuple(t.shape) != shape or not t.is_contiguous():
+            raise PBError(-1, "%s: a contiguous fp32 tensor %s on %s" % (what, list(shape), self.device))
+        return t.data_ptr()
+
+    @property
+    def _int32(self):
+        import torch
+        return torch.int32
+
+    @property
+    def _float32(self):
+        import torch
+        return torch.float32
+
+    def _call(self, fn, args, need, scratch, stream):
+        """fn(*args, scratch, bytes, stream) on the pools' device; need < 0: a function without scratch"""
+        import torch
+        dev = self.device.index
+        if torch.cuda.current_device() != dev:
+            with torch.cuda.device(dev):
+                return self._call(fn, args, need, scratch, stream)
+        s = stream if stream is not None else torch.cuda.current_stream(dev)
+        if need < 0:
+            return check(fn(*args, s.cuda_stream))
+        if scratch is None and need > 0:
+            if stream is None:
+                scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
+            else:   # allocated on the stream that uses it, so that it is not reused under the call
+                with torch.cuda.stream(stream):
+                    scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
+        if scratch is None:
+            return check(fn(*args, None, 0, s.cuda_stream))
+        if scratch.device != self.device or not scratch.is_contiguous():
+            raise PBError(-1, "scratch: a contiguous tensor on %s" % self.device)
+        return check(fn(*args, scratch.data_ptr(), scratch.numel() * scratch.element_size(), s.cuda_stream))
+
+    def append(self, table, seq, slot, pos, qkv, q, q_norm=None, k_norm=None, eps=1e-5, cos=None, sin=None, stream=None):
+        """norm and rotate the heads of qkv [n][>= (n_heads + 2 n_kv) dim] (bf16, fp16 or fp32), query heads to
+        q [n][n_heads][dim] (the cache's dtype), K and V rows to row slot[i] of sequence seq[i]; pos: the rotation's
+        position per token (None: slot); cos, sin [positions][half] (None: no rotation)"""
+        n, nh = q.shape[0], q.shape[1]
+        if qkv.dim() != 2 or qkv.shape[0] != n or qkv.device != self.device or (qkv.numel() and qkv.stride(1) != 1) or \
+                qkv.shape[1] < (nh + 2 * self.n_kv) * self.head_dim:
+            raise PBError(-1, "qkv: a tensor [%d][>= %d] on %s with contiguous rows" % (
+                n, (nh + 2 * self.n_kv) * self.head_dim, self.device))
+        if (cos is None) != (sin is None):
+            raise PBError(-1, "cos and sin go together")
+        half, n_rope = (cos.shape[1], cos.shape[0]) if cos is not None else (0, 0)
+        d = (self.head_dim,)
+        args = (self._r, table.shape[0], self._ints("table", table, 2), table.shape[1],
+                qkv.data_ptr(), _dtype_code(qkv), qkv.stride(0) if n > 1 else qkv.shape[1] // 8 * 8, n, nh,
+                self._ints("seq", seq, 1, n), self._ints("slot", slot, 1, n),
+                self._ints("pos", pos, 1, n) if pos is not None else None, self._floats("q_norm", q_norm, d),
+                self._floats("k_norm", k_norm, d), float(eps), self._floats("cos", cos, (n_rope, half)),
+                self._floats("sin", sin, (n_rope, half)), half, n_rope, self._heads("q", q, self.dtype),
+                q.stride(0) if n > 1 else nh * self.head_dim)
+        self._call(lib().pb_kv_append, args, -1, None, stream)
+
+    def decode(self, table, length, q, out, max_len=0, scale=None, window=0, sinks=0, accumulate=False, scratch=None,
+               stream=None):
+        """attention of one token per sequence: q [n_seq][n_heads][dim] (the cache's dtype) at row length[b] - 1 of
+        each cache, into out (bf16 or fp16, q's shape); scale: 1 / sqrt(dim) by default; accumulate: add each seen
+        row's probabilities to the cache's weight"""
+        L = lib()
+        n, nh = q.shape[0], q.shape[1]
+        args = self._attn_args(table, n, [self._ints("length", length, 1, n)], [], q, out, max_len, scale, window, sinks,
+                               [1 if accumulate else 0])
+        need = L.pb_kv_decode_scratch(self._r, n, max_len or table.shape[1] * self.page_size, nh, 1 if accumulate else 0)
+        self._call(L.pb_kv_decode, args, need, scratch, stream)
+
+    def prefill(self, table, start, length, q, out, max_len=0, scale=None, window=0, sinks=0, scratch=None, stream=None):
+        """attention of the last rows of each sequence: rows start[b] .. start[b+1]-1 of q [n][n_heads][dim] are the
+        tokens at the last rows of sequence b, into out (bf16 or fp16, q's shape)"""
+        L = lib()
+        n = length.shape[0]
+        args = self._attn_args(table, n, [self._ints("start", start, 1, n + 1), self._ints("length", length, 1, n)],
+                               [q.shape[0]], q, out, max_len, scale, window, sinks, [])
+        need = L.pb_kv_prefill_scratch(self._r, n, max_len or table.shape[1] * self.page_size, q.shape[0], q.shape[1])
+        self._call(L.pb_kv_prefill, args, need, scratch, stream)
+
+    def _attn_args(self, table, n_seq, lens, rows, q, out, max_len, scale, window, sinks, more):
+        qp, op = self._heads("q", q, self.dtype), self._heads("out", out)
+        if out.shape != q.shape:
+            raise PBError(-1, "out: q's shape")
+        if table.shape[0] != n_seq:
+            raise PBError(-1, "table: a row for each of %d sequences" % n_seq)
+        n, nh, wide = q.shape[0], q.shape[1], q.shape[1] * self.head_dim
+        return (self._r, n_seq, self._ints("table", table, 2), table.shape[1], *lens, max_len,
+                *rows, nh, qp, q.stride(0) if n > 1 else wide, self.head_dim ** -0.5 if scale is None else scale, window,
+                sinks, *more, op, _dtype_code(out), out.stride(0) if n > 1 else wide)
+
+    def evict(self, table, length, dst_table, new_length, budget, sinks=0, recent=0, max_len=0, scratch=None, stream=None):
+        """keep up to `budget` rows of each sequence and K/V head (the first `sinks`, the last `recent`, then the
+        largest weights), moved in order to the pages of dst_table; new_length (may be length) receives the lengths"""
+        L = lib()
+        n = length.shape[0]
+        if table.shape[0] != n or dst_table.shape[0] != n:
+            raise PBError(-1, "table, dst_table: a row for each of %d sequences" % n)
+        args = (self._r, n, self._ints("table", table, 2), table.shape[1],
+                self._ints("length", length, 1, n), max_len, self._ints("dst_table", dst_table, 2),
+                dst_table.shape[1], self._ints("new_length", new_length, 1, n), budget,
+                sinks, recent)
+        need = L.pb_kv_evict_scratch(self._r, n, max_len or table.shape[1] * self.page_size, budget)
+        self._call(L.pb_kv_evict, args, need, scratch, stream)
 
 
 class Q1Tensor:

@@ -1,0 +1,584 @@
+"""The paged K/V cache on the device (pb_kv_append, pb_kv_decode,
+pb_kv_prefill, pb_kv_evict) against the 64-bit oracle of kv_oracle.py.
+
+Tolerances, from the arithmetic (u = eps / 2 of a type, the half step):
+append: a mean of D squares, a root, and a rotation of two products in fp32:
+(D / 2 + 16) 2^-24 (|a| + |b|) of the pair's values, then one rounding, u of
+the result (and half the smallest fp16 step, 2^-25). V is one rounding: exact.
+Attention: a probability is off by its fp32 score's error (`slack` of the
+oracle, which becomes twice that relative to the sum), ex2's 2^-22, n 2^-24
+for the sum of n terms, and its own rounding to the cache's type for the
+matrix product, u (or 2^-25 of the largest, for an fp16 subnormal); the
+output's rounding adds u of the result. Weights are fp32: no u."""
+import numpy as np
+import pytest
+
+import kv_oracle as KO
+
+pytestmark = pytest.mark.gpu
+
+
+def U(torch, dt):
+    return torch.finfo(dt).eps / 2
+
+
+def f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+class Cache:
+    """pools of n_pages pages full of NaN, in one of three memory orders, and a table of random pages"""
+
+    def __init__(self, pb, torch, lens, nkv, D, ps, dt, layout="head", weights=False, seed=0, spare=3, width=None):
+        g = torch.Generator().manual_seed(seed)
+        need = [-(-n // ps) for n in lens]
+        n_pages = sum(need) + spare
+        nan = float("nan")
+        if layout == "head":
+            k, v = (torch.full((n_pages, nkv, ps, D), nan, dtype=dt, device="cuda") for _ in "kv")
+        elif layout == "row":      # [page][row][head][dim]
+            k, v = (torch.full((n_pages, ps, nkv, D), nan, dtype=dt, device="cuda").transpose(1, 2) for _ in "kv")
+        else:                      # K and V interleaved, rows padded
+            kv = torch.full((n_pages, 2, nkv, ps, D + 8), nan, dtype=dt, device="cuda")
+            k, v = kv[:, 0, :, :, :D], kv[:, 1, :, :, :D]
+        w = torch.rand((n_pages, nkv, ps), generator=g).cuda() if weights else None
+        self.h = pb.KVPages(k, v, w)
+        self.k, self.v, self.w, self.ps, self.nkv, self.D, self.dt = k, v, w, ps, nkv, D, dt
+        ids = torch.randperm(n_pages, generator=g).int()
+        self.table = torch.full((len(lens), width or max(1, max(need))), -1, dtype=torch.int32)
+        at = 0
+        for b, n in enumerate(need):
+            self.table[b, :n] = ids[at:at + n]
+            at += n
+        self.lens, self.g, self.torch, self.n_pages = list(lens), g, torch, n_pages
+        self.fill()
+
+    def fill(self):
+        torch = self.torch
+        for b, n in enumerate(self.lens):
+            if n:
+                pg, r, ok = KO.rows_of(self.table.numpy(), b, n, self.ps, self.n_pages)
+                pg, r = torch.from_numpy(pg).long().cuda(), torch.from_numpy(r).cuda()
+                for t in (self.k, self.v):
+                    t[pg, :, r] = torch.randn((n, self.nkv, self.D), generator=self.g).to(self.dt).cuda()
+
+    def dev(self):
+        return self.table.cuda()
+
+
+def check(torch, got, want, spread, slack, tiny, n, dt, out, what):
+    p_err = 2 * slack[..., None] + 2.0 ** -21 + n * 2.0 ** -24 + U(torch, dt)
+    tol = spread * p_err + 2.0 ** -25 * tiny + U(torch, out) * (np.abs(want) + spread * p_err) + 2.0 ** -25
+    bad = ~(np.abs(got - want) <= tol)
+    assert not bad.any(), (what, np.argwhere(bad)[:5].tolist(), got[bad][:5], want[bad][:5], tol[bad][:5])
+
+
+def oracle_rows(c, q, lens, counts, scale, window, sinks):
+    """(out, spread, slack, tiny) of every row, and the weights' sums per sequence"""
+    k, v, qq, tb = f64(c.k), f64(c.v), f64(q), c.table.numpy()
+    res, sums, r = [], [], 0
+    for b, (n, m) in enumerate(zip(lens, counts)):
+        n = max(0, min(n, c.table.shape[1] * c.ps))
+        for i in range(m):
+            x = KO.attend(qq[r], k, v, None, tb, b, n - m + i, n, scale, window, sinks)
+            res.append(x[:4])
+            sums.append(x[4])
+            r += 1
+    if not res:
+        return None, sums
+    return [np.stack(x) for x in zip(*res)], sums
+
+
+# ------------------------------------------------------------------ append
+APPEND = [  # nh, nkv, D, ps, cache, x, half, layout, weights, pos, norms, n
+    (32, 8, 64, 16, "float16", "bfloat16", 32, "head", True, False, True, 1),
+    (16, 4, 128, 32, "float16", "float32", 32, "row", True, True, True, 9),
+    (4, 4, 128, 64, "bfloat16", "float16", 64, "mixed", False, True, True, 33),
+    (5, 1, 64, 256, "bfloat16", "bfloat16", 5, "head", True, True, True, 70),
+    (12, 2, 64, 128, "float16", "float32", 0, "row", False, False, True, 6),
+    (7, 1, 128, 16, "float16", "float16", 64, "head", False, False, False, 17),
+    (32, 8, 128, 16, "bfloat16", "bfloat16", 64, "head", False, False, True, 2500),
+]
+
+
+@pytest.mark.parametrize("nh,nkv,D,ps,dt,xt,half,layout,weights,pos,norms,n", APPEND)
+def test_append(pb, cuda, nh, nkv, D, ps, dt, xt, half, layout, weights, pos, norms, n):
+    torch = cuda
+    dt, xt = getattr(torch, dt), getattr(torch, xt)
+    rng = np.random.default_rng(n)
+    S = min(n, 4)
+    ctx = [3 + 29 * b for b in range(S)]
+    per = [n // S + (b < n % S) for b in range(S)]
+    c = Cache(pb, torch, [a + m for a, m in zip(ctx, per)], nkv, D, ps, dt, layout, weights, seed=n)
+    seq = np.concatenate([np.full(m, b) for b, m in enumerate(per)]).astype(np.int32)
+    slot = np.concatenate([np.arange(a, a + m) for a, m in zip(ctx, per)]).astype(np.int32)
+    order = rng.permutation(n)
+    seq, slot = seq[order], slot[order]
+    n_rope = int(slot.max()) + 40
+    p = (slot + rng.integers(0, 40, n)).astype(np.int32) if pos else None
+    if n > 8:      # padding of every kind
+        seq[1], slot[2], seq[3], slot[4] = -1, -5, S, c.table.shape[1] * ps
+        if p is not None and half:
+            p[5] = n_rope
+        j = 6      # a row whose page is not one
+        c.table[seq[j], slot[j] // ps] = -1 if n % 2 else c.n_pages
+    wide = (nh + 2 * nkv) * D
+    big = torch.full((n, wide + 24), float("nan"), dtype=xt)
+    big[:, :wide] = torch.from_numpy(rng.standard_normal((n, wide)) * 2).to(xt)
+    q = torch.full((n, nh, D), 7.0, dtype=dt, device="cuda")
+    ang = np.arange(n_rope)[:, None] * 1e4 ** (-np.arange(max(half, 1)) / max(half, 1))
+    cos, sin = np.cos(ang).astype(np.float32), np.sin(ang).astype(np.float32)
+    qn, kn = (rng.standard_normal((2, D)) * 0.1 + 1).astype(np.float32) if norms else (None, None)
+    K, V, Q = f64(c.k), f64(c.v), f64(q)
+    W = f64(c.w) if weights else None
+    KO.append(K, V, W, c.table.numpy(), seq, slot, p, f64(big), nh, qn, kn, 1e-5, cos if half else None, sin, Q)
+    # the size of a value's rotation pair, for the tolerance
+    mq, mk = f64(q) * 0, np.zeros_like(K)
+    for nw in (0,):
+        one, zero = np.ones_like(cos), np.zeros_like(cos)
+        KO.append(mk, np.zeros_like(V), None, c.table.numpy(), seq, slot, p, np.nan_to_num(f64(big)), nh, qn, kn, 1e-5,
+                  one if half else None, zero, mq)
+    d = lambda a: None if a is None else torch.from_numpy(a).cuda()
+    c.h.append(c.dev(), d(seq), d(slot), d(p), big.cuda(), q, q_norm=d(qn), k_norm=d(kn), eps=1e-5,
+               cos=d(cos) if half else None, sin=d(sin) if half else None)
+    torch.cuda.synchronize()
+
+    def close(got, want, mag, what):
+        pair = np.abs(mag) + np.roll(np.abs(mag), D // 2, -1)
+        tol = (D / 2 + 16) * 2.0 ** -24 * pair
+        tol = tol + U(torch, dt) * (np.abs(want) + tol) + 2.0 ** -25
+        same = np.isnan(got) & np.isnan(want)
+        bad = ~(same | (np.abs(got - want) <= tol))
+        assert not bad.any(), (what, np.argwhere(bad)[:5].tolist(), got[bad][:5], want[bad][:5])
+
+    close(f64(q), Q, mq, "q")
+    close(f64(c.k), K, mk, "k")
+    vr = f64(torch.from_numpy(V).to(dt))
+    assert np.array_equal(f64(c.v), vr, equal_nan=True), "v"
+    if weights:
+        assert np.array_equal(f64(c.w), W), "weights"
+
+
+def test_append_refuses_what_the_pointers_do_not_show(pb, cuda):
+    torch = cuda
+    c = Cache(pb, torch, [40], 2, 64, 16, torch.float16)
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    x, q = torch.zeros(1, 8 * 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, 4, 64, dtype=torch.float16, device="cuda")
+    t = c.dev()
+    for bad in (dict(q=q.bfloat16()), dict(qkv=x[:, :-64]), dict(qkv=x.double()), dict(qkv=x.cpu()), dict(seq=i(0).long()),
+                dict(seq=i(0, 0)), dict(slot=i(0).cpu()), dict(table=t.long()), dict(table=t[:, ::2]), dict(cos=torch.zeros(9, 8).cuda()),
+                dict(q_norm=torch.ones(32).cuda()), dict(q=torch.zeros(1, 4, 128, dtype=torch.float16).cuda()[:, :, ::2])):
+        a = dict(table=t, seq=i(0), slot=i(39), pos=None, qkv=x, q=q)
+        a.update(bad)
+        with pytest.raises(pb.PBError):
+            c.h.append(**a)
+    with pytest.raises(pb.PBError):
+        pb.KVPages(c.k, c.v[:2])
+    with pytest.raises(pb.PBError):
+        pb.KVPages(c.k.float(), c.v.float())
+    with pytest.raises(pb.PBError):
+        pb.KVPages(c.k, c.v, torch.zeros(3, device="cuda"))
+
+
+# ------------------------------------------------------------------ decode
+LENS = [0, 1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 130, 255, 257, 500, 777, 1031]
+DECODE = [  # nh, nkv, D, ps, cache, out, layout, window, sinks, lens
+    (32, 8, 64, 16, "float16", "bfloat16", "head", 0, 0, LENS),
+    (8, 2, 128, 32, "bfloat16", "bfloat16", "row", 0, 0, LENS),
+    (4, 4, 128, 64, "float16", "float16", "mixed", 0, 0, LENS),
+    (16, 1, 64, 128, "bfloat16", "float16", "head", 0, 0, LENS),
+    (15, 3, 128, 256, "float16", "bfloat16", "row", 0, 0, LENS),
+    (7, 1, 64, 16, "float16", "float16", "mixed", 0, 0, [1031]),
+    (12, 2, 128, 16, "float16", "float16", "head", 0, 0, [40] * 130),
+    (16, 4, 128, 32, "float16", "bfloat16", "head", 100, 4, LENS),
+    (9, 1, 64, 16, "bfloat16", "bfloat16", "head", 33, 70, LENS),
+    (2, 2, 64, 64, "float16", "float16", "row", 1, 0, LENS),
+    (2, 2, 128, 64, "float16", "float16", "row", 2000, 3, LENS),
+    (8, 8, 128, 128, "float16", "float16", "head", 256, 130, LENS),
+]
+
+
+@pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("nh,nkv,D,ps,dt,ot,layout,window,sinks,lens", DECODE)
+def test_decode(pb, cuda, nh, nkv, D, ps, dt, ot, layout, window, sinks, lens, weights):
+    torch = cuda
+    dt, ot = getattr(torch, dt), getattr(torch, ot)
+    c = Cache(pb, torch, lens, nkv, D, ps, dt, layout, weights, seed=nh + D)
+    if window:      # rows behind the window are gone: their pages freed, the rest of them NaN
+        for b, n in enumerate(lens):
+            pg, r, _ = KO.rows_of(c.table.numpy(), b, n, ps, c.n_pages)
+            hid = np.nonzero(~KO.seen(n - 1, n, window, sinks))[0]
+            for t in (c.k, c.v):
+                t[torch.from_numpy(pg[hid]).long().cuda(), :, torch.from_numpy(r[hid]).cuda()] = float("nan")
+            for p in range(-(-n // ps)):
+                if not KO.seen(n - 1, n, window, sinks)[p * ps:(p + 1) * ps].any():
+                    c.table[b, p] = -1
+    S = len(lens)
+    big = torch.randn((S, nh + 1, D), generator=c.g).to(dt).cuda()
+    q = big[:, :nh]
+    out = torch.full((S + 2, nh, D), 9.0, dtype=ot, device="cuda")
+    w0 = f64(c.w) if weights else None
+    scale = 0.7 * D ** -0.5
+    length = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    c.h.decode(c.dev(), length, q, out[:S], scale=scale, window=window, sinks=sinks, accumulate=weights)
+    torch.cuda.synchronize()
+    (o, spread, slack, tiny), sums = oracle_rows(c, q, lens, [1] * S, scale, window, sinks)
+    check(torch, f64(out)[:S], o, spread, slack, tiny, max(lens), dt, ot, "out")
+    assert (out[S:] == 9.0).all()
+    if weights:
+        w = w0.copy()
+        err = np.zeros_like(w)
+        for b, n in enumerate(lens):
+            pg, r, ok = KO.rows_of(c.table.numpy(), b, n, ps, c.n_pages)
+            for h in range(nkv):
+                grp = slice(h * (nh // nkv), (h + 1) * (nh // nkv))
+                w[pg[ok], h, r[ok]] += sums[b][h][ok]
+                err[pg[ok], h, r[ok]] = sums[b][h][ok] * (2 * slack[b][grp].max() + 2.0 ** -21 + (n + 32) * 2.0 ** -24)
+        got = f64(c.w)
+        bad = ~(np.abs(got - w) <= err + 2.0 ** -22 * np.abs(w))
+        assert not bad.any(), (np.argwhere(bad)[:4].tolist(), got[bad][:4], w[bad][:4])
+        untouched = w == w0
+        assert np.array_equal(got[untouched], w0[untouched])
+
+
+def test_decode_long_cache_split(pb, cuda):
+    """one sequence over every SM, a few around it, the longest row near the type's largest values"""
+    torch = cuda
+    lens = [20011, 1, 3000, 0, 9000]
+    c = Cache(pb, torch, lens, 2, 128, 64, torch.float16, seed=5)
+    q = (torch.randn((5, 8, 128), generator=c.g) * 3).half().cuda()
+    out = torch.empty((5, 8, 128), dtype=torch.float16, device="cuda")
+    length = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    c.h.decode(c.dev(), length, q, out)
+    torch.cuda.synchronize()
+    first = out.clone()
+    (o, spread, slack, tiny), _ = oracle_rows(c, q, lens, [1] * 5, 128 ** -0.5, 0, 0)
+    check(torch, f64(out), o, spread, slack, tiny, max(lens), c.dt, torch.float16, "long")
+    for _ in range(3):
+        out.fill_(3.0)
+        c.h.decode(c.dev(), length, q, out)
+        assert torch.equal(out, first)      # the same bits every time
+
+
+def test_decode_bad_lengths_pages_and_bounds(pb, cuda):
+    """lengths past max_len or the table count as the bound, negative ones as 0; bad pages hide their rows; a sequence
+    that sees nothing gets zeros"""
+    torch = cuda
+    lens = [100, 100, 100, 100, 100]
+    c = Cache(pb, torch, lens, 2, 64, 16, torch.bfloat16, weights=True, seed=9)
+    c.table[1, 2], c.table[1, 5], c.table[2, :] = -7, c.n_pages, -1
+    q = torch.randn((5, 8, 64), generator=c.g).bfloat16().cuda()
+    out = torch.empty((5, 8, 64), dtype=torch.bfloat16, device="cuda")
+    said = torch.tensor([100, 100, 100, -4, 2**31 - 1], dtype=torch.int32, device="cuda")
+    c.table[4, 4:] = -1          # its rows end at 64
+    w0 = f64(c.w)
+    c.h.decode(c.dev(), said, q, out, max_len=80, accumulate=True)
+    torch.cuda.synchronize()
+    (o, spread, slack, tiny), _ = oracle_rows(c, q, [80, 80, 80, 0, 80], [1] * 5, 64 ** -0.5, 0, 0)
+    check(torch, f64(out), o, spread, slack, tiny, 80, c.dt, torch.bfloat16, "bounds")
+    assert (out[2] == 0).all() and (out[3] == 0).all()
+    used = [int(p) for b in (0, 1, 4) for p in c.table[b, :5] if 0 <= p < c.n_pages]
+    rest = [p for p in range(c.n_pages) if p not in used]
+    assert np.array_equal(f64(c.w)[rest], w0[rest])
+
+
+def test_decode_extreme_values(pb, cuda):
+    """scores of +-thousands (one row takes all the weight), an infinite key, a NaN where it is seen"""
+    torch = cuda
+    lens = [300, 300, 300, 300]
+    c = Cache(pb, torch, lens, 1, 128, 32, torch.float16, seed=4)
+    q = torch.randn((4, 4, 128), generator=c.g).half().cuda()
+    q[0] *= 500
+    pg, r, _ = KO.rows_of(c.table.numpy(), 1, 300, 32, c.n_pages)
+    c.k[int(pg[77]), 0, int(r[77]), 3] = -float("inf")
+    q[1, :, 3] = 1.0                       # every head: score -inf there
+    pg2, r2, _ = KO.rows_of(c.table.numpy(), 2, 300, 32, c.n_pages)
+    c.v[int(pg2[10]), 0, int(r2[10]), 5] = float("nan")
+    out = torch.empty((4, 4, 128), dtype=torch.float16, device="cuda")
+    length = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    c.h.decode(c.dev(), length, q, out)
+    torch.cuda.synchronize()
+    (o, spread, slack, tiny), _ = oracle_rows(c, q, lens, [1] * 4, 128 ** -0.5, 0, 0)
+    got = f64(out)
+    slack = np.minimum(slack, 1.0)
+    assert np.isfinite(got[0]).all() and np.isfinite(got[1]).all()
+    check(torch, got[[0, 3]], o[[0, 3]], spread[[0, 3]], slack[[0, 3]], tiny[[0, 3]], 300, c.dt, torch.float16, "large scores")
+    clean = slack[3:4].repeat(1, 0)        # row 1's own slack is infinite with its key
+    check(torch, got[1:2], o[1:2], spread[1:2], clean, tiny[1:2], 300, c.dt, torch.float16, "minus infinity")
+    assert np.isnan(got[2, :, 5]).all() and np.isfinite(np.delete(got[2], 5, -1)).all()
+
+
+# ----------------------------------------------------------------- prefill
+PREFILL = [  # nh, nkv, D, ps, cache, out, layout, window, sinks, (rows in the cache, rows of the chunk)
+    (8, 2, 64, 16, "float16", "bfloat16", "head", 0, 0, [(32, 32), (1, 1), (77, 77), (200, 65), (131, 1)]),
+    (8, 2, 128, 32, "bfloat16", "bfloat16", "row", 0, 0, [(130, 130), (129, 2), (300, 33), (64, 64)]),
+    (4, 4, 128, 64, "float16", "float16", "mixed", 0, 0, [(257, 257), (500, 128)]),
+    (3, 1, 64, 128, "float16", "float16", "head", 0, 0, [(150, 150), (99, 98), (5, 5)]),
+    (5, 1, 128, 16, "float16", "bfloat16", "head", 0, 0, [(90, 60), (31, 31)]),
+    (16, 1, 128, 256, "bfloat16", "float16", "head", 0, 0, [(300, 41), (20, 20)]),
+    (7, 1, 64, 64, "bfloat16", "bfloat16", "row", 0, 0, [(400, 100)]),
+    (8, 2, 64, 16, "float16", "float16", "head", 16, 4, [(200, 200), (33, 33), (400, 17)]),
+    (8, 2, 128, 32, "bfloat16", "bfloat16", "head", 100, 0, [(350, 350), (101, 1)]),
+    (4, 1, 128, 64, "float16", "bfloat16", "mixed", 140, 70, [(500, 300), (64, 64)]),
+    (2, 2, 64, 128, "float16", "float16", "head", 1, 0, [(260, 260)]),
+    (2, 1, 128, 16, "float16", "float16", "head", 5000, 5, [(260, 130)]),
+    (8, 1, 64, 16, "float16", "bfloat16", "head", 24, 200, [(700, 300)]),
+]
+
+
+@pytest.mark.parametrize("nh,nkv,D,ps,dt,ot,layout,window,sinks,seqs", PREFILL)
+def test_prefill(pb, cuda, nh, nkv, D, ps, dt, ot, layout, window, sinks, seqs):
+    torch = cuda
+    dt, ot = getattr(torch, dt), getattr(torch, ot)
+    seqs = seqs[:1] + [(9, 0)] + seqs[1:]      # one sequence has no rows in the batch
+    lens, counts = [a for a, _ in seqs], [m for _, m in seqs]
+    c = Cache(pb, torch, lens, nkv, D, ps, dt, layout, seed=nh + D + window)
+    if window:      # what no query of a chunk sees is NaN, whole pages of it freed
+        for b, (n, m) in enumerate(seqs):
+            any_ = np.zeros(n, bool)
+            for t in range(n - m, n):
+                any_ |= KO.seen(t, n, window, sinks)
+            pg, r, _ = KO.rows_of(c.table.numpy(), b, n, ps, c.n_pages)
+            hid = np.nonzero(~any_)[0]
+            for t in (c.k, c.v):
+                t[torch.from_numpy(pg[hid]).long().cuda(), :, torch.from_numpy(r[hid]).cuda()] = float("nan")
+            for p in range(-(-n // ps)):
+                if not any_[p * ps:(p + 1) * ps].any():
+                    c.table[b, p] = -1
+    pad = 3                                    # rows before the first and behind the last sequence
+    rows = sum(counts)
+    q = torch.randn((rows + 2 * pad, nh, D), generator=c.g).to(dt).cuda()
+    out = torch.full((rows + 2 * pad, nh + 2, D), 9.0, dtype=ot, device="cuda")
+    start = torch.tensor(np.concatenate([[0], np.cumsum(counts)]) + pad, dtype=torch.int32, device="cuda")
+    length = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    scale = 1.3 * D ** -0.5
+    c.h.prefill(c.dev(), start, length, q, out[:, :nh], scale=scale, window=window, sinks=sinks)
+    torch.cuda.synchronize()
+    (o, spread, slack, tiny), _ = oracle_rows(c, q[pad:pad + rows], lens, counts, scale, window, sinks)
+    check(torch, f64(out)[pad:pad + rows, :nh], o, spread, slack, tiny, max(lens), dt, ot, "out")
+    assert (out[:pad] == 9.0).all() and (out[pad + rows:] == 9.0).all() and (out[:, nh:] == 9.0).all()
+
+
+def test_prefill_small_chunk_long_cache(pb, cuda):
+    """few rows against a long cache: the cache is split over the SMs, the same bits every time"""
+    torch = cuda
+    lens, counts = [9001, 16, 4100], [33, 16, 7]
+    c = Cache(pb, torch, lens, 2, 64, 16, torch.float16, seed=3)
+    q = torch.randn((56, 8, 64), generator=c.g).half().cuda()
+    out = torch.empty((56, 8, 64), dtype=torch.float16, device="cuda")
+    start = torch.tensor([0, 33, 49, 56], dtype=torch.int32, device="cuda")
+    length = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    c.h.prefill(c.dev(), start, length, q, out)
+    torch.cuda.synchronize()
+    (o, spread, slack, tiny), _ = oracle_rows(c, q, lens, counts, 64 ** -0.5, 0, 0)
+    check(torch, f64(out), o, spread, slack, tiny, max(lens), c.dt, torch.float16, "chunk")
+    first = out.clone()
+    for _ in range(3):
+        out.fill_(1.0)
+        c.h.prefill(c.dev(), start, length, q, out)
+        assert torch.equal(out, first)
+
+
+def test_prefill_bad_pages_and_lengths(pb, cuda):
+    """bad pages hide their rows; a chunk longer than its cache: the rows before the cache's first see nothing"""
+    torch = cuda
+    c = Cache(pb, torch, [100, 100, 100], 1, 128, 16, torch.float16, seed=6)
+    c.table[0, 1], c.table[0, 3], c.table[1, :] = -1, 10 ** 9, c.n_pages
+    q = torch.randn((60, 4, 128), generator=c.g).half().cuda()
+    out = torch.full((60, 4, 128), 5.0, dtype=torch.float16, device="cuda")
+    start = torch.tensor([0, 30, 40, 60], dtype=torch.int32, device="cuda")
+    said = torch.tensor([100, 100, 12], dtype=torch.int32, device="cuda")
+    c.h.prefill(c.dev(), start, said, q, out)
+    torch.cuda.synchronize()
+    (o, spread, slack, tiny), _ = oracle_rows(c, q, [100, 100, 12], [30, 10, 20], 128 ** -0.5, 0, 0)
+    check(torch, f64(out), o, spread, slack, tiny, 100, c.dt, torch.float16, "bad pages")
+    assert (out[30:40] == 0).all() and (out[40:48] == 0).all()
+
+
+def test_prefill_extreme_scores(pb, cuda):
+    torch = cuda
+    c = Cache(pb, torch, [400], 2, 128, 32, torch.bfloat16, seed=8)
+    q = (torch.randn((400, 8, 128), generator=c.g) * 200).bfloat16().cuda()
+    out = torch.empty((400, 8, 128), dtype=torch.bfloat16, device="cuda")
+    start = torch.tensor([0, 400], dtype=torch.int32, device="cuda")
+    c.h.prefill(c.dev(), start, torch.tensor([400], dtype=torch.int32, device="cuda"), q, out)
+    torch.cuda.synchronize()
+    (o, spread, slack, tiny), _ = oracle_rows(c, q, [400], [400], 128 ** -0.5, 0, 0)
+    check(torch, f64(out), o, spread, np.minimum(slack, 1.0), tiny, 400, c.dt, torch.bfloat16, "large scores")
+
+
+# ------------------------------------------------------------------- evict
+EVICT = [  # nkv, D, ps, dtype, layout, lens, budget, sinks, recent, weights
+    (4, 128, 16, "bfloat16", "head", [300, 200, 201, 0, 1, 77], 200, 4, 50, "random"),
+    (2, 64, 32, "float16", "row", [500, 499, 130], 128, 0, 0, "random"),
+    (1, 64, 64, "float16", "mixed", [1000], 700, 1, 699, "random"),
+    (3, 128, 16, "float16", "head", [400, 333], 160, 2, 30, "ties"),
+    (2, 64, 16, "bfloat16", "head", [400, 333], 160, 0, 16, "zeros"),
+    (2, 64, 16, "float16", "head", [400, 333], 160, 3, 16, "odd"),
+    (1, 64, 256, "float16", "head", [700], 256, 256, 0, "random"),
+    (1, 64, 128, "float16", "head", [12000], 1025, 5, 100, "random"),
+    (8, 64, 16, "float16", "head", [40, 30], 50, 5, 10, "random"),
+]
+
+
+@pytest.mark.parametrize("nkv,D,ps,dt,layout,lens,budget,sinks,recent,kind", EVICT)
+def test_evict(pb, cuda, nkv, D, ps, dt, layout, lens, budget, sinks, recent, kind):
+    torch = cuda
+    S = len(lens)
+    kept = [min(n, budget) for n in lens]
+    c = Cache(pb, torch, lens + kept, nkv, D, ps, getattr(torch, dt), layout, True, seed=budget)
+    table, dst = c.table[:S].contiguous(), c.table[S:].contiguous()
+    rng = np.random.default_rng(budget)
+    w = torch.from_numpy(rng.random(tuple(c.w.shape)).astype(np.float32) ** 6 * 30)
+    if kind == "ties":
+        w = (w * 0.2).round()
+    elif kind == "zeros":
+        w = w * 0
+    elif kind == "odd":
+        w.view(-1)[::7] = float("nan")
+        w.view(-1)[1::11] = -1.0
+        w.view(-1)[2::13] = float("inf")
+        w.view(-1)[3::5] = 1e-42
+    c.w.copy_(w.cuda())
+    K, V, W = f64(c.k), f64(c.v), f64(c.w)
+    length = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    new = torch.full((S,), -1, dtype=torch.int32, device="cuda")
+    c.h.evict(table.cuda(), length, dst.cuda(), new, budget, sinks=sinks, recent=recent)
+    torch.cuda.synchronize()
+    assert new.tolist() == kept
+    K2, V2, W2 = K.copy(), V.copy(), W.copy()
+    for b, n in enumerate(lens):
+        pg, r, _ = KO.rows_of(table.numpy(), b, n, ps, c.n_pages)
+        to, tr, _ = KO.rows_of(dst.numpy(), b, kept[b], ps, c.n_pages)
+        for h in range(nkv):
+            at = KO.evict_rows(W[pg, h, r], n, budget, sinks, recent)
+            assert len(at) == kept[b]
+            K2[to, h, tr], V2[to, h, tr], W2[to, h, tr] = K[pg[at], h, r[at]], V[pg[at], h, r[at]], W[pg[at], h, r[at]]
+    for got, want, what in ((c.k, K2, "k"), (c.v, V2, "v"), (c.w, W2, "weights")):
+        assert np.array_equal(f64(got), want, equal_nan=True), what
+
+
+def test_evict_lengths_in_place_and_bad_pages(pb, cuda):
+    torch = cuda
+    c = Cache(pb, torch, [300, 300, 150, 150], 2, 64, 16, torch.float16, "head", True, seed=2)
+    table, dst = c.table[:2].contiguous(), c.table[2:].contiguous()
+    table[0, 3], dst[1, 1] = -1, c.n_pages
+    W, K = f64(c.w), f64(c.k)
+    length = torch.tensor([300, 2**31 - 1], dtype=torch.int32, device="cuda")
+    c.h.evict(table.cuda(), length, dst.cuda(), length, 150, sinks=0, recent=10, max_len=299)
+    torch.cuda.synchronize()
+    assert length.tolist() == [150, 150]
+    for b in range(2):
+        pg, r, ok = KO.rows_of(table.numpy(), b, 299, 16, c.n_pages)
+        to, tr, dok = KO.rows_of(dst.numpy(), b, 150, 16, c.n_pages)
+        for h in range(2):
+            at = np.asarray(KO.evict_rows(np.where(ok, W[np.where(ok, pg, 0), h, r], 0), 299, 150, 0, 10))
+            m = ok[at] & dok
+            assert np.array_equal(f64(c.k)[to[m], h, tr[m]], K[pg[at[m]], h, r[at[m]]])
+            assert np.array_equal(f64(c.w)[to[m], h, tr[m]], W[pg[at[m]], h, r[at[m]]])
+
+
+# ---------------------------------------------------------------- together
+def test_prompt_decode_evict_decode(pb, cuda):
+    """as a server uses them: prompts appended and attended in chunks, decode steps that add weights, eviction to fresh
+    pages, more steps (slots behind the kept rows, positions going on), each result against the oracle on the cache as
+    it then is; replayed from a captured graph on another stream for the last steps"""
+    torch = cuda
+    nh, nkv, D, ps, dt = 8, 2, 64, 16, torch.float16
+    S, budget = 3, 64
+    prompt = [70, 33, 90]
+    c = Cache(pb, torch, [160] * S + [96] * S, nkv, D, ps, dt, "head", True, seed=12)
+    for t in (c.k, c.v):
+        t.fill_(float("nan"))
+    table, fresh = c.table[:S].contiguous(), c.table[S:].contiguous()
+    rng = np.random.default_rng(3)
+    wide = (nh + 2 * nkv) * D
+    ang = np.arange(200)[:, None] * 1e4 ** (-np.arange(D // 2) / (D // 2))
+    cos, sin = torch.from_numpy(np.cos(ang)).float().cuda(), torch.from_numpy(np.sin(ang)).float().cuda()
+    qn, kn = torch.ones(D).cuda() * 1.1, torch.ones(D).cuda() * 0.9
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    done = [0] * S
+    while any(d < p for d, p in zip(done, prompt)):
+        m = [min(32, p - d) for d, p in zip(done, prompt)]
+        seq = i32(sum([[b] * m[b] for b in range(S)], []))
+        slot = i32(sum([list(range(done[b], done[b] + m[b])) for b in range(S)], []))
+        n = sum(m)
+        x = torch.from_numpy(rng.standard_normal((n, wide))).bfloat16().cuda()
+        q, out = torch.empty((n, nh, D), dtype=dt, device="cuda"), torch.empty((n, nh, D), dtype=torch.bfloat16, device="cuda")
+        c.h.append(table.cuda(), seq, slot, None, x, q, q_norm=qn, k_norm=kn, cos=cos, sin=sin)
+        done = [d + a for d, a in zip(done, m)]
+        c.h.prefill(table.cuda(), i32(np.concatenate([[0], np.cumsum(m)]).tolist()), i32(done), q, out, window=48, sinks=2)
+        torch.cuda.synchronize()
+        c.table = table
+        (o, spread, slack, tiny), _ = oracle_rows(c, q, done, m, D ** -0.5, 48, 2)
+        check(torch, f64(out), o, spread, slack, tiny, 200, dt, torch.bfloat16, "prompt")
+
+    x = torch.empty((S, wide), dtype=torch.float32, device="cuda")
+    q, out = torch.empty((S, nh, D), dtype=dt, device="cuda"), torch.empty((S, nh, D), dtype=torch.bfloat16, device="cuda")
+    seq, slot, pos, length = i32(list(range(S))), i32(done), i32(done), i32(done)
+    scratch = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    tb = table.cuda()
+
+    def step(tb, stream=None):
+        c.h.append(tb, seq, slot, pos, x, q, q_norm=qn, k_norm=kn, cos=cos, sin=sin, stream=stream)
+        c.h.decode(tb, length, q, out, accumulate=True, scratch=scratch, stream=stream)
+
+    def verify(lens, what):
+        (o, spread, slack, tiny), _ = oracle_rows(c, q, lens, [1] * S, D ** -0.5, 0, 0)
+        check(torch, f64(out), o, spread, slack, tiny, 200, dt, torch.bfloat16, what)
+
+    lens = list(done)
+    for k in range(4):
+        x.copy_(torch.from_numpy(rng.standard_normal((S, wide))).float())
+        slot.copy_(i32(lens)); pos.copy_(i32(lens))
+        lens = [n + 1 for n in lens]
+        length.copy_(i32(lens))
+        step(tb)
+        torch.cuda.synchronize()
+        verify(lens, "step %d" % k)
+    position = list(lens)
+    c.h.evict(tb, length, fresh.cuda(), length, budget, sinks=2, recent=16)
+    torch.cuda.synchronize()
+    lens = [min(n, budget) for n in lens]
+    assert length.tolist() == lens
+    c.table, tb = fresh, fresh.cuda()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    before = (c.k.clone(), c.v.clone(), c.w.clone())
+    with torch.cuda.stream(side):
+        slot.copy_(i32(lens)); pos.copy_(i32(position)); length.copy_(i32([n + 1 for n in lens]))
+        step(tb, side)          # once before the capture
+    side.synchronize()
+    for t, o in zip((c.k, c.v, c.w), before):
+        t.copy_(o)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        step(tb, side)
+    for k in range(6):
+        x.copy_(torch.from_numpy(rng.standard_normal((S, wide))).float())
+        slot.copy_(i32(lens)); pos.copy_(i32(position))
+        lens, position = [n + 1 for n in lens], [p + 1 for p in position]
+        length.copy_(i32(lens))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        verify(lens, "replayed step %d" % k)
+
+
+def test_two_streams_at_once(pb, cuda):
+    """the same cache read by calls on two streams, each with scratch of its own"""
+    torch = cuda
+    lens = [3000, 2000, 1500]
+    c = Cache(pb, torch, lens, 2, 128, 32, torch.float16, seed=1)
+    q = torch.randn((3, 8, 128), generator=c.g).half().cuda()
+    length, tb = torch.tensor(lens, dtype=torch.int32, device="cuda"), c.dev()
+    want = torch.empty_like(q)
+    c.h.decode(tb, length, q, want)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [torch.empty_like(q) for _ in range(20)]
+    for n, o in enumerate(outs):
+        c.h.decode(tb, length, q, o, stream=streams[n % 2])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
