@@ -1,6 +1,7 @@
 // pb_kvattn.cu -- attention over the paged K/V cache: one new token per
 // sequence (pb_kv_decode) and the last rows of each sequence (pb_kv_prefill).
 #include "pb_kv.cuh"
+#include <atomic>
 #include <climits>
 
 namespace {
@@ -104,34 +105,490 @@ __global__ void __launch_bounds__(128) k_kv_attn(AttnKvArgs a) {
   }
 }
 
-// the weights: a warp per cache row and K/V head adds the row's probability
-// under every query head of the group
-template <int D, int CT>
-__global__ void __launch_bounds__(128) k_kv_weight(AttnKvArgs a) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 31;
-  const int b = blockIdx.y / a.p.n_kv, kh = blockIdx.y % a.p.n_kv;
-  const int j = blockIdx.x * 4 + (threadIdx.x >> 5), t = kv_len(a.len[b], a.max_len) - 1;
-  if (j > t || (a.window > 0 && j <= t - a.window && j >= a.sinks)) return;
-  const int page = kv_page(a.p, a.p.table + (size_t)b * a.p.table_ld, j);
-  if (page < 0) return;
-  const int row = j & ((1 << a.p.shift) - 1);
-  const char* kp = a.p.k + (long long)page * a.p.ps + (long long)kh * a.p.hs + (long long)row * a.p.rs;
-  float sum = 0.0f;
-  for (int g = 0; g < a.grp; g++) {
-    const int h = kh * a.grp + g;
-    float s = 0.0f;
+// ------------------------------------------------------------------ decode
+// One token per sequence. The work is the K/V bytes: 2 D elements per seen
+// row and K/V head, 4 D (n_heads / n_kv) flops on them, so HBM bounds it and
+// the rest has to keep out of the way:
+//  - the heads of a group share each row: S^T = K Q^T and O^T = V^T P^T as
+//    m16n8k16 matrix products with the group's heads as the 8 columns (two
+//    column tiles for groups of 9 to 16), K and V as they lie in memory;
+//  - every warp streams its own rows through a private ring of shared memory
+//    (16-byte asynchronous copies, rows that are not seen filled with zeros
+//    and never read), with running maximum and sum per head: no barrier
+//    until a piece of work ends;
+//  - the tiles of all sequences and K/V heads form one line, cut into equal
+//    pieces, one per CTA, whatever the lengths are; a sequence and head that a
+//    cut goes through is joined by a second, small kernel from the pieces'
+//    unnormalised sums, in the order of the line (the same bits every time).
+constexpr int DC_W = 4;      // warps per CTA
+
+template <int D>
+struct DcGeo {
+  static constexpr int KT = 2048 / D;            // rows per warp and tile: 4 KB of K, 4 KB of V
+  static constexpr int TILE = DC_W * KT;         // rows per tile
+  static constexpr int NB = KT / 16;             // 16-row blocks: one page each
+  static constexpr int NS = 3;                   // ring stages per warp
+  static constexpr int RING = DC_W * NS * 8192;
+  static constexpr int OP = D + 4;               // padded row of the merge buffer
+  static constexpr int SMEM = RING + DC_W * 8 * OP * 4 + DC_W * 8 * 8;
+};
+
+struct DcArgs {
+  AttnKvArgs a;
+  float* part;       // [2 grid][grp][D] unnormalised sums of pieces that are not a whole item
+  float* ml;         // [2 grid][grp][2] their maximum and sum
+  float* score;      // [item][max_len][grp2] log2-scaled scores (only for the weights)
+  int grid, grp2, out_bf16;
+};
+
+// tiles of sequence b: those of the sinks, then those from the window's first
+// row on (all of them where the two meet). At least one, so that a sequence
+// that sees nothing is written too.
+struct DcSeq {
+  int len, lo, sinks, nst, lot, nt;
+};
+template <int TILE>
+PB_DEV DcSeq dc_seq(const AttnKvArgs& a, int b) {
+  DcSeq s;
+  s.len = kv_len(__ldg(a.len + b), a.max_len);
+  s.lo = a.window > 0 ? max(0, s.len - a.window) : 0;
+  s.sinks = min(a.sinks, s.lo);
+  s.nst = (s.sinks + TILE - 1) / TILE;
+  s.lot = s.lo / TILE;
+  if (s.nst >= s.lot) s.nst = s.lot = 0;
+  s.nt = max(1, s.nst + (s.len + TILE - 1) / TILE - s.lot);
+  return s;
+}
+
+// The line of tiles, sequence by sequence, head by head: its length, and the
+// sequence in which tile x(total) lies with that sequence's first tile. A
+// thread sums a run of sequences; the runs are scanned over the CTA.
+template <int TILE, int T, typename F>
+PB_DEV void dc_locate(const AttnKvArgs& a, F pick, int& total, int& b, int& first) {
+  __shared__ int wsum[T / 32], found[2];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int per = (a.p.n_seq + T - 1) / T, b0 = min(a.p.n_seq, t * per), b1 = min(a.p.n_seq, b0 + per);
+  int own = 0;
+  for (int i = b0; i < b1; i++) own += dc_seq<TILE>(a, i).nt;
+  own *= a.p.n_kv;
+  int inc = own;
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-      const float2 k = kv_up<CT>(*reinterpret_cast<const unsigned*>(kp + (e * 32 + lane) * 4));
-      const float2 q = kv_up<CT>(*reinterpret_cast<const unsigned*>(a.q + (long long)b * a.ldq + (size_t)h * D * 2 + (e * 32 + lane) * 4));
-      s += q.x * k.x + q.y * k.y;
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    sum += kv_ex2(s * a.scale2 - a.lse[(size_t)b * a.nh + h]);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
   }
-  if (lane == 0) a.p.w[((size_t)page * a.p.n_kv + kh) * (1 << a.p.shift) + row] += sum;
+  if (lane == 31) wsum[warp] = inc;
+  __syncthreads();
+  int pre = inc - own;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < T / 32; w++) {
+    if (w < warp) pre += wsum[w];
+    total += wsum[w];
+  }
+  const int x = pick(total);
+  if (x >= pre && x < pre + own) {
+    for (int i = b0; i < b1; i++) {
+      const int n = dc_seq<TILE>(a, i).nt * a.p.n_kv;
+      if (x < pre + n) {
+        found[0] = i;
+        found[1] = pre;
+        break;
+      }
+      pre += n;
+    }
+  }
+  __syncthreads();
+  b = found[0];   // (undefined when x lies past the line: the caller's CTA has no piece)
+  first = found[1];
+}
+
+// the pieces: one per CTA, none of them empty
+PB_DEV int dc_pieces(const DcArgs& d, int total) { return min(d.grid, total); }
+// piece w of `grid` over `total` tiles begins at tile total w / grid
+PB_DEV int dc_cut(int w, int total, int grid) { return (int)((long long)total * w / grid); }
+// the piece that holds tile x
+PB_DEV int dc_piece(int x, int total, int grid) { return (int)((((long long)x + 1) * grid - 1) / total); }
+
+PB_DEV uint32_t kv_s32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+PB_DEV void kv_cp16(uint32_t dst, const char* src, bool in) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+template <int N>
+PB_DEV void kv_cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+PB_DEV void kv_cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+PB_DEV void kv_ldm(uint32_t at, unsigned (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+PB_DEV void kv_ldmt(uint32_t at, unsigned (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+template <int CT>
+PB_DEV void kv_mma(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+  if (CT == PB_DT_F16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+PB_DEV unsigned kv_trans(unsigned x) {
+  unsigned y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// a place on the line of tiles
+struct DcAt {
+  DcSeq s;
+  int b, kh, t;
+};
+template <int TILE>
+PB_DEV void dc_next(const AttnKvArgs& a, DcAt& w) {
+  if (++w.t < w.s.nt) return;
+  w.t = 0;
+  if (++w.kh < a.p.n_kv) return;
+  w.kh = 0;
+  if (++w.b < a.p.n_seq) w.s = dc_seq<TILE>(a, w.b);
+}
+
+// output of one group: normalised rows, or the piece's sums
+template <int D>
+PB_DEV void dc_store(const DcArgs& d, int b, int h, int e, const float4& x) {
+  char* o = d.a.out + (long long)b * d.a.ldo + (size_t)h * (D * 2) + e * 2;
+  uint2 w;
+  if (d.out_bf16) w = make_uint2(kv_down<PB_DT_BF16>(x.x, x.y), kv_down<PB_DT_BF16>(x.z, x.w));
+  else w = make_uint2(kv_down<PB_DT_F16>(x.x, x.y), kv_down<PB_DT_F16>(x.z, x.w));
+  *reinterpret_cast<uint2*>(o) = w;
+}
+
+template <int D, int CT, int NT>
+__global__ void __launch_bounds__(32 * DC_W, 2) k_kv_decode(DcArgs d) {
+  typedef DcGeo<D> G;
+  constexpr int KT = G::KT, TILE = G::TILE, NB = G::NB, NS = G::NS, CPR = D / 8, RS = 32 / CPR;
+  extern __shared__ __align__(128) char dsm[];
+  const AttnKvArgs& a = d.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pb_grid_launch_dependents();
+  int total, b, first;
+  dc_locate<TILE, 32 * DC_W>(a, [&](int n) { return dc_cut(blockIdx.x, n, dc_pieces(d, n)); }, total, b, first);
+  const int pieces = dc_pieces(d, total);
+  if ((int)blockIdx.x >= pieces) return;   // CTA-uniform
+  const int x0 = dc_cut(blockIdx.x, total, pieces), x1 = dc_cut(blockIdx.x + 1, total, pieces);
+  DcAt at;
+  at.b = b;
+  at.s = dc_seq<TILE>(a, b);
+  at.kh = (x0 - first) / at.s.nt;
+  at.t = (x0 - first) % at.s.nt;
+
+  // ---- the issuing side, NS - 1 tiles ahead
+  char* ring = dsm + warp * (NS * 8192);
+  const int cc = lane % CPR, rr = lane / CPR;
+  const uint32_t ring0 = kv_s32(ring);
+  uint32_t soff[16 / RS];   // this lane's chunk of its rows in a 16-row block, swizzled by the row
+#pragma unroll
+  for (int i = 0; i < 16 / RS; i++) {
+    const int r = rr + i * RS;
+    soff[i] = r * (D * 2) + ((cc ^ (r & 7)) << 4);
+  }
+  DcAt ia = at;
+  int ix = x0, islot = 0;
+  unsigned vbits = 0;       // validity of the 16-row blocks in flight, newest lowest
+  int pg[NB];
+  auto key0 = [&](const DcAt& w) {
+    return (w.t < w.s.nst ? w.t : w.t - w.s.nst + w.s.lot) * TILE + warp * KT;
+  };
+  auto pages = [&]() {      // the pages of the tile to be issued next
+    const int* trow = a.p.table + (size_t)ia.b * a.p.table_ld;
+    const int j = key0(ia);
+#pragma unroll
+    for (int n = 0; n < NB; n++) pg[n] = j + n * 16 < ia.s.len ? __ldg(trow + ((j + n * 16) >> a.p.shift)) : -1;
+  };
+  pages();
+  auto issue = [&]() {
+    if (ix < x1) {
+      const int j = key0(ia);
+      const uint32_t st = ring0 + islot * 8192;
+#pragma unroll
+      for (int n = 0; n < NB; n++) {
+        const bool ok = (unsigned)pg[n] < (unsigned)a.p.n_pages;
+        vbits = (vbits << 1) | (ok ? 1u : 0u);
+        const int j0 = j + n * 16;
+        const long long off = ok ? (long long)pg[n] * a.p.ps + (long long)ia.kh * a.p.hs +
+                                       (long long)((j0 & ((1 << a.p.shift) - 1)) + rr) * a.p.rs + cc * 16
+                                 : 0;
+        const char *kp = a.p.k + off, *vp = a.p.v + off;
+#pragma unroll
+        for (int i = 0; i < 16 / RS; i++) {
+          const int r = j0 + rr + i * RS;
+          const bool in = ok && r < ia.s.len && (r >= ia.s.lo || r < ia.s.sinks);
+          const long long o = in ? (long long)(i * RS) * a.p.rs : 0;
+          kv_cp16(st + n * (16 * D * 2) + soff[i], kp + o, in);
+          kv_cp16(st + 4096 + n * (16 * D * 2) + soff[i], vp + o, in);
+        }
+      }
+      if (++ix < x1) {
+        const int was = ia.b, kw = ia.kh;
+        dc_next<TILE>(a, ia);
+        pages();
+        if (ia.b != was || ia.kh != kw) {   // the next group's queries on their way to L1
+          const char* q = a.q + (long long)ia.b * a.ldq + (size_t)ia.kh * a.grp * (D * 2);
+          if (lane * 128 < a.grp * D * 2) asm volatile("prefetch.global.L1 [%0];" ::"l"(q + lane * 128));
+        }
+      }
+      if (++islot == NS) islot = 0;
+    } else {
+      vbits <<= NB;
+    }
+    kv_cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < NS - 1; i++) issue();
+
+  // ---- the consuming side
+  const int g = lane >> 2, c = lane & 3;
+  unsigned qf[NT][D / 16][2];
+  float o[NT][D / 16][4], m[NT][2], l[NT][2];
+  int slot = 0;
+  // ldmatrix: lane i gives the address of row i % 8 of matrix i / 8. K (rows
+  // = keys): matrices (keys 0-7, dims 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15)
+  const int lr = lane & 7, lq = lane >> 3;
+  const int krow = lr + (lq & 1) * 8, kch = lq >> 1;
+  // V transposed (rows = dims): (dims 0-7, keys 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15)
+  const int vrow = lr + (lq >> 1) * 8, vch = lq & 1;
+  float* mo = reinterpret_cast<float*>(dsm + G::RING);
+  float* mml = mo + DC_W * 8 * G::OP;
+  bool fresh = true;
+  int t0 = at.t;            // first tile of this piece in its item
+  for (int x = x0; x < x1; x++) {
+    if (fresh) {
+      fresh = false;
+      t0 = at.t;
+      const char* q = a.q + (long long)at.b * a.ldq + (size_t)at.kh * a.grp * (D * 2);
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        const int h = n * 8 + g;
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) {
+#pragma unroll
+          for (int u = 0; u < 2; u++)
+            qf[n][k][u] = h < a.grp ? __ldg(reinterpret_cast<const unsigned*>(q + (size_t)h * (D * 2) + (k * 16 + u * 8 + 2 * c) * 2)) : 0u;
+        }
+#pragma unroll
+        for (int k = 0; k < D / 16; k++)
+#pragma unroll
+          for (int u = 0; u < 4; u++) o[n][k][u] = 0.0f;
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.0f;
+      }
+    }
+    kv_cp_wait<NS - 2>();
+    __syncwarp();           // the tile has landed for every lane, and its predecessor's slot is free
+    const unsigned vb = vbits >> ((NS - 2) * NB);
+    issue();
+    const int j = key0(at);
+    const uint32_t ks = ring0 + slot * 8192, vs = ks + 4096;
+    if (++slot == NS) slot = 0;
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+      const int j0 = j + nb * 16;
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < D / 16; k++) {
+        unsigned f[4];
+        kv_ldm(ks + (nb * 16 + krow) * (D * 2) + (((2 * k + kch) ^ (krow & 7)) << 4), f);
+#pragma unroll
+        for (int n = 0; n < NT; n++) kv_mma<CT>(s[n], f, qf[n][k][0], qf[n][k][1]);
+      }
+      const bool okb = (vb >> (NB - 1 - nb)) & 1u;
+      const bool whole = okb && j0 + 16 <= at.s.len && (j0 >= at.s.lo || j0 + 16 <= at.s.sinks);   // warp-uniform
+      const int ja = j0 + g, jb = ja + 8;
+      const bool ina = whole || (okb && ja < at.s.len && (ja >= at.s.lo || ja < at.s.sinks));
+      const bool inb = whole || (okb && jb < at.s.len && (jb >= at.s.lo || jb < at.s.sinks));
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          s[n][u] = ina ? s[n][u] * a.scale2 : -INFINITY;
+          s[n][2 + u] = inb ? s[n][2 + u] * a.scale2 : -INFINITY;
+        }
+        if (d.score) {
+          const int h = n * 8 + 2 * c;
+          if (h < d.grp2) {
+            float* sp = d.score + (((size_t)at.b * a.p.n_kv + at.kh) * a.max_len + ja) * d.grp2 + h;
+            if (ina) *reinterpret_cast<float2*>(sp) = make_float2(s[n][0], s[n][1]);
+            if (inb) *reinterpret_cast<float2*>(sp + 8 * d.grp2) = make_float2(s[n][2], s[n][3]);
+          }
+        }
+        float mx[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          mx[u] = fmaxf(s[n][u], s[n][2 + u]);
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], w));
+          mx[u] = fmaxf(mx[u], m[n][u]);
+        }
+        if (__any_sync(0xffffffffu, mx[0] > m[n][0] || mx[1] > m[n][1])) {
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            const float f = mx[u] > m[n][u] ? kv_ex2(m[n][u] - mx[u]) : 1.0f;
+            m[n][u] = mx[u];
+            l[n][u] *= f;
+#pragma unroll
+            for (int k = 0; k < D / 16; k++) { o[n][k][u] *= f; o[n][k][2 + u] *= f; }
+          }
+        }
+        // p in the cache's type for the matrix product; their sum in fp32 from before that rounding
+        float p[4];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const float r = m[n][u] == -INFINITY ? 0.0f : m[n][u];
+          p[u] = kv_ex2(s[n][u] - r);
+          p[2 + u] = kv_ex2(s[n][2 + u] - r);
+          l[n][u] += p[u] + p[2 + u];
+        }
+        const unsigned b0 = kv_trans(kv_down<CT>(p[0], p[1])), b1 = kv_trans(kv_down<CT>(p[2], p[3]));
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) {
+          unsigned f[4];
+          kv_ldmt(vs + (nb * 16 + vrow) * (D * 2) + (((2 * k + vch) ^ (vrow & 7)) << 4), f);
+          kv_mma<CT>(o[n][k], f, b0, b1);
+        }
+      }
+    }
+    const bool ends = at.t == at.s.nt - 1;
+    if (ends || x == x1 - 1) {
+      // the piece of this group is done: merge the warps
+      const bool whole = t0 == 0 && ends;
+      const int slot_p = 2 * blockIdx.x + (t0 == 0 ? 1 : 0);
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) l[n][u] += __shfl_xor_sync(0xffffffffu, l[n][u], w);
+          float* row = mo + (warp * 8 + 2 * c + u) * G::OP;
+#pragma unroll
+          for (int k = 0; k < D / 16; k++) { row[k * 16 + g] = o[n][k][u]; row[k * 16 + g + 8] = o[n][k][2 + u]; }
+          if (g == 0) { mml[(warp * 8 + 2 * c + u) * 2] = m[n][u]; mml[(warp * 8 + 2 * c + u) * 2 + 1] = l[n][u]; }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 8 * (D / 4); i += 32 * DC_W) {
+          const int h = i / (D / 4), e = (i % (D / 4)) * 4, hg = n * 8 + h;
+          if (hg >= a.grp) break;
+          float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+          for (int w = 0; w < DC_W; w++) mm = fmaxf(mm, mml[(w * 8 + h) * 2]);
+          const float r = mm == -INFINITY ? 0.0f : mm;
+          float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+          for (int w = 0; w < DC_W; w++) {
+            const float f = kv_ex2(mml[(w * 8 + h) * 2] - r);
+            const float4 z = *reinterpret_cast<const float4*>(mo + (w * 8 + h) * G::OP + e);
+            ll += f * mml[(w * 8 + h) * 2 + 1];
+            y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
+          }
+          if (whole) {
+            const float f = ll != 0.0f ? 1.0f / ll : 0.0f;   // nothing seen: zeros
+            dc_store<D>(d, at.b, at.kh * a.grp + hg, e, make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
+            if (a.lse && e == 0) a.lse[(size_t)at.b * a.nh + at.kh * a.grp + hg] = mm + log2f(ll);
+          } else {
+            *reinterpret_cast<float4*>(d.part + ((size_t)slot_p * a.grp + hg) * D + e) = y;
+            if (e == 0) *reinterpret_cast<float2*>(d.ml + ((size_t)slot_p * a.grp + hg) * 2) = make_float2(mm, ll);
+          }
+        }
+        __syncthreads();
+      }
+      fresh = true;
+    }
+    dc_next<TILE>(a, at);
+  }
+  kv_cp_wait<0>();
+}
+
+// one CTA per sequence and K/V head: the pieces of a group that was cut
+template <int D>
+__global__ void __launch_bounds__(128) k_kv_join(DcArgs d) {
+  const AttnKvArgs& a = d.a;
+  constexpr int TILE = DcGeo<D>::TILE;
+  const int b = blockIdx.x / a.p.n_kv, kh = blockIdx.x % a.p.n_kv;
+  __shared__ int wsum[4][2];
+  pb_grid_launch_dependents();
+  // tiles of the sequences before b, and of all
+  int pre = 0, total = 0;
+  for (int i = threadIdx.x; i < a.p.n_seq; i += 128) {
+    const int n = dc_seq<TILE>(a, i).nt;
+    total += n;
+    if (i < b) pre += n;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    pre += __shfl_xor_sync(0xffffffffu, pre, o);
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+  }
+  if ((threadIdx.x & 31) == 0) { wsum[threadIdx.x >> 5][0] = pre; wsum[threadIdx.x >> 5][1] = total; }
+  __syncthreads();
+  pre = (wsum[0][0] + wsum[1][0] + wsum[2][0] + wsum[3][0]) * a.p.n_kv;
+  total = (wsum[0][1] + wsum[1][1] + wsum[2][1] + wsum[3][1]) * a.p.n_kv;
+  const int nt = dc_seq<TILE>(a, b).nt, s = pre + kh * nt;
+  const int pieces = dc_pieces(d, total);
+  const int w0 = dc_piece(s, total, pieces), w1 = dc_piece(s + nt - 1, total, pieces);
+  pb_grid_wait();
+  if (w0 == w1) return;     // whole: written by its CTA
+  for (int i = threadIdx.x; i < a.grp * (D / 4); i += 128) {
+    const int h = i / (D / 4), e = (i % (D / 4)) * 4;
+    float mm = -INFINITY, ll = 0.0f;
+    for (int w = w0; w <= w1; w++) mm = fmaxf(mm, __ldcg(d.ml + ((size_t)(2 * w + (w == w0)) * a.grp + h) * 2));
+    const float r = mm == -INFINITY ? 0.0f : mm;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int w = w0; w <= w1; w++) {
+      const size_t at = (size_t)(2 * w + (w == w0)) * a.grp + h;
+      const float2 q = __ldcg(reinterpret_cast<const float2*>(d.ml + at * 2));
+      const float4 z = __ldcg(reinterpret_cast<const float4*>(d.part + at * D + e));
+      const float f = kv_ex2(q.x - r);
+      ll += f * q.y;
+      y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
+    }
+    const float f = ll != 0.0f ? 1.0f / ll : 0.0f;
+    dc_store<D>(d, b, kh * a.grp + h, e, make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
+    if (a.lse && e == 0) a.lse[(size_t)b * a.nh + kh * a.grp + h] = mm + log2f(ll);
+  }
+}
+
+// the weights: a thread per seen row and K/V head adds the row's
+// probabilities under the heads of the group, from the kept scores; the same
+// line of tiles and the same cuts as the attention
+template <int D>
+__global__ void __launch_bounds__(128) k_kv_weight(DcArgs d) {
+  constexpr int TILE = DcGeo<D>::TILE;
+  const AttnKvArgs& a = d.a;
+  int total, b, first;
+  dc_locate<TILE, 128>(a, [&](int n) { return dc_cut(blockIdx.x, n, dc_pieces(d, n)); }, total, b, first);
+  const int pieces = dc_pieces(d, total);
+  pb_grid_wait();
+  if ((int)blockIdx.x >= pieces) return;
+  const int x0 = dc_cut(blockIdx.x, total, pieces), x1 = dc_cut(blockIdx.x + 1, total, pieces);
+  DcAt at;
+  at.b = b;
+  at.s = dc_seq<TILE>(a, b);
+  at.kh = (x0 - first) / at.s.nt;
+  at.t = (x0 - first) % at.s.nt;
+  for (int x = x0; x < x1; x++, dc_next<TILE>(a, at)) {
+    if (threadIdx.x >= TILE) continue;
+    const int j = (at.t < at.s.nst ? at.t : at.t - at.s.nst + at.s.lot) * TILE + threadIdx.x;
+    if (j >= at.s.len || (j < at.s.lo && j >= at.s.sinks)) continue;
+    const int page = kv_page(a.p, a.p.table + (size_t)at.b * a.p.table_ld, j);
+    if (page < 0) continue;
+    const float* sp = d.score + (((size_t)at.b * a.p.n_kv + at.kh) * a.max_len + j) * d.grp2;
+    const float* lp = a.lse + (size_t)at.b * a.nh + at.kh * a.grp;
+    float sum = 0.0f;
+    for (int h = 0; h < a.grp; h++) sum += kv_ex2(__ldcg(sp + h) - __ldcg(lp + h));
+    a.p.w[((size_t)page * a.p.n_kv + at.kh) * (1 << a.p.shift) + (j & ((1 << a.p.shift) - 1))] += sum;
+  }
 }
 
 int attn_check(const char* who, const pb_kv_pages* c, const KvPool& p, const int* d_len, int* max_len, int table_ld, int rows,
@@ -178,44 +635,115 @@ void attn_launch(const AttnKvArgs& a, int ct, int ot, cudaStream_t st) {
   }
 }
 
+// launch shape and scratch of a decode call
+struct DcPlan {
+  int grid, grp2;
+  bool join;
+  long long part, ml, lse, score;   // floats
+};
+template <int D>
+DcPlan dc_plan_t(int n_seq, int n_kv, int max_len, int grp, int accumulate) {
+  DcPlan p{};
+  const long long most = (max_len + DcGeo<D>::TILE - 1) / DcGeo<D>::TILE, items = (long long)n_seq * n_kv;
+  const long long all = items * (most > 0 ? most : 1), cap = 2LL * pb_num_sms();
+  p.grid = (int)(all < cap ? all : cap);
+  p.grp2 = (grp + 1) / 2 * 2;
+  // a sequence of one tile cannot be cut
+  p.join = most > 1;
+  p.part = p.join ? 2LL * p.grid * grp * D : 0;
+  p.ml = p.join ? 2LL * p.grid * grp * 2 : 0;
+  p.lse = accumulate ? (items * grp + 3) / 4 * 4 : 0;
+  p.score = accumulate ? items * max_len * p.grp2 : 0;
+  return p;
+}
+DcPlan dc_plan(const pb_kv_pages* c, int n_seq, int max_len, int n_heads, int accumulate) {
+  return c->head_dim == 64 ? dc_plan_t<64>(n_seq, c->n_kv, max_len, n_heads / c->n_kv, accumulate)
+                           : dc_plan_t<128>(n_seq, c->n_kv, max_len, n_heads / c->n_kv, accumulate);
+}
+
+// dynamic shared memory above 48 KB is allowed once per device and kernel
+template <typename K>
+int kv_smem(K k, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  PB_TRY_CUDA(cudaGetDevice(&dev));
+  if (dev < 64 && (done.load(std::memory_order_acquire) >> dev) & 1) return PB_OK;
+  PB_TRY_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+  return PB_OK;
+}
+
+template <typename... KArgs, typename... Args>
+int kv_launch(void (*k)(KArgs...), unsigned grid, int block, int smem, cudaStream_t st, bool pdl, const char* name, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k, args...);
+  if (e != cudaSuccess) return pb_set_error(PB_ECUDA, "%s: %s", name, cudaGetErrorString(e));
+  pb_count_launch();
+  return PB_OK;
+}
+
+template <int D, int CT, int NT>
+int dc_launch(const DcArgs& d, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  if (int rc = kv_smem(k_kv_decode<D, CT, NT>, DcGeo<D>::SMEM, done)) return rc;
+  return kv_launch(k_kv_decode<D, CT, NT>, (unsigned)d.grid, 32 * DC_W, DcGeo<D>::SMEM, st, false, "k_kv_decode", d);
+}
+
+template <int D>
+int dc_run(const DcArgs& d, int ct, bool join, cudaStream_t st) {
+  const bool two = d.a.grp > 8;
+  int rc;
+  if (ct == PB_DT_F16) rc = two ? dc_launch<D, PB_DT_F16, 2>(d, st) : dc_launch<D, PB_DT_F16, 1>(d, st);
+  else rc = two ? dc_launch<D, PB_DT_BF16, 2>(d, st) : dc_launch<D, PB_DT_BF16, 1>(d, st);
+  if (rc) return rc;
+  if (join && (rc = kv_launch(k_kv_join<D>, (unsigned)(d.a.p.n_seq * d.a.p.n_kv), 128, 0, st, true, "k_kv_join", d))) return rc;
+  if (d.score) rc = kv_launch(k_kv_weight<D>, (unsigned)d.grid, 128, 0, st, true, "k_kv_weight", d);
+  return rc;
+}
+
 }  // namespace
 
 extern "C" long long pb_kv_decode_scratch(const pb_kv_pages* c, int n_seq, int max_len, int n_heads, int accumulate) {
-  if (!c || n_seq < 0 || max_len < 0 || n_heads <= 0) return -1;
-  return accumulate ? (long long)n_seq * n_heads * 4 : 0;
+  if (!c || n_seq < 0 || max_len < 0 || n_heads <= 0 || c->n_kv <= 0 || (c->head_dim != 64 && c->head_dim != 128)) return -1;
+  const DcPlan p = dc_plan(c, n_seq, max_len, n_heads, accumulate);
+  return 4 * (p.part + p.ml + p.lse + p.score);
 }
 
 extern "C" int pb_kv_decode(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const int* d_len, int max_len,
                             int n_heads, const void* d_q, long long ldq, float scale, int window, int sinks, int accumulate,
                             void* d_out, int out_dtype, long long ldo, void* d_scratch, long long scratch_bytes, void* stream) {
+  DcArgs d{};
   KvPool p{};
-  AttnKvArgs a{};
   if (int rc = kv_pool("pb_kv_decode", c, n_seq, d_table, table_ld, &p)) return rc;
   if (int rc = attn_check("pb_kv_decode", c, p, d_len, &max_len, table_ld, n_seq, n_heads, d_q, ldq, scale, window, sinks, d_out,
-                          out_dtype, ldo, &a))
+                          out_dtype, ldo, &d.a))
     return rc;
   if (accumulate && !c->weight) return pb_set_error(PB_EINVAL, "pb_kv_decode: the cache keeps no weights");
+  if ((long long)n_seq * c->n_kv * ((max_len + 63) / 64) > INT_MAX)
+    return pb_set_error(PB_EINVAL, "pb_kv_decode: %d sequences of %d rows", n_seq, max_len);
   const long long need = pb_kv_decode_scratch(c, n_seq, max_len, n_heads, accumulate);
-  if (need > 0 && (!d_scratch || scratch_bytes < need))
-    return pb_set_error(PB_EINVAL, "pb_kv_decode: scratch of %lld bytes, %lld needed", scratch_bytes, need);
+  if (need > 0 && (!d_scratch || scratch_bytes < need || (reinterpret_cast<size_t>(d_scratch) & 15)))
+    return pb_set_error(PB_EINVAL, "pb_kv_decode: scratch of %lld bytes, %lld needed (16-byte aligned)", scratch_bytes, need);
   if (n_seq == 0) return PB_OK;
+  const DcPlan pl = dc_plan(c, n_seq, max_len, n_heads, accumulate);
+  float* f = static_cast<float*>(d_scratch);
+  d.part = f;
+  d.ml = f + pl.part;
+  d.a.lse = accumulate ? d.ml + pl.ml : nullptr;
+  d.score = accumulate ? d.a.lse + pl.lse : nullptr;
+  d.grid = pl.grid;
+  d.grp2 = pl.grp2;
+  d.out_bf16 = out_dtype == PB_DT_BF16;
   cudaStream_t st = (cudaStream_t)stream;
-  a.lse = accumulate ? static_cast<float*>(d_scratch) : nullptr;
-  if (c->head_dim == 64) attn_launch<64>(a, c->dtype, out_dtype, st);
-  else attn_launch<128>(a, c->dtype, out_dtype, st);
-  PB_LAUNCHED("k_kv_attn");
-  if (accumulate) {
-    const dim3 g((unsigned)((max_len + 3) / 4), (unsigned)(n_seq * c->n_kv));
-    if (c->head_dim == 64) {
-      if (c->dtype == PB_DT_F16) k_kv_weight<64, PB_DT_F16><<<g, 128, 0, st>>>(a);
-      else k_kv_weight<64, PB_DT_BF16><<<g, 128, 0, st>>>(a);
-    } else {
-      if (c->dtype == PB_DT_F16) k_kv_weight<128, PB_DT_F16><<<g, 128, 0, st>>>(a);
-      else k_kv_weight<128, PB_DT_BF16><<<g, 128, 0, st>>>(a);
-    }
-    PB_LAUNCHED("k_kv_weight");
-  }
-  return PB_OK;
+  return c->head_dim == 64 ? dc_run<64>(d, c->dtype, pl.join, st) : dc_run<128>(d, c->dtype, pl.join, st);
 }
 
 extern "C" long long pb_kv_prefill_scratch(const pb_kv_pages* c, int n_seq, int max_len, int n_tok, int n_heads) {
