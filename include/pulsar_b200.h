@@ -421,6 +421,9 @@ long long pb_kv_prefill_scratch(const pb_kv_pages* c, int n_seq, int max_len, in
 int pb_kv_prefill(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const int* d_start, const int* d_len,
                   int max_len, int n_tok, int n_heads, const void* d_q, long long ldq, float scale, int window, int sinks,
                   void* d_out, int out_dtype, long long ldo, void* d_scratch, long long scratch_bytes, void* stream);
+/* synchronise `stream` and report a bounded wait inside the current device's
+ * pb_kv_prefill kernels that gave up since the last report: PB_OK or PB_ECUDA */
+int pb_kv_status(void* stream);
 /* per sequence and K/V head, keep the first `sinks` rows, the last `recent`
  * rows and, up to `budget` rows in all, those of the largest weight (equal
  * weights: the lowest row first; a weight that is not above 0 counts as 0).

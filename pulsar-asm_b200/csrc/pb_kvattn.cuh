@@ -1,0 +1,140 @@
+// pb_kvattn.cuh -- what the two attention kernels over the paged K/V cache
+// share (pb_kvattn.cu: one token per sequence; pb_kvprefill.cu: prompt
+// chunks): arguments and their checks, the search of the line of work, copies.
+#pragma once
+#include "pb_kv.cuh"
+#include <atomic>
+#include <climits>
+
+namespace {
+
+struct AttnKvArgs {
+  KvPool p;
+  const int* len;
+  const int* start;     // prefill: row offsets [n_seq + 1]
+  const char* q;
+  char* out;
+  long long ldq, ldo;   // bytes
+  int n_rows, nh, grp, max_len, window, sinks;
+  float scale2;         // scale * log2(e): the softmax runs in powers of two
+  float* lse;           // [row][nh]: log2 of the softmax sum (only for the weights)
+};
+
+PB_DEV float kv_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Sequences laid end to end on a line, count(i) units each: the line's length
+// and, for the unit pick(length), its sequence and that sequence's first unit
+// (undefined when it lies past the line: the caller has no work then). A
+// thread of the CTA's T sums a run of sequences; the runs are scanned.
+template <int T, typename C, typename F>
+PB_DEV void kv_locate(int n_seq, C count, F pick, int& total, int& b, int& first) {
+  __shared__ int wsum[T / 32], found[2];
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const int per = (n_seq + T - 1) / T, b0 = min(n_seq, t * per), b1 = min(n_seq, b0 + per);
+  int own = 0;
+  for (int i = b0; i < b1; i++) own += count(i);
+  int inc = own;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) wsum[warp] = inc;
+  __syncthreads();
+  int pre = inc - own;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < T / 32; w++) {
+    if (w < warp) pre += wsum[w];
+    total += wsum[w];
+  }
+  const int x = pick(total);
+  if (x >= pre && x < pre + own) {
+    for (int i = b0; i < b1; i++) {
+      const int n = count(i);
+      if (x < pre + n) {
+        found[0] = i;
+        found[1] = pre;
+        break;
+      }
+      pre += n;
+    }
+  }
+  __syncthreads();
+  b = found[0];
+  first = found[1];
+}
+
+PB_DEV uint32_t kv_s32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+PB_DEV void kv_cp16(uint32_t dst, const char* src, bool in) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+template <int N>
+PB_DEV void kv_cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+PB_DEV void kv_cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+inline int attn_check(const char* who, const pb_kv_pages* c, const KvPool& p, const int* d_len, int* max_len, int table_ld, int rows,
+               int n_heads, const void* d_q, long long ldq, float scale, int window, int sinks, const void* d_out, int out_dtype,
+               long long ldo, AttnKvArgs* a) {
+  if (!d_len || !d_q || !d_out) return pb_set_error(PB_EINVAL, "%s: null argument", who);
+  if (out_dtype != PB_DT_F16 && out_dtype != PB_DT_BF16)
+    return pb_set_error(PB_ENOTSUP, "%s: out_dtype %d (fp16 or bf16)", who, out_dtype);
+  if (n_heads <= 0 || n_heads % c->n_kv || n_heads / c->n_kv > 16)
+    return pb_set_error(PB_ENOTSUP, "%s: %d query heads over %d K/V heads (a whole number, at most 16)", who, n_heads, c->n_kv);
+  if (rows < 0 || window < 0 || sinks < 0 || !(scale > 0.0f) || scale > 1e30f)
+    return pb_set_error(PB_EINVAL, "%s: %d rows, window %d, %d sinks, scale %g", who, rows, window, sinks, (double)scale);
+  const long long wide = (long long)n_heads * c->head_dim;
+  if (ldq < wide || ldo < wide || ((reinterpret_cast<size_t>(d_q) | reinterpret_cast<size_t>(d_out)) & 15) || ((ldq | ldo) & 7))
+    return pb_set_error(PB_EINVAL, "%s: q and out rows must be 16-byte aligned (row strides %lld, %lld)", who, ldq, ldo);
+  if (rows > 0 && kv_overlap(d_q, ((size_t)(rows - 1) * ldq + wide) * 2, d_out, ((size_t)(rows - 1) * ldo + wide) * 2))
+    return pb_set_error(PB_EINVAL, "%s: out overlaps q", who);
+  if (*max_len <= 0 || *max_len > table_ld * c->page_size) *max_len = table_ld * c->page_size;
+  a->p = p;
+  a->len = d_len;
+  a->q = static_cast<const char*>(d_q);
+  a->out = static_cast<char*>(const_cast<void*>(d_out));
+  a->ldq = ldq * 2;
+  a->ldo = ldo * 2;
+  a->n_rows = rows;
+  a->nh = n_heads;
+  a->grp = n_heads / c->n_kv;
+  a->max_len = *max_len;
+  a->window = window;
+  a->sinks = window > 0 ? sinks : 0;
+  a->scale2 = scale * 1.4426950408889634f;
+  return PB_OK;
+}
+
+// dynamic shared memory above 48 KB is allowed once per device and kernel
+template <typename K>
+inline int kv_smem(K k, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  PB_TRY_CUDA(cudaGetDevice(&dev));
+  if (dev < 64 && (done.load(std::memory_order_acquire) >> dev) & 1) return PB_OK;
+  PB_TRY_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+  return PB_OK;
+}
+
+template <typename... KArgs, typename... Args>
+inline int kv_launch(void (*k)(KArgs...), unsigned grid, int block, int smem, cudaStream_t st, bool pdl, const char* name, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, k, args...);
+  if (e != cudaSuccess) return pb_set_error(PB_ECUDA, "%s: %s", name, cudaGetErrorString(e));
+  pb_count_launch();
+  return PB_OK;
+}
+
+}  // namespace

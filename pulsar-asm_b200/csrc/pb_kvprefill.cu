@@ -1,0 +1,567 @@
+// pb_kvprefill.cu -- attention of the last rows of each sequence over the
+// paged K/V cache (prompt chunks; causal, window and sinks) on the tensor
+// cores: tcgen05.mma kind::f16 with the scores, the probabilities and the
+// output in TMEM.
+//
+// 4 D n_heads flops per visible pair of rows bound it, together with one
+// exponential per pair and head (16 per clock and SM: as long as the matrix
+// products at D = 128, twice as long at D = 64). So both have to run at once:
+//  - a CTA takes up to 256 rows of one K/V head, in two groups of 128: a row
+//    is a token and one of the heads of the group, so that short chunks fill
+//    the tiles and a K/V tile serves all heads at once. Key tiles are 64 rows.
+//  - per group, the scores S = Q K^T of a tile go to one of two TMEM buffers;
+//    128 threads (a row each) turn them into probabilities, in place, while
+//    the tensor cores work on the other group and on the next tile's scores;
+//    O += P V takes P from TMEM and accumulates in TMEM.
+//  - the running maximum only moves when a row's scores pass it by more than
+//    2^8; the output is rescaled in TMEM then, which is rare. The sum of a row
+//    stays with its thread. Any maximum that is near enough gives the same
+//    quotient.
+// Warps 0 and 1 copy K and V (16-byte asynchronous copies into the 128-byte
+// swizzle the tensor cores read; rows that no query of the CTA sees are
+// filled with zeros), warp 2 issues the matrix products, warps 4-7 and 8-11
+// are the two groups' softmax (a warp reads its quarter of the TMEM lanes).
+// All waits are bounded; a wait that gives up
+// records an error (pb_kv_status), every role leaves its loop, copies and
+// products in flight are waited for, and the TMEM is freed.
+#include "pb_kvattn.cuh"
+
+namespace {
+
+constexpr int PF_KT = 64;                 // key rows per tile
+constexpr int PF_T = 12 * 32;
+constexpr int PF_CW = 2;                  // warps that copy (0 and 1), warp 2 issues the products
+constexpr int PF_MMA = 2;
+constexpr unsigned long long PF_WAIT_NS = 1000000000ull;
+
+template <int D>
+struct PfGeo {
+  static constexpr int Q = 128 * D * 2;           // bytes of a group's queries
+  static constexpr int KV = PF_KT * D * 2;        // bytes of a K (or V) tile
+  static constexpr int NST = D == 128 ? 4 : 8;    // K/V stages
+  static constexpr int LAG = 2;                   // copies of this many later stages are in flight when a stage is handed over
+  static constexpr int SMEM = 2 * Q + NST * 2 * KV + 1024;
+  static constexpr uint32_t O_COL = 256;          // S: group * 128 + buffer * 64; O: 256 + group * D
+};
+
+struct PfArgs {
+  AttnKvArgs a;
+  int tq, ns, out_bf16;     // tokens per group of 128 rows; splits of the key line
+  float* part;              // [split][row][head][D] unnormalised sums (ns > 1)
+  float2* ml;               // [split][row][head] maximum and sum
+};
+
+__device__ int kv_pf_err;
+
+PB_DEV void pf_init(uint64_t* b, unsigned c) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(kv_s32(b)), "r"(c) : "memory");
+}
+PB_DEV void pf_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(kv_s32(b)) : "memory");
+}
+PB_DEV bool pf_try(uint64_t* b, unsigned par) {
+  uint32_t ok;
+  asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok) : "r"(kv_s32(b)), "r"(par) : "memory");
+  return ok != 0;
+}
+PB_DEV unsigned long long pf_now() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+// bounded wait; false when it gave up or another role did
+PB_DEV bool pf_wait_slow(uint64_t* b, unsigned par, volatile int* stop) {
+  const unsigned long long t0 = pf_now();
+  for (unsigned i = 0;; i++) {
+    if (pf_try(b, par)) return true;
+    if ((i & 63) == 63 && (*stop || pf_now() - t0 > PF_WAIT_NS)) return false;
+  }
+}
+PB_DEV bool pf_wait(uint64_t* b, unsigned par, volatile int* stop) {
+  return pf_try(b, par) || pf_wait_slow(b, par, stop);
+}
+// the same whatever the other roles did: products in flight before the exit
+PB_DEV void pf_drain(uint64_t* b, unsigned par) {
+  const unsigned long long t0 = pf_now();
+  for (unsigned i = 0; !pf_try(b, par); i++)
+    if ((i & 63) == 63 && pf_now() - t0 > PF_WAIT_NS) return;
+}
+PB_DEV void pf_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+PB_DEV void pf_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+PB_DEV void pf_commit(uint64_t* b) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(kv_s32(b)) : "memory");
+}
+// shared-memory descriptors, 128-byte swizzle (layout 2), version 1. K-major
+// (Q, K): 8-row groups 1024 bytes apart. Row-major V as the N-major operand:
+// 64-column panels `lbo` bytes apart, 8-key groups 1024 bytes apart.
+PB_DEV uint64_t pf_desc(uint32_t at, uint32_t lbo) {
+  return (uint64_t)((at >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+PB_DEV void pf_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc) : "memory");
+}
+PB_DEV void pf_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc) : "memory");
+}
+#define PF_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+#define PF_W8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+// 32 consecutive columns of this thread's TMEM lane
+PB_DEV void pf_ld32(uint32_t at, unsigned* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+               "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+               : PF_R8(v, 0), PF_R8(v, 8), PF_R8(v, 16), PF_R8(v, 24) : "r"(at));
+}
+PB_DEV void pf_st32(uint32_t at, const unsigned* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+               "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+               ::PF_W8(v, 0), PF_W8(v, 8), PF_W8(v, 16), PF_W8(v, 24), "r"(at) : "memory");
+}
+PB_DEV void pf_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+PB_DEV void pf_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// rows of q of sequence b: the first, and how many
+PB_DEV int pf_count(const AttnKvArgs& a, int b, int& s0) {
+  s0 = min(max(__ldg(a.start + b), 0), a.n_rows);
+  return max(0, min(__ldg(a.start + b + 1), a.n_rows) - s0);
+}
+
+// the key tiles of one CTA: those of the sinks, then from the first query's
+// window on (all of them where the two meet), to the last query's row
+struct PfLine {
+  int lo, sinks, end, nst, lot, nt;
+};
+PB_DEV PfLine pf_line(const AttnKvArgs& a, int t_first, int t_last) {
+  PfLine s;
+  s.end = max(0, t_last + 1);
+  s.lo = a.window > 0 ? min(max(0, t_first + 1 - a.window), s.end) : 0;
+  s.sinks = min(a.sinks, s.lo);
+  s.nst = (s.sinks + PF_KT - 1) / PF_KT;
+  s.lot = s.lo / PF_KT;
+  if (s.nst >= s.lot) s.nst = s.lot = 0;
+  s.nt = s.nst + (s.end + PF_KT - 1) / PF_KT - s.lot;
+  return s;
+}
+PB_DEV int pf_key(const PfLine& s, int i) { return (i < s.nst ? i : i - s.nst + s.lot) * PF_KT; }
+
+template <int D>
+PB_DEV void pf_put(const PfArgs& p, int row, int h, int e, const float (&x)[8]) {
+  char* o = p.a.out + (long long)row * p.a.ldo + (size_t)h * (D * 2) + e * 2;
+  uint4 w;
+  if (p.out_bf16)
+    w = make_uint4(kv_down<PB_DT_BF16>(x[0], x[1]), kv_down<PB_DT_BF16>(x[2], x[3]), kv_down<PB_DT_BF16>(x[4], x[5]),
+                   kv_down<PB_DT_BF16>(x[6], x[7]));
+  else
+    w = make_uint4(kv_down<PB_DT_F16>(x[0], x[1]), kv_down<PB_DT_F16>(x[2], x[3]), kv_down<PB_DT_F16>(x[4], x[5]),
+                   kv_down<PB_DT_F16>(x[6], x[7]));
+  *reinterpret_cast<uint4*>(o) = w;
+}
+
+template <int D, int CT>
+__global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
+  typedef PfGeo<D> G;
+  constexpr int NST = G::NST, LAG = G::LAG, KP = PF_KT * 128, QP = 128 * 128;   // bytes of a 64-column panel of K or V, of Q
+  extern __shared__ __align__(128) char psm_raw[];
+  __shared__ uint64_t full[NST], empty[NST], sfull[2][2], pready[2][2], pvdone[2], done;
+  __shared__ uint32_t tbase;
+  __shared__ int stop_f;
+  const AttnKvArgs& a = p.a;
+  char* smq = psm_raw + ((1024u - (kv_s32(psm_raw) & 1023u)) & 1023u);
+  char* smk = smq + 2 * G::Q;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pb_grid_launch_dependents();
+
+  // ---- which rows: the last tiles of the line (the longest keys) first
+  const int split = blockIdx.x % p.ns, kh = blockIdx.x / p.ns % a.p.n_kv, idx = blockIdx.x / p.ns / a.p.n_kv;
+  int total, b, first;
+  kv_locate<PF_T>(a.p.n_seq, [&](int i) { int s0; return (pf_count(a, i, s0) + 2 * p.tq - 1) / (2 * p.tq); },
+                  [&](int n) { return idx < n ? n - 1 - idx : n; }, total, b, first);
+  if (idx >= total) return;   // CTA-uniform
+  int row0;
+  const int cnt = pf_count(a, b, row0), tok0 = (total - 1 - idx - first) * 2 * p.tq, ntok = min(2 * p.tq, cnt - tok0);
+  row0 += tok0;
+  const int len = kv_len(__ldg(a.len + b), a.max_len), t0 = len - cnt + tok0;   // cache row of the first token (negative: before the cache)
+  const PfLine line = pf_line(a, t0, t0 + ntok - 1);
+  const int i0 = (int)((long long)line.nt * split / p.ns), n = (int)((long long)line.nt * (split + 1) / p.ns) - i0;
+  const int ng = ntok > p.tq ? 2 : 1;   // groups with rows
+  const int* trow = a.p.table + (size_t)b * a.p.table_ld;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NST; i++) { pf_init(&full[i], 32 * PF_CW); pf_init(&empty[i], 1); }
+    for (int g = 0; g < 2; g++) {
+      for (int i = 0; i < 2; i++) { pf_init(&sfull[g][i], 1); pf_init(&pready[g][i], 128); }
+      pf_init(&pvdone[g], 1);
+    }
+    pf_init(&done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    stop_f = 0;
+  }
+  if (warp == PF_MMA) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(kv_s32(&tbase)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  pf_fence_before();
+  __syncthreads();
+  pf_fence_after();
+  const uint32_t tmem = tbase;
+  volatile int* stop = &stop_f;
+  auto give_up = [&](int role) {
+    *stop = 1;
+    atomicCAS(&kv_pf_err, 0, role);
+  };
+
+  if (warp < PF_CW) {
+    // ------------------------------------------------------------ copies
+    constexpr int CPR = D / 8, RP = 32 * PF_CW / CPR;   // 16-byte chunks per row, rows per pass
+    const int c = threadIdx.x % CPR, r0 = threadIdx.x / CPR;
+    const uint32_t coff = (c >> 3) * KP, qoff = (c >> 3) * QP;
+    if (n > 0) {
+      for (int i = r0; i < ng * 128; i += RP) {
+        const int g = i >> 7, r = i & 127, tk = g * p.tq + r / a.grp;
+        const bool in = r < p.tq * a.grp && tk < ntok;
+        const char* src = a.q + (in ? (long long)(row0 + tk) * a.ldq + (size_t)(kh * a.grp + r % a.grp) * (D * 2) + c * 16 : 0);
+        kv_cp16(kv_s32(smq) + g * G::Q + qoff + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, in);
+      }
+    }
+    int pg[PF_KT / 16];
+    auto pages = [&](int i) {
+      const int k0 = pf_key(line, i0 + i);
+#pragma unroll
+      for (int u = 0; u < PF_KT / 16; u++) pg[u] = k0 + u * 16 < line.end ? __ldg(trow + ((k0 + u * 16) >> a.p.shift)) : -1;
+    };
+    if (n > 0) pages(0);
+    bool ok = true;
+    for (int i = 0; i < n + LAG; i++) {
+      if (i < n) {
+        const int st = i % NST;
+        if (i >= NST && !(ok = pf_wait(&empty[st], (unsigned)(i / NST - 1) & 1u, stop))) break;
+        const int k0 = pf_key(line, i0 + i);
+        const uint32_t ks = kv_s32(smk) + st * (2 * G::KV) + coff;
+#pragma unroll
+        for (int u = 0; u < PF_KT / RP; u++) {
+          const int r = u * RP + r0, j = k0 + r;
+          const int page = pg[(u * RP) / 16];         // a pass lies in one 16-row block
+          const bool in = (unsigned)page < (unsigned)a.p.n_pages && j < line.end && (j >= line.lo || j < line.sinks);
+          const long long off = in ? (long long)page * a.p.ps + (long long)kh * a.p.hs +
+                                         (long long)(j & ((1 << a.p.shift) - 1)) * a.p.rs + c * 16
+                                   : 0;
+          const uint32_t so = r * 128 + (((c & 7) ^ (r & 7)) << 4);
+          kv_cp16(ks + so, a.p.k + off, in);
+          kv_cp16(ks + G::KV + so, a.p.v + off, in);
+        }
+        if (i + 1 < n) pages(i + 1);
+      }
+      kv_cp_commit();
+      if (i >= LAG) {
+        kv_cp_wait<LAG>();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        pf_arrive(&full[(i - LAG) % NST]);
+      }
+    }
+    if (!ok) give_up(1);
+    kv_cp_wait<0>();
+  } else if (warp == PF_MMA) {
+    // ---------------------------------------------------- matrix products
+    // kind::f16: D fp32 (bits 4-5 = 1), A and B fp16 (0) or bf16 (1) at bits 7 and 10, B N-major at bit 16,
+    // N / 8 at bits 17-22, M / 16 at bits 24-28
+    constexpr uint32_t ty = CT == PB_DT_BF16 ? 1u : 0u;
+    constexpr uint32_t base = (1u << 4) | (ty << 7) | (ty << 10) | (8u << 24);
+    constexpr uint32_t id_s = base | ((uint32_t)(PF_KT >> 3) << 17), id_o = base | (1u << 16) | ((uint32_t)(D >> 3) << 17);
+    const uint64_t dq = pf_desc(kv_s32(smq), 16), dk = pf_desc(kv_s32(smk), 16), dv = pf_desc(kv_s32(smk) + G::KV, KP);
+    bool ok = true;
+    for (int i = 0; i <= n && ok; i++) {
+      if (i < n) {   // scores of tile i
+        const int st = i % NST;
+        if (!(ok = __all_sync(0xffffffffu, pf_wait(&full[st], (unsigned)(i / NST) & 1u, stop)))) break;
+        for (int g = 0; g < ng && ok; g++) {
+          // the buffer held P of tile i - 2: its product is done
+          if (i >= 2 && !(ok = __all_sync(0xffffffffu, pf_wait(&pvdone[g], (unsigned)(i - 2) & 1u, stop)))) break;
+          pf_fence_after();
+          if (lane == 0) {
+            const uint64_t qa = dq + (uint64_t)(g * (G::Q >> 4)), kb = dk + (uint64_t)(st * ((2 * G::KV) >> 4));
+#pragma unroll
+            for (int k = 0; k < D / 16; k++)
+              pf_mma_ss(tmem + (uint32_t)(g * 128 + (i & 1) * 64), qa + (uint64_t)(((k >> 2) * QP + (k & 3) * 32) >> 4),
+                        kb + (uint64_t)(((k >> 2) * KP + (k & 3) * 32) >> 4), id_s, k > 0);
+            pf_commit(&sfull[g][i & 1]);
+          }
+          __syncwarp();
+        }
+      }
+      if (i > 0 && ok) {   // output of tile i - 1
+        const int j = i - 1, st = j % NST;
+        for (int g = 0; g < ng && ok; g++) {
+          if (!(ok = __all_sync(0xffffffffu, pf_wait(&pready[g][j & 1], (unsigned)(j >> 1) & 1u, stop)))) break;
+          pf_fence_after();
+          if (lane == 0) {
+            const uint64_t vb = dv + (uint64_t)(st * ((2 * G::KV) >> 4));
+#pragma unroll
+            for (int k = 0; k < PF_KT / 16; k++)
+              pf_mma_ts(tmem + G::O_COL + (uint32_t)(g * D), tmem + (uint32_t)(g * 128 + (j & 1) * 64 + k * 8),
+                        vb + (uint64_t)((k * 2048) >> 4), id_o, j > 0 || k > 0);
+            pf_commit(&pvdone[g]);
+            if (g == ng - 1) pf_commit(&empty[st]);
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (!ok && lane == 0) give_up(2);
+    // every product has completed before the TMEM is freed (bounded)
+    if (lane == 0) pf_commit(&done);
+    __syncwarp();
+    pf_drain(&done, 0);
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ softmax
+    const int g = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t to = tl + G::O_COL + (uint32_t)(g * D);
+    const int tk = g * p.tq + r / a.grp;                       // token within the CTA
+    const bool live = r < p.tq * a.grp && tk < ntok;
+    const int t = t0 + min(tk, ntok - 1);                      // the row's own cache row
+    const int wlo = a.window > 0 ? t + 1 - a.window : 0;       // it sees [wlo, t] and [0, sinks)
+    // of the group: what all rows see, for tiles that need no masks
+    const int ta = t0 + min(g * p.tq, ntok - 1), tb = t0 + min((g + 1) * p.tq - 1, ntok - 1);
+    const int whi = a.window > 0 ? tb + 1 - a.window : 0;
+    float m = -INFINITY, ms = 0.0f, l = 0.0f;                  // maximum of the raw scores, the same scaled, sum
+    bool ok = g < ng;
+    for (int i = 0; i < n && ok; i++) {
+      const int k0 = pf_key(line, i0 + i);
+      int pg[PF_KT / 16];
+#pragma unroll
+      for (int u = 0; u < PF_KT / 16; u++) pg[u] = k0 + u * 16 < line.end ? __ldg(trow + ((k0 + u * 16) >> a.p.shift)) : -1;
+      const uint32_t ts = tl + (uint32_t)(g * 128 + (i & 1) * 64);
+      if (!(ok = __all_sync(0xffffffffu, pf_wait(&sfull[g][i & 1], (unsigned)(i >> 1) & 1u, stop)))) break;
+      pf_fence_after();
+      unsigned s[PF_KT];
+      pf_ld32(ts, s);
+      pf_ld32(ts + 32, s + 32);
+      unsigned bad = 0;
+#pragma unroll
+      for (int u = 0; u < PF_KT / 16; u++) bad |= (unsigned)pg[u] < (unsigned)a.p.n_pages ? 0u : 1u << u;
+      pf_wait_ld();
+      if (bad || k0 + PF_KT - 1 > ta || (k0 < whi && k0 + PF_KT > a.sinks)) {
+#pragma unroll
+        for (int k = 0; k < PF_KT; k++) {
+          const int j = k0 + k;
+          const bool in = !((bad >> (k >> 4)) & 1u) && j <= t && (j >= wlo || j < a.sinks);
+          s[k] = in ? s[k] : 0xff800000u;
+        }
+      }
+      float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int k = 0; k < PF_KT; k += 4)
+#pragma unroll
+        for (int u = 0; u < 4; u++) x[u] = fmaxf(x[u], __uint_as_float(s[k + u]));
+      const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+      // the reference maximum: the first one, and a new one when a score passes it by 2^8
+      const bool move = mx > m && (m == -INFINITY || (mx - m) * a.scale2 > 8.0f);
+      if (__any_sync(0xffffffffu, move)) {
+        const float f = !move ? 1.0f : (m == -INFINITY ? 0.0f : kv_ex2((m - mx) * a.scale2));
+        if (move) { m = mx; ms = mx * a.scale2; }
+        l *= f;
+        if (i > 0) {   // the output so far, which the product of tile i - 1 has completed
+          if (!(ok = __all_sync(0xffffffffu, pf_wait(&pvdone[g], (unsigned)(i - 1) & 1u, stop)))) break;
+          pf_fence_after();
+#pragma unroll
+          for (int e = 0; e < D; e += 32) {
+            unsigned o[32];
+            pf_ld32(to + e, o);
+            pf_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            pf_st32(to + e, o);
+          }
+        }
+      }
+      float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      unsigned w[32];
+#pragma unroll
+      for (int k = 0; k < PF_KT; k += 2) {
+        const float u = kv_ex2(__fmaf_rn(__uint_as_float(s[k]), a.scale2, -ms));
+        const float v = kv_ex2(__fmaf_rn(__uint_as_float(s[k + 1]), a.scale2, -ms));
+        y[k & 2] += u;
+        y[(k & 2) + 1] += v;
+        // rounded to the cache's type, which the product with V needs; the sum takes the unrounded ones
+        w[k / 2] = kv_down<CT>(u, v);
+      }
+      l += (y[0] + y[1]) + (y[2] + y[3]);
+      pf_st32(ts, w);
+      pf_wait_st();
+      pf_fence_before();
+      pf_arrive(&pready[g][i & 1]);
+    }
+    if (g < ng && !ok && lane == 0) give_up(3);
+    if (ok && n > 0) {
+      // tile by tile: the wait for a phase's parity needs the phase before it to be over
+      ok = (n < 2 || __all_sync(0xffffffffu, pf_wait(&pvdone[g], (unsigned)(n - 2) & 1u, stop))) &&
+           __all_sync(0xffffffffu, pf_wait(&pvdone[g], (unsigned)(n - 1) & 1u, stop));
+      if (!ok && lane == 0) give_up(4);
+    }
+    if (g < ng && ok) {
+      pf_fence_after();
+      const int row = row0 + tk, h = kh * a.grp + r % a.grp;
+      const float f = l != 0.0f ? 1.0f / l : 0.0f;       // nothing seen: zeros
+      const size_t at = ((size_t)split * a.n_rows + row) * a.nh + h;
+#pragma unroll
+      for (int e = 0; e < D; e += 32) {
+        unsigned o[32];
+        if (n > 0) {
+          pf_ld32(to + e, o);
+          pf_wait_ld();
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; k++) o[k] = 0u;
+        }
+        if (live) {
+          if (p.ns == 1) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+              float v[8];
+#pragma unroll
+              for (int u = 0; u < 8; u++) v[u] = __uint_as_float(o[k + u]) * f;
+              pf_put<D>(p, row, h, e + k, v);
+            }
+          } else if (n > 0) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<uint4*>(p.part + at * D + e + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+          }
+        }
+      }
+      if (live && p.ns > 1) p.ml[at] = make_float2(n > 0 ? ms : -INFINITY, n > 0 ? l : 0.0f);
+    }
+    pf_fence_before();
+  }
+  __syncthreads();
+  if (warp == PF_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// the splits of each row and head joined, D / 4 lanes' worth of a warp per
+// head. A row belongs to a sequence or it is left alone.
+template <int D>
+__global__ void __launch_bounds__(128) k_kv_prefill_join(PfArgs p) {
+  const AttnKvArgs& a = p.a;
+  constexpr int L = D / 4;      // lanes per head
+  const int unit = (blockIdx.x * 128 + threadIdx.x) / L, e = (threadIdx.x % L) * 4;
+  const int row = unit / a.nh, h = unit % a.nh;
+  bool mine = row < a.n_rows;
+  if (mine) {
+    // the sequences are in ascending order: the last that starts at or before the row, if it reaches it
+    int lo = 0, hi = a.p.n_seq;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(a.start + mid) <= row) lo = mid;
+      else hi = mid;
+    }
+    int s0;
+    const int c = pf_count(a, lo, s0);
+    mine = row >= s0 && row < s0 + c;
+  }
+  pb_grid_wait();
+  if (!mine) return;
+  float m = -INFINITY;
+  for (int s = 0; s < p.ns; s++) {
+    const float2 q = __ldcg(p.ml + ((size_t)s * a.n_rows + row) * a.nh + h);
+    if (q.y != 0.0f) m = fmaxf(m, q.x);
+  }
+  float l = 0.0f;
+  float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s = 0; s < p.ns; s++) {
+    const size_t at = ((size_t)s * a.n_rows + row) * a.nh + h;
+    const float2 q = __ldcg(p.ml + at);
+    if (q.y == 0.0f) continue;      // an empty split wrote no sums
+    const float f = kv_ex2(q.x - m);
+    const float4 z = __ldcg(reinterpret_cast<const float4*>(p.part + at * D + e));
+    l += f * q.y;
+    y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
+  }
+  const float f = l != 0.0f ? 1.0f / l : 0.0f;
+  char* o = a.out + (long long)row * a.ldo + (size_t)h * (D * 2) + e * 2;
+  uint2 w;
+  if (p.out_bf16) w = make_uint2(kv_down<PB_DT_BF16>(y.x * f, y.y * f), kv_down<PB_DT_BF16>(y.z * f, y.w * f));
+  else w = make_uint2(kv_down<PB_DT_F16>(y.x * f, y.y * f), kv_down<PB_DT_F16>(y.z * f, y.w * f));
+  *reinterpret_cast<uint2*>(o) = w;
+}
+
+// launch shape: CTAs of 2 * tq tokens, and splits of the key line where those
+// leave SMs idle (at least 4 tiles each)
+struct PfPlan {
+  int tq, ns;
+  long long items, part, ml;   // CTAs per split; floats
+};
+PfPlan pf_plan(const pb_kv_pages* c, int n_seq, int max_len, int n_tok, int n_heads) {
+  PfPlan p{};
+  const int grp = n_heads / c->n_kv;
+  p.tq = 128 / (grp > 0 ? grp : 1);
+  p.items = ((long long)n_tok / (2 * p.tq) + (n_seq < n_tok ? n_seq : n_tok)) * c->n_kv;
+  const long long tiles = (max_len + PF_KT - 1) / PF_KT;
+  long long ns = p.items > 0 ? pb_num_sms() / p.items : 1;
+  if (ns > tiles / 4) ns = tiles / 4;
+  p.ns = ns < 1 ? 1 : (int)ns;
+  const long long rows = (long long)p.ns * n_tok * n_heads;
+  p.part = p.ns > 1 ? rows * c->head_dim : 0;
+  p.ml = p.ns > 1 ? rows * 2 : 0;
+  return p;
+}
+
+template <int D, int CT>
+int pf_run(const PfArgs& p, long long items, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  if (int rc = kv_smem(k_kv_prefill<D, CT>, PfGeo<D>::SMEM, done)) return rc;
+  if (int rc = kv_launch(k_kv_prefill<D, CT>, (unsigned)(items * p.ns), PF_T, PfGeo<D>::SMEM, st, false, "k_kv_prefill", p)) return rc;
+  if (p.ns == 1) return PB_OK;
+  const long long blocks = ((long long)p.a.n_rows * p.a.nh * (D / 4) + 127) / 128;
+  return kv_launch(k_kv_prefill_join<D>, (unsigned)blocks, 128, 0, st, true, "k_kv_prefill_join", p);
+}
+
+}  // namespace
+
+extern "C" long long pb_kv_prefill_scratch(const pb_kv_pages* c, int n_seq, int max_len, int n_tok, int n_heads) {
+  if (!c || n_seq < 0 || max_len < 0 || n_tok < 0 || n_heads <= 0 || c->n_kv <= 0 || n_heads / c->n_kv > 16) return -1;
+  const PfPlan p = pf_plan(c, n_seq, max_len, n_tok, n_heads);
+  return 4 * (p.part + p.ml);
+}
+
+extern "C" int pb_kv_prefill(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const int* d_start,
+                             const int* d_len, int max_len, int n_tok, int n_heads, const void* d_q, long long ldq, float scale,
+                             int window, int sinks, void* d_out, int out_dtype, long long ldo, void* d_scratch,
+                             long long scratch_bytes, void* stream) {
+  KvPool pool{};
+  PfArgs p{};
+  if (int rc = kv_pool("pb_kv_prefill", c, n_seq, d_table, table_ld, &pool)) return rc;
+  if (!d_start) return pb_set_error(PB_EINVAL, "pb_kv_prefill: null argument");
+  if (int rc = attn_check("pb_kv_prefill", c, pool, d_len, &max_len, table_ld, n_tok, n_heads, d_q, ldq, scale, window, sinks,
+                          d_out, out_dtype, ldo, &p.a))
+    return rc;
+  if (n_seq == 0 || n_tok == 0) return PB_OK;
+  const PfPlan pl = pf_plan(c, n_seq, max_len, n_tok, n_heads);
+  if (pl.items * pl.ns > INT_MAX || (long long)n_tok * n_heads * 32 > INT_MAX)
+    return pb_set_error(PB_EINVAL, "pb_kv_prefill: %d tokens of %d heads", n_tok, n_heads);
+  const long long need = 4 * (pl.part + pl.ml);
+  if (need > 0 && (!d_scratch || scratch_bytes < need || (reinterpret_cast<size_t>(d_scratch) & 15)))
+    return pb_set_error(PB_EINVAL, "pb_kv_prefill: scratch of %lld bytes, %lld needed (16-byte aligned)", scratch_bytes, need);
+  p.a.start = d_start;
+  p.tq = pl.tq;
+  p.ns = pl.ns;
+  p.out_bf16 = out_dtype == PB_DT_BF16;
+  p.part = static_cast<float*>(d_scratch);
+  p.ml = reinterpret_cast<float2*>(p.part + pl.part);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (c->head_dim == 64) return c->dtype == PB_DT_F16 ? pf_run<64, PB_DT_F16>(p, pl.items, st) : pf_run<64, PB_DT_BF16>(p, pl.items, st);
+  return c->dtype == PB_DT_F16 ? pf_run<128, PB_DT_F16>(p, pl.items, st) : pf_run<128, PB_DT_BF16>(p, pl.items, st);
+}
+
+extern "C" int pb_kv_status(void* stream) {
+  PB_TRY_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+  int e = 0;
+  const int zero = 0;
+  PB_TRY_CUDA(cudaMemcpyFromSymbol(&e, kv_pf_err, sizeof e));
+  if (e) PB_TRY_CUDA(cudaMemcpyToSymbol(kv_pf_err, &zero, sizeof zero));
+  return e ? pb_set_error(PB_ECUDA, "k_kv_prefill: a bounded wait gave up (role %d)", e) : PB_OK;
+}

@@ -99,6 +99,7 @@ def lib():
     L.pb_kv_decode_scratch.argtypes = [kvp, i, i, i, i]
     L.pb_kv_prefill_scratch.argtypes = [kvp, i, i, i, i]
     L.pb_kv_evict_scratch.argtypes = [kvp, i, i, i]
+    L.pb_kv_status.argtypes = [vp]
     for fn in (L.pb_kv_decode_scratch, L.pb_kv_prefill_scratch, L.pb_kv_evict_scratch):
         fn.restype = ll
     L.pb_q1_gemv.argtypes = [vp, vp, vp, vp, vp]
@@ -485,6 +486,12 @@ class KVPages:
                                [q.shape[0]], q, out, max_len, scale, window, sinks, [])
         need = L.pb_kv_prefill_scratch(self._r, n, max_len or table.shape[1] * self.page_size, q.shape[0], q.shape[1])
         self._call(L.pb_kv_prefill, args, need, scratch, stream)
+
+    def status(self, stream=None):
+        """synchronise and raise if a prefill kernel recorded a wait that gave up"""
+        import torch
+        with torch.cuda.device(self.device):
+            check(lib().pb_kv_status(_stream(stream)))
 
     def _attn_args(self, table, n_seq, lens, rows, q, out, max_len, scale, window, sinks, more):
         qp, op = self._heads("q", q, self.dtype), self._heads("out", out)

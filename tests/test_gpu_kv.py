@@ -354,6 +354,7 @@ def test_prefill(pb, cuda, nh, nkv, D, ps, dt, ot, layout, window, sinks, seqs):
     scale = 1.3 * D ** -0.5
     c.h.prefill(c.dev(), start, length, q, out[:, :nh], scale=scale, window=window, sinks=sinks)
     torch.cuda.synchronize()
+    c.h.status()
     (o, spread, slack, tiny), _ = oracle_rows(c, q[pad:pad + rows], lens, counts, scale, window, sinks)
     check(torch, f64(out)[pad:pad + rows, :nh], o, spread, slack, tiny, max(lens), dt, ot, "out")
     assert (out[:pad] == 9.0).all() and (out[pad + rows:] == 9.0).all() and (out[:, nh:] == 9.0).all()
