@@ -38,8 +38,8 @@ template <int D>
 struct PfGeo {
   static constexpr int Q = 128 * D * 2;           // bytes of a group's queries
   static constexpr int KV = PF_KT * D * 2;        // bytes of a K (or V) tile
-  static constexpr int NST = D == 128 ? 4 : 8;    // K/V stages
-  static constexpr int LAG = 2;                   // copies of this many later stages are in flight when a stage is handed over
+  static constexpr int NST = D == 128 ? 5 : 8;    // K/V stages
+  static constexpr int LAG = 2;                   // stages in flight
   static constexpr int SMEM = 2 * Q + NST * 2 * KV + 1024;
   static constexpr uint32_t O_COL = 256;          // S: group * 128 + buffer * 64; O: 256 + group * D
 };
@@ -91,6 +91,11 @@ PB_DEV void pf_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;
 PB_DEV void pf_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 PB_DEV void pf_commit(uint64_t* b) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(kv_s32(b)) : "memory");
+}
+PB_DEV bool pf_elect() {
+  uint32_t one;
+  asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(one));
+  return one != 0;
 }
 // shared-memory descriptors, 128-byte swizzle (layout 2), version 1. K-major
 // (Q, K): 8-row groups 1024 bytes apart. Row-major V as the N-major operand:
@@ -228,6 +233,15 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
         kv_cp16(kv_s32(smq) + g * G::Q + qoff + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, in);
       }
     }
+    // Per thread, chunk c of rows r0, r0 + RP, ...: the shared-memory offsets
+    // repeat every 8 rows (the swizzle), the row addresses step by RP rows
+    // within a 16-row block, which lies in one page.
+    constexpr int PB = 16 / RP, SV = RP < 8 ? 8 / RP : 1;   // passes per block, swizzle variants
+    uint32_t so[SV];
+#pragma unroll
+    for (int u = 0; u < SV; u++) so[u] = coff + r0 * 128 + (((c & 7) ^ ((u * RP + r0) & 7)) << 4);
+    const long long step = (long long)RP * a.p.rs, lane_off = (long long)kh * a.p.hs + (long long)r0 * a.p.rs + c * 16;
+    const long long v_k = a.p.v - a.p.k;
     int pg[PF_KT / 16];
     auto pages = [&](int i) {
       const int k0 = pf_key(line, i0 + i);
@@ -237,31 +251,36 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
     if (n > 0) pages(0);
     bool ok = true;
     for (int i = 0; i < n + LAG; i++) {
+      if (i >= LAG) {    // hand over the stage that has landed, before waiting for room for the next
+        kv_cp_wait<LAG - 1>();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        pf_arrive(&full[(i - LAG) % NST]);
+      }
       if (i < n) {
         const int st = i % NST;
         if (i >= NST && !(ok = pf_wait(&empty[st], (unsigned)(i / NST - 1) & 1u, stop))) break;
         const int k0 = pf_key(line, i0 + i);
-        const uint32_t ks = kv_s32(smk) + st * (2 * G::KV) + coff;
+        const uint32_t ks = kv_s32(smk) + st * (2 * G::KV);
+        const bool edge = k0 + PF_KT > line.end || (k0 < line.lo && k0 + PF_KT > line.sinks);   // rows that no query sees
 #pragma unroll
-        for (int u = 0; u < PF_KT / RP; u++) {
-          const int r = u * RP + r0, j = k0 + r;
-          const int page = pg[(u * RP) / 16];         // a pass lies in one 16-row block
-          const bool in = (unsigned)page < (unsigned)a.p.n_pages && j < line.end && (j >= line.lo || j < line.sinks);
-          const long long off = in ? (long long)page * a.p.ps + (long long)kh * a.p.hs +
-                                         (long long)(j & ((1 << a.p.shift) - 1)) * a.p.rs + c * 16
-                                   : 0;
-          const uint32_t so = r * 128 + (((c & 7) ^ (r & 7)) << 4);
-          kv_cp16(ks + so, a.p.k + off, in);
-          kv_cp16(ks + G::KV + so, a.p.v + off, in);
+        for (int blk = 0; blk < PF_KT / 16; blk++) {
+          const int j0 = k0 + blk * 16;
+          const bool page = (unsigned)pg[blk] < (unsigned)a.p.n_pages;
+          const char* src = a.p.k + (page ? (long long)pg[blk] * a.p.ps + (long long)(j0 & ((1 << a.p.shift) - 1)) * a.p.rs + lane_off : 0);
+          const long long by = page ? step : 0;
+#pragma unroll
+          for (int q = 0; q < PB; q++) {
+            const int u = blk * PB + q, j = j0 + q * RP + r0;
+            const uint32_t dst = ks + so[u % SV] + u * (RP * 128);
+            const bool in = page && (!edge || (j < line.end && (j >= line.lo || j < line.sinks)));
+            kv_cp16(dst, src, in);
+            kv_cp16(dst + G::KV, src + v_k, in);
+            src += by;
+          }
         }
         if (i + 1 < n) pages(i + 1);
       }
       kv_cp_commit();
-      if (i >= LAG) {
-        kv_cp_wait<LAG>();
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        pf_arrive(&full[(i - LAG) % NST]);
-      }
     }
     if (!ok) give_up(1);
     kv_cp_wait<0>();
@@ -273,20 +292,28 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
     constexpr uint32_t base = (1u << 4) | (ty << 7) | (ty << 10) | (8u << 24);
     constexpr uint32_t id_s = base | ((uint32_t)(PF_KT >> 3) << 17), id_o = base | (1u << 16) | ((uint32_t)(D >> 3) << 17);
     const uint64_t dq = pf_desc(kv_s32(smq), 16), dk = pf_desc(kv_s32(smk), 16), dv = pf_desc(kv_s32(smk) + G::KV, KP);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    // One elected thread issues. Descriptors and TMEM columns are warp-uniform
+    // values plus constants (both groups written out): computed per product by
+    // a divergent thread, they cost some 100 cycles each, twice the product.
     bool ok = true;
+    int st = 0, sp = 0;            // stages of tiles i and i - 1
+    unsigned fpar = 0;             // parity of full[st]
     for (int i = 0; i <= n && ok; i++) {
+      const uint32_t sb = (uint32_t)(i & 1) * 64;
       if (i < n) {   // scores of tile i
-        const int st = i % NST;
-        if (!(ok = __all_sync(0xffffffffu, pf_wait(&full[st], (unsigned)(i / NST) & 1u, stop)))) break;
-        for (int g = 0; g < ng && ok; g++) {
+        if (!(ok = __all_sync(0xffffffffu, pf_wait(&full[st], fpar, stop)))) break;
+        const uint64_t kb = dk + (uint64_t)(st * ((2 * G::KV) >> 4));
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+          if (g >= ng) break;
           // the buffer held P of tile i - 2: its product is done
-          if (i >= 2 && !(ok = __all_sync(0xffffffffu, pf_wait(&pvdone[g], (unsigned)(i - 2) & 1u, stop)))) break;
+          if (i >= 2 && !(ok = __all_sync(0xffffffffu, pf_wait(&pvdone[g], (unsigned)i & 1u, stop)))) break;
           pf_fence_after();
-          if (lane == 0) {
-            const uint64_t qa = dq + (uint64_t)(g * (G::Q >> 4)), kb = dk + (uint64_t)(st * ((2 * G::KV) >> 4));
+          if (pf_elect()) {
 #pragma unroll
             for (int k = 0; k < D / 16; k++)
-              pf_mma_ss(tmem + (uint32_t)(g * 128 + (i & 1) * 64), qa + (uint64_t)(((k >> 2) * QP + (k & 3) * 32) >> 4),
+              pf_mma_ss(tm + sb + g * 128, dq + (uint64_t)((g * G::Q + (k >> 2) * QP + (k & 3) * 32) >> 4),
                         kb + (uint64_t)(((k >> 2) * KP + (k & 3) * 32) >> 4), id_s, k > 0);
             pf_commit(&sfull[g][i & 1]);
           }
@@ -294,26 +321,29 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
         }
       }
       if (i > 0 && ok) {   // output of tile i - 1
-        const int j = i - 1, st = j % NST;
-        for (int g = 0; g < ng && ok; g++) {
-          if (!(ok = __all_sync(0xffffffffu, pf_wait(&pready[g][j & 1], (unsigned)(j >> 1) & 1u, stop)))) break;
+        const uint64_t vb = dv + (uint64_t)(sp * ((2 * G::KV) >> 4));
+        const uint32_t pb = 64 - sb;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+          if (g >= ng) break;
+          if (!(ok = __all_sync(0xffffffffu, pf_wait(&pready[g][(i - 1) & 1], (unsigned)((i - 1) >> 1) & 1u, stop)))) break;
           pf_fence_after();
-          if (lane == 0) {
-            const uint64_t vb = dv + (uint64_t)(st * ((2 * G::KV) >> 4));
+          if (pf_elect()) {
 #pragma unroll
             for (int k = 0; k < PF_KT / 16; k++)
-              pf_mma_ts(tmem + G::O_COL + (uint32_t)(g * D), tmem + (uint32_t)(g * 128 + (j & 1) * 64 + k * 8),
-                        vb + (uint64_t)((k * 2048) >> 4), id_o, j > 0 || k > 0);
+              pf_mma_ts(tm + G::O_COL + g * D, tm + pb + g * 128 + k * 8, vb + (uint64_t)((k * 2048) >> 4), id_o, i > 1 || k > 0);
             pf_commit(&pvdone[g]);
-            if (g == ng - 1) pf_commit(&empty[st]);
+            if (g == ng - 1) pf_commit(&empty[sp]);
           }
           __syncwarp();
         }
       }
+      sp = st;
+      if (++st == NST) { st = 0; fpar ^= 1; }
     }
     if (!ok && lane == 0) give_up(2);
     // every product has completed before the TMEM is freed (bounded)
-    if (lane == 0) pf_commit(&done);
+    if (pf_elect()) pf_commit(&done);
     __syncwarp();
     pf_drain(&done, 0);
   } else if (warp >= 4) {
