@@ -130,6 +130,33 @@ PB_DEV void pf_st32(uint32_t at, const unsigned* v) {
 PB_DEV void pf_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 PB_DEV void pf_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// packed pairs of fp32, each operation rounded on its own
+typedef unsigned long long pf_f2;
+PB_DEV pf_f2 pf_pk(float a, float b) {
+  pf_f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+PB_DEV void pf_upk(pf_f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+PB_DEV pf_f2 pf_fma2(pf_f2 a, pf_f2 b, pf_f2 c) {
+  pf_f2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+PB_DEV pf_f2 pf_add2(pf_f2 a, pf_f2 b) {
+  pf_f2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+PB_DEV float pf_max3(float a, float b, float c) {   // NaN if any is
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+PB_DEV void pf_cp16(uint32_t dst, const char* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // rows of q of sequence b: the first, and how many
 PB_DEV int pf_count(const AttnKvArgs& a, int b, int& s0) {
   s0 = min(max(__ldg(a.start + b), 0), a.n_rows);
@@ -152,6 +179,8 @@ PB_DEV PfLine pf_line(const AttnKvArgs& a, int t_first, int t_last) {
   s.nt = s.nst + (s.end + PF_KT - 1) / PF_KT - s.lot;
   return s;
 }
+// bits 0 .. x - 1
+PB_DEV unsigned long long pf_below(int x) { return x <= 0 ? 0ull : (x >= 64 ? ~0ull : (1ull << x) - 1ull); }
 PB_DEV int pf_key(const PfLine& s, int i) { return (i < s.nst ? i : i - s.nst + s.lot) * PF_KT; }
 
 template <int D>
@@ -241,7 +270,6 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
 #pragma unroll
     for (int u = 0; u < SV; u++) so[u] = coff + r0 * 128 + (((c & 7) ^ ((u * RP + r0) & 7)) << 4);
     const long long step = (long long)RP * a.p.rs, lane_off = (long long)kh * a.p.hs + (long long)r0 * a.p.rs + c * 16;
-    const long long v_k = a.p.v - a.p.k;
     int pg[PF_KT / 16];
     auto pages = [&](int i) {
       const int k0 = pf_key(line, i0 + i);
@@ -266,16 +294,27 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
         for (int blk = 0; blk < PF_KT / 16; blk++) {
           const int j0 = k0 + blk * 16;
           const bool page = (unsigned)pg[blk] < (unsigned)a.p.n_pages;
-          const char* src = a.p.k + (page ? (long long)pg[blk] * a.p.ps + (long long)(j0 & ((1 << a.p.shift) - 1)) * a.p.rs + lane_off : 0);
-          const long long by = page ? step : 0;
+          const long long off = (page ? (long long)pg[blk] * a.p.ps + (long long)(j0 & ((1 << a.p.shift) - 1)) * a.p.rs : 0) + lane_off;
+          const char *kp = a.p.k + off, *vp = a.p.v + off;
+          if (page && !edge) {
 #pragma unroll
-          for (int q = 0; q < PB; q++) {
-            const int u = blk * PB + q, j = j0 + q * RP + r0;
-            const uint32_t dst = ks + so[u % SV] + u * (RP * 128);
-            const bool in = page && (!edge || (j < line.end && (j >= line.lo || j < line.sinks)));
-            kv_cp16(dst, src, in);
-            kv_cp16(dst + G::KV, src + v_k, in);
-            src += by;
+            for (int q = 0; q < PB; q++) {
+              const int u = blk * PB + q;
+              pf_cp16(ks + so[u % SV] + u * (RP * 128), kp);
+              pf_cp16(ks + so[u % SV] + (u * (RP * 128) + G::KV), vp);
+              kp += step;
+              vp += step;
+            }
+          } else {
+#pragma unroll
+            for (int q = 0; q < PB; q++) {
+              const int u = blk * PB + q, j = j0 + q * RP + r0;
+              const bool in = page && j < line.end && (j >= line.lo || j < line.sinks);
+              kv_cp16(ks + so[u % SV] + u * (RP * 128), in ? kp : a.p.k, in);
+              kv_cp16(ks + so[u % SV] + u * (RP * 128) + G::KV, in ? vp : a.p.v, in);
+              kp += step;
+              vp += step;
+            }
           }
         }
         if (i + 1 < n) pages(i + 1);
@@ -292,60 +331,58 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
     constexpr uint32_t base = (1u << 4) | (ty << 7) | (ty << 10) | (8u << 24);
     constexpr uint32_t id_s = base | ((uint32_t)(PF_KT >> 3) << 17), id_o = base | (1u << 16) | ((uint32_t)(D >> 3) << 17);
     const uint64_t dq = pf_desc(kv_s32(smq), 16), dk = pf_desc(kv_s32(smk), 16), dv = pf_desc(kv_s32(smk) + G::KV, KP);
-    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-    // One elected thread issues. Descriptors and TMEM columns are warp-uniform
-    // values plus constants (both groups written out): computed per product by
-    // a divergent thread, they cost some 100 cycles each, twice the product.
-    bool ok = true;
-    int st = 0, sp = 0;            // stages of tiles i and i - 1
-    unsigned fpar = 0;             // parity of full[st]
-    for (int i = 0; i <= n && ok; i++) {
-      const uint32_t sb = (uint32_t)(i & 1) * 64;
-      if (i < n) {   // scores of tile i
-        if (!(ok = __all_sync(0xffffffffu, pf_wait(&full[st], fpar, stop)))) break;
-        const uint64_t kb = dk + (uint64_t)(st * ((2 * G::KV) >> 4));
+    // One elected thread waits and issues: a warp-wide wait, with its vote and
+    // election, costs some 150 cycles of a step that has six; and operands
+    // that ptxas does not see as uniform cost 100 cycles per product instead
+    // of 50 (a product takes 48 to 64).
+    if (pf_elect()) {
+      bool ok = true;
+      int st = 0, sp = 0;            // stages of tiles i and i - 1
+      unsigned fpar = 0;             // parity of full[st]
+      for (int i = 0; i <= n; i++) {
+        const uint32_t sb = (uint32_t)(i & 1) * 64;
+        if (i < n) {   // scores of tile i
+          if (!(ok = pf_wait(&full[st], fpar, stop))) break;
+          const uint64_t kb = dk + (uint64_t)(st * ((2 * G::KV) >> 4));
 #pragma unroll
-        for (int g = 0; g < 2; g++) {
-          if (g >= ng) break;
-          // the buffer held P of tile i - 2: its product is done
-          if (i >= 2 && !(ok = __all_sync(0xffffffffu, pf_wait(&pvdone[g], (unsigned)i & 1u, stop)))) break;
-          pf_fence_after();
-          if (pf_elect()) {
+          for (int g = 0; g < 2; g++) {
+            if (g >= ng) break;
+            // the buffer held P of tile i - 2: its product is done
+            if (i >= 2 && !(ok = pf_wait(&pvdone[g], (unsigned)i & 1u, stop))) break;
+            pf_fence_after();
 #pragma unroll
             for (int k = 0; k < D / 16; k++)
-              pf_mma_ss(tm + sb + g * 128, dq + (uint64_t)((g * G::Q + (k >> 2) * QP + (k & 3) * 32) >> 4),
+              pf_mma_ss(tmem + sb + g * 128, dq + (uint64_t)((g * G::Q + (k >> 2) * QP + (k & 3) * 32) >> 4),
                         kb + (uint64_t)(((k >> 2) * KP + (k & 3) * 32) >> 4), id_s, k > 0);
             pf_commit(&sfull[g][i & 1]);
           }
-          __syncwarp();
+          if (!ok) break;
         }
-      }
-      if (i > 0 && ok) {   // output of tile i - 1
-        const uint64_t vb = dv + (uint64_t)(sp * ((2 * G::KV) >> 4));
-        const uint32_t pb = 64 - sb;
+        if (i > 0) {   // output of tile i - 1
+          const uint64_t vb = dv + (uint64_t)(sp * ((2 * G::KV) >> 4));
+          const uint32_t pb = 64 - sb;
 #pragma unroll
-        for (int g = 0; g < 2; g++) {
-          if (g >= ng) break;
-          if (!(ok = __all_sync(0xffffffffu, pf_wait(&pready[g][(i - 1) & 1], (unsigned)((i - 1) >> 1) & 1u, stop)))) break;
-          pf_fence_after();
-          if (pf_elect()) {
+          for (int g = 0; g < 2; g++) {
+            if (g >= ng) break;
+            if (!(ok = pf_wait(&pready[g][(i - 1) & 1], (unsigned)((i - 1) >> 1) & 1u, stop))) break;
+            pf_fence_after();
 #pragma unroll
             for (int k = 0; k < PF_KT / 16; k++)
-              pf_mma_ts(tm + G::O_COL + g * D, tm + pb + g * 128 + k * 8, vb + (uint64_t)((k * 2048) >> 4), id_o, i > 1 || k > 0);
+              pf_mma_ts(tmem + G::O_COL + g * D, tmem + pb + g * 128 + k * 8, vb + (uint64_t)((k * 2048) >> 4), id_o, i > 1 || k > 0);
             pf_commit(&pvdone[g]);
-            if (g == ng - 1) pf_commit(&empty[sp]);
           }
-          __syncwarp();
+          if (!ok) break;
+          pf_commit(&empty[sp]);
         }
+        sp = st;
+        if (++st == NST) { st = 0; fpar ^= 1; }
       }
-      sp = st;
-      if (++st == NST) { st = 0; fpar ^= 1; }
+      if (!ok) give_up(2);
+      // every product has completed before the TMEM is freed (bounded)
+      pf_commit(&done);
+      pf_drain(&done, 0);
     }
-    if (!ok && lane == 0) give_up(2);
-    // every product has completed before the TMEM is freed (bounded)
-    if (pf_elect()) pf_commit(&done);
     __syncwarp();
-    pf_drain(&done, 0);
   } else if (warp >= 4) {
     // ------------------------------------------------------------ softmax
     const int g = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
@@ -359,37 +396,45 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
     const int ta = t0 + min(g * p.tq, ntok - 1), tb = t0 + min((g + 1) * p.tq - 1, ntok - 1);
     const int whi = a.window > 0 ? tb + 1 - a.window : 0;
     float m = -INFINITY, ms = 0.0f, l = 0.0f;                  // maximum of the raw scores, the same scaled, sum
+    const pf_f2 sc2 = pf_pk(a.scale2, a.scale2);
+    // the pages of a tile's 16-row blocks, one per lane, a tile ahead
+    auto page_of = [&](int i) {
+      const int j = pf_key(line, i0 + i) + (lane & (PF_KT / 16 - 1)) * 16;
+      return j < line.end ? __ldg(trow + (j >> a.p.shift)) : -1;
+    };
+    int pg = g < ng && n > 0 ? page_of(0) : 0;
     bool ok = g < ng;
     for (int i = 0; i < n && ok; i++) {
       const int k0 = pf_key(line, i0 + i);
-      int pg[PF_KT / 16];
-#pragma unroll
-      for (int u = 0; u < PF_KT / 16; u++) pg[u] = k0 + u * 16 < line.end ? __ldg(trow + ((k0 + u * 16) >> a.p.shift)) : -1;
       const uint32_t ts = tl + (uint32_t)(g * 128 + (i & 1) * 64);
+      const unsigned bad = ~__ballot_sync(0xffffffffu, (unsigned)pg < (unsigned)a.p.n_pages) & ((1u << (PF_KT / 16)) - 1u);
+      if (i + 1 < n) pg = page_of(i + 1);
       if (!(ok = __all_sync(0xffffffffu, pf_wait(&sfull[g][i & 1], (unsigned)(i >> 1) & 1u, stop)))) break;
       pf_fence_after();
       unsigned s[PF_KT];
       pf_ld32(ts, s);
       pf_ld32(ts + 32, s + 32);
-      unsigned bad = 0;
-#pragma unroll
-      for (int u = 0; u < PF_KT / 16; u++) bad |= (unsigned)pg[u] < (unsigned)a.p.n_pages ? 0u : 1u << u;
       pf_wait_ld();
-      if (bad || k0 + PF_KT - 1 > ta || (k0 < whi && k0 + PF_KT > a.sinks)) {
+      const bool masked = bad || k0 + PF_KT - 1 > ta || (k0 < whi && k0 + PF_KT > a.sinks);   // warp-uniform
+      if (__builtin_expect(masked, 0)) {
+        unsigned long long v = pf_below(t - k0 + 1) & (~pf_below(wlo - k0) | pf_below(a.sinks - k0));
 #pragma unroll
-        for (int k = 0; k < PF_KT; k++) {
-          const int j = k0 + k;
-          const bool in = !((bad >> (k >> 4)) & 1u) && j <= t && (j >= wlo || j < a.sinks);
-          s[k] = in ? s[k] : 0xff800000u;
-        }
+        for (int u = 0; u < PF_KT / 16; u++)
+          if ((bad >> u) & 1u) v &= ~(0xffffull << (16 * u));
+#pragma unroll
+        for (int k = 0; k < PF_KT; k++) s[k] = (v >> k) & 1ull ? s[k] : 0xff800000u;
       }
-      float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float x[4];
 #pragma unroll
-      for (int k = 0; k < PF_KT; k += 4)
+      for (int u = 0; u < 4; u++) x[u] = __uint_as_float(s[u]);
 #pragma unroll
-        for (int u = 0; u < 4; u++) x[u] = fmaxf(x[u], __uint_as_float(s[k + u]));
-      const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-      // the reference maximum: the first one, and a new one when a score passes it by 2^8
+      for (int k = 4; k + 8 <= PF_KT; k += 8)
+#pragma unroll
+        for (int u = 0; u < 4; u++) x[u] = pf_max3(x[u], __uint_as_float(s[k + 2 * u]), __uint_as_float(s[k + 2 * u + 1]));
+      const float mx = pf_max3(pf_max3(x[0], x[1], pf_max3(__uint_as_float(s[60]), __uint_as_float(s[61]), __uint_as_float(s[62]))),
+                               __uint_as_float(s[63]), pf_max3(x[2], x[3], x[2]));
+      // the reference maximum: the first one, and a new one when a score
+      // passes it by 2^8 (a NaN moves nothing: it reaches the sum and the output by itself)
       const bool move = mx > m && (m == -INFINITY || (mx - m) * a.scale2 > 8.0f);
       if (__any_sync(0xffffffffu, move)) {
         const float f = !move ? 1.0f : (m == -INFINITY ? 0.0f : kv_ex2((m - mx) * a.scale2));
@@ -409,18 +454,24 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
           }
         }
       }
-      float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      // p = 2^(scale2 s - ms), rounded to the cache's type, which the product
+      // with V needs; the sum takes the unrounded ones
+      const pf_f2 nms = pf_pk(-ms, -ms);
+      pf_f2 y[2] = {0ull, 0ull};
       unsigned w[32];
 #pragma unroll
-      for (int k = 0; k < PF_KT; k += 2) {
-        const float u = kv_ex2(__fmaf_rn(__uint_as_float(s[k]), a.scale2, -ms));
-        const float v = kv_ex2(__fmaf_rn(__uint_as_float(s[k + 1]), a.scale2, -ms));
-        y[k & 2] += u;
-        y[(k & 2) + 1] += v;
-        // rounded to the cache's type, which the product with V needs; the sum takes the unrounded ones
-        w[k / 2] = kv_down<CT>(u, v);
+      for (int k = 0; k < 32; k++) {
+        float u, v;
+        pf_upk(pf_fma2(pf_pk(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), sc2, nms), u, v);
+        u = kv_ex2(u);
+        v = kv_ex2(v);
+        y[k & 1] = pf_add2(y[k & 1], pf_pk(u, v));
+        w[k] = kv_down<CT>(u, v);
       }
-      l += (y[0] + y[1]) + (y[2] + y[3]);
+      float ya, yb, yc, yd;
+      pf_upk(y[0], ya, yb);
+      pf_upk(y[1], yc, yd);
+      l += (ya + yb) + (yc + yd);
       pf_st32(ts, w);
       pf_wait_st();
       pf_fence_before();
