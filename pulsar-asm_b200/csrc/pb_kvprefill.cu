@@ -17,21 +17,21 @@
 //    2^8; the output is rescaled in TMEM then, which is rare. The sum of a row
 //    stays with its thread. Any maximum that is near enough gives the same
 //    quotient.
-// Warps 0 and 1 copy K and V (16-byte asynchronous copies into the 128-byte
+// Warps 0 to 2 copy K and V (16-byte asynchronous copies into the 128-byte
 // swizzle the tensor cores read; rows that no query of the CTA sees are
-// filled with zeros), warp 2 issues the matrix products, warps 4-7 and 8-11
+// filled with zeros), warp 3 issues the matrix products, warps 4-7 and 8-11
 // are the two groups' softmax (a warp reads its quarter of the TMEM lanes).
 // All waits are bounded; a wait that gives up
-// records an error (pb_kv_status), every role leaves its loop, copies and
-// products in flight are waited for, and the TMEM is freed.
+// records an error (pb_kv_status); copies and products in flight are waited
+// for and the TMEM is freed before the CTA ends.
 #include "pb_kvattn.cuh"
 
 namespace {
 
 constexpr int PF_KT = 64;                 // key rows per tile
 constexpr int PF_T = 12 * 32;
-constexpr int PF_CW = 2;                  // warps that copy (0 and 1), warp 2 issues the products
-constexpr int PF_MMA = 2;
+constexpr int PF_CW = 3;                  // warps that copy: 0, 1 and 2
+constexpr int PF_MMA = 3;                 // the warp that issues the products
 constexpr unsigned long long PF_WAIT_NS = 1000000000ull;
 
 template <int D>
@@ -70,16 +70,25 @@ PB_DEV unsigned long long pf_now() {
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
   return t;
 }
-// bounded wait; false when it gave up or another role did
-PB_DEV bool pf_wait_slow(uint64_t* b, unsigned par, volatile int* stop) {
+// A wait ends after about a second: it then records the role that gave up and
+// raises the CTA's stop flag, at which every further wait returns at once. The
+// roles run on through their loops (all accesses stay in bounds), so copies
+// and products end and the TMEM is freed; the result is void.
+PB_DEV void pf_wait_slow(uint64_t* b, unsigned par, volatile int* stop, int role) {
   const unsigned long long t0 = pf_now();
-  for (unsigned i = 0;; i++) {
-    if (pf_try(b, par)) return true;
-    if ((i & 63) == 63 && (*stop || pf_now() - t0 > PF_WAIT_NS)) return false;
+  for (unsigned i = 1; !pf_try(b, par); i++) {
+    if ((i & 63) == 0) {
+      if (*stop) return;
+      if (pf_now() - t0 > PF_WAIT_NS) {
+        *stop = 1;
+        atomicCAS(&kv_pf_err, 0, role);
+        return;
+      }
+    }
   }
 }
-PB_DEV bool pf_wait(uint64_t* b, unsigned par, volatile int* stop) {
-  return pf_try(b, par) || pf_wait_slow(b, par, stop);
+PB_DEV void pf_wait(uint64_t* b, unsigned par, volatile int* stop, int role) {
+  if (!pf_try(b, par)) pf_wait_slow(b, par, stop, role);
 }
 // the same whatever the other roles did: products in flight before the exit
 PB_DEV void pf_drain(uint64_t* b, unsigned par) {
@@ -201,7 +210,7 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
   typedef PfGeo<D> G;
   constexpr int NST = G::NST, LAG = G::LAG, KP = PF_KT * 128, QP = 128 * 128;   // bytes of a 64-column panel of K or V, of Q
   extern __shared__ __align__(128) char psm_raw[];
-  __shared__ uint64_t full[NST], empty[NST], sfull[2][2], pready[2][2], pvdone[2], done;
+  __shared__ uint64_t full[NST], empty[NST], sfull[2][2], pready[2][2], pvdone[2], ofin[2], done;
   __shared__ uint32_t tbase;
   __shared__ int stop_f;
   const AttnKvArgs& a = p.a;
@@ -230,6 +239,7 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
     for (int g = 0; g < 2; g++) {
       for (int i = 0; i < 2; i++) { pf_init(&sfull[g][i], 1); pf_init(&pready[g][i], 128); }
       pf_init(&pvdone[g], 1);
+      pf_init(&ofin[g], 1);
     }
     pf_init(&done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -239,89 +249,87 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(kv_s32(&tbase)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  // does every 16-row block of the line have its page?
+  bool gap = false;
+  for (int u = threadIdx.x; u < n * (PF_KT / 16); u += PF_T) {
+    const int j = pf_key(line, i0 + u / (PF_KT / 16)) + u % (PF_KT / 16) * 16;
+    if (j < line.end && kv_page(a.p, trow, j) < 0) gap = true;
+  }
   pf_fence_before();
-  __syncthreads();
+  const bool gaps = __syncthreads_or(gap);
   pf_fence_after();
   const uint32_t tmem = tbase;
   volatile int* stop = &stop_f;
-  auto give_up = [&](int role) {
-    *stop = 1;
-    atomicCAS(&kv_pf_err, 0, role);
-  };
 
   if (warp < PF_CW) {
     // ------------------------------------------------------------ copies
-    constexpr int CPR = D / 8, RP = 32 * PF_CW / CPR;   // 16-byte chunks per row, rows per pass
-    const int c = threadIdx.x % CPR, r0 = threadIdx.x / CPR;
+    // A unit is one 16-row block (one page) of K or of V; the warps take the
+    // 8 units of a tile in turn. A lane copies chunk c of rows r0, r0 + RP, ...
+    // The swizzle of the destination repeats every 8 rows.
+    constexpr int CPR = D / 8, RP = 32 / CPR, PB = 16 / RP, SV = 8 / RP, BLK = PF_KT / 16;
+    const int c = lane % CPR, r0 = lane / CPR;
     const uint32_t coff = (c >> 3) * KP, qoff = (c >> 3) * QP;
     if (n > 0) {
-      for (int i = r0; i < ng * 128; i += RP) {
+      for (int i = warp * RP + r0; i < ng * 128; i += RP * PF_CW) {
         const int g = i >> 7, r = i & 127, tk = g * p.tq + r / a.grp;
         const bool in = r < p.tq * a.grp && tk < ntok;
         const char* src = a.q + (in ? (long long)(row0 + tk) * a.ldq + (size_t)(kh * a.grp + r % a.grp) * (D * 2) + c * 16 : 0);
         kv_cp16(kv_s32(smq) + g * G::Q + qoff + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, in);
       }
     }
-    // Per thread, chunk c of rows r0, r0 + RP, ...: the shared-memory offsets
-    // repeat every 8 rows (the swizzle), the row addresses step by RP rows
-    // within a 16-row block, which lies in one page.
-    constexpr int PB = 16 / RP, SV = RP < 8 ? 8 / RP : 1;   // passes per block, swizzle variants
     uint32_t so[SV];
 #pragma unroll
-    for (int u = 0; u < SV; u++) so[u] = coff + r0 * 128 + (((c & 7) ^ ((u * RP + r0) & 7)) << 4);
+    for (int u = 0; u < SV; u++) so[u] = kv_s32(smk) + coff + r0 * 128 + (((c & 7) ^ ((u * RP + r0) & 7)) << 4);
     const long long step = (long long)RP * a.p.rs, lane_off = (long long)kh * a.p.hs + (long long)r0 * a.p.rs + c * 16;
-    int pg[PF_KT / 16];
-    auto pages = [&](int i) {
-      const int k0 = pf_key(line, i0 + i);
-#pragma unroll
-      for (int u = 0; u < PF_KT / 16; u++) pg[u] = k0 + u * 16 < line.end ? __ldg(trow + ((k0 + u * 16) >> a.p.shift)) : -1;
+    // the page of the tile's block `lane % BLK`, a tile ahead
+    auto page_of = [&](int i) {
+      const int j = pf_key(line, i0 + i) + lane % BLK * 16;
+      return j < line.end ? __ldg(trow + (j >> a.p.shift)) : -1;
     };
-    if (n > 0) pages(0);
-    bool ok = true;
+    int pg = n > 0 ? page_of(0) : 0, st = 0, sl = 0;
+    unsigned epar = 1;
     for (int i = 0; i < n + LAG; i++) {
       if (i >= LAG) {    // hand over the stage that has landed, before waiting for room for the next
         kv_cp_wait<LAG - 1>();
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        pf_arrive(&full[(i - LAG) % NST]);
+        pf_arrive(&full[sl]);
+        if (++sl == NST) sl = 0;
       }
       if (i < n) {
-        const int st = i % NST;
-        if (i >= NST && !(ok = pf_wait(&empty[st], (unsigned)(i / NST - 1) & 1u, stop))) break;
+        const int now = pg;
+        if (i + 1 < n) pg = page_of(i + 1);
+        if (i >= NST) pf_wait(&empty[st], epar, stop, 1);
         const int k0 = pf_key(line, i0 + i);
-        const uint32_t ks = kv_s32(smk) + st * (2 * G::KV);
         const bool edge = k0 + PF_KT > line.end || (k0 < line.lo && k0 + PF_KT > line.sinks);   // rows that no query sees
 #pragma unroll
-        for (int blk = 0; blk < PF_KT / 16; blk++) {
-          const int j0 = k0 + blk * 16;
-          const bool page = (unsigned)pg[blk] < (unsigned)a.p.n_pages;
-          const long long off = (page ? (long long)pg[blk] * a.p.ps + (long long)(j0 & ((1 << a.p.shift) - 1)) * a.p.rs : 0) + lane_off;
-          const char *kp = a.p.k + off, *vp = a.p.v + off;
+        for (int z = 0; z < (2 * BLK + PF_CW - 1) / PF_CW; z++) {
+          const int unit = z * PF_CW + warp;
+          if (unit >= 2 * BLK) break;                       // warp-uniform
+          const int blk = unit >> 1, j0 = k0 + blk * 16, e = __shfl_sync(0xffffffffu, now, blk);
+          const bool page = (unsigned)e < (unsigned)a.p.n_pages;
+          const char* pool = unit & 1 ? a.p.v : a.p.k;
+          const char* src = pool + (page ? (long long)e * a.p.ps + (long long)(j0 & ((1 << a.p.shift) - 1)) * a.p.rs : 0) + lane_off;
+          const uint32_t dst = (uint32_t)(st * (2 * G::KV) + (unit & 1) * G::KV + blk * (16 * 128));
           if (page && !edge) {
 #pragma unroll
             for (int q = 0; q < PB; q++) {
-              const int u = blk * PB + q;
-              pf_cp16(ks + so[u % SV] + u * (RP * 128), kp);
-              pf_cp16(ks + so[u % SV] + (u * (RP * 128) + G::KV), vp);
-              kp += step;
-              vp += step;
+              pf_cp16(so[q % SV] + dst + q * (RP * 128), src);
+              src += step;
             }
           } else {
 #pragma unroll
             for (int q = 0; q < PB; q++) {
-              const int u = blk * PB + q, j = j0 + q * RP + r0;
+              const int j = j0 + q * RP + r0;
               const bool in = page && j < line.end && (j >= line.lo || j < line.sinks);
-              kv_cp16(ks + so[u % SV] + u * (RP * 128), in ? kp : a.p.k, in);
-              kv_cp16(ks + so[u % SV] + u * (RP * 128) + G::KV, in ? vp : a.p.v, in);
-              kp += step;
-              vp += step;
+              kv_cp16(so[q % SV] + dst + q * (RP * 128), in ? src : pool, in);
+              src += step;
             }
           }
         }
-        if (i + 1 < n) pages(i + 1);
+        if (++st == NST) { st = 0; epar ^= 1; }
       }
       kv_cp_commit();
     }
-    if (!ok) give_up(1);
     kv_cp_wait<0>();
   } else if (warp == PF_MMA) {
     // ---------------------------------------------------- matrix products
@@ -336,48 +344,53 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
     // that ptxas does not see as uniform cost 100 cycles per product instead
     // of 50 (a product takes 48 to 64).
     if (pf_elect()) {
-      bool ok = true;
-      int st = 0, sp = 0;            // stages of tiles i and i - 1
-      unsigned fpar = 0;             // parity of full[st]
-      for (int i = 0; i <= n; i++) {
-        const uint32_t sb = (uint32_t)(i & 1) * 64;
-        if (i < n) {   // scores of tile i
-          if (!(ok = pf_wait(&full[st], fpar, stop))) break;
-          const uint64_t kb = dk + (uint64_t)(st * ((2 * G::KV) >> 4));
+      // scores of tile j: its stage is `st`, first used with parity `par`
+      auto scores = [&](int g, int j, int st, unsigned par) {
+        if (g == 0) pf_wait(&full[st], par, stop, 2);
+        // the buffer held P of tile j - 2: its product is done
+        if (j >= 2) pf_wait(&pvdone[g], (unsigned)j & 1u, stop, 3);
+        pf_fence_after();
+        const uint64_t kb = dk + (uint64_t)(st * ((2 * G::KV) >> 4));
+        const uint32_t d = tmem + g * 128 + (uint32_t)(j & 1) * 64;
 #pragma unroll
-          for (int g = 0; g < 2; g++) {
-            if (g >= ng) break;
-            // the buffer held P of tile i - 2: its product is done
-            if (i >= 2 && !(ok = pf_wait(&pvdone[g], (unsigned)i & 1u, stop))) break;
-            pf_fence_after();
+        for (int k = 0; k < D / 16; k++)
+          pf_mma_ss(d, dq + (uint64_t)((g * G::Q + (k >> 2) * QP + (k & 3) * 32) >> 4),
+                    kb + (uint64_t)(((k >> 2) * KP + (k & 3) * 32) >> 4), id_s, k > 0);
+        pf_commit(&sfull[g][j & 1]);
+      };
+      // output of tile j
+      auto output = [&](int g, int j, int st) {
+        pf_wait(&pready[g][j & 1], (unsigned)(j >> 1) & 1u, stop, 4);
+        pf_fence_after();
+        const uint64_t vb = dv + (uint64_t)(st * ((2 * G::KV) >> 4));
+        const uint32_t pb = tmem + g * 128 + (uint32_t)(j & 1) * 64;
 #pragma unroll
-            for (int k = 0; k < D / 16; k++)
-              pf_mma_ss(tmem + sb + g * 128, dq + (uint64_t)((g * G::Q + (k >> 2) * QP + (k & 3) * 32) >> 4),
-                        kb + (uint64_t)(((k >> 2) * KP + (k & 3) * 32) >> 4), id_s, k > 0);
-            pf_commit(&sfull[g][i & 1]);
-          }
-          if (!ok) break;
-        }
-        if (i > 0) {   // output of tile i - 1
-          const uint64_t vb = dv + (uint64_t)(sp * ((2 * G::KV) >> 4));
-          const uint32_t pb = 64 - sb;
-#pragma unroll
-          for (int g = 0; g < 2; g++) {
-            if (g >= ng) break;
-            if (!(ok = pf_wait(&pready[g][(i - 1) & 1], (unsigned)((i - 1) >> 1) & 1u, stop))) break;
-            pf_fence_after();
-#pragma unroll
-            for (int k = 0; k < PF_KT / 16; k++)
-              pf_mma_ts(tmem + G::O_COL + g * D, tmem + pb + g * 128 + k * 8, vb + (uint64_t)((k * 2048) >> 4), id_o, i > 1 || k > 0);
-            pf_commit(&pvdone[g]);
-          }
-          if (!ok) break;
-          pf_commit(&empty[sp]);
-        }
-        sp = st;
-        if (++st == NST) { st = 0; fpar ^= 1; }
+        for (int k = 0; k < PF_KT / 16; k++)
+          pf_mma_ts(tmem + G::O_COL + g * D, pb + k * 8, vb + (uint64_t)((k * 2048) >> 4), id_o, j > 0 || k > 0);
+        pf_commit(j + 1 < n ? &pvdone[g] : &ofin[g]);
+      };
+      // The groups half a step apart: each one's next scores follow the
+      // other's output, so that its last output has had time to complete and
+      // the groups' exponentials fall beside each other's other work.
+      int s0 = 0, s1 = 1, s2 = 2;       // stages of tiles i, i + 1, i + 2
+      unsigned p2 = 0;                  // parity of full[s2]
+      if (n > 0) {
+        scores(0, 0, 0, 0);
+        if (ng == 2) scores(1, 0, 0, 0);
+        if (n > 1) scores(0, 1, 1, 0);
       }
-      if (!ok) give_up(2);
+      for (int i = 0; i < n; i++) {
+        output(0, i, s0);
+        if (ng == 2) {
+          if (i + 1 < n) scores(1, i + 1, s1, 0);
+          output(1, i, s0);
+        }
+        pf_commit(&empty[s0]);
+        if (i + 2 < n) scores(0, i + 2, s2, p2);
+        s0 = s1;
+        s1 = s2;
+        if (++s2 == NST) { s2 = 0; p2 ^= 1; }
+      }
       // every product has completed before the TMEM is freed (bounded)
       pf_commit(&done);
       pf_drain(&done, 0);
@@ -397,19 +410,19 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
     const int whi = a.window > 0 ? tb + 1 - a.window : 0;
     float m = -INFINITY, ms = 0.0f, l = 0.0f;                  // maximum of the raw scores, the same scaled, sum
     const pf_f2 sc2 = pf_pk(a.scale2, a.scale2);
-    // the pages of a tile's 16-row blocks, one per lane, a tile ahead
-    auto page_of = [&](int i) {
-      const int j = pf_key(line, i0 + i) + (lane & (PF_KT / 16 - 1)) * 16;
-      return j < line.end ? __ldg(trow + (j >> a.p.shift)) : -1;
-    };
-    int pg = g < ng && n > 0 ? page_of(0) : 0;
-    bool ok = g < ng;
-    for (int i = 0; i < n && ok; i++) {
+    const float over = 8.0f / a.scale2;
+    float thr = -INFINITY;                                     // m + over
+    const int steps = g < ng ? n : 0;
+    for (int i = 0; i < steps; i++) {
       const int k0 = pf_key(line, i0 + i);
       const uint32_t ts = tl + (uint32_t)(g * 128 + (i & 1) * 64);
-      const unsigned bad = ~__ballot_sync(0xffffffffu, (unsigned)pg < (unsigned)a.p.n_pages) & ((1u << (PF_KT / 16)) - 1u);
-      if (i + 1 < n) pg = page_of(i + 1);
-      if (!(ok = __all_sync(0xffffffffu, pf_wait(&sfull[g][i & 1], (unsigned)(i >> 1) & 1u, stop)))) break;
+      unsigned bad = 0;
+      if (gaps) {
+        const int j = k0 + (lane & (PF_KT / 16 - 1)) * 16;
+        bad = ~__ballot_sync(0xffffffffu, j >= line.end || kv_page(a.p, trow, j) >= 0) & ((1u << (PF_KT / 16)) - 1u);
+      }
+      pf_wait(&sfull[g][i & 1], (unsigned)(i >> 1) & 1u, stop, 5);
+      __syncwarp();
       pf_fence_after();
       unsigned s[PF_KT];
       pf_ld32(ts, s);
@@ -434,14 +447,17 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
       const float mx = pf_max3(pf_max3(x[0], x[1], pf_max3(__uint_as_float(s[60]), __uint_as_float(s[61]), __uint_as_float(s[62]))),
                                __uint_as_float(s[63]), pf_max3(x[2], x[3], x[2]));
       // the reference maximum: the first one, and a new one when a score
-      // passes it by 2^8 (a NaN moves nothing: it reaches the sum and the output by itself)
-      const bool move = mx > m && (m == -INFINITY || (mx - m) * a.scale2 > 8.0f);
-      if (__any_sync(0xffffffffu, move)) {
+      // passes it by 2^8. A NaN or +inf makes the row's sum, and so its output, NaN.
+      const bool over_it = !(mx <= thr);
+      if (__any_sync(0xffffffffu, over_it)) {
+        const bool move = mx > thr;
         const float f = !move ? 1.0f : (m == -INFINITY ? 0.0f : kv_ex2((m - mx) * a.scale2));
-        if (move) { m = mx; ms = mx * a.scale2; }
+        if (move) { m = mx; ms = mx * a.scale2; thr = mx + over; }
+        if (over_it && !(mx < INFINITY)) l = __int_as_float(0x7fffffff);
         l *= f;
         if (i > 0) {   // the output so far, which the product of tile i - 1 has completed
-          if (!(ok = __all_sync(0xffffffffu, pf_wait(&pvdone[g], (unsigned)(i - 1) & 1u, stop)))) break;
+          pf_wait(&pvdone[g], (unsigned)(i - 1) & 1u, stop, 6);
+          __syncwarp();
           pf_fence_after();
 #pragma unroll
           for (int e = 0; e < D; e += 32) {
@@ -459,10 +475,13 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
       const pf_f2 nms = pf_pk(-ms, -ms);
       pf_f2 y[2] = {0ull, 0ull};
       unsigned w[32];
+      pf_f2 z[32];
+#pragma unroll
+      for (int k = 0; k < 32; k++) z[k] = pf_fma2(pf_pk(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), sc2, nms);
 #pragma unroll
       for (int k = 0; k < 32; k++) {
         float u, v;
-        pf_upk(pf_fma2(pf_pk(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), sc2, nms), u, v);
+        pf_upk(z[k], u, v);
         u = kv_ex2(u);
         v = kv_ex2(v);
         y[k & 1] = pf_add2(y[k & 1], pf_pk(u, v));
@@ -477,14 +496,11 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
       pf_fence_before();
       pf_arrive(&pready[g][i & 1]);
     }
-    if (g < ng && !ok && lane == 0) give_up(3);
-    if (ok && n > 0) {
-      // tile by tile: the wait for a phase's parity needs the phase before it to be over
-      ok = (n < 2 || __all_sync(0xffffffffu, pf_wait(&pvdone[g], (unsigned)(n - 2) & 1u, stop))) &&
-           __all_sync(0xffffffffu, pf_wait(&pvdone[g], (unsigned)(n - 1) & 1u, stop));
-      if (!ok && lane == 0) give_up(4);
-    }
-    if (g < ng && ok) {
+    if (g < ng) {
+      if (n > 0) {
+        pf_wait(&ofin[g], 0, stop, 8);   // (a barrier of its own: pvdone may be one or two phases on)
+        __syncwarp();
+      }
       pf_fence_after();
       const int row = row0 + tk, h = kh * a.grp + r % a.grp;
       const float f = l != 0.0f ? 1.0f / l : 0.0f;       // nothing seen: zeros
