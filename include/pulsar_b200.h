@@ -365,8 +365,9 @@ int pb_tq_attention(int bits, const float* d_q, const uint32_t* d_kcode, const f
  *  - head_dim 64 or 128; page_size 16, 32, 64, 128 or 256; dtype (of K, V and
  *    q) PB_DT_F16 or PB_DT_BF16; n_heads / n_kv a whole number up to 16.
  *  - Strides are in elements, the last dimension is contiguous, rows start on
- *    16 bytes, and no two rows overlap; [page][head][row] and
- *    [page][row][head] orders and interleaved K and V pools all do.
+ *    16 bytes, no two rows overlap, and each stride is a multiple of the next
+ *    smaller one; [page][head][row] and [page][row][head] orders, interleaved
+ *    K and V pools and slices of larger ones all do.
  *  - A table entry outside [0, n_pages) names no page: rows there are not
  *    seen, stored or moved. Entries that no seen row needs are not used.
  *  - Lengths live on the device and are read there, so a captured graph

@@ -352,13 +352,15 @@ int kv_pool(const char* who, const pb_kv_pages* c, int n_seq, const int* d_table
   for (int i = 0; i < 2; i++)
     for (int j = 0; j < 2 - i; j++)
       if (d[j].st > d[j + 1].st) { const auto x = d[j]; d[j] = d[j + 1]; d[j + 1] = x; }
-  long long span = c->head_dim;
+  long long span = c->head_dim, below = 8;
   for (int i = 0; i < 3; i++) {
     if (d[i].n == 1) continue;
-    if (d[i].st < span || d[i].st > (1ll << 52) / d[i].n)
-      return pb_set_error(PB_EINVAL, "%s: strides %lld (page), %lld (head), %lld (row) make rows overlap", who, c->page_stride,
-                          c->head_stride, c->row_stride);
+    // (2^38 elements, and whole multiples of the next smaller stride: what a tensor map takes)
+    if (d[i].st < span || d[i].st > (1ll << 38) / d[i].n || d[i].st % below)
+      return pb_set_error(PB_EINVAL, "%s: strides %lld (page), %lld (head), %lld (row): rows overlap, or one is not a multiple of the next smaller",
+                          who, c->page_stride, c->head_stride, c->row_stride);
     span += d[i].st * (d[i].n - 1);
+    below = d[i].st;
   }
   p->k = static_cast<char*>(c->k);
   p->v = static_cast<char*>(c->v);

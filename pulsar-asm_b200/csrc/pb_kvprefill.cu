@@ -17,21 +17,24 @@
 //    2^8; the output is rescaled in TMEM then, which is rare. The sum of a row
 //    stays with its thread. Any maximum that is near enough gives the same
 //    quotient.
-// Warps 0 to 2 copy K and V (16-byte asynchronous copies into the 128-byte
-// swizzle the tensor cores read; rows that no query of the CTA sees are
-// filled with zeros), warp 3 issues the matrix products, warps 4-7 and 8-11
-// are the two groups' softmax (a warp reads its quarter of the TMEM lanes).
+// Warp 0 brings K and V tiles by TMA (a box per page, or part of one, and 64
+// columns, in the 128-byte swizzle the tensor cores read; a table entry that
+// names no page becomes a box outside the pool, which reads as zeros), warps 2
+// and 3 issue the two groups' matrix products, warps 4-7 and 8-11 are the two
+// groups' softmax (a warp reads its quarter of the TMEM lanes). In a tile at
+// the end of what the queries see, V rows behind it are set to zero: they may
+// hold anything, and 0 times that must be 0.
 // All waits are bounded; a wait that gives up
 // records an error (pb_kv_status); copies and products in flight are waited
 // for and the TMEM is freed before the CTA ends.
 #include "pb_kvattn.cuh"
+#include <cuda.h>
 
 namespace {
 
 constexpr int PF_KT = 64;                 // key rows per tile
 constexpr int PF_T = 12 * 32;
-constexpr int PF_CW = 3;                  // warps that copy: 0, 1 and 2
-constexpr int PF_MMA = 3;                 // the warp that issues the products
+constexpr int PF_MMA = 2;                 // the warp that issues the first group's products, the next one the second's
 constexpr unsigned long long PF_WAIT_NS = 1000000000ull;
 
 template <int D>
@@ -39,13 +42,13 @@ struct PfGeo {
   static constexpr int Q = 128 * D * 2;           // bytes of a group's queries
   static constexpr int KV = PF_KT * D * 2;        // bytes of a K (or V) tile
   static constexpr int NST = D == 128 ? 5 : 8;    // K/V stages
-  static constexpr int LAG = 2;                   // stages in flight
   static constexpr int SMEM = 2 * Q + NST * 2 * KV + 1024;
   static constexpr uint32_t O_COL = 256;          // S: group * 128 + buffer * 64; O: 256 + group * D
 };
 
 struct PfArgs {
   AttnKvArgs a;
+  int d_row, d_head, box;   // which of the tensor map's dimensions 1-3 are the row and the head (the third is the page); rows per box
   int tq, ns, out_bf16;     // tokens per group of 128 rows; splits of the key line
   float* part;              // [split][row][head][D] unnormalised sums (ns > 1)
   float2* ml;               // [split][row][head] maximum and sum
@@ -162,8 +165,12 @@ PB_DEV float pf_max3(float a, float b, float c) {   // NaN if any is
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-PB_DEV void pf_cp16(uint32_t dst, const char* src) {
-  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+PB_DEV void pf_expect(uint64_t* b, unsigned bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(kv_s32(b)), "r"(bytes) : "memory");
+}
+PB_DEV void pf_tma(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+               ::"r"(dst), "l"(m), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(kv_s32(bar)) : "memory");
 }
 
 // rows of q of sequence b: the first, and how many
@@ -190,6 +197,8 @@ PB_DEV PfLine pf_line(const AttnKvArgs& a, int t_first, int t_last) {
 }
 // bits 0 .. x - 1
 PB_DEV unsigned long long pf_below(int x) { return x <= 0 ? 0ull : (x >= 64 ? ~0ull : (1ull << x) - 1ull); }
+// a tile with rows that no query of the CTA sees
+PB_DEV bool pf_edge(const PfLine& s, int k0) { return k0 + PF_KT > s.end || (k0 < s.lo && k0 + PF_KT > s.sinks); }
 PB_DEV int pf_key(const PfLine& s, int i) { return (i < s.nst ? i : i - s.nst + s.lot) * PF_KT; }
 
 template <int D>
@@ -206,11 +215,11 @@ PB_DEV void pf_put(const PfArgs& p, int row, int h, int e, const float (&x)[8]) 
 }
 
 template <int D, int CT>
-__global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
+__global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, PfArgs p) {
   typedef PfGeo<D> G;
-  constexpr int NST = G::NST, LAG = G::LAG, KP = PF_KT * 128, QP = 128 * 128;   // bytes of a 64-column panel of K or V, of Q
+  constexpr int NST = G::NST, KP = PF_KT * 128, QP = 128 * 128;   // bytes of a 64-column panel of K or V, of Q
   extern __shared__ __align__(128) char psm_raw[];
-  __shared__ uint64_t full[NST], empty[NST], sfull[2][2], pready[2][2], pvdone[2], ofin[2], done;
+  __shared__ uint64_t full[NST], empty[NST], sfull[2][2], pready[2][2], pvdone[2], ofin[2], lock[4], qfull, vfix[3], done[2];
   __shared__ uint32_t tbase;
   __shared__ int stop_f;
   const AttnKvArgs& a = p.a;
@@ -235,13 +244,17 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
   const int* trow = a.p.table + (size_t)b * a.p.table_ld;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NST; i++) { pf_init(&full[i], 32 * PF_CW); pf_init(&empty[i], 1); }
+    for (int i = 0; i < NST; i++) { pf_init(&full[i], 1); pf_init(&empty[i], ng); }
     for (int g = 0; g < 2; g++) {
       for (int i = 0; i < 2; i++) { pf_init(&sfull[g][i], 1); pf_init(&pready[g][i], 128); }
       pf_init(&pvdone[g], 1);
       pf_init(&ofin[g], 1);
     }
-    pf_init(&done, 1);
+    pf_init(&qfull, 256);
+    for (int i = 0; i < 4; i++) pf_init(&lock[i], 1);
+    for (int i = 0; i < 3; i++) pf_init(&vfix[i], 1);
+    pf_init(&done[0], 1);
+    pf_init(&done[1], 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     stop_f = 0;
   }
@@ -261,77 +274,64 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
   const uint32_t tmem = tbase;
   volatile int* stop = &stop_f;
 
-  if (warp < PF_CW) {
+  if (warp == 0) {
     // ------------------------------------------------------------ copies
-    // A unit is one 16-row block (one page) of K or of V; the warps take the
-    // 8 units of a tile in turn. A lane copies chunk c of rows r0, r0 + RP, ...
-    // The swizzle of the destination repeats every 8 rows.
-    constexpr int CPR = D / 8, RP = 32 / CPR, PB = 16 / RP, SV = 8 / RP, BLK = PF_KT / 16;
-    const int c = lane % CPR, r0 = lane / CPR;
-    const uint32_t coff = (c >> 3) * KP, qoff = (c >> 3) * QP;
-    if (n > 0) {
-      for (int i = warp * RP + r0; i < ng * 128; i += RP * PF_CW) {
-        const int g = i >> 7, r = i & 127, tk = g * p.tq + r / a.grp;
-        const bool in = r < p.tq * a.grp && tk < ntok;
-        const char* src = a.q + (in ? (long long)(row0 + tk) * a.ldq + (size_t)(kh * a.grp + r % a.grp) * (D * 2) + c * 16 : 0);
-        kv_cp16(kv_s32(smq) + g * G::Q + qoff + r * 128 + (((c & 7) ^ (r & 7)) << 4), src, in);
-      }
-    }
-    uint32_t so[SV];
-#pragma unroll
-    for (int u = 0; u < SV; u++) so[u] = kv_s32(smk) + coff + r0 * 128 + (((c & 7) ^ ((u * RP + r0) & 7)) << 4);
-    const long long step = (long long)RP * a.p.rs, lane_off = (long long)kh * a.p.hs + (long long)r0 * a.p.rs + c * 16;
-    // the page of the tile's block `lane % BLK`, a tile ahead
+    // the page of the tile's 16-row block `lane % 4`, a tile ahead
     auto page_of = [&](int i) {
-      const int j = pf_key(line, i0 + i) + lane % BLK * 16;
-      return j < line.end ? __ldg(trow + (j >> a.p.shift)) : -1;
+      const int j = pf_key(line, i0 + i) + lane % (PF_KT / 16) * 16;
+      const int e = j < line.end ? __ldg(trow + (j >> a.p.shift)) : -1;
+      return (unsigned)e < (unsigned)a.p.n_pages ? e : a.p.n_pages;   // the box behind the last page: zeros
     };
-    int pg = n > 0 ? page_of(0) : 0, st = 0, sl = 0;
-    unsigned epar = 1;
-    for (int i = 0; i < n + LAG; i++) {
-      if (i >= LAG) {    // hand over the stage that has landed, before waiting for room for the next
-        kv_cp_wait<LAG - 1>();
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        pf_arrive(&full[sl]);
-        if (++sl == NST) sl = 0;
-      }
+    int pg = n > 0 ? page_of(0) : 0, st = 0, sf = 0;
+    unsigned epar = 1, fpar = 0;
+    int fixes = 0;    // at most 3: where the sinks end, where the window begins, the last tile
+    for (int i = 0; i < n + 2; i++) {
       if (i < n) {
-        const int now = pg;
+        const int now = pg, k0 = pf_key(line, i0 + i);
         if (i + 1 < n) pg = page_of(i + 1);
         if (i >= NST) pf_wait(&empty[st], epar, stop, 1);
-        const int k0 = pf_key(line, i0 + i);
-        const bool edge = k0 + PF_KT > line.end || (k0 < line.lo && k0 + PF_KT > line.sinks);   // rows that no query sees
+        __syncwarp();
+        const uint32_t ks = kv_s32(smk) + st * (2 * G::KV);
+        if (lane == 0) pf_expect(&full[st], 2 * G::KV);
+        for (int r = 0; r < PF_KT; r += p.box) {
+          const int page = __shfl_sync(0xffffffffu, now, r >> 4), row = (k0 + r) & ((1 << a.p.shift) - 1);
+          if (lane == 0) {
+            const int c1 = p.d_row == 1 ? row : (p.d_head == 1 ? kh : page), c2 = p.d_row == 2 ? row : (p.d_head == 2 ? kh : page),
+                      c3 = p.d_row == 3 ? row : (p.d_head == 3 ? kh : page);
 #pragma unroll
-        for (int z = 0; z < (2 * BLK + PF_CW - 1) / PF_CW; z++) {
-          const int unit = z * PF_CW + warp;
-          if (unit >= 2 * BLK) break;                       // warp-uniform
-          const int blk = unit >> 1, j0 = k0 + blk * 16, e = __shfl_sync(0xffffffffu, now, blk);
-          const bool page = (unsigned)e < (unsigned)a.p.n_pages;
-          const char* pool = unit & 1 ? a.p.v : a.p.k;
-          const char* src = pool + (page ? (long long)e * a.p.ps + (long long)(j0 & ((1 << a.p.shift) - 1)) * a.p.rs : 0) + lane_off;
-          const uint32_t dst = (uint32_t)(st * (2 * G::KV) + (unit & 1) * G::KV + blk * (16 * 128));
-          if (page && !edge) {
-#pragma unroll
-            for (int q = 0; q < PB; q++) {
-              pf_cp16(so[q % SV] + dst + q * (RP * 128), src);
-              src += step;
-            }
-          } else {
-#pragma unroll
-            for (int q = 0; q < PB; q++) {
-              const int j = j0 + q * RP + r0;
-              const bool in = page && j < line.end && (j >= line.lo || j < line.sinks);
-              kv_cp16(so[q % SV] + dst + q * (RP * 128), in ? src : pool, in);
-              src += step;
+            for (int c = 0; c < D / 64; c++) {
+              pf_tma(ks + c * KP + r * 128, &mk, c * 64, c1, c2, c3, &full[st]);
+              pf_tma(ks + G::KV + c * KP + r * 128, &mv, c * 64, c1, c2, c3, &full[st]);
             }
           }
         }
         if (++st == NST) { st = 0; epar ^= 1; }
       }
-      kv_cp_commit();
+      if (i >= 2) {     // two tiles later: V rows behind what is seen
+        const int k0 = pf_key(line, i0 + i - 2);
+        if (pf_edge(line, k0)) {
+          pf_wait(&full[sf], fpar, stop, 9);
+          char* vs = smk + sf * (2 * G::KV) + G::KV;
+          for (int u = lane; u < PF_KT * (D / 8); u += 32) {
+            const int r = u & (PF_KT - 1), j = k0 + r;
+            if (j >= line.end || (j < line.lo && j >= line.sinks))
+              *reinterpret_cast<uint4*>(vs + (u / PF_KT >> 3) * KP + r * 128 + (u / PF_KT & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && fixes < 3) pf_arrive(&vfix[fixes]);
+          fixes++;
+        }
+        if (++sf == NST) { sf = 0; fpar ^= 1; }
+      }
     }
-    kv_cp_wait<0>();
-  } else if (warp == PF_MMA) {
+    // no copy may land after the CTA ends: every tile was waited for by the products; where those
+    // gave up, by time
+    if (*stop) {
+      const unsigned long long t1 = pf_now();
+      while (pf_now() - t1 < 1000000ull) {}
+    }
+  } else if (warp == PF_MMA || warp == PF_MMA + 1) {
     // ---------------------------------------------------- matrix products
     // kind::f16: D fp32 (bits 4-5 = 1), A and B fp16 (0) or bf16 (1) at bits 7 and 10, B N-major at bit 16,
     // N / 8 at bits 17-22, M / 16 at bits 24-28
@@ -339,61 +339,71 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
     constexpr uint32_t base = (1u << 4) | (ty << 7) | (ty << 10) | (8u << 24);
     constexpr uint32_t id_s = base | ((uint32_t)(PF_KT >> 3) << 17), id_o = base | (1u << 16) | ((uint32_t)(D >> 3) << 17);
     const uint64_t dq = pf_desc(kv_s32(smq), 16), dk = pf_desc(kv_s32(smk), 16), dv = pf_desc(kv_s32(smk) + G::KV, KP);
-    // One elected thread waits and issues: a warp-wide wait, with its vote and
-    // election, costs some 150 cycles of a step that has six; and operands
-    // that ptxas does not see as uniform cost 100 cycles per product instead
-    // of 50 (a product takes 48 to 64).
-    if (pf_elect()) {
-      // scores of tile j: its stage is `st`, first used with parity `par`
-      auto scores = [&](int g, int j, int st, unsigned par) {
-        if (g == 0) pf_wait(&full[st], par, stop, 2);
+    // A warp per group, in which one elected thread waits and issues: with a
+    // warp-wide wait, its vote and election, a step's waits took half its
+    // time; operands that ptxas does not see as uniform cost 100 cycles per
+    // product instead of 25 (a product takes 48 to 64); and one thread for
+    // both groups spent 1900 cycles a step on its own waits and commits.
+    const int g = warp - PF_MMA;
+    if (g < ng && pf_elect()) {
+      // scores of tile j
+      auto scores = [&](int j, int st, unsigned par) {
+        pf_wait(&full[st], par, stop, 2);
         // the buffer held P of tile j - 2: its product is done
         if (j >= 2) pf_wait(&pvdone[g], (unsigned)j & 1u, stop, 3);
         pf_fence_after();
-        const uint64_t kb = dk + (uint64_t)(st * ((2 * G::KV) >> 4));
+        const uint64_t kb = dk + (uint64_t)(st * ((2 * G::KV) >> 4)), qb = dq + (uint64_t)((g * G::Q) >> 4);
         const uint32_t d = tmem + g * 128 + (uint32_t)(j & 1) * 64;
 #pragma unroll
         for (int k = 0; k < D / 16; k++)
-          pf_mma_ss(d, dq + (uint64_t)((g * G::Q + (k >> 2) * QP + (k & 3) * 32) >> 4),
-                    kb + (uint64_t)(((k >> 2) * KP + (k & 3) * 32) >> 4), id_s, k > 0);
+          pf_mma_ss(d, qb + (uint64_t)(((k >> 2) * QP + (k & 3) * 32) >> 4), kb + (uint64_t)(((k >> 2) * KP + (k & 3) * 32) >> 4),
+                    id_s, k > 0);
         pf_commit(&sfull[g][j & 1]);
       };
-      // output of tile j
-      auto output = [&](int g, int j, int st) {
-        pf_wait(&pready[g][j & 1], (unsigned)(j >> 1) & 1u, stop, 4);
-        pf_fence_after();
-        const uint64_t vb = dv + (uint64_t)(st * ((2 * G::KV) >> 4));
-        const uint32_t pb = tmem + g * 128 + (uint32_t)(j & 1) * 64;
-#pragma unroll
-        for (int k = 0; k < PF_KT / 16; k++)
-          pf_mma_ts(tmem + G::O_COL + g * D, pb + k * 8, vb + (uint64_t)((k * 2048) >> 4), id_o, j > 0 || k > 0);
-        pf_commit(j + 1 < n ? &pvdone[g] : &ofin[g]);
-      };
-      // The groups half a step apart: each one's next scores follow the
-      // other's output, so that its last output has had time to complete and
-      // the groups' exponentials fall beside each other's other work.
-      int s0 = 0, s1 = 1, s2 = 2;       // stages of tiles i, i + 1, i + 2
-      unsigned p2 = 0;                  // parity of full[s2]
+      // The groups are held half a step apart, so that one's exponentials
+      // fall beside the other's other work: the second group's next scores
+      // wait for the first's probabilities, and the first's next but one for
+      // the second's. (At their own pace they fell into step: 540 us instead
+      // of 502 for 8192 tokens of 32/8 heads x 128; a share of the
+      // exponentials by polynomial on the FMA pipe, 509 in step, did not help
+      // further here.)
+      int fixes = 0;                    // edge tiles so far
+      int st = 0, s1 = 1, s2 = 2;       // stages of tiles i, i + 1, i + 2
+      unsigned p1 = 0, p2 = 0;          // parities of full[s1], full[s2]
       if (n > 0) {
-        scores(0, 0, 0, 0);
-        if (ng == 2) scores(1, 0, 0, 0);
-        if (n > 1) scores(0, 1, 1, 0);
+        pf_wait(&qfull, 0, stop, 10);
+        scores(0, 0, 0);
+        if (g == 0 && n > 1) scores(1, 1, 0);
       }
       for (int i = 0; i < n; i++) {
-        output(0, i, s0);
-        if (ng == 2) {
-          if (i + 1 < n) scores(1, i + 1, s1, 0);
-          output(1, i, s0);
+        const bool edge = pf_edge(line, pf_key(line, i0 + i));
+        if (g == 1 && i + 1 < n) {
+          pf_wait(&pready[0][i & 1], (unsigned)(i >> 1) & 1u, stop, 7);
+          scores(i + 1, s1, p1);
         }
-        pf_commit(&empty[s0]);
-        if (i + 2 < n) scores(0, i + 2, s2, p2);
-        s0 = s1;
+        if (edge && fixes < 3) pf_wait(&vfix[fixes++], 0, stop, 11);
+        pf_wait(&pready[g][i & 1], (unsigned)(i >> 1) & 1u, stop, 4);
+        if (g == 1) pf_arrive(&lock[i & 3]);
+        pf_fence_after();
+        const uint64_t vb = dv + (uint64_t)(st * ((2 * G::KV) >> 4));
+        const uint32_t pb = tmem + g * 128 + (uint32_t)(i & 1) * 64, o = tmem + G::O_COL + g * D;
+#pragma unroll
+        for (int k = 0; k < PF_KT / 16; k++) pf_mma_ts(o, pb + k * 8, vb + (uint64_t)((k * 2048) >> 4), id_o, i > 0 || k > 0);
+        pf_commit(i + 1 < n ? &pvdone[g] : &ofin[g]);
+        pf_commit(&empty[st]);
+        if (g == 0 && i + 2 < n) {
+          // (of four, as the other thread may be up to three tiles ahead)
+          if (ng == 2) pf_wait(&lock[i & 3], (unsigned)(i >> 2) & 1u, stop, 12);
+          scores(i + 2, s2, p2);
+        }
+        st = s1;
         s1 = s2;
+        p1 = p2;
         if (++s2 == NST) { s2 = 0; p2 ^= 1; }
       }
       // every product has completed before the TMEM is freed (bounded)
-      pf_commit(&done);
-      pf_drain(&done, 0);
+      pf_commit(&done[g]);
+      pf_drain(&done[g], 0);
     }
     __syncwarp();
   } else if (warp >= 4) {
@@ -405,6 +415,18 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(PfArgs p) {
     const bool live = r < p.tq * a.grp && tk < ntok;
     const int t = t0 + min(tk, ntok - 1);                      // the row's own cache row
     const int wlo = a.window > 0 ? t + 1 - a.window : 0;       // it sees [wlo, t] and [0, sinks)
+    // its query, swizzled; rows past the last token are zeros
+    if (n > 0) {
+      const char* src = a.q + (long long)(row0 + min(tk, ntok - 1)) * a.ldq + (size_t)(kh * a.grp + r % a.grp) * (D * 2);
+#pragma unroll
+      for (int c = 0; c < D / 8; c++) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (live) v = pb_ldg_stream(src + c * 16);
+        *reinterpret_cast<uint4*>(smq + g * G::Q + (c >> 3) * QP + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      pf_arrive(&qfull);
+    }
     // of the group: what all rows see, for tiles that need no masks
     const int ta = t0 + min(g * p.tq, ntok - 1), tb = t0 + min((g + 1) * p.tq - 1, ntok - 1);
     const int whi = a.window > 0 ? tb + 1 - a.window : 0;
@@ -607,11 +629,57 @@ PfPlan pf_plan(const pb_kv_pages* c, int n_seq, int max_len, int n_tok, int n_he
   return p;
 }
 
+// The pools as tensors of rank 4, dimension 0 the columns, the others by
+// ascending stride; a box is up to 64 rows of one page and 64 columns.
+typedef CUresult (*PfEncode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+int pf_maps(const pb_kv_pages* c, PfArgs* p, CUtensorMap* mk, CUtensorMap* mv) {
+  static std::atomic<void*> fn{nullptr};
+  void* f = fn.load(std::memory_order_acquire);
+  if (!f) {
+    cudaDriverEntryPointQueryResult found;
+    PB_TRY_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found));
+    if (found != cudaDriverEntryPointSuccess || !f) return pb_set_error(PB_ECUDA, "pb_kv_prefill: no cuTensorMapEncodeTiled");
+    fn.store(f, std::memory_order_release);
+  }
+  struct Dim { long long st; int n, box, what; } d[3] = {{c->row_stride, c->page_size, c->page_size < PF_KT ? c->page_size : PF_KT, 0},
+                                                         {c->head_stride, c->n_kv, 1, 1},
+                                                         {c->page_stride, c->n_pages, 1, 2}};
+  p->box = d[0].box;
+  // a dimension of size 1 takes part with the stride behind the larger ones
+  long long far = c->head_dim;
+  for (const Dim& x : d)
+    if (x.n > 1 && x.st * x.n > far) far = x.st * x.n;
+  for (Dim& x : d)
+    if (x.n == 1) x.st = far;
+  for (int i = 0; i < 2; i++)
+    for (int j = 0; j < 2 - i; j++)
+      if (d[j].st > d[j + 1].st) { const Dim x = d[j]; d[j] = d[j + 1]; d[j + 1] = x; }
+  cuuint64_t dims[4] = {(cuuint64_t)c->head_dim}, strides[3];
+  cuuint32_t box[4] = {64}, one[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 3; i++) {
+    dims[i + 1] = (cuuint64_t)d[i].n;
+    strides[i] = (cuuint64_t)d[i].st * 2;
+    box[i + 1] = (cuuint32_t)d[i].box;
+    if (d[i].what == 0) p->d_row = i + 1;
+    if (d[i].what == 1) p->d_head = i + 1;
+  }
+  const CUtensorMapDataType ty = c->dtype == PB_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  for (int i = 0; i < 2; i++) {
+    const CUresult r = reinterpret_cast<PfEncode>(f)(i ? mv : mk, ty, 4, i ? c->v : c->k, dims, strides, box, one,
+                                                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return pb_set_error(PB_EINVAL, "pb_kv_prefill: strides the tensor map does not take (%d)", (int)r);
+  }
+  return PB_OK;
+}
+
 template <int D, int CT>
-int pf_run(const PfArgs& p, long long items, cudaStream_t st) {
+int pf_run(const CUtensorMap& mk, const CUtensorMap& mv, const PfArgs& p, long long items, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
   if (int rc = kv_smem(k_kv_prefill<D, CT>, PfGeo<D>::SMEM, done)) return rc;
-  if (int rc = kv_launch(k_kv_prefill<D, CT>, (unsigned)(items * p.ns), PF_T, PfGeo<D>::SMEM, st, false, "k_kv_prefill", p)) return rc;
+  if (int rc = kv_launch(k_kv_prefill<D, CT>, (unsigned)(items * p.ns), PF_T, PfGeo<D>::SMEM, st, false, "k_kv_prefill", mk, mv, p)) return rc;
   if (p.ns == 1) return PB_OK;
   const long long blocks = ((long long)p.a.n_rows * p.a.nh * (D / 4) + 127) / 128;
   return kv_launch(k_kv_prefill_join<D>, (unsigned)blocks, 128, 0, st, true, "k_kv_prefill_join", p);
@@ -650,8 +718,11 @@ extern "C" int pb_kv_prefill(const pb_kv_pages* c, int n_seq, const int* d_table
   p.part = static_cast<float*>(d_scratch);
   p.ml = reinterpret_cast<float2*>(p.part + pl.part);
   cudaStream_t st = (cudaStream_t)stream;
-  if (c->head_dim == 64) return c->dtype == PB_DT_F16 ? pf_run<64, PB_DT_F16>(p, pl.items, st) : pf_run<64, PB_DT_BF16>(p, pl.items, st);
-  return c->dtype == PB_DT_F16 ? pf_run<128, PB_DT_F16>(p, pl.items, st) : pf_run<128, PB_DT_BF16>(p, pl.items, st);
+  CUtensorMap mk, mv;
+  if (int rc = pf_maps(c, &p, &mk, &mv)) return rc;
+  if (c->head_dim == 64)
+    return c->dtype == PB_DT_F16 ? pf_run<64, PB_DT_F16>(mk, mv, p, pl.items, st) : pf_run<64, PB_DT_BF16>(mk, mv, p, pl.items, st);
+  return c->dtype == PB_DT_F16 ? pf_run<128, PB_DT_F16>(mk, mv, p, pl.items, st) : pf_run<128, PB_DT_BF16>(mk, mv, p, pl.items, st);
 }
 
 extern "C" int pb_kv_status(void* stream) {
