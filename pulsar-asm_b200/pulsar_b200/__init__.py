@@ -338,19 +338,20 @@ def sample_topkpp(logits, temp, topp, topk, minp, rng, ids, stream=None):
                                  _stream(stream)))
 
 
+_DTYPES = {}
+
+
 def _dtype_code(t):
     """PB_DT_* of a torch tensor's dtype (int16 tensors hold bf16 bits, as elsewhere in this module)"""
-    import torch
-    if not _DTYPES:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        import torch
         _DTYPES.update({torch.bfloat16: PB_DT_BF16, torch.int16: PB_DT_BF16, torch.float32: PB_DT_F32,
                         torch.float16: PB_DT_F16})
-    try:
-        return _DTYPES[t.dtype]
-    except KeyError:
-        raise PBError(-1, "dtype %s" % t.dtype) from None
-
-
-_DTYPES = {}
+        code = _DTYPES.get(t.dtype)
+        if code is None:
+            raise PBError(-1, "dtype %s" % t.dtype)
+    return code
 
 
 class KVPages:
@@ -379,6 +380,9 @@ class KVPages:
                            n, r, h, d, k.stride(0), k.stride(1), k.stride(2))
         self._r = C.byref(self._c)
         self.n_kv, self.page_size, self.head_dim = h, r, d
+        self._torch, self._dev, self._i32, self._f32 = torch, k.get_device(), torch.int32, torch.float32
+        self._scale = d ** -0.5
+        self._need = {}     # scratch bytes by call shape
 
     @classmethod
     def alloc(cls, n_pages, page_size, n_kv, head_dim, dtype=None, weights=False, device="cuda"):
@@ -389,81 +393,94 @@ class KVPages:
         return cls(k, torch.zeros_like(k),
                    torch.zeros(shape[:3], dtype=torch.float32, device=device) if weights else None)
 
-    def _ints(self, what, t, dim=1, n=None):
-        if t.dtype != self._int32 or t.device != self.device or t.dim() != dim or not t.is_contiguous() or \
-                (n is not None and t.shape[0] != n):
-            raise PBError(-1, "%s: an int32 tensor on %s of %d dimension%s%s, contiguous" % (
-                what, self.device, dim, "" if dim == 1 else "s", "" if n is None else " and length %d" % n))
+    # the checks below are on the path of every call: a decode step makes one or two per layer
+    def _ints(self, what, t, shape):
+        if t.dtype is not self._i32 or t.shape != shape or t.get_device() != self._dev or not t.is_contiguous():
+            raise PBError(-1, "%s: a contiguous int32 tensor %s on %s" % (what, list(shape), self.device))
         return t.data_ptr()
 
-    def _heads(self, what, t, dtype=None):
-        """a tensor [row][head][dim] whose rows are contiguous"""
-        if t.dim() != 3 or t.device != self.device or t.shape[2] != self.head_dim or (dtype and t.dtype != dtype) or \
-                (t.numel() and (t.stride(2) != 1 or t.stride(1) != self.head_dim)):
-            raise PBError(-1, "%s: a tensor [row][head][%d]%s on %s with contiguous rows" % (
+    def _heads(self, what, t, shape, dtype):
+        """a tensor [row][head][dim] with contiguous rows: (pointer, row stride)"""
+        st = t.stride()
+        if len(shape) != 3 or t.shape != shape or shape[2] != self.head_dim or t.get_device() != self._dev or \
+                (dtype is not None and t.dtype is not dtype) or \
+                (shape[0] and (st[2] != 1 or (st[1] != shape[2] and shape[1] > 1))):
+            raise PBError(-1, "%s: a tensor [row][head][%d]%s on %s with contiguous rows, q and out alike" % (
                 what, self.head_dim, " of %s" % dtype if dtype else "", self.device))
-        return t.data_ptr()
+        return t.data_ptr(), st[0] if shape[0] > 1 else shape[1] * shape[2]
+
+    def _table(self, what, t, n):
+        """(pointer, width) of a table for n sequences"""
+        shape = t.shape
+        if len(shape) != 2 or shape[0] != n:
+            raise PBError(-1, "%s: a tensor [%d][pages]" % (what, n))
+        return self._ints(what, t, shape), shape[1]
 
     def _floats(self, what, t, shape):
-        if t is None:
-            return None
-        if t.dtype != self._float32 or t.device != self.device or tuple(t.shape) != shape or not t.is_contiguous():
+        if t.dtype is not self._f32 or t.get_device() != self._dev or t.shape != shape or not t.is_contiguous():
             raise PBError(-1, "%s: a contiguous fp32 tensor %s on %s" % (what, list(shape), self.device))
         return t.data_ptr()
 
-    @property
-    def _int32(self):
-        import torch
-        return torch.int32
-
-    @property
-    def _float32(self):
-        import torch
-        return torch.float32
-
     def _call(self, fn, args, need, scratch, stream):
-        """fn(*args, scratch, bytes, stream) on the pools' device; need < 0: a function without scratch"""
-        import torch
-        dev = self.device.index
-        if torch.cuda.current_device() != dev:
+        """fn(*args[, scratch, bytes], stream) on the pools' device; need None: a function without scratch"""
+        torch, dev = self._torch, self._dev
+        if torch._C._cuda_getDevice() != dev:
             with torch.cuda.device(dev):
                 return self._call(fn, args, need, scratch, stream)
-        s = stream if stream is not None else torch.cuda.current_stream(dev)
-        if need < 0:
-            return check(fn(*args, s.cuda_stream))
-        if scratch is None and need > 0:
+        s = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
+        if need is None:
+            rc = fn(*args, s)
+        elif scratch is None and need > 0:
             if stream is None:
                 scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
             else:   # allocated on the stream that uses it, so that it is not reused under the call
                 with torch.cuda.stream(stream):
                     scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
-        if scratch is None:
-            return check(fn(*args, None, 0, s.cuda_stream))
-        if scratch.device != self.device or not scratch.is_contiguous():
-            raise PBError(-1, "scratch: a contiguous tensor on %s" % self.device)
-        return check(fn(*args, scratch.data_ptr(), scratch.numel() * scratch.element_size(), s.cuda_stream))
+            rc = fn(*args, scratch.data_ptr(), need, s)
+        elif scratch is None:
+            rc = fn(*args, None, 0, s)
+        else:
+            if scratch.get_device() != dev or not scratch.is_contiguous():
+                raise PBError(-1, "scratch: a contiguous tensor on %s" % self.device)
+            rc = fn(*args, scratch.data_ptr(), scratch.numel() * scratch.element_size(), s)
+        if rc:
+            check(rc)
+
+    def _bytes(self, fn, *shape):
+        # (a negative max_len or count, which the call itself refuses, needs no scratch)
+        need = self._need.get((fn.__name__, shape))
+        if need is None:
+            need = self._need[fn.__name__, shape] = fn(self._r, *shape)
+        return need
 
     def append(self, table, seq, slot, pos, qkv, q, q_norm=None, k_norm=None, eps=1e-5, cos=None, sin=None, stream=None):
         """norm and rotate the heads of qkv [n][>= (n_heads + 2 n_kv) dim] (bf16, fp16 or fp32), query heads to
         q [n][n_heads][dim] (the cache's dtype), K and V rows to row slot[i] of sequence seq[i]; pos: the rotation's
         position per token (None: slot); cos, sin [positions][half] (None: no rotation)"""
-        n, nh = q.shape[0], q.shape[1]
-        if qkv.dim() != 2 or qkv.shape[0] != n or qkv.device != self.device or (qkv.numel() and qkv.stride(1) != 1) or \
-                qkv.shape[1] < (nh + 2 * self.n_kv) * self.head_dim:
-            raise PBError(-1, "qkv: a tensor [%d][>= %d] on %s with contiguous rows" % (
-                n, (nh + 2 * self.n_kv) * self.head_dim, self.device))
+        shape = q.shape
+        qp, ldq = self._heads("q", q, shape, self.dtype)
+        n, nh = shape[0], shape[1]
+        wide = (nh + 2 * self.n_kv) * self.head_dim
+        xs, xt = qkv.shape, qkv.stride()
+        if len(xs) != 2 or xs[0] != n or xs[1] < wide or qkv.get_device() != self._dev or (n and xt[1] != 1):
+            raise PBError(-1, "qkv: a tensor [%d][>= %d] on %s with contiguous rows" % (n, wide, self.device))
         if (cos is None) != (sin is None):
             raise PBError(-1, "cos and sin go together")
-        half, n_rope = (cos.shape[1], cos.shape[0]) if cos is not None else (0, 0)
-        d = (self.head_dim,)
-        args = (self._r, table.shape[0], self._ints("table", table, 2), table.shape[1],
-                qkv.data_ptr(), _dtype_code(qkv), qkv.stride(0) if n > 1 else qkv.shape[1] // 8 * 8, n, nh,
-                self._ints("seq", seq, 1, n), self._ints("slot", slot, 1, n),
-                self._ints("pos", pos, 1, n) if pos is not None else None, self._floats("q_norm", q_norm, d),
-                self._floats("k_norm", k_norm, d), float(eps), self._floats("cos", cos, (n_rope, half)),
-                self._floats("sin", sin, (n_rope, half)), half, n_rope, self._heads("q", q, self.dtype),
-                q.stride(0) if n > 1 else nh * self.head_dim)
-        self._call(lib().pb_kv_append, args, -1, None, stream)
+        ns = len(table)
+        tp, pages = self._table("table", table, ns)
+        one, d = (n,), (self.head_dim,)
+        if cos is None:
+            rope = None, None, 0, 0
+        else:
+            cs = cos.shape
+            if len(cs) != 2:
+                raise PBError(-1, "cos: a tensor [positions][half]")
+            rope = self._floats("cos", cos, cs), self._floats("sin", sin, cs), cs[1], cs[0]
+        self._call(lib().pb_kv_append, (
+            self._r, ns, tp, pages, qkv.data_ptr(), _dtype_code(qkv), xt[0] if n > 1 else wide, n, nh,
+            self._ints("seq", seq, one), self._ints("slot", slot, one), None if pos is None else self._ints("pos", pos, one),
+            None if q_norm is None else self._floats("q_norm", q_norm, d),
+            None if k_norm is None else self._floats("k_norm", k_norm, d), eps, *rope, qp, ldq), None, None, stream)
 
     def decode(self, table, length, q, out, max_len=0, scale=None, window=0, sinks=0, accumulate=False, scratch=None,
                stream=None):
@@ -471,52 +488,46 @@ class KVPages:
         each cache, into out (bf16 or fp16, q's shape); scale: 1 / sqrt(dim) by default; accumulate: add each seen
         row's probabilities to the cache's weight"""
         L = lib()
-        n, nh = q.shape[0], q.shape[1]
-        args = self._attn_args(table, n, [self._ints("length", length, 1, n)], [], q, out, max_len, scale, window, sinks,
-                               [1 if accumulate else 0])
-        need = L.pb_kv_decode_scratch(self._r, n, max_len or table.shape[1] * self.page_size, nh, 1 if accumulate else 0)
-        self._call(L.pb_kv_decode, args, need, scratch, stream)
+        shape = q.shape
+        qp, ldq = self._heads("q", q, shape, self.dtype)
+        op, ldo = self._heads("out", out, shape, None)
+        n, nh, acc = shape[0], shape[1], 1 if accumulate else 0
+        tp, pages = self._table("table", table, n)
+        need = self._bytes(L.pb_kv_decode_scratch, n, min(max_len, pages * self.page_size) or pages * self.page_size, nh, acc)
+        self._call(L.pb_kv_decode, (
+            self._r, n, tp, pages, self._ints("length", length, (n,)), max_len, nh, qp, ldq,
+            self._scale if scale is None else scale, window, sinks, acc, op, _dtype_code(out), ldo), need, scratch, stream)
 
     def prefill(self, table, start, length, q, out, max_len=0, scale=None, window=0, sinks=0, scratch=None, stream=None):
         """attention of the last rows of each sequence: rows start[b] .. start[b+1]-1 of q [n][n_heads][dim] are the
         tokens at the last rows of sequence b, into out (bf16 or fp16, q's shape)"""
         L = lib()
-        n = length.shape[0]
-        args = self._attn_args(table, n, [self._ints("start", start, 1, n + 1), self._ints("length", length, 1, n)],
-                               [q.shape[0]], q, out, max_len, scale, window, sinks, [])
-        need = L.pb_kv_prefill_scratch(self._r, n, max_len or table.shape[1] * self.page_size, q.shape[0], q.shape[1])
-        self._call(L.pb_kv_prefill, args, need, scratch, stream)
+        shape = q.shape
+        qp, ldq = self._heads("q", q, shape, self.dtype)
+        op, ldo = self._heads("out", out, shape, None)
+        n, nt, nh = len(length), shape[0], shape[1]
+        tp, pages = self._table("table", table, n)
+        need = self._bytes(L.pb_kv_prefill_scratch, n, min(max_len, pages * self.page_size) or pages * self.page_size, nt, nh)
+        self._call(L.pb_kv_prefill, (
+            self._r, n, tp, pages, self._ints("start", start, (n + 1,)), self._ints("length", length, (n,)), max_len, nt, nh,
+            qp, ldq, self._scale if scale is None else scale, window, sinks, op, _dtype_code(out), ldo), need, scratch, stream)
 
     def status(self, stream=None):
         """synchronise and raise if a prefill kernel recorded a wait that gave up"""
-        import torch
-        with torch.cuda.device(self.device):
+        with self._torch.cuda.device(self.device):
             check(lib().pb_kv_status(_stream(stream)))
-
-    def _attn_args(self, table, n_seq, lens, rows, q, out, max_len, scale, window, sinks, more):
-        qp, op = self._heads("q", q, self.dtype), self._heads("out", out)
-        if out.shape != q.shape:
-            raise PBError(-1, "out: q's shape")
-        if table.shape[0] != n_seq:
-            raise PBError(-1, "table: a row for each of %d sequences" % n_seq)
-        n, nh, wide = q.shape[0], q.shape[1], q.shape[1] * self.head_dim
-        return (self._r, n_seq, self._ints("table", table, 2), table.shape[1], *lens, max_len,
-                *rows, nh, qp, q.stride(0) if n > 1 else wide, self.head_dim ** -0.5 if scale is None else scale, window,
-                sinks, *more, op, _dtype_code(out), out.stride(0) if n > 1 else wide)
 
     def evict(self, table, length, dst_table, new_length, budget, sinks=0, recent=0, max_len=0, scratch=None, stream=None):
         """keep up to `budget` rows of each sequence and K/V head (the first `sinks`, the last `recent`, then the
         largest weights), moved in order to the pages of dst_table; new_length (may be length) receives the lengths"""
         L = lib()
-        n = length.shape[0]
-        if table.shape[0] != n or dst_table.shape[0] != n:
-            raise PBError(-1, "table, dst_table: a row for each of %d sequences" % n)
-        args = (self._r, n, self._ints("table", table, 2), table.shape[1],
-                self._ints("length", length, 1, n), max_len, self._ints("dst_table", dst_table, 2),
-                dst_table.shape[1], self._ints("new_length", new_length, 1, n), budget,
-                sinks, recent)
-        need = L.pb_kv_evict_scratch(self._r, n, max_len or table.shape[1] * self.page_size, budget)
-        self._call(L.pb_kv_evict, args, need, scratch, stream)
+        n = len(length)
+        tp, pages = self._table("table", table, n)
+        dp, fresh = self._table("dst_table", dst_table, n)
+        need = self._bytes(L.pb_kv_evict_scratch, n, min(max_len, pages * self.page_size) or pages * self.page_size, budget)
+        self._call(L.pb_kv_evict, (
+            self._r, n, tp, pages, self._ints("length", length, (n,)), max_len, dp, fresh,
+            self._ints("new_length", new_length, (n,)), budget, sinks, recent), need, scratch, stream)
 
 
 class Q1Tensor:
