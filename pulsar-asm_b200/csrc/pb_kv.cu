@@ -10,11 +10,15 @@ namespace {
 // i < half the pair (y_i, y_{i+D/2}) turned by the token's angle. All of it in
 // fp32 with one rounding at the store. V heads are only rounded.
 //
-// D / 8 lanes hold a head, 8 consecutive values each (16-byte loads and
-// stores); the partner of a lane's values is D / 16 lanes away, so the
-// rotation is one exchange by shuffle. A warp takes one token and every
-// parts-th group of heads, so the angles and the norm weights are read once
-// per warp.
+// Bytes bound it (each row in, each row out) as long as the instructions stay
+// few: D / 16 lanes hold a head, each 8 values and their 8 partners of the
+// rotation (16-byte loads and stores, nothing to exchange but the mean's
+// sum), a warp 4 (D 128) or 8 (D 64) heads at a time, two such groups' loads
+// in flight. A warp takes one token and every parts-th of its groups; its
+// angles stay in registers, the norm weights in shared memory. (One lane per 8
+// consecutive values, with shuffles for the partners, needed twice the
+// instructions: 74 us for 8191 tokens of 32/8 heads x 128 in bf16, now 43,
+// 4.8 TB/s; without any arithmetic 36.)
 struct AppendArgs {
   KvPool p;
   const char* x;
@@ -24,15 +28,14 @@ struct AppendArgs {
   const int* slot;
   const int* pos;          // null: the slot
   const float *qn, *kn, *cs, *sn;
-  int n_tok, nh, half, n_rope, rows, parts;
+  int n_tok, nh, half, n_rope, rows, parts, n_qk, n_groups;   // groups of query and key heads, and with those of value heads
   float eps;
 };
 
 template <int XT>
-struct KvRaw {
+struct KvRaw {             // 8 values
   uint4 a, b;
 };
-
 template <int XT>
 PB_DEV void ap_load(KvRaw<XT>& r, const char* p) {
   r.a = pb_ldg_stream(p);
@@ -53,17 +56,74 @@ PB_DEV void ap_up(const KvRaw<XT>& r, float (&x)[8]) {
     }
   }
 }
+template <int CT>
+PB_DEV uint4 ap_down(const float (&y)[8]) {
+  return make_uint4(kv_down<CT>(y[0], y[1]), kv_down<CT>(y[2], y[3]), kv_down<CT>(y[4], y[5]), kv_down<CT>(y[6], y[7]));
+}
+PB_DEV void ap_floats(const float* p, int n, float past, float (&o)[8]) {   // p[0 .. 7], `past` from n on
+  if (n >= 8 && (reinterpret_cast<size_t>(p) & 15) == 0) {
+    const float4 x = __ldg(reinterpret_cast<const float4*>(p)), y = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    o[0] = x.x; o[1] = x.y; o[2] = x.z; o[3] = x.w; o[4] = y.x; o[5] = y.y; o[6] = y.z; o[7] = y.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) o[i] = i < n ? __ldg(p + i) : past;
+  }
+}
+
+
+// packed pairs of fp32 (each operation rounds on its own)
+typedef unsigned long long ap_f2;
+PB_DEV ap_f2 ap_pk(float a, float b) {
+  ap_f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+PB_DEV void ap_upk(ap_f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+PB_DEV ap_f2 ap_fma2(ap_f2 a, ap_f2 b, ap_f2 c) {
+  ap_f2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+PB_DEV ap_f2 ap_mul2(ap_f2 a, ap_f2 b) {
+  ap_f2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 
 constexpr int AP_W = 8;    // warps per CTA
-constexpr int AP_U = 4;    // head groups whose loads are in flight together
+constexpr int AP_U = 2;    // groups whose loads are in flight together
 
 template <int D, int XT, int CT>
-__global__ void __launch_bounds__(32 * AP_W) k_kv_append(AppendArgs a) {
-  constexpr int LPH = D / 8, HPW = 32 / LPH, XB = XT == PB_DT_F32 ? 4 : 2;
-  const int lane = threadIdx.x & 31, l = lane % LPH, sub = lane / LPH;
+__global__ void __launch_bounds__(32 * AP_W, XT == PB_DT_F32 ? 3 : 4) k_kv_append(AppendArgs a) {
+  constexpr int L = D / 16, HPW = 32 / L, XB = XT == PB_DT_F32 ? 4 : 2;
+  __shared__ __align__(16) float nw[2][D];   // the norms' weights, of queries and of keys
+  for (int i = threadIdx.x; i < 2 * D; i += 32 * AP_W) {
+    const float* w = i < D ? a.qn : a.kn;
+    nw[i / D][i % D] = w ? __ldg(w + i % D) : 1.0f;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L;
   const long long unit = (long long)blockIdx.x * AP_W + (threadIdx.x >> 5);
   const int t = (int)(unit / a.parts), part = (int)(unit % a.parts);
   if (t >= a.n_tok) return;
+  const int nk = a.p.n_kv;
+  const char* x0 = a.x + (long long)t * a.ldx + l * 8 * XB;
+  // head of this lane in group g: query and key heads, then (from n_qk on) value heads
+  auto head = [&](int g) { return g < a.n_qk ? g * HPW + sub : a.nh + nk + (g - a.n_qk) * HPW + sub; };
+  auto live = [&](int g, int h) { return g < a.n_groups && h < (g < a.n_qk ? a.nh + nk : a.nh + 2 * nk); };
+  KvRaw<XT> lo[AP_U], hi[AP_U];
+  auto fetch = [&](int g, int u) {
+    const int h = head(g);
+    if (live(g, h)) {
+      ap_load<XT>(lo[u], x0 + (size_t)h * (D * XB));
+      ap_load<XT>(hi[u], x0 + (size_t)h * (D * XB) + D / 2 * XB);
+    } else {
+      lo[u].a = lo[u].b = hi[u].a = hi[u].b = make_uint4(0, 0, 0, 0);
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < AP_U; u++) fetch(part + u * a.parts, u);   // before the look-ups of the destination
+
   const int seq = __ldg(a.seq + t), slot = __ldg(a.slot + t), pos = a.pos ? __ldg(a.pos + t) : slot;
   if ((unsigned)seq >= (unsigned)a.p.n_seq || (unsigned)slot >= (unsigned)a.rows) return;
   if (a.half > 0 && (unsigned)pos >= (unsigned)a.n_rope) return;
@@ -71,81 +131,70 @@ __global__ void __launch_bounds__(32 * AP_W) k_kv_append(AppendArgs a) {
   if (page < 0) return;
   const int row = slot & ((1 << a.p.shift) - 1);
   const long long at = (long long)page * a.p.ps + (long long)row * a.p.rs + l * 16;
+  char* q0 = a.q + (long long)t * a.ldq + l * 16;
+  float c[8], s[8];        // of pairs 8l .. 8l + 7
+  ap_floats(a.cs + (size_t)pos * a.half + 8 * l, a.half - 8 * l, 1.0f, c);
+  ap_floats(a.sn + (size_t)pos * a.half + 8 * l, a.half - 8 * l, 0.0f, s);
+  const bool whole = a.half == D / 2;
 
-  // this lane's angles (both lanes of a pair hold the same ones): index
-  // i = 8l mod D/2; past `half` the angle is zero
-  float c[8], s[8];
-  const int i0 = (8 * l) % (D / 2);
-  const float *cp = a.cs + (size_t)pos * a.half + i0, *sp = a.sn + (size_t)pos * a.half + i0;
-  if (a.half == D / 2 && (reinterpret_cast<size_t>(a.cs) & 15) == 0 && (reinterpret_cast<size_t>(a.sn) & 15) == 0) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      const float4 x = __ldg(reinterpret_cast<const float4*>(cp + i)), y = __ldg(reinterpret_cast<const float4*>(sp + i));
-      c[i] = x.x; c[i + 1] = x.y; c[i + 2] = x.z; c[i + 3] = x.w;
-      s[i] = y.x; s[i + 1] = y.y; s[i + 2] = y.z; s[i + 3] = y.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const bool in = i0 + i < a.half;
-      c[i] = in ? __ldg(cp + i) : 1.0f;
-      s[i] = in ? __ldg(sp + i) : 0.0f;
-    }
-  }
-  const bool upper = 8 * l >= D / 2;   // the second of each pair: y' = y c + partner s; the first: y c - partner s
-#pragma unroll
-  for (int i = 0; i < 8; i++) s[i] = upper ? s[i] : -s[i];
-  float qw[8], kw[8];
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    qw[i] = a.qn ? __ldg(a.qn + 8 * l + i) : 1.0f;
-    kw[i] = a.kn ? __ldg(a.kn + 8 * l + i) : 1.0f;
-  }
-
-  const int nk = a.p.n_kv, all = a.nh + 2 * nk, step = a.parts * HPW;
-  const char* x0 = a.x + (long long)t * a.ldx + (size_t)(l * 8 * XB);
-  for (int h0 = part * HPW; h0 < all; h0 += AP_U * step) {
-    KvRaw<XT> raw[AP_U];
+  for (int g0 = part; g0 < a.n_groups; g0 += AP_U * a.parts) {
 #pragma unroll
     for (int u = 0; u < AP_U; u++) {
-      const int h = h0 + u * step + sub;
-      if (h < all) ap_load<XT>(raw[u], x0 + (size_t)h * (D * XB));
-      else raw[u].a = raw[u].b = make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int u = 0; u < AP_U; u++) {
-      if (h0 + u * step >= all) break;   // warp-uniform
-      const int h = h0 + u * step + sub;
-      const bool isq = h < a.nh, isv = h >= a.nh + nk;
-      float x[8];
-      ap_up<XT>(raw[u], x);
-      float ss = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; i++) ss = __fmaf_rn(x[i], x[i], ss);
-#pragma unroll
-      for (int o = 1; o < LPH; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const bool norm = isq ? a.qn != nullptr : (!isv && a.kn != nullptr);
-      const float r = norm ? __fdiv_rn(1.0f, __fsqrt_rn(ss * (1.0f / D) + a.eps)) : 1.0f;
-      float y[8];
-#pragma unroll
-      for (int i = 0; i < 8; i++) y[i] = isv ? x[i] : x[i] * r * (isq ? qw[i] : kw[i]);
-      if (a.half > 0) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float o = __shfl_xor_sync(0xffffffffu, y[i], LPH / 2);
-          if (!isv && i0 + i < a.half) y[i] = __fmaf_rn(o, s[i], y[i] * c[i]);
-        }
+      const int g = g0 + u * a.parts;
+      if (g >= a.n_groups) break;      // warp-uniform
+      const int h = head(g);
+      const bool on = live(g, h);
+      float x[8], y[8];
+      ap_up<XT>(lo[u], x);
+      ap_up<XT>(hi[u], y);
+      fetch(g + AP_U * a.parts, u);    // the slot's next group
+      if (g >= a.n_qk) {
+        if (!on) continue;
+        const int kh = h - a.nh - nk;
+        char* v = a.p.v + at + (long long)kh * a.p.hs;
+        *reinterpret_cast<uint4*>(v) = ap_down<CT>(x);
+        *reinterpret_cast<uint4*>(v + D) = ap_down<CT>(y);
+        if (a.p.w && l == 0) a.p.w[((size_t)page * nk + kh) * (1 << a.p.shift) + row] = 0.0f;
+        continue;
       }
-      if (h >= all) continue;
-      const uint4 w = make_uint4(kv_down<CT>(y[0], y[1]), kv_down<CT>(y[2], y[3]), kv_down<CT>(y[4], y[5]),
-                                 kv_down<CT>(y[6], y[7]));
-      if (isq) {
-        *reinterpret_cast<uint4*>(a.q + (long long)t * a.ldq + (size_t)h * (D * 2) + l * 16) = w;
-      } else {
-        const int kh = isv ? h - a.nh - nk : h - a.nh;
-        *reinterpret_cast<uint4*>((isv ? a.p.v : a.p.k) + at + (long long)kh * a.p.hs) = w;
-        if (isv && a.p.w && l == 0) a.p.w[((size_t)page * nk + kh) * (1 << a.p.shift) + row] = 0.0f;
+      const bool isq = h < a.nh;
+      ap_f2 X[4], Y[4], sq = 0ull;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        X[i] = ap_pk(x[2 * i], x[2 * i + 1]);
+        Y[i] = ap_pk(y[2 * i], y[2 * i + 1]);
+        sq = ap_fma2(X[i], X[i], ap_fma2(Y[i], Y[i], sq));
       }
+      float ss, s1;
+      ap_upk(sq, ss, s1);
+      ss += s1;
+#pragma unroll
+      for (int o = 1; o < L; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float r = (isq ? a.qn : a.kn) ? rsqrtf(ss * (1.0f / D) + a.eps) : 1.0f;
+      const ap_f2 R = ap_pk(r, r);
+      const ulonglong2* wl = reinterpret_cast<const ulonglong2*>(nw[isq ? 0 : 1] + 8 * l);
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const ulonglong2 w = wl[i], z = wl[i + D / 8];
+        X[2 * i] = ap_mul2(X[2 * i], ap_mul2(R, w.x)); X[2 * i + 1] = ap_mul2(X[2 * i + 1], ap_mul2(R, w.y));
+        Y[2 * i] = ap_mul2(Y[2 * i], ap_mul2(R, z.x)); Y[2 * i + 1] = ap_mul2(Y[2 * i + 1], ap_mul2(R, z.y));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const ap_f2 C = ap_pk(c[2 * i], c[2 * i + 1]), S = ap_pk(s[2 * i], s[2 * i + 1]), T = ap_pk(-s[2 * i], -s[2 * i + 1]);
+        const ap_f2 n0 = ap_fma2(Y[i], T, ap_mul2(X[i], C)), n1 = ap_fma2(X[i], S, ap_mul2(Y[i], C));
+        float p, q, v, w;
+        ap_upk(X[i], x[2 * i], x[2 * i + 1]);
+        ap_upk(Y[i], y[2 * i], y[2 * i + 1]);
+        ap_upk(n0, p, q);
+        ap_upk(n1, v, w);
+        if (whole || 8 * l + 2 * i < a.half) { x[2 * i] = p; y[2 * i] = v; }
+        if (whole || 8 * l + 2 * i + 1 < a.half) { x[2 * i + 1] = q; y[2 * i + 1] = w; }
+      }
+      if (!on) continue;
+      char* o = isq ? q0 + (size_t)h * (D * 2) : a.p.k + at + (long long)(h - a.nh) * a.p.hs;
+      *reinterpret_cast<uint4*>(o) = ap_down<CT>(x);
+      *reinterpret_cast<uint4*>(o + D) = ap_down<CT>(y);
     }
   }
 }
@@ -407,11 +456,15 @@ extern "C" int pb_kv_append(const pb_kv_pages* c, int n_seq, const int* d_table,
   a.n_tok = n_tok; a.nh = n_heads; a.half = half; a.n_rope = n_rope;
   a.rows = table_ld * c->page_size;
   a.eps = eps;
-  // few tokens: a warp per group of heads; many: a warp per token
-  const int groups = (int)((n_heads + 2 * c->n_kv + 256 / D - 1) / (256 / D));
-  const long long per = (long long)n_tok * groups / ((long long)pb_num_sms() * 48);
-  const int iters = per < 1 ? 1 : (per > groups ? groups : (int)per);
-  a.parts = (groups + iters - 1) / iters;
+  // few tokens: a warp per group of heads; many: up to 6 groups a warp (12,
+  // a whole token of 48 heads, left a longer tail: 47 against 43 us; 1 paid
+  // the look-ups each time: 81)
+  const int hpw = 512 / D, nk = c->n_kv;
+  a.n_qk = (n_heads + nk + hpw - 1) / hpw;
+  a.n_groups = a.n_qk + (nk + hpw - 1) / hpw;
+  const long long per = (long long)n_tok * a.n_groups / ((long long)pb_num_sms() * 24);
+  const int iters = per < 1 ? 1 : (per > 6 ? 6 : (int)per);
+  a.parts = (a.n_groups + iters - 1) / iters;
   const long long blocks = ((long long)n_tok * a.parts + AP_W - 1) / AP_W;
   if (blocks > INT_MAX) return pb_set_error(PB_EINVAL, "pb_kv_append: %d tokens", n_tok);
   const dim3 grid((unsigned)blocks);

@@ -359,17 +359,23 @@ __global__ void __launch_bounds__(32 * DC_W, 2) k_kv_decode(DcArgs d) {
   kv_cp_wait<0>();
 }
 
-// one CTA per sequence and K/V head: the pieces of a group that was cut
+// One CTA per sequence and K/V head joins the pieces of a group that was cut,
+// in the order of the line: the pieces' factors first (a warp per head), then
+// the sums, a float4 per thread, with many pieces' loads in flight.
+constexpr int JN_T = 128;
+
 template <int D>
-__global__ void __launch_bounds__(128) k_kv_join(DcArgs d) {
+__global__ void __launch_bounds__(JN_T) k_kv_join(DcArgs d) {
   const AttnKvArgs& a = d.a;
   constexpr int TILE = DcGeo<D>::TILE;
-  const int b = blockIdx.x / a.p.n_kv, kh = blockIdx.x % a.p.n_kv;
-  __shared__ int wsum[4][2];
+  extern __shared__ float fac[];      // [head][piece]
+  __shared__ float inv[16];
+  __shared__ int wsum[JN_T / 32][2];
+  const int b = blockIdx.x / a.p.n_kv, kh = blockIdx.x % a.p.n_kv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pb_grid_launch_dependents();
   // tiles of the sequences before b, and of all
   int pre = 0, total = 0;
-  for (int i = threadIdx.x; i < a.p.n_seq; i += 128) {
+  for (int i = threadIdx.x; i < a.p.n_seq; i += JN_T) {
     const int n = dc_seq<TILE>(a, i).nt;
     total += n;
     if (i < b) pre += n;
@@ -379,46 +385,66 @@ __global__ void __launch_bounds__(128) k_kv_join(DcArgs d) {
     pre += __shfl_xor_sync(0xffffffffu, pre, o);
     total += __shfl_xor_sync(0xffffffffu, total, o);
   }
-  if ((threadIdx.x & 31) == 0) { wsum[threadIdx.x >> 5][0] = pre; wsum[threadIdx.x >> 5][1] = total; }
+  if (lane == 0) { wsum[warp][0] = pre; wsum[warp][1] = total; }
   __syncthreads();
-  pre = (wsum[0][0] + wsum[1][0] + wsum[2][0] + wsum[3][0]) * a.p.n_kv;
-  total = (wsum[0][1] + wsum[1][1] + wsum[2][1] + wsum[3][1]) * a.p.n_kv;
+  pre = total = 0;
+#pragma unroll
+  for (int w = 0; w < JN_T / 32; w++) { pre += wsum[w][0]; total += wsum[w][1]; }
+  pre *= a.p.n_kv;
+  total *= a.p.n_kv;
   const int nt = dc_seq<TILE>(a, b).nt, s = pre + kh * nt;
   const int pieces = dc_pieces(d, total);
-  const int w0 = dc_piece(s, total, pieces), w1 = dc_piece(s + nt - 1, total, pieces);
+  const int w0 = dc_piece(s, total, pieces), np = dc_piece(s + nt - 1, total, pieces) - w0 + 1;
   pb_grid_wait();
-  if (w0 == w1) return;     // whole: written by its CTA
-  for (int i = threadIdx.x; i < a.grp * (D / 4); i += 128) {
-    const int h = i / (D / 4), e = (i % (D / 4)) * 4;
+  if (np == 1) return;     // whole: written by its CTA
+  // piece k of this group lies in slot 2 (w0 + k), the first one in 2 w0 + 1
+  for (int h = warp; h < a.grp; h += JN_T / 32) {
     float mm = -INFINITY, ll = 0.0f;
-    for (int w = w0; w <= w1; w++) mm = fmaxf(mm, __ldcg(d.ml + ((size_t)(2 * w + (w == w0)) * a.grp + h) * 2));
+    for (int k = lane; k < np; k += 32) mm = fmaxf(mm, __ldcg(d.ml + ((size_t)(2 * (w0 + k) + (k == 0)) * a.grp + h) * 2));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
     const float r = mm == -INFINITY ? 0.0f : mm;
-    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int w = w0; w <= w1; w++) {
-      const size_t at = (size_t)(2 * w + (w == w0)) * a.grp + h;
-      const float2 q = __ldcg(reinterpret_cast<const float2*>(d.ml + at * 2));
-      const float4 z = __ldcg(reinterpret_cast<const float4*>(d.part + at * D + e));
+    for (int k = lane; k < np; k += 32) {
+      const float2 q = __ldcg(reinterpret_cast<const float2*>(d.ml + ((size_t)(2 * (w0 + k) + (k == 0)) * a.grp + h) * 2));
       const float f = kv_ex2(q.x - r);
+      fac[h * np + k] = f;
       ll += f * q.y;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+    if (lane == 0) {
+      inv[h] = ll != 0.0f ? 1.0f / ll : 0.0f;
+      if (a.lse) a.lse[(size_t)b * a.nh + kh * a.grp + h] = mm + log2f(ll);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.grp * (D / 4); i += JN_T) {
+    const int h = i / (D / 4), e = (i % (D / 4)) * 4;
+    float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int k = 0; k < np; k++) {
+      const float4 z = __ldcg(reinterpret_cast<const float4*>(d.part + ((size_t)(2 * (w0 + k) + (k == 0)) * a.grp + h) * D + e));
+      const float f = fac[h * np + k];
       y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
     }
-    const float f = ll != 0.0f ? 1.0f / ll : 0.0f;
+    const float f = inv[h];
     dc_store<D>(d, b, kh * a.grp + h, e, make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
-    if (a.lse && e == 0) a.lse[(size_t)b * a.nh + kh * a.grp + h] = mm + log2f(ll);
   }
 }
 
-// the weights: a thread per seen row and K/V head adds the row's
-// probabilities under the heads of the group, from the kept scores; the same
-// line of tiles and the same cuts as the attention
+// The weights: a thread per seen row and K/V head adds the row's
+// probabilities under the heads of the group, from the kept scores. The same
+// line of tiles, in finer pieces: its few loads depend on one another, so it
+// takes many small CTAs (one piece per CTA of the attention: 46 us for 16
+// sequences of 2048 to 4352 rows, 32/8 heads x 128; now X).
 template <int D>
-__global__ void __launch_bounds__(128) k_kv_weight(DcArgs d) {
+__global__ void __launch_bounds__(DcGeo<D>::TILE) k_kv_weight(DcArgs d) {
   constexpr int TILE = DcGeo<D>::TILE;
   const AttnKvArgs& a = d.a;
   int total, b, first;
-  kv_locate<128>(a.p.n_seq, [&](int i) { return dc_seq<TILE>(a, i).nt * a.p.n_kv; }, [&](int n) { return dc_cut(blockIdx.x, n, dc_pieces(d, n)); }, total, b, first);
-  const int pieces = dc_pieces(d, total);
-  pb_grid_wait();
+  kv_locate<TILE>(a.p.n_seq, [&](int i) { return dc_seq<TILE>(a, i).nt * a.p.n_kv; },
+                  [&](int n) { return dc_cut(blockIdx.x, n, min(n, (int)gridDim.x)); }, total, b, first);
+  const int pieces = min(total, (int)gridDim.x);
   if ((int)blockIdx.x >= pieces) return;
   const int x0 = dc_cut(blockIdx.x, total, pieces), x1 = dc_cut(blockIdx.x + 1, total, pieces);
   DcAt at;
@@ -426,17 +452,23 @@ __global__ void __launch_bounds__(128) k_kv_weight(DcArgs d) {
   at.s = dc_seq<TILE>(a, b);
   at.kh = (x0 - first) / at.s.nt;
   at.t = (x0 - first) % at.s.nt;
+  pb_grid_wait();
   for (int x = x0; x < x1; x++, dc_next<TILE>(a, at)) {
-    if (threadIdx.x >= TILE) continue;
     const int j = (at.t < at.s.nst ? at.t : at.t - at.s.nst + at.s.lot) * TILE + threadIdx.x;
     if (j >= at.s.len || (j < at.s.lo && j >= at.s.sinks)) continue;
     const int page = kv_page(a.p, a.p.table + (size_t)at.b * a.p.table_ld, j);
     if (page < 0) continue;
+    float* w = a.p.w + ((size_t)page * a.p.n_kv + at.kh) * (1 << a.p.shift) + (j & ((1 << a.p.shift) - 1));
     const float* sp = d.score + (((size_t)at.b * a.p.n_kv + at.kh) * a.max_len + j) * d.grp2;
     const float* lp = a.lse + (size_t)at.b * a.nh + at.kh * a.grp;
+    const float was = *w;
     float sum = 0.0f;
-    for (int h = 0; h < a.grp; h++) sum += kv_ex2(__ldcg(sp + h) - __ldcg(lp + h));
-    a.p.w[((size_t)page * a.p.n_kv + at.kh) * (1 << a.p.shift) + (j & ((1 << a.p.shift) - 1))] += sum;
+    for (int h = 0; h < a.grp; h += 2) {
+      const float2 s = __ldcg(reinterpret_cast<const float2*>(sp + h));
+      sum += kv_ex2(s.x - __ldcg(lp + h));
+      if (h + 1 < a.grp) sum += kv_ex2(s.y - __ldcg(lp + h + 1));
+    }
+    *w = was + sum;
   }
 }
 
@@ -480,8 +512,14 @@ int dc_run(const DcArgs& d, int ct, bool join, cudaStream_t st) {
   if (ct == PB_DT_F16) rc = two ? dc_launch<D, PB_DT_F16, 2>(d, st) : dc_launch<D, PB_DT_F16, 1>(d, st);
   else rc = two ? dc_launch<D, PB_DT_BF16, 2>(d, st) : dc_launch<D, PB_DT_BF16, 1>(d, st);
   if (rc) return rc;
-  if (join && (rc = kv_launch(k_kv_join<D>, (unsigned)(d.a.p.n_seq * d.a.p.n_kv), 128, 0, st, true, "k_kv_join", d))) return rc;
-  if (d.score) rc = kv_launch(k_kv_weight<D>, (unsigned)d.grid, 128, 0, st, true, "k_kv_weight", d);
+  // (a group's pieces: at most one per tile and per CTA)
+  const int tiles = (d.a.max_len + DcGeo<D>::TILE - 1) / DcGeo<D>::TILE, np = d.grid < tiles ? d.grid : tiles;
+  if (join && (rc = kv_launch(k_kv_join<D>, (unsigned)(d.a.p.n_seq * d.a.p.n_kv), JN_T, d.a.grp * np * 4, st, true, "k_kv_join", d)))
+    return rc;
+  if (d.score) {
+    const long long all = (long long)d.a.p.n_seq * d.a.p.n_kv * (tiles > 0 ? tiles : 1), cap = 32LL * pb_num_sms();
+    rc = kv_launch(k_kv_weight<D>, (unsigned)(all < cap ? all : cap), DcGeo<D>::TILE, 0, st, true, "k_kv_weight", d);
+  }
   return rc;
 }
 
