@@ -360,15 +360,20 @@ __global__ void __launch_bounds__(32 * DC_W, 2) k_kv_decode(DcArgs d) {
 }
 
 // One CTA per sequence and K/V head joins the pieces of a group that was cut,
-// in the order of the line: the pieces' factors first (a warp per head), then
-// the sums, a float4 per thread, with many pieces' loads in flight.
-constexpr int JN_T = 128;
+// always in the same order: the pieces' factors first (a warp per head), then
+// the sums, a float4 per thread; where a group has fewer of those than the CTA
+// threads, slices of the pieces go to the others, so that the loads of all
+// pieces are in flight at once (a thread per float4 alone took 11 us to join
+// 32 pieces). JN_T is 512 for few groups, 128 where the CTAs fill the GPU
+// several times and most groups are whole (64 x 8 groups: 33 against 35 us
+// for the whole call).
 
-template <int D>
+template <int D, int JN_T>
 __global__ void __launch_bounds__(JN_T) k_kv_join(DcArgs d) {
   const AttnKvArgs& a = d.a;
   constexpr int TILE = DcGeo<D>::TILE;
   extern __shared__ float fac[];      // [head][piece]
+  __shared__ float4 sum[JN_T];
   __shared__ float inv[16];
   __shared__ int wsum[JN_T / 32][2];
   const int b = blockIdx.x / a.p.n_kv, kh = blockIdx.x % a.p.n_kv, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -418,17 +423,31 @@ __global__ void __launch_bounds__(JN_T) k_kv_join(DcArgs d) {
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < a.grp * (D / 4); i += JN_T) {
+  const int items = a.grp * (D / 4), pass = min(items, JN_T), slices = JN_T / pass;
+  const int slice = threadIdx.x / pass;
+  for (int i = threadIdx.x % pass; i < items; i += pass) {      // one round, unless items > JN_T
     const int h = i / (D / 4), e = (i % (D / 4)) * 4;
     float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (slice < slices) {
+      const int k0 = np * slice / slices, k1 = np * (slice + 1) / slices;
 #pragma unroll 8
-    for (int k = 0; k < np; k++) {
-      const float4 z = __ldcg(reinterpret_cast<const float4*>(d.part + ((size_t)(2 * (w0 + k) + (k == 0)) * a.grp + h) * D + e));
-      const float f = fac[h * np + k];
-      y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
+      for (int k = k0; k < k1; k++) {
+        const float4 z = __ldcg(reinterpret_cast<const float4*>(d.part + ((size_t)(2 * (w0 + k) + (k == 0)) * a.grp + h) * D + e));
+        const float f = fac[h * np + k];
+        y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
+      }
+    }
+    if (slices > 1) {            // (one round then: every thread is here)
+      sum[threadIdx.x] = y;
+      __syncthreads();
+      if (slice == 0)
+        for (int s2 = 1; s2 < slices; s2++) {
+          const float4 z = sum[s2 * pass + i];
+          y.x += z.x; y.y += z.y; y.z += z.z; y.w += z.w;
+        }
     }
     const float f = inv[h];
-    dc_store<D>(d, b, kh * a.grp + h, e, make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
+    if (slice == 0) dc_store<D>(d, b, kh * a.grp + h, e, make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
   }
 }
 
@@ -514,8 +533,12 @@ int dc_run(const DcArgs& d, int ct, bool join, cudaStream_t st) {
   if (rc) return rc;
   // (a group's pieces: at most one per tile and per CTA)
   const int tiles = (d.a.max_len + DcGeo<D>::TILE - 1) / DcGeo<D>::TILE, np = d.grid < tiles ? d.grid : tiles;
-  if (join && (rc = kv_launch(k_kv_join<D>, (unsigned)(d.a.p.n_seq * d.a.p.n_kv), JN_T, d.a.grp * np * 4, st, true, "k_kv_join", d)))
-    return rc;
+  if (join) {
+    const unsigned groups = (unsigned)(d.a.p.n_seq * d.a.p.n_kv);
+    rc = (int)groups <= 2 * pb_num_sms() ? kv_launch(k_kv_join<D, 512>, groups, 512, d.a.grp * np * 4, st, true, "k_kv_join", d)
+                                         : kv_launch(k_kv_join<D, 128>, groups, 128, d.a.grp * np * 4, st, true, "k_kv_join", d);
+    if (rc) return rc;
+  }
   if (d.score) {
     const long long all = (long long)d.a.p.n_seq * d.a.p.n_kv * (tiles > 0 ? tiles : 1), cap = 32LL * pb_num_sms();
     rc = kv_launch(k_kv_weight<D>, (unsigned)(all < cap ? all : cap), DcGeo<D>::TILE, 0, st, true, "k_kv_weight", d);
