@@ -28,7 +28,8 @@ struct DcGeo {
   static constexpr int NB = KT / 16;             // 16-row blocks: one page each
   static constexpr int NS = 3;                   // ring stages per warp
   static constexpr int RING = DC_W * NS * 8192;
-  static constexpr int OP = D + 4;               // padded row of the merge buffer
+  static constexpr int OP = 64 + 4;              // padded row of the merge buffer: 64 columns at a time, so
+                                                 // that the join's CTAs fit beside two of these
   static constexpr int SMEM = RING + DC_W * 8 * OP * 4 + DC_W * 8 * 8;
 };
 
@@ -320,37 +321,48 @@ __global__ void __launch_bounds__(32 * DC_W, 2) k_kv_decode(DcArgs d) {
         for (int u = 0; u < 2; u++) {
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) l[n][u] += __shfl_xor_sync(0xffffffffu, l[n][u], w);
-          float* row = mo + (warp * 8 + 2 * c + u) * G::OP;
-#pragma unroll
-          for (int k = 0; k < D / 16; k++) { row[k * 16 + g] = o[n][k][u]; row[k * 16 + g + 8] = o[n][k][2 + u]; }
-          if (g == 0) { mml[(warp * 8 + 2 * c + u) * 2] = m[n][u]; mml[(warp * 8 + 2 * c + u) * 2 + 1] = l[n][u]; }
         }
-        __syncthreads();
-        for (int i = threadIdx.x; i < 8 * (D / 4); i += 32 * DC_W) {
-          const int h = i / (D / 4), e = (i % (D / 4)) * 4, hg = n * 8 + h;
-          if (hg >= a.grp) break;
-          float mm = -INFINITY, ll = 0.0f;
 #pragma unroll
-          for (int w = 0; w < DC_W; w++) mm = fmaxf(mm, mml[(w * 8 + h) * 2]);
-          const float r = mm == -INFINITY ? 0.0f : mm;
-          float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int half = 0; half < D / 64; half++) {
 #pragma unroll
-          for (int w = 0; w < DC_W; w++) {
-            const float f = kv_ex2(mml[(w * 8 + h) * 2] - r);
-            const float4 z = *reinterpret_cast<const float4*>(mo + (w * 8 + h) * G::OP + e);
-            ll += f * mml[(w * 8 + h) * 2 + 1];
-            y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
+          for (int u = 0; u < 2; u++) {
+            float* row = mo + (warp * 8 + 2 * c + u) * G::OP;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              row[k * 16 + g] = o[n][half * 4 + k][u];
+              row[k * 16 + g + 8] = o[n][half * 4 + k][2 + u];
+            }
+            if (g == 0) { mml[(warp * 8 + 2 * c + u) * 2] = m[n][u]; mml[(warp * 8 + 2 * c + u) * 2 + 1] = l[n][u]; }
           }
-          if (whole) {
-            const float f = ll != 0.0f ? 1.0f / ll : 0.0f;   // nothing seen: zeros
-            dc_store<D>(d, at.b, at.kh * a.grp + hg, e, make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
-            if (a.lse && e == 0) a.lse[(size_t)at.b * a.nh + at.kh * a.grp + hg] = mm + log2f(ll);
-          } else {
-            *reinterpret_cast<float4*>(d.part + ((size_t)slot_p * a.grp + hg) * D + e) = y;
-            if (e == 0) *reinterpret_cast<float2*>(d.ml + ((size_t)slot_p * a.grp + hg) * 2) = make_float2(mm, ll);
+          __syncthreads();
+          {
+            const int h = threadIdx.x / 16, e = (threadIdx.x % 16) * 4, hg = n * 8 + h;      // 8 heads x 16 float4
+            if (hg < a.grp) {
+              float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+              for (int w = 0; w < DC_W; w++) mm = fmaxf(mm, mml[(w * 8 + h) * 2]);
+              const float r = mm == -INFINITY ? 0.0f : mm;
+              float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+              for (int w = 0; w < DC_W; w++) {
+                const float f = kv_ex2(mml[(w * 8 + h) * 2] - r);
+                const float4 z = *reinterpret_cast<const float4*>(mo + (w * 8 + h) * G::OP + e);
+                ll += f * mml[(w * 8 + h) * 2 + 1];
+                y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
+              }
+              const bool first_of = half == 0 && e == 0;
+              if (whole) {
+                const float f = ll != 0.0f ? 1.0f / ll : 0.0f;   // nothing seen: zeros
+                dc_store<D>(d, at.b, at.kh * a.grp + hg, half * 64 + e, make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
+                if (a.lse && first_of) a.lse[(size_t)at.b * a.nh + at.kh * a.grp + hg] = mm + log2f(ll);
+              } else {
+                *reinterpret_cast<float4*>(d.part + ((size_t)slot_p * a.grp + hg) * D + half * 64 + e) = y;
+                if (first_of) *reinterpret_cast<float2*>(d.ml + ((size_t)slot_p * a.grp + hg) * 2) = make_float2(mm, ll);
+              }
+            }
           }
+          __syncthreads();
         }
-        __syncthreads();
       }
       fresh = true;
     }
