@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(32 * DC_W, 2) k_kv_decode(DcArgs d) {
     const int r = rr + i * RS;
     soff[i] = r * (D * 2) + ((cc ^ (r & 7)) << 4);
   }
+  const long long step = (long long)RS * a.p.rs, lane_off = (long long)rr * a.p.rs + cc * 16;
   DcAt ia = at;
   int ix = x0, islot = 0;
   unsigned vbits = 0;       // validity of the 16-row blocks in flight, newest lowest
@@ -166,17 +167,29 @@ __global__ void __launch_bounds__(32 * DC_W, 2) k_kv_decode(DcArgs d) {
         const bool ok = (unsigned)pg[n] < (unsigned)a.p.n_pages;
         vbits = (vbits << 1) | (ok ? 1u : 0u);
         const int j0 = j + n * 16;
-        const long long off = ok ? (long long)pg[n] * a.p.ps + (long long)ia.kh * a.p.hs +
-                                       (long long)((j0 & ((1 << a.p.shift) - 1)) + rr) * a.p.rs + cc * 16
-                                 : 0;
+        const uint32_t dst = st + n * (16 * D * 2);
+        const bool some = ok && j0 < ia.s.len;
+        const long long off = (some ? (long long)pg[n] * a.p.ps + (long long)(j0 & ((1 << a.p.shift) - 1)) * a.p.rs : 0) +
+                              (long long)ia.kh * a.p.hs + lane_off;
         const char *kp = a.p.k + off, *vp = a.p.v + off;
+        if (some && j0 + 16 <= ia.s.len && (j0 >= ia.s.lo || j0 + 16 <= ia.s.sinks)) {   // all 16 rows: no tests, no sizes
 #pragma unroll
-        for (int i = 0; i < 16 / RS; i++) {
-          const int r = j0 + rr + i * RS;
-          const bool in = ok && r < ia.s.len && (r >= ia.s.lo || r < ia.s.sinks);
-          const long long o = in ? (long long)(i * RS) * a.p.rs : 0;
-          kv_cp16(st + n * (16 * D * 2) + soff[i], kp + o, in);
-          kv_cp16(st + 4096 + n * (16 * D * 2) + soff[i], vp + o, in);
+          for (int i = 0; i < 16 / RS; i++) {
+            kv_cp16(dst + soff[i], kp);
+            kv_cp16(dst + 4096 + soff[i], vp);
+            kp += step;
+            vp += step;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16 / RS; i++) {
+            const int r = j0 + rr + i * RS;
+            const bool in = ok && r < ia.s.len && (r >= ia.s.lo || r < ia.s.sinks);
+            kv_cp16(dst + soff[i], in ? kp : a.p.k, in);
+            kv_cp16(dst + 4096 + soff[i], in ? vp : a.p.v, in);
+            kp += step;
+            vp += step;
+          }
         }
       }
       if (++ix < x1) {

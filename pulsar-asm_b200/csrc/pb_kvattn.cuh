@@ -73,6 +73,9 @@ PB_DEV uint32_t kv_s32(const void* p) { return (uint32_t)__cvta_generic_to_share
 PB_DEV void kv_cp16(uint32_t dst, const char* src, bool in) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
+PB_DEV void kv_cp16(uint32_t dst, const char* src) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 template <int N>
 PB_DEV void kv_cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 PB_DEV void kv_cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
