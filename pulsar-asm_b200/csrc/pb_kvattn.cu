@@ -26,7 +26,9 @@ struct DcGeo {
   static constexpr int KT = 2048 / D;            // rows per warp and tile: 4 KB of K, 4 KB of V
   static constexpr int TILE = DC_W * KT;         // rows per tile
   static constexpr int NB = KT / 16;             // 16-row blocks: one page each
-  static constexpr int NS = 3;                   // ring stages per warp
+  static constexpr int NS = 2;                   // ring stages per warp: with 3 CTAs an SM faster than 3 stages and 2 CTAs
+                                                 // (64 ragged: 29.7 against 32.1 us, long: 138 against 146): a warp's step is
+                                                 // a chain of some 3000 cycles, which other warps have to fill
   static constexpr int RING = DC_W * NS * 8192;
   static constexpr int OP = 64 + 4;              // padded row of the merge buffer: 64 columns at a time, so
                                                  // that the join's CTAs fit beside two of these
@@ -115,7 +117,7 @@ PB_DEV void dc_store(const DcArgs& d, int b, int h, int e, const float4& x) {
 }
 
 template <int D, int CT, int NT>
-__global__ void __launch_bounds__(32 * DC_W, 2) k_kv_decode(DcArgs d) {
+__global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs d) {
   typedef DcGeo<D> G;
   constexpr int KT = G::KT, TILE = G::TILE, NB = G::NB, NS = G::NS, CPR = D / 8, RS = 32 / CPR;
   extern __shared__ __align__(128) char dsm[];
@@ -526,7 +528,7 @@ template <int D>
 DcPlan dc_plan_t(int n_seq, int n_kv, int max_len, int grp, int accumulate) {
   DcPlan p{};
   const long long most = (max_len + DcGeo<D>::TILE - 1) / DcGeo<D>::TILE, items = (long long)n_seq * n_kv;
-  const long long all = items * (most > 0 ? most : 1), cap = 2LL * pb_num_sms();
+  const long long all = items * (most > 0 ? most : 1), cap = (grp > 8 ? 2LL : 3LL) * pb_num_sms();
   p.grid = (int)(all < cap ? all : cap);
   p.grp2 = (grp + 1) / 2 * 2;
   // a sequence of one tile cannot be cut
