@@ -7,7 +7,7 @@
 // exponential per pair and head (16 per clock and SM: as long as the matrix
 // products at D = 128, twice as long at D = 64). So both have to run at once:
 //  - a CTA takes up to 256 rows of one K/V head, in two groups of 128: a row
-//    is a token and one of the heads of the group, so that short chunks fill
+//    is one of the heads of the group and a token, so that short chunks fill
 //    the tiles and a K/V tile serves all heads at once. Key tiles are 64 rows.
 //  - per group, the scores S = Q K^T of a tile go to one of two TMEM buffers;
 //    128 threads (a row each) turn them into probabilities, in place, while
@@ -33,17 +33,20 @@
 namespace {
 
 constexpr int PF_KT = 64;                 // key rows per tile
-constexpr int PF_T = 12 * 32;
 constexpr int PF_MMA = 2;                 // the warp that issues the first group's products, the next one the second's
 constexpr unsigned long long PF_WAIT_NS = 1000000000ull;
 
-template <int D>
+// NG groups of 128 rows per CTA: 2, sharing every K/V tile, or 1 with two CTAs
+// an SM (see pf_plan)
+template <int D, int NG>
 struct PfGeo {
+  static constexpr int T = 128 + 128 * NG;        // threads
   static constexpr int Q = 128 * D * 2;           // bytes of a group's queries
   static constexpr int KV = PF_KT * D * 2;        // bytes of a K (or V) tile
-  static constexpr int NST = D == 128 ? 5 : 8;    // K/V stages
-  static constexpr int SMEM = 2 * Q + NST * 2 * KV + 1024;
-  static constexpr uint32_t O_COL = 256;          // S: group * 128 + buffer * 64; O: 256 + group * D
+  static constexpr int NST = NG == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 2 : 4);   // stages of the K ring, and of the V ring
+  static constexpr int SMEM = NG * Q + NST * 2 * KV + 1024;
+  static constexpr int COLS = NG * 256;           // TMEM columns allocated
+  static constexpr uint32_t O_COL = NG * 128;     // S: group * 128 + buffer * 64; O: O_COL + group * D
 };
 
 struct PfArgs {
@@ -134,10 +137,16 @@ PB_DEV void pf_ld32(uint32_t at, unsigned* v) {
                "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
                : PF_R8(v, 0), PF_R8(v, 8), PF_R8(v, 16), PF_R8(v, 24) : "r"(at));
 }
-PB_DEV void pf_st32(uint32_t at, const unsigned* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-               "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
-               ::PF_W8(v, 0), PF_W8(v, 8), PF_W8(v, 16), PF_W8(v, 24), "r"(at) : "memory");
+PB_DEV void pf_ld16(uint32_t at, unsigned* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : PF_R8(v, 0), PF_R8(v, 8) : "r"(at));
+}
+PB_DEV void pf_st16(uint32_t at, const unsigned* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+               ::PF_W8(v, 0), PF_W8(v, 8), "r"(at) : "memory");
+}
+PB_DEV void pf_st8(uint32_t at, const unsigned* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::PF_W8(v, 0), "r"(at) : "memory");
 }
 PB_DEV void pf_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 PB_DEV void pf_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -167,6 +176,10 @@ PB_DEV float pf_max3(float a, float b, float c) {   // NaN if any is
 }
 PB_DEV void pf_expect(uint64_t* b, unsigned bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(kv_s32(b)), "r"(bytes) : "memory");
+}
+PB_DEV void pf_tma2(uint32_t dst, const CUtensorMap* m, int c0, int c1, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               ::"r"(dst), "l"(m), "r"(c0), "r"(c1), "r"(kv_s32(bar)) : "memory");
 }
 PB_DEV void pf_tma(uint32_t dst, const CUtensorMap* m, int c0, int c1, int c2, int c3, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
@@ -201,70 +214,62 @@ PB_DEV unsigned long long pf_below(int x) { return x <= 0 ? 0ull : (x >= 64 ? ~0
 PB_DEV bool pf_edge(const PfLine& s, int k0) { return k0 + PF_KT > s.end || (k0 < s.lo && k0 + PF_KT > s.sinks); }
 PB_DEV int pf_key(const PfLine& s, int i) { return (i < s.nst ? i : i - s.nst + s.lot) * PF_KT; }
 
-template <int D>
-PB_DEV void pf_put(const PfArgs& p, int row, int h, int e, const float (&x)[8]) {
-  char* o = p.a.out + (long long)row * p.a.ldo + (size_t)h * (D * 2) + e * 2;
-  uint4 w;
-  if (p.out_bf16)
-    w = make_uint4(kv_down<PB_DT_BF16>(x[0], x[1]), kv_down<PB_DT_BF16>(x[2], x[3]), kv_down<PB_DT_BF16>(x[4], x[5]),
-                   kv_down<PB_DT_BF16>(x[6], x[7]));
-  else
-    w = make_uint4(kv_down<PB_DT_F16>(x[0], x[1]), kv_down<PB_DT_F16>(x[2], x[3]), kv_down<PB_DT_F16>(x[4], x[5]),
-                   kv_down<PB_DT_F16>(x[6], x[7]));
-  *reinterpret_cast<uint4*>(o) = w;
-}
-
-template <int D, int CT>
-__global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, PfArgs p) {
-  typedef PfGeo<D> G;
+template <int D, int CT, int NG>
+__global__ void __launch_bounds__(PfGeo<D, NG>::T, NG == 1 ? 2 : 1) k_kv_prefill(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mq,
+             PfArgs p) {
+  typedef PfGeo<D, NG> G;
   constexpr int NST = G::NST, KP = PF_KT * 128, QP = 128 * 128;   // bytes of a 64-column panel of K or V, of Q
   extern __shared__ __align__(128) char psm_raw[];
-  __shared__ uint64_t full[NST], empty[NST], sfull[2][2], pready[2][2], pvdone[2], ofin[2], lock[4], qfull, vfix[3], done[2];
+  __shared__ uint64_t kfull[NST], kempty[NST], vfull[NST], vempty[NST], sfull[NG][2], pready[NG][2], pvdone[NG], ofin[NG], lock[4], qfull, vfix[3], done[NG];
   __shared__ uint32_t tbase;
   __shared__ int stop_f;
   const AttnKvArgs& a = p.a;
   char* smq = psm_raw + ((1024u - (kv_s32(psm_raw) & 1023u)) & 1023u);
-  char* smk = smq + 2 * G::Q;
+  char* smk = smq + NG * G::Q;     // stage: K, V
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pb_grid_launch_dependents();
 
   // ---- which rows: the last tiles of the line (the longest keys) first
   const int split = blockIdx.x % p.ns, kh = blockIdx.x / p.ns % a.p.n_kv, idx = blockIdx.x / p.ns / a.p.n_kv;
   int total, b, first;
-  kv_locate<PF_T>(a.p.n_seq, [&](int i) { int s0; return (pf_count(a, i, s0) + 2 * p.tq - 1) / (2 * p.tq); },
+  kv_locate<G::T>(a.p.n_seq, [&](int i) { int s0; return (pf_count(a, i, s0) + NG * p.tq - 1) / (NG * p.tq); },
                   [&](int n) { return idx < n ? n - 1 - idx : n; }, total, b, first);
   if (idx >= total) return;   // CTA-uniform
   int row0;
-  const int cnt = pf_count(a, b, row0), tok0 = (total - 1 - idx - first) * 2 * p.tq, ntok = min(2 * p.tq, cnt - tok0);
+  const int cnt = pf_count(a, b, row0), tok0 = (total - 1 - idx - first) * NG * p.tq, ntok = min(NG * p.tq, cnt - tok0);
   row0 += tok0;
   const int len = kv_len(__ldg(a.len + b), a.max_len), t0 = len - cnt + tok0;   // cache row of the first token (negative: before the cache)
   const PfLine line = pf_line(a, t0, t0 + ntok - 1);
   const int i0 = (int)((long long)line.nt * split / p.ns), n = (int)((long long)line.nt * (split + 1) / p.ns) - i0;
-  const int ng = ntok > p.tq ? 2 : 1;   // groups with rows
+  const int ng = NG == 2 && ntok > p.tq ? 2 : 1;   // groups with rows
   const int* trow = a.p.table + (size_t)b * a.p.table_ld;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NST; i++) { pf_init(&full[i], 1); pf_init(&empty[i], ng); }
-    for (int g = 0; g < 2; g++) {
+    for (int i = 0; i < NST; i++) {
+      pf_init(&kfull[i], 1);
+      pf_init(&vfull[i], 1);
+      pf_init(&kempty[i], ng);
+      pf_init(&vempty[i], ng);
+    }
+    for (int g = 0; g < NG; g++) {
       for (int i = 0; i < 2; i++) { pf_init(&sfull[g][i], 1); pf_init(&pready[g][i], 128); }
       pf_init(&pvdone[g], 1);
       pf_init(&ofin[g], 1);
+      pf_init(&done[g], 1);
     }
-    pf_init(&qfull, 256);
     for (int i = 0; i < 4; i++) pf_init(&lock[i], 1);
     for (int i = 0; i < 3; i++) pf_init(&vfix[i], 1);
-    pf_init(&done[0], 1);
-    pf_init(&done[1], 1);
+    pf_init(&qfull, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     stop_f = 0;
   }
   if (warp == PF_MMA) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(kv_s32(&tbase)));
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(kv_s32(&tbase)), "n"(G::COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   // does every 16-row block of the line have its page?
   bool gap = false;
-  for (int u = threadIdx.x; u < n * (PF_KT / 16); u += PF_T) {
+  for (int u = threadIdx.x; u < n * (PF_KT / 16); u += G::T) {
     const int j = pf_key(line, i0 + u / (PF_KT / 16)) + u % (PF_KT / 16) * 16;
     if (j < line.end && kv_page(a.p, trow, j) < 0) gap = true;
   }
@@ -282,35 +287,49 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(const __grid_constant__ 
       const int e = j < line.end ? __ldg(trow + (j >> a.p.shift)) : -1;
       return (unsigned)e < (unsigned)a.p.n_pages ? e : a.p.n_pages;   // the box behind the last page: zeros
     };
+    if (n > 0 && lane == 0) {
+      // the queries: a box of tq tokens and 64 columns for each head (rows past the sequence's last
+      // token are another's or zeros, and go nowhere)
+      pf_expect(&qfull, ng * a.grp * p.tq * (D * 2));
+      for (int g = 0; g < ng; g++)
+        for (int h = 0; h < a.grp; h++)
+#pragma unroll
+          for (int c = 0; c < D / 64; c++)
+            pf_tma2(kv_s32(smq) + g * G::Q + c * QP + h * p.tq * 128, &mq, (kh * a.grp + h) * D + c * 64, row0 + g * p.tq, &qfull);
+    }
     int pg = n > 0 ? page_of(0) : 0, st = 0, sf = 0;
     unsigned epar = 1, fpar = 0;
     int fixes = 0;    // at most 3: where the sinks end, where the window begins, the last tile
-    for (int i = 0; i < n + 2; i++) {
+    // a tile's V is looked at LAG tiles later: by then another is on its way,
+    // and issuing that one has not waited for this one's product
+    constexpr int LAG = NST > 2 ? 2 : 1;
+    for (int i = 0; i < n + LAG; i++) {
       if (i < n) {
         const int now = pg, k0 = pf_key(line, i0 + i);
         if (i + 1 < n) pg = page_of(i + 1);
-        if (i >= NST) pf_wait(&empty[st], epar, stop, 1);
-        __syncwarp();
         const uint32_t ks = kv_s32(smk) + st * (2 * G::KV);
-        if (lane == 0) pf_expect(&full[st], 2 * G::KV);
-        for (int r = 0; r < PF_KT; r += p.box) {
-          const int page = __shfl_sync(0xffffffffu, now, r >> 4), row = (k0 + r) & ((1 << a.p.shift) - 1);
-          if (lane == 0) {
-            const int c1 = p.d_row == 1 ? row : (p.d_head == 1 ? kh : page), c2 = p.d_row == 2 ? row : (p.d_head == 2 ? kh : page),
-                      c3 = p.d_row == 3 ? row : (p.d_head == 3 ? kh : page);
 #pragma unroll
-            for (int c = 0; c < D / 64; c++) {
-              pf_tma(ks + c * KP + r * 128, &mk, c * 64, c1, c2, c3, &full[st]);
-              pf_tma(ks + G::KV + c * KP + r * 128, &mv, c * 64, c1, c2, c3, &full[st]);
+        for (int z = 0; z < 2; z++) {        // K, then V
+          if (i >= NST) pf_wait(z ? &vempty[st] : &kempty[st], epar, stop, 1);
+          __syncwarp();
+          uint64_t* bar = z ? &vfull[st] : &kfull[st];
+          if (lane == 0) pf_expect(bar, G::KV);
+          for (int r = 0; r < PF_KT; r += p.box) {
+            const int page = __shfl_sync(0xffffffffu, now, r >> 4), row = (k0 + r) & ((1 << a.p.shift) - 1);
+            if (lane == 0) {
+              const int c1 = p.d_row == 1 ? row : (p.d_head == 1 ? kh : page), c2 = p.d_row == 2 ? row : (p.d_head == 2 ? kh : page),
+                        c3 = p.d_row == 3 ? row : (p.d_head == 3 ? kh : page);
+#pragma unroll
+              for (int c = 0; c < D / 64; c++) pf_tma(ks + z * G::KV + c * KP + r * 128, z ? &mv : &mk, c * 64, c1, c2, c3, bar);
             }
           }
         }
         if (++st == NST) { st = 0; epar ^= 1; }
       }
-      if (i >= 2) {     // two tiles later: V rows behind what is seen
-        const int k0 = pf_key(line, i0 + i - 2);
+      if (i >= LAG) {   // V rows behind what is seen
+        const int k0 = pf_key(line, i0 + i - LAG);
         if (pf_edge(line, k0)) {
-          pf_wait(&full[sf], fpar, stop, 9);
+          pf_wait(&vfull[sf], fpar, stop, 9);
           char* vs = smk + sf * (2 * G::KV) + G::KV;
           for (int u = lane; u < PF_KT * (D / 8); u += 32) {
             const int r = u & (PF_KT - 1), j = k0 + r;
@@ -331,7 +350,7 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(const __grid_constant__ 
       const unsigned long long t1 = pf_now();
       while (pf_now() - t1 < 1000000ull) {}
     }
-  } else if (warp == PF_MMA || warp == PF_MMA + 1) {
+  } else if (warp == PF_MMA || (NG == 2 && warp == PF_MMA + 1)) {
     // ---------------------------------------------------- matrix products
     // kind::f16: D fp32 (bits 4-5 = 1), A and B fp16 (0) or bf16 (1) at bits 7 and 10, B N-major at bit 16,
     // N / 8 at bits 17-22, M / 16 at bits 24-28
@@ -348,7 +367,7 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(const __grid_constant__ 
     if (g < ng && pf_elect()) {
       // scores of tile j
       auto scores = [&](int j, int st, unsigned par) {
-        pf_wait(&full[st], par, stop, 2);
+        pf_wait(&kfull[st], par, stop, 2);
         // the buffer held P of tile j - 2: its product is done
         if (j >= 2) pf_wait(&pvdone[g], (unsigned)j & 1u, stop, 3);
         pf_fence_after();
@@ -359,6 +378,7 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(const __grid_constant__ 
           pf_mma_ss(d, qb + (uint64_t)(((k >> 2) * QP + (k & 3) * 32) >> 4), kb + (uint64_t)(((k >> 2) * KP + (k & 3) * 32) >> 4),
                     id_s, k > 0);
         pf_commit(&sfull[g][j & 1]);
+        pf_commit(&kempty[st]);
       };
       // The groups are held half a step apart, so that one's exponentials
       // fall beside the other's other work: the second group's next scores
@@ -368,8 +388,8 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(const __grid_constant__ 
       // exponentials by polynomial on the FMA pipe, 509 in step, did not help
       // further here.)
       int fixes = 0;                    // edge tiles so far
-      int st = 0, s1 = 1, s2 = 2;       // stages of tiles i, i + 1, i + 2
-      unsigned p1 = 0, p2 = 0;          // parities of full[s1], full[s2]
+      int st = 0, s1 = 1, s2 = 2 % NST;                  // stages of tiles i, i + 1, i + 2
+      unsigned p0 = 0, p1 = 0, p2 = (2 / NST) & 1;       // and the parities of their use
       if (n > 0) {
         pf_wait(&qfull, 0, stop, 10);
         scores(0, 0, 0);
@@ -377,26 +397,28 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(const __grid_constant__ 
       }
       for (int i = 0; i < n; i++) {
         const bool edge = pf_edge(line, pf_key(line, i0 + i));
-        if (g == 1 && i + 1 < n) {
+        if (NG == 2 && g == 1 && i + 1 < n) {
           pf_wait(&pready[0][i & 1], (unsigned)(i >> 1) & 1u, stop, 7);
           scores(i + 1, s1, p1);
         }
+        pf_wait(&vfull[st], p0, stop, 13);
         if (edge && fixes < 3) pf_wait(&vfix[fixes++], 0, stop, 11);
         pf_wait(&pready[g][i & 1], (unsigned)(i >> 1) & 1u, stop, 4);
-        if (g == 1) pf_arrive(&lock[i & 3]);
+        if (NG == 2 && g == 1) pf_arrive(&lock[i & 3]);
         pf_fence_after();
         const uint64_t vb = dv + (uint64_t)(st * ((2 * G::KV) >> 4));
         const uint32_t pb = tmem + g * 128 + (uint32_t)(i & 1) * 64, o = tmem + G::O_COL + g * D;
 #pragma unroll
         for (int k = 0; k < PF_KT / 16; k++) pf_mma_ts(o, pb + k * 8, vb + (uint64_t)((k * 2048) >> 4), id_o, i > 0 || k > 0);
         pf_commit(i + 1 < n ? &pvdone[g] : &ofin[g]);
-        pf_commit(&empty[st]);
+        pf_commit(&vempty[st]);
         if (g == 0 && i + 2 < n) {
           // (of four, as the other thread may be up to three tiles ahead)
           if (ng == 2) pf_wait(&lock[i & 3], (unsigned)(i >> 2) & 1u, stop, 12);
           scores(i + 2, s2, p2);
         }
         st = s1;
+        p0 = p1;
         s1 = s2;
         p1 = p2;
         if (++s2 == NST) { s2 = 0; p2 ^= 1; }
@@ -411,22 +433,10 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(const __grid_constant__ 
     const int g = (warp - 4) >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t to = tl + G::O_COL + (uint32_t)(g * D);
-    const int tk = g * p.tq + r / a.grp;                       // token within the CTA
-    const bool live = r < p.tq * a.grp && tk < ntok;
+    const int tk = g * p.tq + r % p.tq, hq = r / p.tq;         // token within the CTA, head within the group
+    const bool live = hq < a.grp && tk < ntok;
     const int t = t0 + min(tk, ntok - 1);                      // the row's own cache row
     const int wlo = a.window > 0 ? t + 1 - a.window : 0;       // it sees [wlo, t] and [0, sinks)
-    // its query, swizzled; rows past the last token are zeros
-    if (n > 0) {
-      const char* src = a.q + (long long)(row0 + min(tk, ntok - 1)) * a.ldq + (size_t)(kh * a.grp + r % a.grp) * (D * 2);
-#pragma unroll
-      for (int c = 0; c < D / 8; c++) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (live) v = pb_ldg_stream(src + c * 16);
-        *reinterpret_cast<uint4*>(smq + g * G::Q + (c >> 3) * QP + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      pf_arrive(&qfull);
-    }
     // of the group: what all rows see, for tiles that need no masks
     const int ta = t0 + min(g * p.tq, ntok - 1), tb = t0 + min((g + 1) * p.tq - 1, ntok - 1);
     const int whi = a.window > 0 ? tb + 1 - a.window : 0;
@@ -481,14 +491,14 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(const __grid_constant__ 
           pf_wait(&pvdone[g], (unsigned)(i - 1) & 1u, stop, 6);
           __syncwarp();
           pf_fence_after();
-#pragma unroll
-          for (int e = 0; e < D; e += 32) {
-            unsigned o[32];
-            pf_ld32(to + e, o);
+#pragma unroll 2
+          for (int e = 0; e < D; e += 16) {
+            unsigned o[16];
+            pf_ld16(to + e, o);
             pf_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-            pf_st32(to + e, o);
+            for (int k = 0; k < 16; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            pf_st16(to + e, o);
           }
         }
       }
@@ -496,24 +506,24 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(const __grid_constant__ 
       // with V needs; the sum takes the unrounded ones
       const pf_f2 nms = pf_pk(-ms, -ms);
       pf_f2 y[2] = {0ull, 0ull};
-      unsigned w[32];
-      pf_f2 z[32];
 #pragma unroll
-      for (int k = 0; k < 32; k++) z[k] = pf_fma2(pf_pk(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), sc2, nms);
+      for (int q = 0; q < 4; q++) {
+        unsigned w[8];
 #pragma unroll
-      for (int k = 0; k < 32; k++) {
-        float u, v;
-        pf_upk(z[k], u, v);
-        u = kv_ex2(u);
-        v = kv_ex2(v);
-        y[k & 1] = pf_add2(y[k & 1], pf_pk(u, v));
-        w[k] = kv_down<CT>(u, v);
+        for (int k = 0; k < 8; k++) {
+          float u, v;
+          pf_upk(pf_fma2(pf_pk(__uint_as_float(s[16 * q + 2 * k]), __uint_as_float(s[16 * q + 2 * k + 1])), sc2, nms), u, v);
+          u = kv_ex2(u);
+          v = kv_ex2(v);
+          y[k & 1] = pf_add2(y[k & 1], pf_pk(u, v));
+          w[k] = kv_down<CT>(u, v);
+        }
+        pf_st8(ts + q * 8, w);
       }
       float ya, yb, yc, yd;
       pf_upk(y[0], ya, yb);
       pf_upk(y[1], yc, yd);
       l += (ya + yb) + (yc + yd);
-      pf_st32(ts, w);
       pf_wait_st();
       pf_fence_before();
       pf_arrive(&pready[g][i & 1]);
@@ -524,33 +534,56 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(const __grid_constant__ 
         __syncwarp();
       }
       pf_fence_after();
-      const int row = row0 + tk, h = kh * a.grp + r % a.grp;
+      const int row = row0 + tk, h = kh * a.grp + hq;   // (of a live row)
       const float f = l != 0.0f ? 1.0f / l : 0.0f;       // nothing seen: zeros
       const size_t at = ((size_t)split * a.n_rows + row) * a.nh + h;
+      if (p.ns == 1) {
+        // by way of the (now idle) queries' rows, so that a warp writes whole rows together
+        char* sr = smq + g * G::Q + r * 128;
 #pragma unroll
-      for (int e = 0; e < D; e += 32) {
-        unsigned o[32];
-        if (n > 0) {
-          pf_ld32(to + e, o);
-          pf_wait_ld();
-        } else {
+        for (int e = 0; e < D; e += 16) {
+          unsigned o[16];
+          if (n > 0) {
+            pf_ld16(to + e, o);
+            pf_wait_ld();
+          } else {
 #pragma unroll
-          for (int k = 0; k < 32; k++) o[k] = 0u;
-        }
-        if (live) {
-          if (p.ns == 1) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-              float v[8];
-#pragma unroll
-              for (int u = 0; u < 8; u++) v[u] = __uint_as_float(o[k + u]) * f;
-              pf_put<D>(p, row, h, e + k, v);
-            }
-          } else if (n > 0) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              *reinterpret_cast<uint4*>(p.part + at * D + e + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+            for (int k = 0; k < 16; k++) o[k] = 0u;
           }
+          float v[16];
+#pragma unroll
+          for (int k = 0; k < 16; k++) v[k] = __uint_as_float(o[k]) * f;
+#pragma unroll
+          for (int k = 0; k < 2; k++) {
+            const float* y = v + 8 * k;
+            const uint4 w = p.out_bf16 ? make_uint4(kv_down<PB_DT_BF16>(y[0], y[1]), kv_down<PB_DT_BF16>(y[2], y[3]),
+                                                    kv_down<PB_DT_BF16>(y[4], y[5]), kv_down<PB_DT_BF16>(y[6], y[7]))
+                                       : make_uint4(kv_down<PB_DT_F16>(y[0], y[1]), kv_down<PB_DT_F16>(y[2], y[3]),
+                                                    kv_down<PB_DT_F16>(y[4], y[5]), kv_down<PB_DT_F16>(y[6], y[7]));
+            const int c = e / 8 + k;
+            *reinterpret_cast<uint4*>(sr + (c >> 3) * QP + (((c & 7) ^ (r & 7)) << 4)) = w;
+          }
+        }
+        __syncwarp();
+        constexpr int CPR = D / 8, RP = 32 / CPR;      // chunks of a row, rows at a time
+        const int c = lane % CPR;
+#pragma unroll 4
+        for (int i = lane / CPR; i < 32; i += RP) {
+          const int r2 = (warp & 3) * 32 + i, tk2 = g * p.tq + r2 % p.tq, h2 = r2 / p.tq;
+          if (h2 < a.grp && tk2 < ntok)
+            *reinterpret_cast<uint4*>(a.out + (long long)(row0 + tk2) * a.ldo + (size_t)(kh * a.grp + h2) * (D * 2) + c * 16) =
+                *reinterpret_cast<const uint4*>(smq + g * G::Q + (c >> 3) * QP + r2 * 128 + (((c & 7) ^ (r2 & 7)) << 4));
+        }
+      } else if (n > 0) {
+#pragma unroll
+        for (int e = 0; e < D; e += 16) {
+          unsigned o[16];
+          pf_ld16(to + e, o);
+          pf_wait_ld();
+          if (live)
+#pragma unroll
+            for (int k = 0; k < 16; k += 4)
+              *reinterpret_cast<uint4*>(p.part + at * D + e + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
         }
       }
       if (live && p.ns > 1) p.ml[at] = make_float2(n > 0 ? ms : -INFINITY, n > 0 ? l : 0.0f);
@@ -558,7 +591,7 @@ __global__ void __launch_bounds__(PF_T, 1) k_kv_prefill(const __grid_constant__ 
     pf_fence_before();
   }
   __syncthreads();
-  if (warp == PF_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  if (warp == PF_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(G::COLS));
 }
 
 // the splits of each row and head joined, D / 4 lanes' worth of a warp per
@@ -608,19 +641,28 @@ __global__ void __launch_bounds__(128) k_kv_prefill_join(PfArgs p) {
   *reinterpret_cast<uint2*>(o) = w;
 }
 
-// launch shape: CTAs of 2 * tq tokens, and splits of the key line where those
+// launch shape: CTAs of ng * tq tokens, and splits of the key line where those
 // leave SMs idle (at least 4 tiles each)
+#ifndef PF_NG
+#define PF_NG 0
+#endif
 struct PfPlan {
-  int tq, ns;
+  int tq, ng, ns;
   long long items, part, ml;   // CTAs per split; floats
 };
-PfPlan pf_plan(const pb_kv_pages* c, int n_seq, int max_len, int n_tok, int n_heads) {
+PfPlan pf_plan(const pb_kv_pages* c, int n_seq, int max_len, int n_tok, int n_heads, int window, int sinks) {
   PfPlan p{};
   const int grp = n_heads / c->n_kv;
-  p.tq = 128 / (grp > 0 ? grp : 1);
-  p.items = ((long long)n_tok / (2 * p.tq) + (n_seq < n_tok ? n_seq : n_tok)) * c->n_kv;
-  const long long tiles = (max_len + PF_KT - 1) / PF_KT;
-  long long ns = p.items > 0 ? pb_num_sms() / p.items : 1;
+  p.tq = 128 / (grp > 0 ? grp : 1) / 8 * 8;       // whole 8-row groups of the swizzle
+  p.ng = PF_NG ? PF_NG : 2;
+  const int tok = p.ng * p.tq, sms = pb_num_sms() * (p.ng == 1 ? 2 : 1);
+  p.items = ((long long)n_tok / tok + (n_seq < n_tok ? n_seq : n_tok)) * c->n_kv;
+  long long tiles = (max_len + PF_KT - 1) / PF_KT;
+  if (window > 0) {
+    const long long seen = ((long long)window + tok + 2 * PF_KT - 1) / PF_KT + (sinks + PF_KT - 1) / PF_KT;
+    if (seen < tiles) tiles = seen;
+  }
+  long long ns = p.items > 0 ? sms / p.items : 1;
   if (ns > tiles / 4) ns = tiles / 4;
   p.ns = ns < 1 ? 1 : (int)ns;
   const long long rows = (long long)p.ns * n_tok * n_heads;
@@ -634,7 +676,7 @@ PfPlan pf_plan(const pb_kv_pages* c, int n_seq, int max_len, int n_tok, int n_he
 typedef CUresult (*PfEncode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-int pf_maps(const pb_kv_pages* c, PfArgs* p, CUtensorMap* mk, CUtensorMap* mv) {
+int pf_maps(const pb_kv_pages* c, PfArgs* p, CUtensorMap* mk, CUtensorMap* mv, CUtensorMap* mq) {
   static std::atomic<void*> fn{nullptr};
   void* f = fn.load(std::memory_order_acquire);
   if (!f) {
@@ -672,24 +714,39 @@ int pf_maps(const pb_kv_pages* c, PfArgs* p, CUtensorMap* mk, CUtensorMap* mv) {
                                                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return pb_set_error(PB_EINVAL, "pb_kv_prefill: strides the tensor map does not take (%d)", (int)r);
   }
+  // the queries as a matrix [token][head and column]
+  const cuuint64_t qdims[2] = {(cuuint64_t)p->a.nh * c->head_dim, (cuuint64_t)p->a.n_rows};
+  const cuuint64_t qstride[1] = {(cuuint64_t)p->a.ldq};
+  const cuuint32_t qbox[2] = {64, (cuuint32_t)p->tq};
+  const CUresult r = reinterpret_cast<PfEncode>(f)(mq, ty, 2, const_cast<char*>(p->a.q), qdims, qstride, qbox, one,
+                                                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return pb_set_error(PB_EINVAL, "pb_kv_prefill: a row stride of q that the tensor map does not take (%d)", (int)r);
   return PB_OK;
 }
 
-template <int D, int CT>
-int pf_run(const CUtensorMap& mk, const CUtensorMap& mv, const PfArgs& p, long long items, cudaStream_t st) {
+template <int D, int CT, int NG>
+int pf_launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const PfArgs& p, long long items, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
-  if (int rc = kv_smem(k_kv_prefill<D, CT>, PfGeo<D>::SMEM, done)) return rc;
-  if (int rc = kv_launch(k_kv_prefill<D, CT>, (unsigned)(items * p.ns), PF_T, PfGeo<D>::SMEM, st, false, "k_kv_prefill", mk, mv, p)) return rc;
+  if (int rc = kv_smem(k_kv_prefill<D, CT, NG>, PfGeo<D, NG>::SMEM, done)) return rc;
+  if (int rc = kv_launch(k_kv_prefill<D, CT, NG>, (unsigned)(items * p.ns), PfGeo<D, NG>::T, PfGeo<D, NG>::SMEM, st, false,
+                         "k_kv_prefill", mk, mv, mq, p))
+    return rc;
   if (p.ns == 1) return PB_OK;
   const long long blocks = ((long long)p.a.n_rows * p.a.nh * (D / 4) + 127) / 128;
   return kv_launch(k_kv_prefill_join<D>, (unsigned)blocks, 128, 0, st, true, "k_kv_prefill_join", p);
+}
+template <int D, int CT>
+int pf_run(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const PfArgs& p, const PfPlan& pl, cudaStream_t st) {
+  return pl.ng == 1 ? pf_launch<D, CT, 1>(mk, mv, mq, p, pl.items, st) : pf_launch<D, CT, 2>(mk, mv, mq, p, pl.items, st);
 }
 
 }  // namespace
 
 extern "C" long long pb_kv_prefill_scratch(const pb_kv_pages* c, int n_seq, int max_len, int n_tok, int n_heads) {
   if (!c || n_seq < 0 || max_len < 0 || n_tok < 0 || n_heads <= 0 || c->n_kv <= 0 || n_heads / c->n_kv > 16) return -1;
-  const PfPlan p = pf_plan(c, n_seq, max_len, n_tok, n_heads);
+  // (a window may need fewer splits: the whole cache's need covers both)
+  const PfPlan p = pf_plan(c, n_seq, max_len, n_tok, n_heads, 0, 0);
   return 4 * (p.part + p.ml);
 }
 
@@ -705,7 +762,7 @@ extern "C" int pb_kv_prefill(const pb_kv_pages* c, int n_seq, const int* d_table
                           d_out, out_dtype, ldo, &p.a))
     return rc;
   if (n_seq == 0 || n_tok == 0) return PB_OK;
-  const PfPlan pl = pf_plan(c, n_seq, max_len, n_tok, n_heads);
+  const PfPlan pl = pf_plan(c, n_seq, max_len, n_tok, n_heads, window, sinks);
   if (pl.items * pl.ns > INT_MAX || (long long)n_tok * n_heads * 32 > INT_MAX)
     return pb_set_error(PB_EINVAL, "pb_kv_prefill: %d tokens of %d heads", n_tok, n_heads);
   const long long need = 4 * (pl.part + pl.ml);
@@ -718,11 +775,11 @@ extern "C" int pb_kv_prefill(const pb_kv_pages* c, int n_seq, const int* d_table
   p.part = static_cast<float*>(d_scratch);
   p.ml = reinterpret_cast<float2*>(p.part + pl.part);
   cudaStream_t st = (cudaStream_t)stream;
-  CUtensorMap mk, mv;
-  if (int rc = pf_maps(c, &p, &mk, &mv)) return rc;
+  CUtensorMap mk, mv, mq;
+  if (int rc = pf_maps(c, &p, &mk, &mv, &mq)) return rc;
   if (c->head_dim == 64)
-    return c->dtype == PB_DT_F16 ? pf_run<64, PB_DT_F16>(mk, mv, p, pl.items, st) : pf_run<64, PB_DT_BF16>(mk, mv, p, pl.items, st);
-  return c->dtype == PB_DT_F16 ? pf_run<128, PB_DT_F16>(mk, mv, p, pl.items, st) : pf_run<128, PB_DT_BF16>(mk, mv, p, pl.items, st);
+    return c->dtype == PB_DT_F16 ? pf_run<64, PB_DT_F16>(mk, mv, mq, p, pl, st) : pf_run<64, PB_DT_BF16>(mk, mv, mq, p, pl, st);
+  return c->dtype == PB_DT_F16 ? pf_run<128, PB_DT_F16>(mk, mv, mq, p, pl, st) : pf_run<128, PB_DT_BF16>(mk, mv, mq, p, pl, st);
 }
 
 extern "C" int pb_kv_status(void* stream) {
