@@ -36,16 +36,18 @@ constexpr int PF_KT = 64;                 // key rows per tile
 constexpr int PF_MMA = 2;                 // the warp that issues the first group's products, the next one the second's
 constexpr unsigned long long PF_WAIT_NS = 1000000000ull;
 
-// NG groups of 128 rows per CTA: 2, sharing every K/V tile, or 1 with two CTAs
-// an SM (see pf_plan)
-template <int D, int NG>
+// (One group per CTA and two CTAs an SM took as long or longer on every shape
+// tried: 515 against 500 us for 8192 tokens of 32/8 heads x 128, 419 against
+// 393 at head_dim 64, 86 against 82 for the ragged batch with a window.)
+constexpr int NG = 2;                     // groups of 128 rows per CTA
+template <int D>
 struct PfGeo {
   static constexpr int T = 128 + 128 * NG;        // threads
   static constexpr int Q = 128 * D * 2;           // bytes of a group's queries
   static constexpr int KV = PF_KT * D * 2;        // bytes of a K (or V) tile
-  static constexpr int NST = NG == 2 ? (D == 128 ? 5 : 8) : (D == 128 ? 2 : 4);   // stages of the K ring, and of the V ring
+  static constexpr int NST = D == 128 ? 5 : 8;    // stages of the K ring, and of the V ring
   static constexpr int SMEM = NG * Q + NST * 2 * KV + 1024;
-  static constexpr int COLS = NG * 256;           // TMEM columns allocated
+  static constexpr int COLS = 512;                // TMEM columns allocated
   static constexpr uint32_t O_COL = NG * 128;     // S: group * 128 + buffer * 64; O: O_COL + group * D
 };
 
@@ -214,10 +216,10 @@ PB_DEV unsigned long long pf_below(int x) { return x <= 0 ? 0ull : (x >= 64 ? ~0
 PB_DEV bool pf_edge(const PfLine& s, int k0) { return k0 + PF_KT > s.end || (k0 < s.lo && k0 + PF_KT > s.sinks); }
 PB_DEV int pf_key(const PfLine& s, int i) { return (i < s.nst ? i : i - s.nst + s.lot) * PF_KT; }
 
-template <int D, int CT, int NG>
-__global__ void __launch_bounds__(PfGeo<D, NG>::T, NG == 1 ? 2 : 1) k_kv_prefill(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mq,
+template <int D, int CT>
+__global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mq,
              PfArgs p) {
-  typedef PfGeo<D, NG> G;
+  typedef PfGeo<D> G;
   constexpr int NST = G::NST, KP = PF_KT * 128, QP = 128 * 128;   // bytes of a 64-column panel of K or V, of Q
   extern __shared__ __align__(128) char psm_raw[];
   __shared__ uint64_t kfull[NST], kempty[NST], vfull[NST], vempty[NST], sfull[NG][2], pready[NG][2], pvdone[NG], ofin[NG], lock[4], qfull, vfix[3], done[NG];
@@ -241,7 +243,7 @@ __global__ void __launch_bounds__(PfGeo<D, NG>::T, NG == 1 ? 2 : 1) k_kv_prefill
   const int len = kv_len(__ldg(a.len + b), a.max_len), t0 = len - cnt + tok0;   // cache row of the first token (negative: before the cache)
   const PfLine line = pf_line(a, t0, t0 + ntok - 1);
   const int i0 = (int)((long long)line.nt * split / p.ns), n = (int)((long long)line.nt * (split + 1) / p.ns) - i0;
-  const int ng = NG == 2 && ntok > p.tq ? 2 : 1;   // groups with rows
+  const int ng = ntok > p.tq ? 2 : 1;   // groups with rows
   const int* trow = a.p.table + (size_t)b * a.p.table_ld;
 
   if (threadIdx.x == 0) {
@@ -300,9 +302,9 @@ __global__ void __launch_bounds__(PfGeo<D, NG>::T, NG == 1 ? 2 : 1) k_kv_prefill
     int pg = n > 0 ? page_of(0) : 0, st = 0, sf = 0;
     unsigned epar = 1, fpar = 0;
     int fixes = 0;    // at most 3: where the sinks end, where the window begins, the last tile
-    // a tile's V is looked at LAG tiles later: by then another is on its way,
-    // and issuing that one has not waited for this one's product
-    constexpr int LAG = NST > 2 ? 2 : 1;
+    // a tile's V is looked at LAG tiles later: by then others are on their way
+    // (fewer than NST, so that issuing them has not waited for this one's product)
+    constexpr int LAG = 2;
     for (int i = 0; i < n + LAG; i++) {
       if (i < n) {
         const int now = pg, k0 = pf_key(line, i0 + i);
@@ -350,7 +352,7 @@ __global__ void __launch_bounds__(PfGeo<D, NG>::T, NG == 1 ? 2 : 1) k_kv_prefill
       const unsigned long long t1 = pf_now();
       while (pf_now() - t1 < 1000000ull) {}
     }
-  } else if (warp == PF_MMA || (NG == 2 && warp == PF_MMA + 1)) {
+  } else if (warp == PF_MMA || warp == PF_MMA + 1) {
     // ---------------------------------------------------- matrix products
     // kind::f16: D fp32 (bits 4-5 = 1), A and B fp16 (0) or bf16 (1) at bits 7 and 10, B N-major at bit 16,
     // N / 8 at bits 17-22, M / 16 at bits 24-28
@@ -388,8 +390,8 @@ __global__ void __launch_bounds__(PfGeo<D, NG>::T, NG == 1 ? 2 : 1) k_kv_prefill
       // exponentials by polynomial on the FMA pipe, 509 in step, did not help
       // further here.)
       int fixes = 0;                    // edge tiles so far
-      int st = 0, s1 = 1, s2 = 2 % NST;                  // stages of tiles i, i + 1, i + 2
-      unsigned p0 = 0, p1 = 0, p2 = (2 / NST) & 1;       // and the parities of their use
+      int st = 0, s1 = 1, s2 = 2;                  // stages of tiles i, i + 1, i + 2
+      unsigned p0 = 0, p1 = 0, p2 = 0;       // and the parities of their use
       if (n > 0) {
         pf_wait(&qfull, 0, stop, 10);
         scores(0, 0, 0);
@@ -397,14 +399,14 @@ __global__ void __launch_bounds__(PfGeo<D, NG>::T, NG == 1 ? 2 : 1) k_kv_prefill
       }
       for (int i = 0; i < n; i++) {
         const bool edge = pf_edge(line, pf_key(line, i0 + i));
-        if (NG == 2 && g == 1 && i + 1 < n) {
+        if (g == 1 && i + 1 < n) {
           pf_wait(&pready[0][i & 1], (unsigned)(i >> 1) & 1u, stop, 7);
           scores(i + 1, s1, p1);
         }
         pf_wait(&vfull[st], p0, stop, 13);
         if (edge && fixes < 3) pf_wait(&vfix[fixes++], 0, stop, 11);
         pf_wait(&pready[g][i & 1], (unsigned)(i >> 1) & 1u, stop, 4);
-        if (NG == 2 && g == 1) pf_arrive(&lock[i & 3]);
+        if (g == 1) pf_arrive(&lock[i & 3]);
         pf_fence_after();
         const uint64_t vb = dv + (uint64_t)(st * ((2 * G::KV) >> 4));
         const uint32_t pb = tmem + g * 128 + (uint32_t)(i & 1) * 64, o = tmem + G::O_COL + g * D;
@@ -541,38 +543,43 @@ __global__ void __launch_bounds__(PfGeo<D, NG>::T, NG == 1 ? 2 : 1) k_kv_prefill
         // by way of the (now idle) queries' rows, so that a warp writes whole rows together
         char* sr = smq + g * G::Q + r * 128;
 #pragma unroll
-        for (int e = 0; e < D; e += 16) {
-          unsigned o[16];
+        for (int e = 0; e < D; e += 32) {
+          unsigned o[32];
           if (n > 0) {
-            pf_ld16(to + e, o);
+            pf_ld32(to + e, o);
             pf_wait_ld();
           } else {
 #pragma unroll
-            for (int k = 0; k < 16; k++) o[k] = 0u;
+            for (int k = 0; k < 32; k++) o[k] = 0u;
           }
-          float v[16];
 #pragma unroll
-          for (int k = 0; k < 16; k++) v[k] = __uint_as_float(o[k]) * f;
+          for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
 #pragma unroll
-          for (int k = 0; k < 2; k++) {
-            const float* y = v + 8 * k;
-            const uint4 w = p.out_bf16 ? make_uint4(kv_down<PB_DT_BF16>(y[0], y[1]), kv_down<PB_DT_BF16>(y[2], y[3]),
-                                                    kv_down<PB_DT_BF16>(y[4], y[5]), kv_down<PB_DT_BF16>(y[6], y[7]))
-                                       : make_uint4(kv_down<PB_DT_F16>(y[0], y[1]), kv_down<PB_DT_F16>(y[2], y[3]),
-                                                    kv_down<PB_DT_F16>(y[4], y[5]), kv_down<PB_DT_F16>(y[6], y[7]));
+          for (int k = 0; k < 4; k++) {
+            uint4 w;
+            unsigned* x = &w.x;
+#pragma unroll
+            for (int z = 0; z < 4; z++) {
+              const float y0 = __uint_as_float(o[8 * k + 2 * z]), y1 = __uint_as_float(o[8 * k + 2 * z + 1]);
+              x[z] = p.out_bf16 ? kv_down<PB_DT_BF16>(y0, y1) : kv_down<PB_DT_F16>(y0, y1);
+            }
             const int c = e / 8 + k;
             *reinterpret_cast<uint4*>(sr + (c >> 3) * QP + (((c & 7) ^ (r & 7)) << 4)) = w;
           }
         }
         __syncwarp();
-        constexpr int CPR = D / 8, RP = 32 / CPR;      // chunks of a row, rows at a time
+        // D / 8 lanes write a row; where it goes is known to the lane whose row it is
+        constexpr int CPR = D / 8, RP = 32 / CPR;
         const int c = lane % CPR;
-#pragma unroll 4
-        for (int i = lane / CPR; i < 32; i += RP) {
-          const int r2 = (warp & 3) * 32 + i, tk2 = g * p.tq + r2 % p.tq, h2 = r2 / p.tq;
-          if (h2 < a.grp && tk2 < ntok)
-            *reinterpret_cast<uint4*>(a.out + (long long)(row0 + tk2) * a.ldo + (size_t)(kh * a.grp + h2) * (D * 2) + c * 16) =
-                *reinterpret_cast<const uint4*>(smq + g * G::Q + (c >> 3) * QP + r2 * 128 + (((c & 7) ^ (r2 & 7)) << 4));
+        const long long off = live ? (long long)row * a.ldo + h * (D * 2) : -1;
+        const char* from = smq + g * G::Q + (c >> 3) * QP + (warp & 3) * (32 * 128);
+#pragma unroll
+        for (int i0 = 0; i0 < 32; i0 += RP) {
+          const int i = i0 + lane / CPR;
+          const long long to_row = __shfl_sync(0xffffffffu, off, i);
+          if (to_row >= 0)
+            *reinterpret_cast<uint4*>(a.out + to_row + c * 16) =
+                *reinterpret_cast<const uint4*>(from + i * 128 + (((c & 7) ^ (i & 7)) << 4));
         }
       } else if (n > 0) {
 #pragma unroll
@@ -594,13 +601,15 @@ __global__ void __launch_bounds__(PfGeo<D, NG>::T, NG == 1 ? 2 : 1) k_kv_prefill
   if (warp == PF_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(G::COLS));
 }
 
-// the splits of each row and head joined, D / 4 lanes' worth of a warp per
-// head. A row belongs to a sequence or it is left alone.
+// The splits of each row and head joined, by D / 4 lanes: a lane reads the
+// maximum and sum of every (D / 4)-th split, the factors go around by shuffle,
+// and the sums of 8 splits are in flight together. A row belongs to a sequence
+// or it is left alone.
 template <int D>
 __global__ void __launch_bounds__(128) k_kv_prefill_join(PfArgs p) {
   const AttnKvArgs& a = p.a;
-  constexpr int L = D / 4;      // lanes per head
-  const int unit = (blockIdx.x * 128 + threadIdx.x) / L, e = (threadIdx.x % L) * 4;
+  constexpr int L = D / 4, MOST = 160 / L;      // lanes per head; splits per lane (at most one split per SM)
+  const int unit = (blockIdx.x * 128 + threadIdx.x) / L, l = threadIdx.x % L, e = l * 4;
   const int row = unit / a.nh, h = unit % a.nh;
   bool mine = row < a.n_rows;
   if (mine) {
@@ -616,24 +625,41 @@ __global__ void __launch_bounds__(128) k_kv_prefill_join(PfArgs p) {
     mine = row >= s0 && row < s0 + c;
   }
   pb_grid_wait();
-  if (!mine) return;
+  // (every lane of a head has the same `mine`; the others follow for the shuffles)
+  const size_t step = (size_t)a.n_rows * a.nh, at = mine ? (size_t)row * a.nh + h : 0;
+  float2 q[MOST];
   float m = -INFINITY;
-  for (int s = 0; s < p.ns; s++) {
-    const float2 q = __ldcg(p.ml + ((size_t)s * a.n_rows + row) * a.nh + h);
-    if (q.y != 0.0f) m = fmaxf(m, q.x);
+#pragma unroll
+  for (int i = 0; i < MOST; i++) {
+    const int s = i * L + l;
+    q[i] = mine && s < p.ns ? __ldcg(p.ml + s * step + at) : make_float2(-INFINITY, 0.0f);
+    if (q[i].y != 0.0f) m = fmaxf(m, q[i].x);      // an empty split wrote no sums
   }
-  float l = 0.0f;
+#pragma unroll
+  for (int o = L / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float ll = 0.0f;
+#pragma unroll
+  for (int i = 0; i < MOST; i++) {
+    q[i].x = q[i].y != 0.0f ? kv_ex2(q[i].x - m) : 0.0f;
+    ll += q[i].x * q[i].y;
+  }
+#pragma unroll
+  for (int o = L / 2; o; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
   float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int s = 0; s < p.ns; s++) {
-    const size_t at = ((size_t)s * a.n_rows + row) * a.nh + h;
-    const float2 q = __ldcg(p.ml + at);
-    if (q.y == 0.0f) continue;      // an empty split wrote no sums
-    const float f = kv_ex2(q.x - m);
-    const float4 z = __ldcg(reinterpret_cast<const float4*>(p.part + at * D + e));
-    l += f * q.y;
-    y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
+#pragma unroll
+  for (int i = 0; i < MOST; i++) {
+    if (i * L >= p.ns) break;
+    const int n = min(L, p.ns - i * L);
+#pragma unroll 8
+    for (int k = 0; k < n; k++) {
+      const float f = __shfl_sync(0xffffffffu, q[i].x, (threadIdx.x & 31) / L * L + k);
+      if (!mine || f == 0.0f) continue;
+      const float4 z = __ldcg(reinterpret_cast<const float4*>(p.part + ((i * L + k) * step + at) * D + e));
+      y.x += f * z.x; y.y += f * z.y; y.z += f * z.z; y.w += f * z.w;
+    }
   }
-  const float f = l != 0.0f ? 1.0f / l : 0.0f;
+  if (!mine) return;
+  const float f = ll != 0.0f ? 1.0f / ll : 0.0f;
   char* o = a.out + (long long)row * a.ldo + (size_t)h * (D * 2) + e * 2;
   uint2 w;
   if (p.out_bf16) w = make_uint2(kv_down<PB_DT_BF16>(y.x * f, y.y * f), kv_down<PB_DT_BF16>(y.z * f, y.w * f));
@@ -641,30 +667,26 @@ __global__ void __launch_bounds__(128) k_kv_prefill_join(PfArgs p) {
   *reinterpret_cast<uint2*>(o) = w;
 }
 
-// launch shape: CTAs of ng * tq tokens, and splits of the key line where those
+// launch shape: CTAs of NG * tq tokens, and splits of the key line where those
 // leave SMs idle (at least 4 tiles each)
-#ifndef PF_NG
-#define PF_NG 0
-#endif
 struct PfPlan {
-  int tq, ng, ns;
+  int tq, ns;
   long long items, part, ml;   // CTAs per split; floats
 };
 PfPlan pf_plan(const pb_kv_pages* c, int n_seq, int max_len, int n_tok, int n_heads, int window, int sinks) {
   PfPlan p{};
   const int grp = n_heads / c->n_kv;
   p.tq = 128 / (grp > 0 ? grp : 1) / 8 * 8;       // whole 8-row groups of the swizzle
-  p.ng = PF_NG ? PF_NG : 2;
-  const int tok = p.ng * p.tq, sms = pb_num_sms() * (p.ng == 1 ? 2 : 1);
+  const int tok = NG * p.tq;
   p.items = ((long long)n_tok / tok + (n_seq < n_tok ? n_seq : n_tok)) * c->n_kv;
   long long tiles = (max_len + PF_KT - 1) / PF_KT;
   if (window > 0) {
     const long long seen = ((long long)window + tok + 2 * PF_KT - 1) / PF_KT + (sinks + PF_KT - 1) / PF_KT;
     if (seen < tiles) tiles = seen;
   }
-  long long ns = p.items > 0 ? sms / p.items : 1;
+  long long ns = p.items > 0 ? pb_num_sms() / p.items : 1;
   if (ns > tiles / 4) ns = tiles / 4;
-  p.ns = ns < 1 ? 1 : (int)ns;
+  p.ns = ns < 1 ? 1 : (ns > 160 ? 160 : (int)ns);     // (what the join's lanes hold)
   const long long rows = (long long)p.ns * n_tok * n_heads;
   p.part = p.ns > 1 ? rows * c->head_dim : 0;
   p.ml = p.ns > 1 ? rows * 2 : 0;
@@ -725,20 +747,16 @@ int pf_maps(const pb_kv_pages* c, PfArgs* p, CUtensorMap* mk, CUtensorMap* mv, C
   return PB_OK;
 }
 
-template <int D, int CT, int NG>
-int pf_launch(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const PfArgs& p, long long items, cudaStream_t st) {
+template <int D, int CT>
+int pf_run(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const PfArgs& p, const PfPlan& pl, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
-  if (int rc = kv_smem(k_kv_prefill<D, CT, NG>, PfGeo<D, NG>::SMEM, done)) return rc;
-  if (int rc = kv_launch(k_kv_prefill<D, CT, NG>, (unsigned)(items * p.ns), PfGeo<D, NG>::T, PfGeo<D, NG>::SMEM, st, false,
-                         "k_kv_prefill", mk, mv, mq, p))
+  if (int rc = kv_smem(k_kv_prefill<D, CT>, PfGeo<D>::SMEM, done)) return rc;
+  if (int rc = kv_launch(k_kv_prefill<D, CT>, (unsigned)(pl.items * p.ns), PfGeo<D>::T, PfGeo<D>::SMEM, st, false, "k_kv_prefill",
+                         mk, mv, mq, p))
     return rc;
   if (p.ns == 1) return PB_OK;
   const long long blocks = ((long long)p.a.n_rows * p.a.nh * (D / 4) + 127) / 128;
   return kv_launch(k_kv_prefill_join<D>, (unsigned)blocks, 128, 0, st, true, "k_kv_prefill_join", p);
-}
-template <int D, int CT>
-int pf_run(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const PfArgs& p, const PfPlan& pl, cudaStream_t st) {
-  return pl.ng == 1 ? pf_launch<D, CT, 1>(mk, mv, mq, p, pl.items, st) : pf_launch<D, CT, 2>(mk, mv, mq, p, pl.items, st);
 }
 
 }  // namespace
