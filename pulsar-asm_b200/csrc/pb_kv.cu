@@ -1,7 +1,6 @@
 // pb_kv.cu -- the paged K/V cache: append (head norms, rotation and store in
 // one pass) and evict (the rows of largest accumulated weight to fresh pages).
-#include "pb_kv.cuh"
-#include <climits>
+#include "pb_kvattn.cuh"
 
 namespace {
 
@@ -223,6 +222,7 @@ struct EvictArgs {
 };
 
 constexpr int EV_T = 1024;
+static_assert(EV_T == 32 * 32, "one lane of warp 0 scans each warp's sum");
 
 PB_DEV unsigned ev_key(const EvictArgs& a, const int* trow, int h, int j) {
   const int page = kv_page(a.p, trow, j);
@@ -238,6 +238,7 @@ __global__ void __launch_bounds__(EV_T) k_kv_select(EvictArgs a) {
   __shared__ int s_bin, s_need;
   const int b = blockIdx.x / a.p.n_kv, h = blockIdx.x % a.p.n_kv;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  pb_grid_launch_dependents();
   const int len = kv_len(a.len[b], a.max_len);
   if (len <= a.budget) return;   // every row stays: the gather needs no list
   const int* trow = a.p.table + (size_t)b * a.p.table_ld;
@@ -345,6 +346,7 @@ __global__ void __launch_bounds__(EV_GT) k_kv_gather(EvictArgs a, int chunks) {
   const int l = threadIdx.x % LPH, g = threadIdx.x / LPH;
   const int len = kv_len(a.len[b], a.max_len), n = min(len, a.budget);
   const int ps = 1 << a.p.shift;
+  pb_grid_wait();      // the lists
   if (chunk == 0 && h == 0 && threadIdx.x == 0) a.new_len[b] = n;   // may be len[b]: min(n, budget) = n either way
   const int* trow = a.p.table + (size_t)b * a.p.table_ld;
   const int* drow = a.dst + (size_t)b * a.dst_ld;
@@ -519,8 +521,7 @@ extern "C" int pb_kv_evict(const pb_kv_pages* c, int n_seq, const int* d_table, 
   const int per = EV_GT / (c->head_dim / 8) * EV_R, chunks = (cap + per - 1) / per;
   const long long blocks = (long long)n_seq * c->n_kv * chunks;
   if (blocks > INT_MAX) return pb_set_error(PB_EINVAL, "pb_kv_evict: %d sequences of %d rows", n_seq, cap);
-  if (c->head_dim == 64) k_kv_gather<64><<<(unsigned)blocks, EV_GT, 0, st>>>(a, chunks);
-  else k_kv_gather<128><<<(unsigned)blocks, EV_GT, 0, st>>>(a, chunks);
-  PB_LAUNCHED("k_kv_gather");
-  return PB_OK;
+  const bool pdl = max_len > budget;   // (behind the select)
+  return c->head_dim == 64 ? kv_launch(k_kv_gather<64>, (unsigned)blocks, EV_GT, 0, st, pdl, "k_kv_gather", a, chunks)
+                           : kv_launch(k_kv_gather<128>, (unsigned)blocks, EV_GT, 0, st, pdl, "k_kv_gather", a, chunks);
 }
