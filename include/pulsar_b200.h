@@ -387,41 +387,73 @@ typedef struct {
   int dtype, n_pages, page_size, n_kv, head_dim;
   long long page_stride, head_stride, row_stride;
 } pb_kv_pages;
-/* n_tok rows d_qkv [n_tok][ldx] (bf16, fp16 or fp32; q heads | k heads | v
- * heads, anything behind them ignored: the gate values of a q|k|v|gate
- * projection): RMS norm of every query and key head (weights d_qnorm,
- * d_knorm fp32 [head_dim]; NULL: no norm), rotation of the pairs (i, i +
- * head_dim/2), i < half, by row d_pos[i] (NULL: d_slot[i]) of d_cos / d_sin
- * (fp32 [n_rope][half]; half 0: none), the query heads to d_q [n_tok][ldq],
- * the K and V rows to row d_slot[i] of sequence d_seq[i], whose weight
- * becomes 0. A row whose sequence, slot, page or position is out of range is
- * padding: nothing is written for it. Two rows of a call with the same
- * sequence and slot leave that cache row undefined. q must not overlap qkv. */
-int pb_kv_append(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const void* d_qkv, int x_dtype,
-                 long long ldx, int n_tok, int n_heads, const int* d_seq, const int* d_slot, const int* d_pos,
-                 const float* d_qnorm, const float* d_knorm, float eps, const float* d_cos, const float* d_sin, int half,
-                 int n_rope, void* d_q, long long ldq, void* stream);
+/* The arguments of the calls, every pointer a device pointer; `table` holds
+ * n_seq rows of table_ld page numbers. */
+typedef struct {
+  const int* table;
+  const void* qkv;
+  const int* seq;
+  const int* slot;
+  const int* pos;
+  const float* qnorm;
+  const float* knorm;
+  const float* cos;
+  const float* sin;
+  void* q;
+  long long ldx, ldq;
+  int n_seq, table_ld, x_dtype, n_tok, n_heads, half, n_rope;
+  float eps;
+} pb_kv_append_args;
+typedef struct {
+  const int* table;
+  const int* start;            /* pb_kv_prefill only */
+  const int* len;
+  const void* q;
+  void* out;
+  void* scratch;
+  long long ldq, ldo, scratch_bytes;
+  int n_seq, table_ld, max_len, n_heads, window, sinks, out_dtype;
+  int n_tok;                   /* pb_kv_prefill: rows of q */
+  int accumulate;              /* pb_kv_decode only */
+  float scale;
+} pb_kv_attention_args;
+typedef struct {
+  const int* table;
+  const int* len;
+  const int* dst_table;
+  int* new_len;
+  void* scratch;
+  long long scratch_bytes;
+  int n_seq, table_ld, max_len, dst_ld, budget, sinks, recent;
+} pb_kv_evict_args;
+/* n_tok rows qkv [n_tok][ldx] (x_dtype bf16, fp16 or fp32; q heads | k heads |
+ * v heads, anything behind them ignored: the gate values of a q|k|v|gate
+ * projection): RMS norm of every query and key head (weights qnorm, knorm
+ * fp32 [head_dim]; NULL: no norm), rotation of the pairs (i, i + head_dim/2),
+ * i < half, by row pos[i] (NULL: slot[i]) of cos / sin (fp32 [n_rope][half];
+ * half 0: none), the query heads to q [n_tok][ldq] (the cache's dtype), the K
+ * and V rows to row slot[i] of sequence seq[i], whose weight becomes 0. A row
+ * whose sequence, slot, page or position is out of range is padding: nothing
+ * is written for it. Two rows of a call with the same sequence and slot leave
+ * that cache row undefined. q must not overlap qkv. */
+int pb_kv_append(const pb_kv_pages* c, const pb_kv_append_args* a, void* stream);
 /* attention of one token per sequence: row b of q (heads [n_heads][head_dim],
- * row stride ldq) is the token at row t = d_len[b] - 1 of sequence b, whose
- * K and V are stored. It sees row j <= t, and with a window > 0 only
+ * row stride ldq) is the token at row t = len[b] - 1 of sequence b, whose K
+ * and V are stored. It sees row j <= t, and with a window > 0 only
  * j > t - window or j < sinks. out[b] = sum_j p_j v_j, p = softmax(scale
  * q.k_j); 0 where nothing is seen. out_dtype PB_DT_BF16 or PB_DT_F16.
  * accumulate: the cache's weight of every seen row and K/V head grows by the
  * sum of p_j over the query heads of its group; two sequences of one call
  * then share no page. out must not overlap q.                                */
 long long pb_kv_decode_scratch(const pb_kv_pages* c, int n_seq, int max_len, int n_heads, int accumulate);
-int pb_kv_decode(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const int* d_len, int max_len,
-                 int n_heads, const void* d_q, long long ldq, float scale, int window, int sinks, int accumulate,
-                 void* d_out, int out_dtype, long long ldo, void* d_scratch, long long scratch_bytes, void* stream);
+int pb_kv_decode(const pb_kv_pages* c, const pb_kv_attention_args* a, void* stream);
 /* attention of the last rows of each sequence (prompt chunks, whole prompts,
- * a ragged batch of them): rows d_start[b] .. d_start[b+1]-1 of q (d_start
- * int32 [n_seq + 1], ascending, within [0, n_tok]) are the tokens at the
- * last rows of sequence b, each with the masks of pb_kv_decode. Rows of out
- * outside every sequence are left as they were.                              */
+ * a ragged batch of them): rows start[b] .. start[b+1]-1 of q (start int32
+ * [n_seq + 1], ascending, within [0, n_tok]) are the tokens at the last rows
+ * of sequence b, each with the masks of pb_kv_decode. Rows of out outside
+ * every sequence are left as they were.                                      */
 long long pb_kv_prefill_scratch(const pb_kv_pages* c, int n_seq, int max_len, int n_tok, int n_heads);
-int pb_kv_prefill(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const int* d_start, const int* d_len,
-                  int max_len, int n_tok, int n_heads, const void* d_q, long long ldq, float scale, int window, int sinks,
-                  void* d_out, int out_dtype, long long ldo, void* d_scratch, long long scratch_bytes, void* stream);
+int pb_kv_prefill(const pb_kv_pages* c, const pb_kv_attention_args* a, void* stream);
 /* synchronise `stream` and report a bounded wait inside the current device's
  * pb_kv_prefill kernels that gave up since the last report: PB_OK or PB_ECUDA */
 int pb_kv_status(void* stream);
@@ -429,15 +461,13 @@ int pb_kv_status(void* stream);
  * rows and, up to `budget` rows in all, those of the largest weight (equal
  * weights: the lowest row first; a weight that is not above 0 counts as 0).
  * The kept rows move in order, with their weights, to rows 0.. of the pages
- * of d_dst_table (row stride dst_ld), which must share no page with the
- * sequences' own; d_new_len[b] = min(d_len[b], budget) (may be d_len). A
- * sequence within the budget moves whole. The old pages are left as they are.
- * Kept rows stay rotated by their own positions, so later tokens go to slot
- * new_len.. with their true positions in pb_kv_append's d_pos.               */
+ * of dst_table (rows of dst_ld), which must share no page with the sequences'
+ * own; new_len[b] = min(len[b], budget) (may be len itself). A sequence
+ * within the budget moves whole. The old pages are left as they are. Kept
+ * rows stay rotated by their own positions, so later tokens go to slot
+ * new_len.. with their true positions in pb_kv_append's pos.                 */
 long long pb_kv_evict_scratch(const pb_kv_pages* c, int n_seq, int max_len, int budget);
-int pb_kv_evict(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const int* d_len, int max_len,
-                const int* d_dst_table, int dst_ld, int* d_new_len, int budget, int sinks, int recent, void* d_scratch,
-                long long scratch_bytes, void* stream);
+int pb_kv_evict(const pb_kv_pages* c, const pb_kv_evict_args* a, void* stream);
 
 /* ---- sampler: sample_topkpp + frand01 (pulsar_arm/bonsai2/fwd8.c:465-521) ----
  * for each of B rows of fp32 logits (row b at d_logits + b*ld, n values):

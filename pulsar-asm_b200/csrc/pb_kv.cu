@@ -428,36 +428,36 @@ int kv_pool(const char* who, const pb_kv_pages* c, int n_seq, const int* d_table
   return PB_OK;
 }
 
-extern "C" int pb_kv_append(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const void* d_qkv, int x_dtype,
-                            long long ldx, int n_tok, int n_heads, const int* d_seq, const int* d_slot, const int* d_pos,
-                            const float* d_qnorm, const float* d_knorm, float eps, const float* d_cos, const float* d_sin,
-                            int half, int n_rope, void* d_q, long long ldq, void* stream) {
+extern "C" int pb_kv_append(const pb_kv_pages* c, const pb_kv_append_args* g, void* stream) {
+  if (!g) return pb_set_error(PB_EINVAL, "pb_kv_append: null argument");
+  const int n_tok = g->n_tok, n_heads = g->n_heads, half = g->half, x_dtype = g->x_dtype;
+  const long long ldx = g->ldx, ldq = g->ldq;
   AppendArgs a{};
-  if (int rc = kv_pool("pb_kv_append", c, n_seq, d_table, table_ld, &a.p)) return rc;
+  if (int rc = kv_pool("pb_kv_append", c, g->n_seq, g->table, g->table_ld, &a.p)) return rc;
   const int D = c->head_dim;
-  if (!d_qkv || !d_seq || !d_slot || !d_q) return pb_set_error(PB_EINVAL, "pb_kv_append: null argument");
+  if (!g->qkv || !g->seq || !g->slot || !g->q) return pb_set_error(PB_EINVAL, "pb_kv_append: null argument");
   if (x_dtype != PB_DT_BF16 && x_dtype != PB_DT_F32 && x_dtype != PB_DT_F16)
     return pb_set_error(PB_EINVAL, "pb_kv_append: x_dtype %d", x_dtype);
   if (n_tok < 0 || n_heads <= 0 || n_heads > 65536) return pb_set_error(PB_EINVAL, "pb_kv_append: %d tokens, %d heads", n_tok, n_heads);
-  if (half < 0 || half > D / 2 || (half > 0 && (!d_cos || !d_sin || n_rope <= 0)))
-    return pb_set_error(PB_EINVAL, "pb_kv_append: half %d of head_dim %d, %d positions", half, D, n_rope);
+  if (half < 0 || half > D / 2 || (half > 0 && (!g->cos || !g->sin || g->n_rope <= 0)))
+    return pb_set_error(PB_EINVAL, "pb_kv_append: half %d of head_dim %d, %d positions", half, D, g->n_rope);
   const long long wide = (long long)(n_heads + 2 * c->n_kv) * D;
   const int xb = x_dtype == PB_DT_F32 ? 4 : 2;
   if (ldx < wide || ldq < (long long)n_heads * D) return pb_set_error(PB_EINVAL, "pb_kv_append: row strides %lld, %lld", ldx, ldq);
-  if (((reinterpret_cast<size_t>(d_qkv) | reinterpret_cast<size_t>(d_q) | (size_t)(ldx * xb) | (size_t)(ldq * 2)) & 15))
+  if (((reinterpret_cast<size_t>(g->qkv) | reinterpret_cast<size_t>(g->q) | (size_t)(ldx * xb) | (size_t)(ldq * 2)) & 15))
     return pb_set_error(PB_EINVAL, "pb_kv_append: qkv and q rows must be 16-byte aligned");
   if (n_tok == 0) return PB_OK;
-  if (kv_overlap(d_qkv, ((size_t)(n_tok - 1) * ldx + wide) * xb, d_q, ((size_t)(n_tok - 1) * ldq + (size_t)n_heads * D) * 2))
+  if (kv_overlap(g->qkv, ((size_t)(n_tok - 1) * ldx + wide) * xb, g->q, ((size_t)(n_tok - 1) * ldq + (size_t)n_heads * D) * 2))
     return pb_set_error(PB_EINVAL, "pb_kv_append: q overlaps qkv");
-  a.x = static_cast<const char*>(d_qkv);
+  a.x = static_cast<const char*>(g->qkv);
   a.ldx = ldx * xb;
-  a.q = static_cast<char*>(d_q);
+  a.q = static_cast<char*>(g->q);
   a.ldq = ldq * 2;
-  a.seq = d_seq; a.slot = d_slot; a.pos = d_pos;
-  a.qn = d_qnorm; a.kn = d_knorm; a.cs = d_cos; a.sn = d_sin;
-  a.n_tok = n_tok; a.nh = n_heads; a.half = half; a.n_rope = n_rope;
-  a.rows = table_ld * c->page_size;
-  a.eps = eps;
+  a.seq = g->seq; a.slot = g->slot; a.pos = g->pos;
+  a.qn = g->qnorm; a.kn = g->knorm; a.cs = g->cos; a.sn = g->sin;
+  a.n_tok = n_tok; a.nh = n_heads; a.half = half; a.n_rope = g->n_rope;
+  a.rows = g->table_ld * c->page_size;
+  a.eps = g->eps;
   // few tokens: a warp per group of heads; many: up to 6 groups a warp (12,
   // a whole token of 48 heads, left a longer tail: 47 against 43 us; 1 paid
   // the look-ups each time: 81)
@@ -490,13 +490,14 @@ extern "C" long long pb_kv_evict_scratch(const pb_kv_pages* c, int n_seq, int ma
   return (long long)n_seq * c->n_kv * cap * 4;
 }
 
-extern "C" int pb_kv_evict(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const int* d_len, int max_len,
-                           const int* d_dst_table, int dst_ld, int* d_new_len, int budget, int sinks, int recent,
-                           void* d_scratch, long long scratch_bytes, void* stream) {
+extern "C" int pb_kv_evict(const pb_kv_pages* c, const pb_kv_evict_args* g, void* stream) {
+  if (!g) return pb_set_error(PB_EINVAL, "pb_kv_evict: null argument");
+  const int n_seq = g->n_seq, table_ld = g->table_ld, budget = g->budget, sinks = g->sinks, recent = g->recent, dst_ld = g->dst_ld;
+  int max_len = g->max_len;
   EvictArgs a{};
-  if (int rc = kv_pool("pb_kv_evict", c, n_seq, d_table, table_ld, &a.p)) return rc;
-  if (!c->weight || !d_len || !d_dst_table || !d_new_len) return pb_set_error(PB_EINVAL, "pb_kv_evict: null argument");
-  if (d_dst_table == d_table) return pb_set_error(PB_EINVAL, "pb_kv_evict: the fresh pages must not be the old ones");
+  if (int rc = kv_pool("pb_kv_evict", c, n_seq, g->table, table_ld, &a.p)) return rc;
+  if (!c->weight || !g->len || !g->dst_table || !g->new_len) return pb_set_error(PB_EINVAL, "pb_kv_evict: null argument");
+  if (g->dst_table == g->table) return pb_set_error(PB_EINVAL, "pb_kv_evict: the fresh pages must not be the old ones");
   if (max_len <= 0 || max_len > table_ld * c->page_size) max_len = table_ld * c->page_size;
   if (budget <= 0 || sinks < 0 || recent < 0 || sinks > budget || recent > budget - sinks)
     return pb_set_error(PB_EINVAL, "pb_kv_evict: budget %d, %d first and %d last rows", budget, sinks, recent);
@@ -504,13 +505,13 @@ extern "C" int pb_kv_evict(const pb_kv_pages* c, int n_seq, const int* d_table, 
   if (dst_ld <= 0 || dst_ld < (cap + c->page_size - 1) / c->page_size)
     return pb_set_error(PB_EINVAL, "pb_kv_evict: %d rows need more than %d pages", cap, dst_ld);
   const long long need = pb_kv_evict_scratch(c, n_seq, max_len, budget);
-  if (need > 0 && (!d_scratch || scratch_bytes < need))
-    return pb_set_error(PB_EINVAL, "pb_kv_evict: scratch of %lld bytes, %lld needed", scratch_bytes, need);
+  if (need > 0 && (!g->scratch || g->scratch_bytes < need))
+    return pb_set_error(PB_EINVAL, "pb_kv_evict: scratch of %lld bytes, %lld needed", g->scratch_bytes, need);
   if (n_seq == 0) return PB_OK;
-  a.len = d_len; a.new_len = d_new_len; a.dst = d_dst_table; a.dst_ld = dst_ld;
+  a.len = g->len; a.new_len = g->new_len; a.dst = g->dst_table; a.dst_ld = dst_ld;
   a.max_len = max_len; a.budget = budget; a.sinks = sinks; a.recent = recent;
   a.lcap = cap;
-  a.list = static_cast<int*>(d_scratch);
+  a.list = static_cast<int*>(g->scratch);
   cudaStream_t st = (cudaStream_t)stream;
   if (max_len > budget) {
     // keys in shared memory up to 40 KB (no opt-in needed), the rest re-read

@@ -581,31 +581,24 @@ extern "C" long long pb_kv_decode_scratch(const pb_kv_pages* c, int n_seq, int m
   return 4 * (p.part + p.ml + p.lse + p.score);
 }
 
-extern "C" int pb_kv_decode(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const int* d_len, int max_len,
-                            int n_heads, const void* d_q, long long ldq, float scale, int window, int sinks, int accumulate,
-                            void* d_out, int out_dtype, long long ldo, void* d_scratch, long long scratch_bytes, void* stream) {
+extern "C" int pb_kv_decode(const pb_kv_pages* c, const pb_kv_attention_args* g, void* stream) {
   DcArgs d{};
-  KvPool p{};
-  if (int rc = kv_pool("pb_kv_decode", c, n_seq, d_table, table_ld, &p)) return rc;
-  if (int rc = attn_check("pb_kv_decode", c, p, d_len, &max_len, table_ld, n_seq, n_heads, d_q, ldq, scale, window, sinks, d_out,
-                          out_dtype, ldo, &d.a))
-    return rc;
+  if (int rc = attn_check("pb_kv_decode", c, g, g ? g->n_seq : 0, &d.a)) return rc;
+  const int n_seq = g->n_seq, max_len = d.a.max_len, accumulate = g->accumulate;
   if (accumulate && !c->weight) return pb_set_error(PB_EINVAL, "pb_kv_decode: the cache keeps no weights");
   if ((long long)n_seq * c->n_kv * ((max_len + 63) / 64) > INT_MAX)
     return pb_set_error(PB_EINVAL, "pb_kv_decode: %d sequences of %d rows", n_seq, max_len);
-  const long long need = pb_kv_decode_scratch(c, n_seq, max_len, n_heads, accumulate);
-  if (need > 0 && (!d_scratch || scratch_bytes < need || (reinterpret_cast<size_t>(d_scratch) & 15)))
-    return pb_set_error(PB_EINVAL, "pb_kv_decode: scratch of %lld bytes, %lld needed (16-byte aligned)", scratch_bytes, need);
+  const DcPlan pl = dc_plan(c, n_seq, max_len, g->n_heads, accumulate);
+  if (int rc = attn_scratch("pb_kv_decode", g, 4 * (pl.part + pl.ml + pl.lse + pl.score))) return rc;
   if (n_seq == 0) return PB_OK;
-  const DcPlan pl = dc_plan(c, n_seq, max_len, n_heads, accumulate);
-  float* f = static_cast<float*>(d_scratch);
+  float* f = static_cast<float*>(g->scratch);
   d.part = f;
   d.ml = f + pl.part;
   d.a.lse = accumulate ? d.ml + pl.ml : nullptr;
   d.score = accumulate ? d.a.lse + pl.lse : nullptr;
   d.grid = pl.grid;
   d.grp2 = pl.grp2;
-  d.out_bf16 = out_dtype == PB_DT_BF16;
+  d.out_bf16 = g->out_dtype == PB_DT_BF16;
   cudaStream_t st = (cudaStream_t)stream;
   return c->head_dim == 64 ? dc_run<64>(d, c->dtype, pl.join, st) : dc_run<128>(d, c->dtype, pl.join, st);
 }

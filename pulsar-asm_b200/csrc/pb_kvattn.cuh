@@ -79,35 +79,42 @@ PB_DEV void kv_cp16(uint32_t dst, const char* src) {
 template <int N>
 PB_DEV void kv_cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 PB_DEV void kv_cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-inline int attn_check(const char* who, const pb_kv_pages* c, const KvPool& p, const int* d_len, int* max_len, int table_ld, int rows,
-               int n_heads, const void* d_q, long long ldq, float scale, int window, int sinks, const void* d_out, int out_dtype,
-               long long ldo, AttnKvArgs* a) {
-  if (!d_len || !d_q || !d_out) return pb_set_error(PB_EINVAL, "%s: null argument", who);
-  if (out_dtype != PB_DT_F16 && out_dtype != PB_DT_BF16)
-    return pb_set_error(PB_ENOTSUP, "%s: out_dtype %d (fp16 or bf16)", who, out_dtype);
-  if (n_heads <= 0 || n_heads % c->n_kv || n_heads / c->n_kv > 16)
-    return pb_set_error(PB_ENOTSUP, "%s: %d query heads over %d K/V heads (a whole number, at most 16)", who, n_heads, c->n_kv);
-  if (rows < 0 || window < 0 || sinks < 0 || !(scale > 0.0f) || scale > 1e30f)
-    return pb_set_error(PB_EINVAL, "%s: %d rows, window %d, %d sinks, scale %g", who, rows, window, sinks, (double)scale);
-  const long long wide = (long long)n_heads * c->head_dim;
-  if (ldq < wide || ldo < wide || ((reinterpret_cast<size_t>(d_q) | reinterpret_cast<size_t>(d_out)) & 15) || ((ldq | ldo) & 7))
-    return pb_set_error(PB_EINVAL, "%s: q and out rows must be 16-byte aligned (row strides %lld, %lld)", who, ldq, ldo);
-  if (rows > 0 && kv_overlap(d_q, ((size_t)(rows - 1) * ldq + wide) * 2, d_out, ((size_t)(rows - 1) * ldo + wide) * 2))
+// the checks of an attention call of `rows` query rows; fills a but for its
+// prefill part
+inline int attn_check(const char* who, const pb_kv_pages* c, const pb_kv_attention_args* g, int rows, AttnKvArgs* a) {
+  if (!g) return pb_set_error(PB_EINVAL, "%s: null argument", who);
+  if (int rc = kv_pool(who, c, g->n_seq, g->table, g->table_ld, &a->p)) return rc;
+  if (!g->len || !g->q || !g->out) return pb_set_error(PB_EINVAL, "%s: null argument", who);
+  if (g->out_dtype != PB_DT_F16 && g->out_dtype != PB_DT_BF16)
+    return pb_set_error(PB_ENOTSUP, "%s: out_dtype %d (fp16 or bf16)", who, g->out_dtype);
+  if (g->n_heads <= 0 || g->n_heads % c->n_kv || g->n_heads / c->n_kv > 16)
+    return pb_set_error(PB_ENOTSUP, "%s: %d query heads over %d K/V heads (a whole number, at most 16)", who, g->n_heads, c->n_kv);
+  if (rows < 0 || g->window < 0 || g->sinks < 0 || !(g->scale > 0.0f) || g->scale > 1e30f)
+    return pb_set_error(PB_EINVAL, "%s: %d rows, window %d, %d sinks, scale %g", who, rows, g->window, g->sinks, (double)g->scale);
+  const long long wide = (long long)g->n_heads * c->head_dim;
+  if (g->ldq < wide || g->ldo < wide || ((reinterpret_cast<size_t>(g->q) | reinterpret_cast<size_t>(g->out)) & 15) ||
+      ((g->ldq | g->ldo) & 7))
+    return pb_set_error(PB_EINVAL, "%s: q and out rows must be 16-byte aligned (row strides %lld, %lld)", who, g->ldq, g->ldo);
+  if (rows > 0 && kv_overlap(g->q, ((size_t)(rows - 1) * g->ldq + wide) * 2, g->out, ((size_t)(rows - 1) * g->ldo + wide) * 2))
     return pb_set_error(PB_EINVAL, "%s: out overlaps q", who);
-  if (*max_len <= 0 || *max_len > table_ld * c->page_size) *max_len = table_ld * c->page_size;
-  a->p = p;
-  a->len = d_len;
-  a->q = static_cast<const char*>(d_q);
-  a->out = static_cast<char*>(const_cast<void*>(d_out));
-  a->ldq = ldq * 2;
-  a->ldo = ldo * 2;
+  const int most = g->table_ld * c->page_size;
+  a->len = g->len;
+  a->q = static_cast<const char*>(g->q);
+  a->out = static_cast<char*>(g->out);
+  a->ldq = g->ldq * 2;
+  a->ldo = g->ldo * 2;
   a->n_rows = rows;
-  a->nh = n_heads;
-  a->grp = n_heads / c->n_kv;
-  a->max_len = *max_len;
-  a->window = window;
-  a->sinks = window > 0 ? sinks : 0;
-  a->scale2 = scale * 1.4426950408889634f;
+  a->nh = g->n_heads;
+  a->grp = g->n_heads / c->n_kv;
+  a->max_len = g->max_len <= 0 || g->max_len > most ? most : g->max_len;
+  a->window = g->window;
+  a->sinks = g->window > 0 ? g->sinks : 0;
+  a->scale2 = g->scale * 1.4426950408889634f;
+  return PB_OK;
+}
+inline int attn_scratch(const char* who, const pb_kv_attention_args* g, long long need) {
+  if (need > 0 && (!g->scratch || g->scratch_bytes < need || (reinterpret_cast<size_t>(g->scratch) & 15)))
+    return pb_set_error(PB_EINVAL, "%s: scratch of %lld bytes, %lld needed (16-byte aligned)", who, g->scratch_bytes, need);
   return PB_OK;
 }
 

@@ -768,29 +768,21 @@ extern "C" long long pb_kv_prefill_scratch(const pb_kv_pages* c, int n_seq, int 
   return 4 * (p.part + p.ml);
 }
 
-extern "C" int pb_kv_prefill(const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, const int* d_start,
-                             const int* d_len, int max_len, int n_tok, int n_heads, const void* d_q, long long ldq, float scale,
-                             int window, int sinks, void* d_out, int out_dtype, long long ldo, void* d_scratch,
-                             long long scratch_bytes, void* stream) {
-  KvPool pool{};
+extern "C" int pb_kv_prefill(const pb_kv_pages* c, const pb_kv_attention_args* g, void* stream) {
   PfArgs p{};
-  if (int rc = kv_pool("pb_kv_prefill", c, n_seq, d_table, table_ld, &pool)) return rc;
-  if (!d_start) return pb_set_error(PB_EINVAL, "pb_kv_prefill: null argument");
-  if (int rc = attn_check("pb_kv_prefill", c, pool, d_len, &max_len, table_ld, n_tok, n_heads, d_q, ldq, scale, window, sinks,
-                          d_out, out_dtype, ldo, &p.a))
-    return rc;
-  if (n_seq == 0 || n_tok == 0) return PB_OK;
-  const PfPlan pl = pf_plan(c, n_seq, max_len, n_tok, n_heads, window, sinks);
+  if (int rc = attn_check("pb_kv_prefill", c, g, g ? g->n_tok : 0, &p.a)) return rc;
+  if (!g->start) return pb_set_error(PB_EINVAL, "pb_kv_prefill: null argument");
+  const int n_tok = g->n_tok, n_heads = g->n_heads;
+  if (g->n_seq == 0 || n_tok == 0) return PB_OK;
+  const PfPlan pl = pf_plan(c, g->n_seq, p.a.max_len, n_tok, n_heads, g->window, g->sinks);
   if (pl.items * pl.ns > INT_MAX || (long long)n_tok * n_heads * 32 > INT_MAX)
     return pb_set_error(PB_EINVAL, "pb_kv_prefill: %d tokens of %d heads", n_tok, n_heads);
-  const long long need = 4 * (pl.part + pl.ml);
-  if (need > 0 && (!d_scratch || scratch_bytes < need || (reinterpret_cast<size_t>(d_scratch) & 15)))
-    return pb_set_error(PB_EINVAL, "pb_kv_prefill: scratch of %lld bytes, %lld needed (16-byte aligned)", scratch_bytes, need);
-  p.a.start = d_start;
+  if (int rc = attn_scratch("pb_kv_prefill", g, 4 * (pl.part + pl.ml))) return rc;
+  p.a.start = g->start;
   p.tq = pl.tq;
   p.ns = pl.ns;
-  p.out_bf16 = out_dtype == PB_DT_BF16;
-  p.part = static_cast<float*>(d_scratch);
+  p.out_bf16 = g->out_dtype == PB_DT_BF16;
+  p.part = static_cast<float*>(g->scratch);
   p.ml = reinterpret_cast<float2*>(p.part + pl.part);
   cudaStream_t st = (cudaStream_t)stream;
   CUtensorMap mk, mv, mq;

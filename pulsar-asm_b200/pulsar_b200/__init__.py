@@ -16,6 +16,7 @@ The interface mirrors the reference engine's entry points:
 """
 import ctypes as C
 import os
+import struct
 import subprocess
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -91,11 +92,10 @@ def lib():
     L.pb_tq_store.argtypes = [i, vp, i, vp, vp, vp, vp, i, i, vp]
     L.pb_tq_attention.argtypes = [i, vp, vp, vp, vp, vp, i, i, i, vp, vp, vp]
     L.pb_sample_topkpp.argtypes = [vp, i, i, C.c_longlong, C.c_float, C.c_float, i, C.c_float, vp, vp, vp]
-    ll, f, kvp = C.c_longlong, C.c_float, C.POINTER(_KVPages)
-    L.pb_kv_append.argtypes = [kvp, i, vp, i, vp, i, ll, i, i, vp, vp, vp, vp, vp, f, vp, vp, i, i, vp, ll, vp]
-    L.pb_kv_decode.argtypes = [kvp, i, vp, i, vp, i, i, vp, ll, f, i, i, i, vp, i, ll, vp, ll, vp]
-    L.pb_kv_prefill.argtypes = [kvp, i, vp, i, vp, vp, i, i, i, vp, ll, f, i, i, vp, i, ll, vp, ll, vp]
-    L.pb_kv_evict.argtypes = [kvp, i, vp, i, vp, i, vp, i, vp, i, i, i, vp, ll, vp]
+    ll, kvp = C.c_longlong, C.POINTER(_KVPages)
+    # (their argument structs are passed as packed bytes, see KVPages)
+    for fn in (L.pb_kv_append, L.pb_kv_decode, L.pb_kv_prefill, L.pb_kv_evict):
+        fn.argtypes = [kvp, C.c_char_p, vp]
     L.pb_kv_decode_scratch.argtypes = [kvp, i, i, i, i]
     L.pb_kv_prefill_scratch.argtypes = [kvp, i, i, i, i]
     L.pb_kv_evict_scratch.argtypes = [kvp, i, i, i]
@@ -421,30 +421,36 @@ class KVPages:
             raise PBError(-1, "%s: a contiguous fp32 tensor %s on %s" % (what, list(shape), self.device))
         return t.data_ptr()
 
-    def _call(self, fn, args, need, scratch, stream):
-        """fn(*args[, scratch, bytes], stream) on the pools' device; need None: a function without scratch"""
-        torch, dev = self._torch, self._dev
-        if torch._C._cuda_getDevice() != dev:
-            with torch.cuda.device(dev):
-                return self._call(fn, args, need, scratch, stream)
-        s = torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream
-        if need is None:
-            rc = fn(*args, s)
-        elif scratch is None and need > 0:
+    # pb_kv_append_args, pb_kv_attention_args, pb_kv_evict_args: pointers, long longs, ints, a float. A ctypes
+    # argument costs 0.1 us, a packed one a quarter of that.
+    _APPEND, _ATTEND, _EVICT = struct.Struct("@10P2q7if"), struct.Struct("@6P3q9if"), struct.Struct("@5Pq7i")
+
+    def _stream_of(self, stream):
+        return self._torch._C._cuda_getCurrentRawStream(self._dev) if stream is None else stream.cuda_stream
+
+    def _scratch(self, need, scratch, stream):
+        """(pointer, bytes, what keeps it alive)"""
+        torch = self._torch
+        if scratch is None:
+            if need <= 0:
+                return 0, 0, None
             if stream is None:
                 scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
             else:   # allocated on the stream that uses it, so that it is not reused under the call
                 with torch.cuda.stream(stream):
                     scratch = torch.empty(need, dtype=torch.uint8, device=self.device)
-            rc = fn(*args, scratch.data_ptr(), need, s)
-        elif scratch is None:
-            rc = fn(*args, None, 0, s)
-        else:
-            if scratch.get_device() != dev or not scratch.is_contiguous():
-                raise PBError(-1, "scratch: a contiguous tensor on %s" % self.device)
-            rc = fn(*args, scratch.data_ptr(), scratch.numel() * scratch.element_size(), s)
-        if rc:
-            check(rc)
+            return scratch.data_ptr(), need, scratch
+        if scratch.get_device() != self._dev or not scratch.is_contiguous():
+            raise PBError(-1, "scratch: a contiguous tensor on %s" % self.device)
+        return scratch.data_ptr(), scratch.numel() * scratch.element_size(), scratch
+
+    def _on_device(self, method, *args, **kw):
+        """the call again, with the pools' device as the current one"""
+        with self._torch.cuda.device(self._dev):
+            return method(*args, **kw)
+
+    def _away(self):
+        return self._torch._C._cuda_getDevice() != self._dev
 
     def _bytes(self, fn, *shape):
         # (a negative max_len or count, which the call itself refuses, needs no scratch)
@@ -457,6 +463,8 @@ class KVPages:
         """norm and rotate the heads of qkv [n][>= (n_heads + 2 n_kv) dim] (bf16, fp16 or fp32), query heads to
         q [n][n_heads][dim] (the cache's dtype), K and V rows to row slot[i] of sequence seq[i]; pos: the rotation's
         position per token (None: slot); cos, sin [positions][half] (None: no rotation)"""
+        if self._away():
+            return self._on_device(self.append, table, seq, slot, pos, qkv, q, q_norm, k_norm, eps, cos, sin, stream)
         shape = q.shape
         qp, ldq = self._heads("q", q, shape, self.dtype)
         n, nh = shape[0], shape[1]
@@ -469,48 +477,64 @@ class KVPages:
         ns = len(table)
         tp, pages = self._table("table", table, ns)
         one, d = (n,), (self.head_dim,)
-        if cos is None:
-            rope = None, None, 0, 0
-        else:
+        cp, sp, half, n_rope = 0, 0, 0, 0
+        if cos is not None:
             cs = cos.shape
             if len(cs) != 2:
                 raise PBError(-1, "cos: a tensor [positions][half]")
-            rope = self._floats("cos", cos, cs), self._floats("sin", sin, cs), cs[1], cs[0]
-        self._call(lib().pb_kv_append, (
-            self._r, ns, tp, pages, qkv.data_ptr(), _dtype_code(qkv), xt[0] if n > 1 else wide, n, nh,
-            self._ints("seq", seq, one), self._ints("slot", slot, one), None if pos is None else self._ints("pos", pos, one),
-            None if q_norm is None else self._floats("q_norm", q_norm, d),
-            None if k_norm is None else self._floats("k_norm", k_norm, d), eps, *rope, qp, ldq), None, None, stream)
+            n_rope, half = cs
+            cp, sp = self._floats("cos", cos, cs), self._floats("sin", sin, cs)
+        args = self._APPEND.pack(
+            tp, qkv.data_ptr(), self._ints("seq", seq, one), self._ints("slot", slot, one),
+            0 if pos is None else self._ints("pos", pos, one), 0 if q_norm is None else self._floats("q_norm", q_norm, d),
+            0 if k_norm is None else self._floats("k_norm", k_norm, d), cp, sp, qp, xt[0] if n > 1 else wide, ldq, ns, pages,
+            _dtype_code(qkv), n, nh, half, n_rope, eps)
+        rc = lib().pb_kv_append(self._r, args, self._stream_of(stream))
+        if rc:
+            check(rc)
 
     def decode(self, table, length, q, out, max_len=0, scale=None, window=0, sinks=0, accumulate=False, scratch=None,
                stream=None):
         """attention of one token per sequence: q [n_seq][n_heads][dim] (the cache's dtype) at row length[b] - 1 of
         each cache, into out (bf16 or fp16, q's shape); scale: 1 / sqrt(dim) by default; accumulate: add each seen
         row's probabilities to the cache's weight"""
+        if self._away():
+            return self._on_device(self.decode, table, length, q, out, max_len, scale, window, sinks, accumulate, scratch, stream)
         L = lib()
         shape = q.shape
         qp, ldq = self._heads("q", q, shape, self.dtype)
         op, ldo = self._heads("out", out, shape, None)
         n, nh, acc = shape[0], shape[1], 1 if accumulate else 0
         tp, pages = self._table("table", table, n)
-        need = self._bytes(L.pb_kv_decode_scratch, n, min(max_len, pages * self.page_size) or pages * self.page_size, nh, acc)
-        self._call(L.pb_kv_decode, (
-            self._r, n, tp, pages, self._ints("length", length, (n,)), max_len, nh, qp, ldq,
-            self._scale if scale is None else scale, window, sinks, acc, op, _dtype_code(out), ldo), need, scratch, stream)
+        rows = pages * self.page_size
+        need = self._bytes(L.pb_kv_decode_scratch, n, max_len if 0 < max_len < rows else rows, nh, acc)
+        wp, wn, _keep = self._scratch(need, scratch, stream)
+        args = self._ATTEND.pack(tp, 0, self._ints("length", length, (n,)), qp, op, wp, ldq, ldo, wn, n, pages, max_len, nh,
+                                 window, sinks, _dtype_code(out), 0, acc, self._scale if scale is None else scale)
+        rc = L.pb_kv_decode(self._r, args, self._stream_of(stream))
+        if rc:
+            check(rc)
 
     def prefill(self, table, start, length, q, out, max_len=0, scale=None, window=0, sinks=0, scratch=None, stream=None):
         """attention of the last rows of each sequence: rows start[b] .. start[b+1]-1 of q [n][n_heads][dim] are the
         tokens at the last rows of sequence b, into out (bf16 or fp16, q's shape)"""
+        if self._away():
+            return self._on_device(self.prefill, table, start, length, q, out, max_len, scale, window, sinks, scratch, stream)
         L = lib()
         shape = q.shape
         qp, ldq = self._heads("q", q, shape, self.dtype)
         op, ldo = self._heads("out", out, shape, None)
         n, nt, nh = len(length), shape[0], shape[1]
         tp, pages = self._table("table", table, n)
-        need = self._bytes(L.pb_kv_prefill_scratch, n, min(max_len, pages * self.page_size) or pages * self.page_size, nt, nh)
-        self._call(L.pb_kv_prefill, (
-            self._r, n, tp, pages, self._ints("start", start, (n + 1,)), self._ints("length", length, (n,)), max_len, nt, nh,
-            qp, ldq, self._scale if scale is None else scale, window, sinks, op, _dtype_code(out), ldo), need, scratch, stream)
+        rows = pages * self.page_size
+        need = self._bytes(L.pb_kv_prefill_scratch, n, max_len if 0 < max_len < rows else rows, nt, nh)
+        wp, wn, _keep = self._scratch(need, scratch, stream)
+        args = self._ATTEND.pack(tp, self._ints("start", start, (n + 1,)), self._ints("length", length, (n,)), qp, op, wp, ldq,
+                                 ldo, wn, n, pages, max_len, nh, window, sinks, _dtype_code(out), nt, 0,
+                                 self._scale if scale is None else scale)
+        rc = L.pb_kv_prefill(self._r, args, self._stream_of(stream))
+        if rc:
+            check(rc)
 
     def status(self, stream=None):
         """synchronise and raise if a prefill kernel recorded a wait that gave up"""
@@ -520,14 +544,20 @@ class KVPages:
     def evict(self, table, length, dst_table, new_length, budget, sinks=0, recent=0, max_len=0, scratch=None, stream=None):
         """keep up to `budget` rows of each sequence and K/V head (the first `sinks`, the last `recent`, then the
         largest weights), moved in order to the pages of dst_table; new_length (may be length) receives the lengths"""
+        if self._away():
+            return self._on_device(self.evict, table, length, dst_table, new_length, budget, sinks, recent, max_len, scratch, stream)
         L = lib()
         n = len(length)
         tp, pages = self._table("table", table, n)
         dp, fresh = self._table("dst_table", dst_table, n)
-        need = self._bytes(L.pb_kv_evict_scratch, n, min(max_len, pages * self.page_size) or pages * self.page_size, budget)
-        self._call(L.pb_kv_evict, (
-            self._r, n, tp, pages, self._ints("length", length, (n,)), max_len, dp, fresh,
-            self._ints("new_length", new_length, (n,)), budget, sinks, recent), need, scratch, stream)
+        rows = pages * self.page_size
+        need = self._bytes(L.pb_kv_evict_scratch, n, max_len if 0 < max_len < rows else rows, budget)
+        wp, wn, _keep = self._scratch(need, scratch, stream)
+        args = self._EVICT.pack(tp, self._ints("length", length, (n,)), dp, self._ints("new_length", new_length, (n,)), wp, wn, n,
+                                pages, max_len, fresh, budget, sinks, recent)
+        rc = L.pb_kv_evict(self._r, args, self._stream_of(stream))
+        if rc:
+            check(rc)
 
 
 class Q1Tensor:

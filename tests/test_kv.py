@@ -19,36 +19,51 @@ def pool(pb, **over):
     return pb._KVPages(**d)
 
 
-def append(pb, c=None, **over):
-    a = dict(n_seq=4, table=P, table_ld=10, x=P + (1 << 36), x_dtype=pb.PB_DT_BF16, ldx=48 * 128, n_tok=7, nh=32, seq=P,
-             slot=P, pos=P, qn=P, kn=P, eps=1e-5, cos=P, sin=P, half=64, n_rope=1000, q=P + (1 << 38), ldq=32 * 128, st=None)
-    a.update(over)
+class Append(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in "table x seq slot pos qn kn cos sin q".split()] + \
+               [(n, C.c_longlong) for n in ("ldx", "ldq")] + \
+               [(n, C.c_int) for n in "n_seq table_ld x_dtype n_tok nh half n_rope".split()] + [("eps", C.c_float)]
+
+
+class Attend(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in "table start len q out scratch".split()] + \
+               [(n, C.c_longlong) for n in ("ldq", "ldo", "bytes")] + \
+               [(n, C.c_int) for n in "n_seq table_ld max_len nh window sinks od n_tok acc".split()] + [("scale", C.c_float)]
+
+
+class Evict(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in "table len dst new scratch".split()] + [("bytes", C.c_longlong)] + \
+               [(n, C.c_int) for n in "n_seq table_ld max_len dst_ld budget sinks recent".split()]
+
+
+def call(pb, fn, kind, base, c, over):
     c = pool(pb) if c is None else c
-    return pb.lib().pb_kv_append(C.byref(c), *a.values())
+    a = kind(**{**base, **over})
+    return getattr(pb.lib(), fn)(C.byref(c), C.cast(C.byref(a), C.c_char_p), None)
+
+
+def append(pb, c=None, **over):
+    return call(pb, "pb_kv_append", Append,
+                dict(n_seq=4, table=P, table_ld=10, x=P + (1 << 36), x_dtype=pb.PB_DT_BF16, ldx=48 * 128, n_tok=7, nh=32, seq=P,
+                     slot=P, pos=P, qn=P, kn=P, eps=1e-5, cos=P, sin=P, half=64, n_rope=1000, q=P + (1 << 38), ldq=32 * 128), c, over)
+
+
+ATTEND = dict(n_seq=4, table=P, table_ld=10, len=P, max_len=0, nh=32, q=P + (1 << 36), ldq=32 * 128, scale=0.1, window=0,
+              sinks=0, out=P + (1 << 38), od=0, ldo=32 * 128, scratch=P, bytes=1 << 40)
 
 
 def decode(pb, c=None, **over):
-    a = dict(n_seq=4, table=P, table_ld=10, len=P, max_len=0, nh=32, q=P + (1 << 36), ldq=32 * 128, scale=0.1, window=0,
-             sinks=0, acc=0, out=P + (1 << 38), od=pb.PB_DT_BF16, ldo=32 * 128, scratch=P, bytes=1 << 40, st=None)
-    a.update(over)
-    c = pool(pb) if c is None else c
-    return pb.lib().pb_kv_decode(C.byref(c), *a.values())
+    return call(pb, "pb_kv_decode", Attend, ATTEND, c, over)
 
 
 def prefill(pb, c=None, **over):
-    a = dict(n_seq=4, table=P, table_ld=10, start=P, len=P, max_len=0, n_tok=9, nh=32, q=P + (1 << 36), ldq=32 * 128,
-             scale=0.1, window=0, sinks=0, out=P + (1 << 38), od=pb.PB_DT_BF16, ldo=32 * 128, scratch=P, bytes=1 << 40, st=None)
-    a.update(over)
-    c = pool(pb) if c is None else c
-    return pb.lib().pb_kv_prefill(C.byref(c), *a.values())
+    return call(pb, "pb_kv_prefill", Attend, dict(ATTEND, start=P, n_tok=9), c, over)
 
 
 def evict(pb, c=None, **over):
-    a = dict(n_seq=4, table=P, table_ld=10, len=P, max_len=0, dst=P + 4096, dst_ld=8, new=P, budget=200, sinks=4, recent=50,
-             scratch=P, bytes=1 << 40, st=None)
-    a.update(over)
-    c = pool(pb) if c is None else c
-    return pb.lib().pb_kv_evict(C.byref(c), *a.values())
+    return call(pb, "pb_kv_evict", Evict,
+                dict(n_seq=4, table=P, table_ld=10, len=P, max_len=0, dst=P + 4096, dst_ld=8, new=P, budget=200, sinks=4, recent=50,
+                     scratch=P, bytes=1 << 40), c, over)
 
 
 EINVAL, ENOTSUP = -1, -8
@@ -125,6 +140,20 @@ def test_weights_are_needed(pb):
                                   dict(recent=-1), dict(sinks=151), dict(sinks=201, recent=0), dict(dst_ld=6), dict(dst_ld=0)])
 def test_evict_refusals(pb, over):
     assert evict(pb, **over) == EINVAL
+
+
+def test_null_arguments(pb):
+    L = pb.lib()
+    for fn in (L.pb_kv_append, L.pb_kv_decode, L.pb_kv_prefill, L.pb_kv_evict):
+        assert fn(C.byref(pool(pb)), None, None) == EINVAL and fn(None, b"\0" * 256, None) == EINVAL
+    assert prefill(pb, start=None) == EINVAL
+
+
+def test_packed_arguments_match_the_structs(pb):
+    for fmt, kind in ((pb.KVPages._APPEND, Append), (pb.KVPages._ATTEND, Attend), (pb.KVPages._EVICT, Evict)):
+        vals = [float(i) if t is C.c_float else i for i, (_, t) in enumerate(kind._fields_, 1)]
+        s = kind.from_buffer_copy(fmt.pack(*vals).ljust(C.sizeof(kind), b"\0"))
+        assert [getattr(s, n) for n, _ in kind._fields_] == vals
 
 
 def test_calls_of_no_sequence(pb):
