@@ -370,6 +370,7 @@ int pb_tq_attention(int bits, const float* d_q, const uint32_t* d_kcode, const f
  *    K and V pools and slices of larger ones all do.
  *  - A table entry outside [0, n_pages) names no page: rows there are not
  *    seen, stored or moved. Entries that no seen row needs are not used.
+ *  - Sequences may share pages (a common prefix) where they are only read.
  *  - Lengths live on the device and are read there, so a captured graph
  *    replays with each step's lengths. max_len bounds them (0: the table's
  *    rows); a length above it counts as max_len, one below 0 as 0.
@@ -443,8 +444,8 @@ int pb_kv_append(const pb_kv_pages* c, const pb_kv_append_args* a, void* stream)
  * j > t - window or j < sinks. out[b] = sum_j p_j v_j, p = softmax(scale
  * q.k_j); 0 where nothing is seen. out_dtype PB_DT_BF16 or PB_DT_F16.
  * accumulate: the cache's weight of every seen row and K/V head grows by the
- * sum of p_j over the query heads of its group; two sequences of one call
- * then share no page. out must not overlap q.                                */
+ * sum of p_j over the query heads of its group; the rows that the call sees
+ * then lie on different pages, no page twice. out must not overlap q.        */
 long long pb_kv_decode_scratch(const pb_kv_pages* c, int n_seq, int max_len, int n_heads, int accumulate);
 int pb_kv_decode(const pb_kv_pages* c, const pb_kv_attention_args* a, void* stream);
 /* attention of the last rows of each sequence (prompt chunks, whole prompts,

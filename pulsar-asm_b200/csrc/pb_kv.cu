@@ -383,15 +383,15 @@ __global__ void __launch_bounds__(EV_GT) k_kv_gather(EvictArgs a, int chunks) {
 }  // namespace
 
 int kv_pool(const char* who, const pb_kv_pages* c, int n_seq, const int* d_table, int table_ld, KvPool* p) {
-  if (!c || !c->k || !c->v || !d_table) return pb_set_error(PB_EINVAL, "%s: null argument", who);
+  if (!c || !c->k || !c->v || (n_seq > 0 && !d_table)) return pb_set_error(PB_EINVAL, "%s: null argument", who);
   if (c->dtype != PB_DT_F16 && c->dtype != PB_DT_BF16)
     return pb_set_error(PB_ENOTSUP, "%s: cache dtype %d (fp16 or bf16)", who, c->dtype);
   if (c->head_dim != 64 && c->head_dim != 128)
     return pb_set_error(PB_ENOTSUP, "%s: head_dim %d (64 or 128)", who, c->head_dim);
   if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1)))
     return pb_set_error(PB_ENOTSUP, "%s: page_size %d (16, 32, 64, 128 or 256)", who, c->page_size);
-  if (c->n_pages <= 0 || c->n_kv <= 0 || c->n_kv > 1024 || n_seq < 0 || n_seq > (1 << 20) || table_ld <= 0 ||
-      table_ld > (1 << 30) / c->page_size)
+  if (c->n_pages <= 0 || c->n_kv <= 0 || c->n_kv > 1024 || n_seq < 0 || n_seq > (1 << 20) ||
+      (n_seq > 0 && table_ld <= 0) || table_ld > (1 << 30) / c->page_size)
     return pb_set_error(PB_EINVAL, "%s: %d pages, %d K/V heads, %d sequences, table of %d pages", who, c->n_pages, c->n_kv,
                         n_seq, table_ld);
   if (((reinterpret_cast<size_t>(c->k) | reinterpret_cast<size_t>(c->v)) & 15) ||
@@ -435,6 +435,7 @@ extern "C" int pb_kv_append(const pb_kv_pages* c, const pb_kv_append_args* g, vo
   AppendArgs a{};
   if (int rc = kv_pool("pb_kv_append", c, g->n_seq, g->table, g->table_ld, &a.p)) return rc;
   const int D = c->head_dim;
+  if (n_tok == 0) return PB_OK;
   if (!g->qkv || !g->seq || !g->slot || !g->q) return pb_set_error(PB_EINVAL, "pb_kv_append: null argument");
   if (x_dtype != PB_DT_BF16 && x_dtype != PB_DT_F32 && x_dtype != PB_DT_F16)
     return pb_set_error(PB_EINVAL, "pb_kv_append: x_dtype %d", x_dtype);
@@ -446,7 +447,6 @@ extern "C" int pb_kv_append(const pb_kv_pages* c, const pb_kv_append_args* g, vo
   if (ldx < wide || ldq < (long long)n_heads * D) return pb_set_error(PB_EINVAL, "pb_kv_append: row strides %lld, %lld", ldx, ldq);
   if (((reinterpret_cast<size_t>(g->qkv) | reinterpret_cast<size_t>(g->q) | (size_t)(ldx * xb) | (size_t)(ldq * 2)) & 15))
     return pb_set_error(PB_EINVAL, "pb_kv_append: qkv and q rows must be 16-byte aligned");
-  if (n_tok == 0) return PB_OK;
   if (kv_overlap(g->qkv, ((size_t)(n_tok - 1) * ldx + wide) * xb, g->q, ((size_t)(n_tok - 1) * ldq + (size_t)n_heads * D) * 2))
     return pb_set_error(PB_EINVAL, "pb_kv_append: q overlaps qkv");
   a.x = static_cast<const char*>(g->qkv);
@@ -496,6 +496,7 @@ extern "C" int pb_kv_evict(const pb_kv_pages* c, const pb_kv_evict_args* g, void
   int max_len = g->max_len;
   EvictArgs a{};
   if (int rc = kv_pool("pb_kv_evict", c, n_seq, g->table, table_ld, &a.p)) return rc;
+  if (n_seq == 0) return PB_OK;
   if (!c->weight || !g->len || !g->dst_table || !g->new_len) return pb_set_error(PB_EINVAL, "pb_kv_evict: null argument");
   if (g->dst_table == g->table) return pb_set_error(PB_EINVAL, "pb_kv_evict: the fresh pages must not be the old ones");
   if (max_len <= 0 || max_len > table_ld * c->page_size) max_len = table_ld * c->page_size;
@@ -507,7 +508,6 @@ extern "C" int pb_kv_evict(const pb_kv_pages* c, const pb_kv_evict_args* g, void
   const long long need = pb_kv_evict_scratch(c, n_seq, max_len, budget);
   if (need > 0 && (!g->scratch || g->scratch_bytes < need))
     return pb_set_error(PB_EINVAL, "pb_kv_evict: scratch of %lld bytes, %lld needed", g->scratch_bytes, need);
-  if (n_seq == 0) return PB_OK;
   a.len = g->len; a.new_len = g->new_len; a.dst = g->dst_table; a.dst_ld = dst_ld;
   a.max_len = max_len; a.budget = budget; a.sinks = sinks; a.recent = recent;
   a.lcap = cap;

@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs
   int total, b, first;
   kv_locate<32 * DC_W>(a.p.n_seq, [&](int i) { return dc_seq<TILE>(a, i).nt * a.p.n_kv; }, [&](int n) { return dc_cut(blockIdx.x, n, dc_pieces(d, n)); }, total, b, first);
   const int pieces = dc_pieces(d, total);
-  if ((int)blockIdx.x >= pieces) return;   // CTA-uniform
+  if ((int)blockIdx.x >= pieces || b < 0) return;   // CTA-uniform
   const int x0 = dc_cut(blockIdx.x, total, pieces), x1 = dc_cut(blockIdx.x + 1, total, pieces);
   DcAt at;
   at.b = b;
@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(DcGeo<D>::TILE) k_kv_weight(DcArgs d) {
   kv_locate<TILE>(a.p.n_seq, [&](int i) { return dc_seq<TILE>(a, i).nt * a.p.n_kv; },
                   [&](int n) { return dc_cut(blockIdx.x, n, min(n, (int)gridDim.x)); }, total, b, first);
   const int pieces = min(total, (int)gridDim.x);
-  if ((int)blockIdx.x >= pieces) return;
+  if ((int)blockIdx.x >= pieces || b < 0) return;
   const int x0 = dc_cut(blockIdx.x, total, pieces), x1 = dc_cut(blockIdx.x + 1, total, pieces);
   DcAt at;
   at.b = b;
@@ -585,12 +585,12 @@ extern "C" int pb_kv_decode(const pb_kv_pages* c, const pb_kv_attention_args* g,
   DcArgs d{};
   if (int rc = attn_check("pb_kv_decode", c, g, g ? g->n_seq : 0, &d.a)) return rc;
   const int n_seq = g->n_seq, max_len = d.a.max_len, accumulate = g->accumulate;
+  if (n_seq == 0) return PB_OK;
   if (accumulate && !c->weight) return pb_set_error(PB_EINVAL, "pb_kv_decode: the cache keeps no weights");
   if ((long long)n_seq * c->n_kv * ((max_len + 63) / 64) > INT_MAX)
     return pb_set_error(PB_EINVAL, "pb_kv_decode: %d sequences of %d rows", n_seq, max_len);
   const DcPlan pl = dc_plan(c, n_seq, max_len, g->n_heads, accumulate);
   if (int rc = attn_scratch("pb_kv_decode", g, 4 * (pl.part + pl.ml + pl.lse + pl.score))) return rc;
-  if (n_seq == 0) return PB_OK;
   float* f = static_cast<float*>(g->scratch);
   d.part = f;
   d.ml = f + pl.part;

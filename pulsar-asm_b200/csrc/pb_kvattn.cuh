@@ -28,8 +28,8 @@ PB_DEV float kv_ex2(float x) {
 
 // Sequences laid end to end on a line, count(i) units each: the line's length
 // and, for the unit pick(length), its sequence and that sequence's first unit
-// (undefined when it lies past the line: the caller has no work then). A
-// thread of the CTA's T sums a run of sequences; the runs are scanned.
+// (b = -1 when it lies past the line: the caller has no work then). A thread
+// of the CTA's T sums a run of sequences; the runs are scanned.
 template <int T, typename C, typename F>
 PB_DEV void kv_locate(int n_seq, C count, F pick, int& total, int& b, int& first) {
   __shared__ int wsum[T / 32], found[2];
@@ -44,6 +44,7 @@ PB_DEV void kv_locate(int n_seq, C count, F pick, int& total, int& b, int& first
     if (lane >= o) inc += v;
   }
   if (lane == 31) wsum[warp] = inc;
+  if (t == 0) found[0] = -1;
   __syncthreads();
   int pre = inc - own;
   total = 0;
@@ -84,18 +85,20 @@ PB_DEV void kv_cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory")
 inline int attn_check(const char* who, const pb_kv_pages* c, const pb_kv_attention_args* g, int rows, AttnKvArgs* a) {
   if (!g) return pb_set_error(PB_EINVAL, "%s: null argument", who);
   if (int rc = kv_pool(who, c, g->n_seq, g->table, g->table_ld, &a->p)) return rc;
+  if (rows < 0) return pb_set_error(PB_EINVAL, "%s: %d rows", who, rows);
+  if (rows == 0 || g->n_seq == 0) return PB_OK;      // nothing to do: the caller returns
   if (!g->len || !g->q || !g->out) return pb_set_error(PB_EINVAL, "%s: null argument", who);
   if (g->out_dtype != PB_DT_F16 && g->out_dtype != PB_DT_BF16)
     return pb_set_error(PB_ENOTSUP, "%s: out_dtype %d (fp16 or bf16)", who, g->out_dtype);
   if (g->n_heads <= 0 || g->n_heads % c->n_kv || g->n_heads / c->n_kv > 16)
     return pb_set_error(PB_ENOTSUP, "%s: %d query heads over %d K/V heads (a whole number, at most 16)", who, g->n_heads, c->n_kv);
-  if (rows < 0 || g->window < 0 || g->sinks < 0 || !(g->scale > 0.0f) || g->scale > 1e30f)
-    return pb_set_error(PB_EINVAL, "%s: %d rows, window %d, %d sinks, scale %g", who, rows, g->window, g->sinks, (double)g->scale);
+  if (g->window < 0 || g->sinks < 0 || !(g->scale > 0.0f) || g->scale > 1e30f)
+    return pb_set_error(PB_EINVAL, "%s: window %d, %d sinks, scale %g", who, g->window, g->sinks, (double)g->scale);
   const long long wide = (long long)g->n_heads * c->head_dim;
   if (g->ldq < wide || g->ldo < wide || ((reinterpret_cast<size_t>(g->q) | reinterpret_cast<size_t>(g->out)) & 15) ||
       ((g->ldq | g->ldo) & 7))
     return pb_set_error(PB_EINVAL, "%s: q and out rows must be 16-byte aligned (row strides %lld, %lld)", who, g->ldq, g->ldo);
-  if (rows > 0 && kv_overlap(g->q, ((size_t)(rows - 1) * g->ldq + wide) * 2, g->out, ((size_t)(rows - 1) * g->ldo + wide) * 2))
+  if (kv_overlap(g->q, ((size_t)(rows - 1) * g->ldq + wide) * 2, g->out, ((size_t)(rows - 1) * g->ldo + wide) * 2))
     return pb_set_error(PB_EINVAL, "%s: out overlaps q", who);
   const int most = g->table_ld * c->page_size;
   a->len = g->len;

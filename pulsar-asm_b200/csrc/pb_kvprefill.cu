@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
   int total, b, first;
   kv_locate<G::T>(a.p.n_seq, [&](int i) { int s0; return (pf_count(a, i, s0) + NG * p.tq - 1) / (NG * p.tq); },
                   [&](int n) { return idx < n ? n - 1 - idx : n; }, total, b, first);
-  if (idx >= total) return;   // CTA-uniform
+  if (idx >= total || b < 0) return;   // CTA-uniform
   int row0;
   const int cnt = pf_count(a, b, row0), tok0 = (total - 1 - idx - first) * NG * p.tq, ntok = min(NG * p.tq, cnt - tok0);
   row0 += tok0;
@@ -681,7 +681,7 @@ PfPlan pf_plan(const pb_kv_pages* c, int n_seq, int max_len, int n_tok, int n_he
   p.items = ((long long)n_tok / tok + (n_seq < n_tok ? n_seq : n_tok)) * c->n_kv;
   long long tiles = (max_len + PF_KT - 1) / PF_KT;
   if (window > 0) {
-    const long long seen = ((long long)window + tok + 2 * PF_KT - 1) / PF_KT + (sinks + PF_KT - 1) / PF_KT;
+    const long long seen = ((long long)window + tok + 2 * PF_KT - 1) / PF_KT + ((long long)sinks + PF_KT - 1) / PF_KT;
     if (seen < tiles) tiles = seen;
   }
   long long ns = p.items > 0 ? pb_num_sms() / p.items : 1;
@@ -771,11 +771,11 @@ extern "C" long long pb_kv_prefill_scratch(const pb_kv_pages* c, int n_seq, int 
 extern "C" int pb_kv_prefill(const pb_kv_pages* c, const pb_kv_attention_args* g, void* stream) {
   PfArgs p{};
   if (int rc = attn_check("pb_kv_prefill", c, g, g ? g->n_tok : 0, &p.a)) return rc;
-  if (!g->start) return pb_set_error(PB_EINVAL, "pb_kv_prefill: null argument");
   const int n_tok = g->n_tok, n_heads = g->n_heads;
   if (g->n_seq == 0 || n_tok == 0) return PB_OK;
+  if (!g->start) return pb_set_error(PB_EINVAL, "pb_kv_prefill: null argument");
   const PfPlan pl = pf_plan(c, g->n_seq, p.a.max_len, n_tok, n_heads, g->window, g->sinks);
-  if (pl.items * pl.ns > INT_MAX || (long long)n_tok * n_heads * 32 > INT_MAX)
+  if (pl.items * pl.ns > INT_MAX || (long long)n_tok * n_heads > INT_MAX)
     return pb_set_error(PB_EINVAL, "pb_kv_prefill: %d tokens of %d heads", n_tok, n_heads);
   if (int rc = attn_scratch("pb_kv_prefill", g, 4 * (pl.part + pl.ml))) return rc;
   p.a.start = g->start;

@@ -583,3 +583,142 @@ def test_two_streams_at_once(pb, cuda):
         c.h.decode(tb, length, q, o, stream=streams[n % 2])
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+def test_empty_calls(pb, cuda):
+    torch = cuda
+    c = Cache(pb, torch, [40, 20], 2, 64, 16, torch.float16, weights=True)
+    e = lambda *s, dt=torch.int32: torch.empty(s, dtype=dt, device="cuda")
+    q, none = e(0, 4, 64, dt=torch.float16), e(0)
+    c.h.append(c.dev(), none, none, None, e(0, 8 * 64, dt=torch.bfloat16), q)
+    c.h.decode(e(0, 3), none, q, q.clone(), accumulate=True)
+    c.h.prefill(e(0, 3), torch.zeros(1, dtype=torch.int32, device="cuda"), none, q, q.clone())
+    c.h.prefill(c.dev(), torch.zeros(3, dtype=torch.int32, device="cuda"), torch.tensor([40, 20], dtype=torch.int32, device="cuda"),
+                q, q.clone())
+    c.h.evict(e(0, 3), none, e(0, 3), none.clone(), 5)
+    torch.cuda.synchronize()
+
+
+def test_offsets_past_32_bits(pb, cuda):
+    """pages 2^30 elements apart: the third begins 2^32 bytes in"""
+    torch = cuda
+    ps, nkv, D, far = 32, 2, 64, 1 << 30
+    big = torch.zeros(2 * far + (1 << 20), dtype=torch.float16, device="cuda")
+    k = big.as_strided((3, nkv, ps, D), (far, ps * D, D, 1))
+    v = big.as_strided((3, nkv, ps, D), (far, ps * D, D, 1), storage_offset=1 << 16)
+    w = torch.rand((3, nkv, ps), device="cuda")
+    h = pb.KVPages(k, v, w)
+    rng = np.random.default_rng(0)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    table = i32([2, 1], [0, -1]).view(2, 2)
+    n = 50
+    x = torch.from_numpy(rng.standard_normal((n, 8 * D))).half().cuda()
+    q = torch.empty((n, 4, D), dtype=torch.float16, device="cuda")
+    h.append(table, torch.zeros(n, dtype=torch.int32, device="cuda"), torch.arange(n, dtype=torch.int32, device="cuda"), None, x, q)
+    torch.cuda.synchronize()
+    xs = x.view(n, 8, D)
+    assert torch.equal(q, xs[:, :4])
+    assert torch.equal(k[2].transpose(0, 1), xs[:32, 4:6]) and torch.equal(v[1, :, :18].transpose(0, 1), xs[32:, 6:])
+
+    class C_:
+        pass
+    c = C_()
+    c.k, c.v, c.table, c.ps = k, v, table[:1].cpu(), ps
+    out = torch.empty_like(q)
+    h.prefill(table[:1].contiguous(), i32(0, n), i32(n), q, out)
+    last = torch.empty((1, 4, D), dtype=torch.float16, device="cuda")
+    h.decode(table[:1].contiguous(), i32(n), q[-1:], last)
+    torch.cuda.synchronize()
+    (o, spread, slack, tiny), _ = oracle_rows(c, q, [n], [n], D ** -0.5, 0, 0)
+    check(torch, f64(out), o, spread, slack, tiny, n, torch.float16, torch.float16, "prefill")
+    check(torch, f64(last), o[-1:], spread[-1:], slack[-1:], tiny[-1:], n, torch.float16, torch.float16, "decode")
+    keep = KO.evict_rows(torch.cat([w[2, 1], w[1, 1]]).cpu().numpy(), n, 20, 1, 3)
+    new = i32(0)
+    rows = torch.cat([k[2, 1], k[1, 1]])[torch.tensor(keep).cuda()].clone()
+    h.evict(table[:1].contiguous(), i32(n), i32(0).view(1, 1), new, 20, sinks=1, recent=3)
+    torch.cuda.synchronize()
+    assert new.item() == 20 and torch.equal(k[0, 1, :20], rows)
+
+
+def test_shared_prefix_pages(pb, cuda):
+    """sequences whose tables begin with the same pages"""
+    torch = cuda
+    c = Cache(pb, torch, [64, 30, 45, 9], 2, 128, 16, torch.bfloat16, seed=11)
+    own = c.table.clone()
+    c.table = torch.full((3, 8), -1, dtype=torch.int32)
+    lens = [64 + 30, 64 + 45, 64 + 9]
+    for b in range(3):
+        c.table[b, :4] = own[0, :4]
+        m = -(-(lens[b] - 64) // 16)
+        c.table[b, 4:4 + m] = own[b + 1, :m]
+    counts = [30, 45, 9]
+    q = torch.randn((84, 8, 128), generator=c.g).bfloat16().cuda()
+    out, one = torch.empty_like(q), torch.empty((3, 8, 128), dtype=torch.bfloat16, device="cuda")
+    length = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    c.h.prefill(c.dev(), torch.tensor([0, 30, 75, 84], dtype=torch.int32, device="cuda"), length, q, out)
+    last = q[[29, 74, 83]].contiguous()
+    c.h.decode(c.dev(), length, last, one)
+    torch.cuda.synchronize()
+    (o, spread, slack, tiny), _ = oracle_rows(c, q, lens, counts, 128 ** -0.5, 0, 0)
+    check(torch, f64(out), o, spread, slack, tiny, 110, c.dt, torch.bfloat16, "prefill")
+    at = [29, 74, 83]
+    check(torch, f64(one), o[at], spread[at], slack[at], tiny[at], 110, c.dt, torch.bfloat16, "decode")
+
+
+def test_captured_prefill_and_evict(pb, cuda):
+    """replays follow the starts, lengths and tables that lie on the device then; scratch in the graph's own pool"""
+    torch = cuda
+    lens, counts = [700, 90], [20, 12]
+    c = Cache(pb, torch, lens + [64, 64], 2, 64, 16, torch.float16, "head", True, seed=21)
+    table, dst = c.table[:2].contiguous(), c.table[2:].contiguous()
+    c.table = table
+    q = torch.randn((40, 8, 64), generator=c.g).half().cuda()
+    out = torch.zeros_like(q)
+    start = torch.tensor([0, 20, 32], dtype=torch.int32, device="cuda")
+    length, new = torch.tensor(lens, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    tb, db = table.cuda(), dst.cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.h.prefill(tb, start, length, q, out, window=300, sinks=3)
+        c.h.evict(tb, length, db, new, 64, sinks=2, recent=8)
+    for lens, counts in (([700, 90], [20, 12]), ([333, 40], [5, 33]), ([64, 17], [1, 1])):
+        length.copy_(torch.tensor(lens, dtype=torch.int32))
+        start.copy_(torch.tensor(np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32))
+        out.fill_(2.0)
+        W, K = f64(c.w), f64(c.k)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        rows = sum(counts)
+        (o, spread, slack, tiny), _ = oracle_rows(c, q[:rows], lens, counts, 64 ** -0.5, 300, 3)
+        check(torch, f64(out)[:rows], o, spread, slack, tiny, 700, c.dt, torch.float16, lens)
+        assert (out[rows:] == 2.0).all() and new.tolist() == [min(n, 64) for n in lens]
+        for b, n in enumerate(lens):
+            pg, r, _ = KO.rows_of(table.numpy(), b, n, 16, c.n_pages)
+            to, tr, _ = KO.rows_of(dst.numpy(), b, min(n, 64), 16, c.n_pages)
+            for h in range(2):
+                at = KO.evict_rows(W[pg, h, r], n, 64, 2, 8)
+                assert np.array_equal(f64(c.k)[to, h, tr], K[pg[at], h, r[at]])
+
+
+def test_prefill_of_many_sequences(pb, cuda):
+    """more sequences than a CTA has threads; some without rows, one token each; the rows between them stay"""
+    torch = cuda
+    S = 500
+    rng = np.random.default_rng(4)
+    lens = rng.integers(1, 20, S).tolist()
+    counts = [int(rng.integers(0, min(4, n + 1))) for n in lens]
+    c = Cache(pb, torch, lens, 1, 64, 16, torch.float16, seed=31)
+    rows = sum(counts)
+    q = torch.randn((rows, 2, 64), generator=c.g).half().cuda()
+    out, one = torch.empty_like(q), torch.empty((S, 2, 64), dtype=torch.float16, device="cuda")
+    start = torch.tensor(np.concatenate([[0], np.cumsum(counts)]), dtype=torch.int32, device="cuda")
+    length = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    c.h.prefill(c.dev(), start, length, q, out)
+    q1 = torch.randn((S, 2, 64), generator=c.g).half().cuda()
+    c.h.decode(c.dev(), length, q1, one)
+    torch.cuda.synchronize()
+    (o, spread, slack, tiny), _ = oracle_rows(c, q, lens, counts, 64 ** -0.5, 0, 0)
+    check(torch, f64(out), o, spread, slack, tiny, 20, c.dt, torch.float16, "prefill")
+    (o, spread, slack, tiny), _ = oracle_rows(c, q1, lens, [1] * S, 64 ** -0.5, 0, 0)
+    check(torch, f64(one), o, spread, slack, tiny, 20, c.dt, torch.float16, "decode")

@@ -149,6 +149,18 @@ def test_null_arguments(pb):
     assert prefill(pb, start=None) == EINVAL
 
 
+def test_empty_calls_need_no_pointers(pb):
+    """empty torch tensors have null addresses"""
+    nothing = dict(table=None, table_ld=0, n_seq=0)
+    assert append(pb, n_tok=0, x=None, seq=None, slot=None, q=None) == 0
+    assert append(pb, n_tok=0, x=None, seq=None, slot=None, q=None, **nothing) == 0
+    assert decode(pb, len=None, q=None, out=None, scratch=None, bytes=0, **nothing) == 0
+    assert prefill(pb, n_tok=0, start=None, len=None, q=None, out=None, scratch=None, bytes=0, **nothing) == 0
+    assert prefill(pb, n_tok=0, q=None, out=None) == 0
+    assert evict(pb, len=None, dst=None, new=None, scratch=None, bytes=0, **nothing) == 0
+    assert prefill(pb, n_tok=-1) == EINVAL
+
+
 def test_packed_arguments_match_the_structs(pb):
     for fmt, kind in ((pb.KVPages._APPEND, Append), (pb.KVPages._ATTEND, Attend), (pb.KVPages._EVICT, Evict)):
         vals = [float(i) if t is C.c_float else i for i, (_, t) in enumerate(kind._fields_, 1)]
