@@ -33,6 +33,13 @@ PB_DEV float kv_ex2(float x) {
 template <int T, typename C, typename F>
 PB_DEV void kv_locate(int n_seq, C count, F pick, int& total, int& b, int& first) {
   __shared__ int wsum[T / 32], found[2];
+  if (n_seq == 1) {      // no search: one sequence's latency counts
+    total = count(0);
+    const int x = pick(total);
+    b = x >= 0 && x < total ? 0 : -1;
+    first = 0;
+    return;
+  }
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   const int per = (n_seq + T - 1) / T, b0 = min(n_seq, t * per), b1 = min(n_seq, b0 + per);
   int own = 0;

@@ -230,13 +230,27 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
   char* smk = smq + NG * G::Q;     // stage: K, V
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pb_grid_launch_dependents();
+  if (warp == PF_MMA) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(kv_s32(&tbase)), "n"(G::COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
 
   // ---- which rows: the last tiles of the line (the longest keys) first
   const int split = blockIdx.x % p.ns, kh = blockIdx.x / p.ns % a.p.n_kv, idx = blockIdx.x / p.ns / a.p.n_kv;
   int total, b, first;
-  kv_locate<G::T>(a.p.n_seq, [&](int i) { int s0; return (pf_count(a, i, s0) + NG * p.tq - 1) / (NG * p.tq); },
+  kv_locate<G::T>(a.p.n_seq, [&](int i) {
+                    int s0;
+                    asm volatile("prefetch.global.L1 [%0];" ::"l"(a.len + i));
+                    return (pf_count(a, i, s0) + NG * p.tq - 1) / (NG * p.tq);
+                  },
                   [&](int n) { return idx < n ? n - 1 - idx : n; }, total, b, first);
-  if (idx >= total || b < 0) return;   // CTA-uniform
+  if (idx >= total || b < 0) {         // CTA-uniform: no work
+    pf_fence_before();
+    __syncthreads();
+    pf_fence_after();
+    if (warp == PF_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tbase), "n"(G::COLS));
+    return;
+  }
   int row0;
   const int cnt = pf_count(a, b, row0), tok0 = (total - 1 - idx - first) * NG * p.tq, ntok = min(NG * p.tq, cnt - tok0);
   row0 += tok0;
@@ -265,18 +279,8 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     stop_f = 0;
   }
-  if (warp == PF_MMA) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(kv_s32(&tbase)), "n"(G::COLS));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  // does every 16-row block of the line have its page?
-  bool gap = false;
-  for (int u = threadIdx.x; u < n * (PF_KT / 16); u += G::T) {
-    const int j = pf_key(line, i0 + u / (PF_KT / 16)) + u % (PF_KT / 16) * 16;
-    if (j < line.end && kv_page(a.p, trow, j) < 0) gap = true;
-  }
   pf_fence_before();
-  const bool gaps = __syncthreads_or(gap);
+  __syncthreads();
   pf_fence_after();
   const uint32_t tmem = tbase;
   volatile int* stop = &stop_f;
@@ -443,6 +447,14 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
     const int ta = t0 + min(g * p.tq, ntok - 1), tb = t0 + min((g + 1) * p.tq - 1, ntok - 1);
     const int whi = a.window > 0 ? tb + 1 - a.window : 0;
     float m = -INFINITY, ms = 0.0f, l = 0.0f;                  // maximum of the raw scores, the same scaled, sum
+    // does every 16-row block of the line have its page? (while the first tile is on its way)
+    bool gap = false;
+    if (g < ng)
+      for (int u = lane; u < n * (PF_KT / 16); u += 32) {
+        const int j = pf_key(line, i0 + u / (PF_KT / 16)) + u % (PF_KT / 16) * 16;
+        if (j < line.end && kv_page(a.p, trow, j) < 0) gap = true;
+      }
+    const bool gaps = __any_sync(0xffffffffu, gap);
     const pf_f2 sc2 = pf_pk(a.scale2, a.scale2);
     const float over = 8.0f / a.scale2;
     float thr = -INFINITY;                                     // m + over
