@@ -435,6 +435,11 @@ __device__ __noinline__ void step_prologue(const StepArgs& a, float* sx, float* 
       default: gw_pass<SYNC>(gw); break;
     }
   }
+  // zeros behind an input shorter than its padded segments (the plain prologue
+  // writes its own): the padding's codes are zero, and 0 times what an earlier
+  // kernel left in shared memory may be NaN
+  if (pro != PRO_PLAIN)
+    for (int i = a.K + threadIdx.x; i < pb_kpad(a.K); i += 256) sx[padx(i)] = 0.0f;
   csync<SYNC>();
 }
 
