@@ -1069,6 +1069,9 @@ int bs_state_create(pb_bonsai* m, int max_ctx, uint16_t* kv_ext, int kv_bits, co
     if (cudaMemcpy(s->rope, tab.data(), tab.size() * 4, cudaMemcpyHostToDevice) != cudaSuccess)
       rc = pb_set_error(PB_ECUDA, "pb_bonsai_state_create: rope table");
   }
+  // the fills and the table are there before a stream that does not wait for the default one uses them
+  if (rc == PB_OK && cudaStreamSynchronize(nullptr) != cudaSuccess)
+    rc = pb_set_error(PB_ECUDA, "pb_bonsai_state_create: fill");
   if (rc != PB_OK) {
     cudaFree(s->mem); if (s->h_ctl) cudaFreeHost(s->h_ctl); cudaFree(s->tq_mem);
     delete s;
@@ -1224,7 +1227,10 @@ int bs_carve(const size_t* sizes, int n, char** mem, char** parts) {
     *mem = nullptr;
     return pb_set_error(PB_ENOMEM, "bonsai blocks: %zu bytes", tot);
   }
-  if (cudaMemset(*mem, 0, tot) != cudaSuccess) {
+  // The callers' streams do not wait for the default stream, on which the fill
+  // runs behind whatever is queued there: it is done before any of them writes here.
+  if (cudaMemset(*mem, 0, tot) != cudaSuccess || cudaStreamSynchronize(nullptr) != cudaSuccess) {
+    cudaGetLastError();
     cudaFree(*mem);
     *mem = nullptr;
     return pb_set_error(PB_ECUDA, "bonsai blocks: memset");

@@ -183,6 +183,12 @@ HookSession& session() {
   return S;
 }
 
+// Zeros in a new cache, there when it returns: the hooks' stream does not wait
+// for the default stream, which runs the fill behind whatever is queued on it.
+bool zeroed(void* p, size_t bytes) {
+  return cudaMemset(p, 0, bytes) == cudaSuccess && cudaStreamSynchronize(nullptr) == cudaSuccess;
+}
+
 // the session's K/V cache for the announced shape; false: decline (the
 // shape changed after the cache was made, or is too long for the attention
 // kernel)
@@ -207,7 +213,7 @@ bool ensure_kv(HookSession& S) {
     const size_t rows = (size_t)g_h.nl * g_h.nkv * mc;
     const size_t kcb = rows * pb_tq_cw(pb_tq_bk(tq)) * 4, vcb = rows * pb_tq_cw(pb_tq_bv(tq)) * 4;
     const size_t bytes = kcb + vcb + 2 * rows * 4 + (size_t)2 * g_h.nkv * 128 * 2;
-    if (cudaMalloc(&S.tq_mem, bytes) != cudaSuccess || cudaMemset(S.tq_mem, 0, bytes) != cudaSuccess) {
+    if (cudaMalloc(&S.tq_mem, bytes) != cudaSuccess || !zeroed(S.tq_mem, bytes)) {
       cudaGetLastError();
       if (S.tq_mem) cudaFree(S.tq_mem);
       S.tq_mem = nullptr;
@@ -223,7 +229,7 @@ bool ensure_kv(HookSession& S) {
     S.tq = tq;
   } else {
     const size_t bytes = (size_t)g_h.nl * 2 * g_h.nkv * mc * 128 * 2;
-    if (cudaMalloc(&S.kv, bytes) != cudaSuccess || cudaMemset(S.kv, 0, bytes) != cudaSuccess) {
+    if (cudaMalloc(&S.kv, bytes) != cudaSuccess || !zeroed(S.kv, bytes)) {
       cudaGetLastError();
       if (S.kv) cudaFree(S.kv);
       S.kv = nullptr;
@@ -292,7 +298,9 @@ const float* hnorm_of(const float* w) {
   auto it = g_h.hnorm.find(w);
   if (it != g_h.hnorm.end()) return it->second;
   float* d = nullptr;
-  if (cudaMalloc(&d, 128 * 4) != cudaSuccess || cudaMemcpy(d, w, 128 * 4, cudaMemcpyHostToDevice) != cudaSuccess) {
+  // a copy from pageable memory may return before the device has it
+  if (cudaMalloc(&d, 128 * 4) != cudaSuccess || cudaMemcpy(d, w, 128 * 4, cudaMemcpyHostToDevice) != cudaSuccess ||
+      cudaStreamSynchronize(nullptr) != cudaSuccess) {
     cudaGetLastError();
     if (d) cudaFree(d);
     pb_set_error(PB_ECUDA, "pq1 hooks: head-norm weights");
