@@ -217,7 +217,7 @@ struct EvictArgs {
   const int* dst;       // table of the fresh pages
   int dst_ld, max_len, budget, sinks, recent;
   int lcap;             // rows of a list: min(budget, max_len)
-  int* list;            // [sequence][kv head][lcap]
+  int* list;            // [sequence][kv head][lcap], or null: no sequence passes the budget
   int staged;           // rows whose keys fit in shared memory
 };
 
@@ -240,7 +240,10 @@ __global__ void __launch_bounds__(EV_T) k_kv_select(EvictArgs a) {
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   pb_grid_launch_dependents();
   const int len = kv_len(a.len[b], a.max_len);
-  if (len <= a.budget) return;   // every row stays: the gather needs no list
+  if (len <= a.budget) {         // every row stays
+    for (int j = t; j < len; j += EV_T) a.list[(size_t)blockIdx.x * a.lcap + j] = j;
+    return;
+  }
   const int* trow = a.p.table + (size_t)b * a.p.table_ld;
   const int lo = min(a.sinks, len), hi = max(lo, len - a.recent);   // [lo, hi) competes
   int need = a.budget - (len - (hi - lo));                          // how many of it stay (>= 0: sinks + recent <= budget)
@@ -298,7 +301,7 @@ __global__ void __launch_bounds__(EV_T) k_kv_select(EvictArgs a) {
   // kept: outside [lo, hi), a key above prefix, or one of the first `need`
   // keys equal to it. (need == 0 here only when nothing of [lo, hi) stays.)
   const bool none = need == 0;
-  int* out = a.list + ((size_t)b * a.p.n_kv + h) * a.lcap;
+  int* out = a.list + (size_t)blockIdx.x * a.lcap;
   const int seg = (len + EV_T - 1) / EV_T * 32, j0 = warp * seg, j1 = min(len, j0 + seg);
   int ngt = 0, neq = 0;
   for (int j = j0 + lane; j - lane < j1; j += 32) {
@@ -347,10 +350,13 @@ __global__ void __launch_bounds__(EV_GT) k_kv_gather(EvictArgs a, int chunks) {
   const int len = kv_len(a.len[b], a.max_len), n = min(len, a.budget);
   const int ps = 1 << a.p.shift;
   pb_grid_wait();      // the lists
-  if (chunk == 0 && h == 0 && threadIdx.x == 0) a.new_len[b] = n;   // may be len[b]: min(n, budget) = n either way
+  // May be len[b], which CTAs that start later read: min(n, budget) = n, and
+  // nothing but n may depend on it here (so the list of a sequence within the
+  // budget is there too).
+  if (chunk == 0 && h == 0 && threadIdx.x == 0) a.new_len[b] = n;
   const int* trow = a.p.table + (size_t)b * a.p.table_ld;
   const int* drow = a.dst + (size_t)b * a.dst_ld;
-  const int* list = a.list + ((size_t)b * a.p.n_kv + h) * a.lcap;
+  const int* list = a.list ? a.list + ((size_t)b * a.p.n_kv + h) * a.lcap : nullptr;
   const int i0 = chunk * (G * EV_R) + g;
   uint4 kk[EV_R], vv[EV_R];
   float w[EV_R];
@@ -361,7 +367,7 @@ __global__ void __launch_bounds__(EV_GT) k_kv_gather(EvictArgs a, int chunks) {
     const int i = i0 + r * G;
     to[r] = -1;
     if (i >= n) continue;
-    const int j = len > a.budget ? list[i] : i;
+    const int j = list ? list[i] : i;
     const int sp = kv_page(a.p, trow, j), dp = kv_page(a.p, drow, i);
     if (sp < 0 || dp < 0) continue;
     const long long from = (long long)sp * a.p.ps + (long long)h * a.p.hs + (long long)(j & (ps - 1)) * a.p.rs + l * 16;
@@ -511,7 +517,7 @@ extern "C" int pb_kv_evict(const pb_kv_pages* c, const pb_kv_evict_args* g, void
   a.len = g->len; a.new_len = g->new_len; a.dst = g->dst_table; a.dst_ld = dst_ld;
   a.max_len = max_len; a.budget = budget; a.sinks = sinks; a.recent = recent;
   a.lcap = cap;
-  a.list = static_cast<int*>(g->scratch);
+  a.list = max_len > budget ? static_cast<int*>(g->scratch) : nullptr;
   cudaStream_t st = (cudaStream_t)stream;
   if (max_len > budget) {
     // keys in shared memory up to 40 KB (no opt-in needed), the rest re-read

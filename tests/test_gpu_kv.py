@@ -479,6 +479,34 @@ def test_evict_lengths_in_place_and_bad_pages(pb, cuda):
             assert np.array_equal(f64(c.w)[to[m], h, tr[m]], W[pg[at[m]], h, r[at[m]]])
 
 
+def test_evict_lengths_in_place_of_more_rows_than_run_at_once(pb, cuda):
+    """the lengths are replaced while CTAs that read them have not started: 64
+    K/V heads of 4096 kept rows; and a sequence within the budget beside it"""
+    torch = cuda
+    lens, budget, nkv, D, ps = [4200, 100], 4096, 64, 128, 64
+    kept = [4096, 100]
+    c = Cache(pb, torch, lens + kept, nkv, D, ps, torch.float16, "head", True, seed=9)
+    table, dst = c.table[:2].contiguous(), c.table[2:].contiguous()
+    W = c.w.cpu().numpy()
+    length = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = []
+    for b, n in enumerate(lens):
+        pg, r, _ = KO.rows_of(table.numpy(), b, n, ps, c.n_pages)
+        for h in range(nkv):
+            at = np.asarray(KO.evict_rows(W[pg, h, r].astype(np.float64), n, budget, 0, 8))
+            pa, ra = (torch.from_numpy(np.ascontiguousarray(x)).cuda().long() for x in (pg[at], r[at]))
+            want.append((c.k[pa, h, ra], c.v[pa, h, ra], c.w[pa, h, ra]))
+    c.h.evict(table.cuda(), length, dst.cuda(), length, budget, sinks=0, recent=8)
+    torch.cuda.synchronize()
+    assert length.tolist() == kept
+    for b, n in enumerate(kept):
+        to, tr, _ = KO.rows_of(dst.numpy(), b, n, ps, c.n_pages)
+        to, tr = torch.from_numpy(np.ascontiguousarray(to)).cuda().long(), torch.from_numpy(np.ascontiguousarray(tr)).cuda().long()
+        for h in range(nkv):
+            k, v, w = want[b * nkv + h]
+            assert torch.equal(c.k[to, h, tr], k) and torch.equal(c.v[to, h, tr], v) and torch.equal(c.w[to, h, tr], w), (b, h)
+
+
 # ---------------------------------------------------------------- together
 def test_prompt_decode_evict_decode(pb, cuda):
     """as a server uses them: prompts appended and attended in chunks, decode steps that add weights, eviction to fresh
