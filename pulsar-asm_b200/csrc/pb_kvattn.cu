@@ -116,7 +116,9 @@ PB_DEV void dc_store(const DcArgs& d, int b, int h, int e, const float4& x) {
   *reinterpret_cast<uint2*>(o) = w;
 }
 
-template <int D, int CT, int NT>
+// P2: the probabilities as two numbers of the cache's type, for an output with
+// more bits than that has.
+template <int D, int CT, int NT, bool P2>
 __global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs d) {
   typedef DcGeo<D> G;
   constexpr int KT = G::KT, TILE = G::TILE, NB = G::NB, NS = G::NS, CPR = D / 8, RS = 32 / CPR;
@@ -307,7 +309,8 @@ __global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs
             for (int k = 0; k < D / 16; k++) { o[n][k][u] *= f; o[n][k][2 + u] *= f; }
           }
         }
-        // p in the cache's type for the matrix product; their sum in fp32 from before that rounding
+        // p in the cache's type for the matrix product (as exact as an output of that type: the
+        // roundings of many rows average out); their sum in fp32 from before that rounding
         float p[4];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
@@ -316,12 +319,20 @@ __global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs
           p[2 + u] = kv_ex2(s[n][2 + u] - r);
           l[n][u] += p[u] + p[2 + u];
         }
-        const unsigned b0 = kv_trans(kv_down<CT>(p[0], p[1])), b1 = kv_trans(kv_down<CT>(p[2], p[3]));
+        const unsigned w0 = kv_down<CT>(p[0], p[1]), w1 = kv_down<CT>(p[2], p[3]);
+        const unsigned b0 = kv_trans(w0), b1 = kv_trans(w1);
+        unsigned c0 = 0, c1 = 0;
+        if (P2) {                // what that rounding left
+          const float2 x = kv_up<CT>(w0), y = kv_up<CT>(w1);
+          c0 = kv_trans(kv_down<CT>(p[0] - x.x, p[1] - x.y));
+          c1 = kv_trans(kv_down<CT>(p[2] - y.x, p[3] - y.y));
+        }
 #pragma unroll
         for (int k = 0; k < D / 16; k++) {
           unsigned f[4];
           kv_ldmt(vs + (nb * 16 + vrow) * (D * 2) + (((2 * k + vch) ^ (vrow & 7)) << 4), f);
           kv_mma<CT>(o[n][k], f, b0, b1);
+          if (P2) kv_mma<CT>(o[n][k], f, c0, c1);
         }
       }
     }
@@ -544,19 +555,20 @@ DcPlan dc_plan(const pb_kv_pages* c, int n_seq, int max_len, int n_heads, int ac
                            : dc_plan_t<128>(n_seq, c->n_kv, max_len, n_heads / c->n_kv, accumulate);
 }
 
-template <int D, int CT, int NT>
+template <int D, int CT, int NT, bool P2>
 int dc_launch(const DcArgs& d, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
-  if (int rc = kv_smem(k_kv_decode<D, CT, NT>, DcGeo<D>::SMEM, done)) return rc;
-  return kv_launch(k_kv_decode<D, CT, NT>, (unsigned)d.grid, 32 * DC_W, DcGeo<D>::SMEM, st, false, "k_kv_decode", d);
+  if (int rc = kv_smem(k_kv_decode<D, CT, NT, P2>, DcGeo<D>::SMEM, done)) return rc;
+  return kv_launch(k_kv_decode<D, CT, NT, P2>, (unsigned)d.grid, 32 * DC_W, DcGeo<D>::SMEM, st, false, "k_kv_decode", d);
 }
 
 template <int D>
 int dc_run(const DcArgs& d, int ct, bool join, cudaStream_t st) {
   const bool two = d.a.grp > 8;
   int rc;
-  if (ct == PB_DT_F16) rc = two ? dc_launch<D, PB_DT_F16, 2>(d, st) : dc_launch<D, PB_DT_F16, 1>(d, st);
-  else rc = two ? dc_launch<D, PB_DT_BF16, 2>(d, st) : dc_launch<D, PB_DT_BF16, 1>(d, st);
+  if (ct == PB_DT_F16) rc = two ? dc_launch<D, PB_DT_F16, 2, false>(d, st) : dc_launch<D, PB_DT_F16, 1, false>(d, st);
+  else if (d.out_bf16) rc = two ? dc_launch<D, PB_DT_BF16, 2, false>(d, st) : dc_launch<D, PB_DT_BF16, 1, false>(d, st);
+  else rc = two ? dc_launch<D, PB_DT_BF16, 2, true>(d, st) : dc_launch<D, PB_DT_BF16, 1, true>(d, st);
   if (rc) return rc;
   // (a group's pieces: at most one per tile and per CTA)
   const int tiles = (d.a.max_len + DcGeo<D>::TILE - 1) / DcGeo<D>::TILE, np = d.grid < tiles ? d.grid : tiles;

@@ -216,7 +216,10 @@ PB_DEV unsigned long long pf_below(int x) { return x <= 0 ? 0ull : (x >= 64 ? ~0
 PB_DEV bool pf_edge(const PfLine& s, int k0) { return k0 + PF_KT > s.end || (k0 < s.lo && k0 + PF_KT > s.sinks); }
 PB_DEV int pf_key(const PfLine& s, int i) { return (i < s.nst ? i : i - s.nst + s.lot) * PF_KT; }
 
-template <int D, int CT>
+// P2: the probabilities as two numbers of the cache's type, for an output with
+// more bits than that has; the second ones take the other half of the scores'
+// columns.
+template <int D, int CT, bool P2>
 __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mq,
              PfArgs p) {
   typedef PfGeo<D> G;
@@ -415,7 +418,8 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
         const uint64_t vb = dv + (uint64_t)(st * ((2 * G::KV) >> 4));
         const uint32_t pb = tmem + g * 128 + (uint32_t)(i & 1) * 64, o = tmem + G::O_COL + g * D;
 #pragma unroll
-        for (int k = 0; k < PF_KT / 16; k++) pf_mma_ts(o, pb + k * 8, vb + (uint64_t)((k * 2048) >> 4), id_o, i > 0 || k > 0);
+        for (int k = 0; k < (P2 ? 2 : 1) * (PF_KT / 16); k++)
+          pf_mma_ts(o, pb + k * 8, vb + (uint64_t)((k % (PF_KT / 16) * 2048) >> 4), id_o, i > 0 || k > 0);
         pf_commit(i + 1 < n ? &pvdone[g] : &ofin[g]);
         pf_commit(&vempty[st]);
         if (g == 0 && i + 2 < n) {
@@ -517,12 +521,13 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
         }
       }
       // p = 2^(scale2 s - ms), rounded to the cache's type, which the product
-      // with V needs; the sum takes the unrounded ones
+      // with V needs (as exact as an output of that type); the sum takes the
+      // unrounded ones
       const pf_f2 nms = pf_pk(-ms, -ms);
       pf_f2 y[2] = {0ull, 0ull};
 #pragma unroll
       for (int q = 0; q < 4; q++) {
-        unsigned w[8];
+        unsigned w[8], z[8];
 #pragma unroll
         for (int k = 0; k < 8; k++) {
           float u, v;
@@ -531,8 +536,13 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
           v = kv_ex2(v);
           y[k & 1] = pf_add2(y[k & 1], pf_pk(u, v));
           w[k] = kv_down<CT>(u, v);
+          if (P2) {              // what that rounding left
+            const float2 x = kv_up<CT>(w[k]);
+            z[k] = kv_down<CT>(u - x.x, v - x.y);
+          }
         }
         pf_st8(ts + q * 8, w);
+        if (P2) pf_st8(ts + PF_KT / 2 + q * 8, z);
       }
       float ya, yb, yc, yd;
       pf_upk(y[0], ya, yb);
@@ -759,16 +769,21 @@ int pf_maps(const pb_kv_pages* c, PfArgs* p, CUtensorMap* mk, CUtensorMap* mv, C
   return PB_OK;
 }
 
-template <int D, int CT>
+template <int D, int CT, bool P2>
 int pf_run(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const PfArgs& p, const PfPlan& pl, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
-  if (int rc = kv_smem(k_kv_prefill<D, CT>, PfGeo<D>::SMEM, done)) return rc;
-  if (int rc = kv_launch(k_kv_prefill<D, CT>, (unsigned)(pl.items * p.ns), PfGeo<D>::T, PfGeo<D>::SMEM, st, false, "k_kv_prefill",
+  if (int rc = kv_smem(k_kv_prefill<D, CT, P2>, PfGeo<D>::SMEM, done)) return rc;
+  if (int rc = kv_launch(k_kv_prefill<D, CT, P2>, (unsigned)(pl.items * p.ns), PfGeo<D>::T, PfGeo<D>::SMEM, st, false, "k_kv_prefill",
                          mk, mv, mq, p))
     return rc;
   if (p.ns == 1) return PB_OK;
   const long long blocks = ((long long)p.a.n_rows * p.a.nh * (D / 4) + 127) / 128;
   return kv_launch(k_kv_prefill_join<D>, (unsigned)blocks, 128, 0, st, true, "k_kv_prefill_join", p);
+}
+template <int D>
+int pf_types(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq, const PfArgs& p, const PfPlan& pl, int ct, cudaStream_t st) {
+  if (ct == PB_DT_F16) return pf_run<D, PB_DT_F16, false>(mk, mv, mq, p, pl, st);
+  return p.out_bf16 ? pf_run<D, PB_DT_BF16, false>(mk, mv, mq, p, pl, st) : pf_run<D, PB_DT_BF16, true>(mk, mv, mq, p, pl, st);
 }
 
 }  // namespace
@@ -799,9 +814,7 @@ extern "C" int pb_kv_prefill(const pb_kv_pages* c, const pb_kv_attention_args* g
   cudaStream_t st = (cudaStream_t)stream;
   CUtensorMap mk, mv, mq;
   if (int rc = pf_maps(c, &p, &mk, &mv, &mq)) return rc;
-  if (c->head_dim == 64)
-    return c->dtype == PB_DT_F16 ? pf_run<64, PB_DT_F16>(mk, mv, mq, p, pl, st) : pf_run<64, PB_DT_BF16>(mk, mv, mq, p, pl, st);
-  return c->dtype == PB_DT_F16 ? pf_run<128, PB_DT_F16>(mk, mv, mq, p, pl, st) : pf_run<128, PB_DT_BF16>(mk, mv, mq, p, pl, st);
+  return c->head_dim == 64 ? pf_types<64>(mk, mv, mq, p, pl, c->dtype, st) : pf_types<128>(mk, mv, mq, p, pl, c->dtype, st);
 }
 
 extern "C" int pb_kv_status(void* stream) {

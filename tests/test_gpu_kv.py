@@ -66,8 +66,8 @@ class Cache:
         return self.table.cuda()
 
 
-def check(torch, got, want, spread, slack, tiny, n, dt, out, what):
-    p_err = 2 * slack[..., None] + 2.0 ** -21 + n * 2.0 ** -24 + U(torch, dt)
+def check(torch, got, want, spread, slack, tiny, n, dt, out, what, u=None):
+    p_err = 2 * slack[..., None] + 2.0 ** -21 + n * 2.0 ** -24 + (U(torch, dt) if u is None else u)
     tol = spread * p_err + 2.0 ** -25 * tiny + U(torch, out) * (np.abs(want) + spread * p_err) + 2.0 ** -25
     bad = ~(np.abs(got - want) <= tol)
     assert not bad.any(), (what, np.argwhere(bad)[:5].tolist(), got[bad][:5], want[bad][:5], tol[bad][:5])
@@ -406,6 +406,29 @@ def test_prefill_extreme_scores(pb, cuda):
     torch.cuda.synchronize()
     (o, spread, slack, tiny), _ = oracle_rows(c, q, [400], [400], 128 ** -0.5, 0, 0)
     check(torch, f64(out), o, spread, np.minimum(slack, 1.0), tiny, 400, c.dt, torch.bfloat16, "large scores")
+
+
+@pytest.mark.parametrize("nh,nkv,D", [(8, 2, 64), (16, 1, 128), (4, 4, 128)])
+def test_fp16_output_of_a_bf16_cache(pb, cuda, nh, nkv, D):
+    """an output with more bits than the cache's type: the probabilities keep two numbers of that type, each a half
+    step of 2^-8 (2^-16 together), so that the output's own rounding is the largest error"""
+    torch = cuda
+    lens, counts = [2, 3, 17, 200, 70, 2600], [2, 3, 5, 130, 1, 40]
+    c = Cache(pb, torch, lens, nkv, D, 32, torch.bfloat16, seed=D + nh)
+    S = len(lens)
+    length = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    for m in ([1] * S, counts):
+        q = (torch.randn((sum(m), nh, D), generator=c.g) * 0.5).bfloat16().cuda()
+        out = torch.empty((sum(m), nh, D), dtype=torch.float16, device="cuda")
+        if m is counts:
+            start = torch.tensor(np.concatenate([[0], np.cumsum(m)]), dtype=torch.int32, device="cuda")
+            c.h.prefill(c.dev(), start, length, q, out)
+            c.h.status()
+        else:
+            c.h.decode(c.dev(), length, q, out)
+        torch.cuda.synchronize()
+        (o, spread, slack, tiny), _ = oracle_rows(c, q, lens, m, D ** -0.5, 0, 0)
+        check(torch, f64(out), o, spread, slack, tiny * 0, max(lens), c.dt, torch.float16, "%d rows" % sum(m), u=2.0 ** -16)
 
 
 # ------------------------------------------------------------------- evict
