@@ -463,7 +463,7 @@ int pb_kv_status(void* stream);
  * weights: the lowest row first; a weight that is not above 0 counts as 0).
  * The kept rows move in order, with their weights, to rows 0.. of the pages
  * of dst_table (rows of dst_ld), which must share no page with the sequences'
- * own; new_len[b] = min(len[b], budget) (may be len itself). A sequence
+ * own; new_len[b] = min(len[b], budget) (len itself, or apart from it). A sequence
  * within the budget moves whole. The old pages are left as they are. Kept
  * rows stay rotated by their own positions, so later tokens go to slot
  * new_len.. with their true positions in pb_kv_append's pos.                 */

@@ -142,6 +142,13 @@ def test_evict_refusals(pb, over):
     assert evict(pb, **over) == EINVAL
 
 
+@pytest.mark.parametrize("over", [dict(new=P + 4), dict(new=P - 12), dict(scratch=P + 4)])
+def test_evict_lengths_in_place_or_apart(pb, over):
+    """new_len beside len but sharing entries with it, which the kernels would read after they are replaced; a scratch
+    that is not aligned"""
+    assert evict(pb, **over) == EINVAL
+
+
 def test_null_arguments(pb):
     L = pb.lib()
     for fn in (L.pb_kv_append, L.pb_kv_decode, L.pb_kv_prefill, L.pb_kv_evict):
