@@ -266,7 +266,11 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
   row0 += tok0;
   const int len = kv_len(__ldg(a.len + b), a.max_len), t0 = len - cnt + tok0;   // cache row of the first token (negative: before the cache)
   const PfLine line = pf_line(a, t0, t0 + ntok - 1);
-  const int i0 = (int)((long long)line.nt * split / p.ns), n = (int)((long long)line.nt * (split + 1) / p.ns) - i0;
+  int i0 = 0, n = line.nt;
+  if (p.ns > 1) {    // (nt is below 2^24, ns at most 160)
+    i0 = (int)((unsigned)line.nt * split / (unsigned)p.ns);
+    n = (int)((unsigned)line.nt * (split + 1) / (unsigned)p.ns) - i0;
+  }
   const int ng = ntok > p.tq ? 2 : 1;   // groups with rows
   const int* trow = a.p.table + (size_t)b * a.p.table_ld;
 
@@ -297,10 +301,11 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
 
   if (warp == 0) {
     // ------------------------------------------------------------ copies
-    // the page of the tile's 16-row block `lane % 4`, a tile ahead
-    auto page_of = [&](int i) {
-      const int j = pf_key(line, i0 + i) + lane % (PF_KT / 16) * 16;
-      const int e = j < line.end ? __ldg(trow + (j >> a.p.shift)) : -1;
+    // the pages of 8 tiles, 4 blocks of 16 rows each, a lane for each; the next 8 tiles' 8 tiles ahead
+    constexpr int BT = PF_KT / 16, AHEAD = 32 / BT;
+    auto pages = [&](int i) {
+      const int j = pf_key(line, i0 + i + lane / BT) + lane % BT * 16;
+      const int e = i + lane / BT < n && j < line.end ? __ldg(trow + (j >> a.p.shift)) : -1;
       return (unsigned)e < (unsigned)a.p.n_pages ? e : a.p.n_pages;   // the box behind the last page: zeros
     };
     if (n > 0 && lane == 0) {
@@ -313,7 +318,7 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
           for (int c = 0; c < D / 64; c++)
             pf_tma2(kv_s32(smq) + g * G::Q + c * QP + h * p.tq * 128, &mq, (kh * a.grp + h) * D + c * 64, row0 + g * p.tq, &qfull);
     }
-    int pg = n > 0 ? page_of(0) : 0, st = 0, sf = 0;
+    int now = pages(0), pg = 0, st = 0, sf = 0;
     unsigned epar = 1, fpar = 0;
     int fixes = 0;    // at most 3: where the sinks end, where the window begins, the last tile
     // a tile's V is looked at LAG tiles later: by then others are on their way
@@ -321,8 +326,11 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
     constexpr int LAG = 2;
     for (int i = 0; i < n + LAG; i++) {
       if (i < n) {
-        const int now = pg, k0 = pf_key(line, i0 + i);
-        if (i + 1 < n) pg = page_of(i + 1);
+        const int k0 = pf_key(line, i0 + i), it = i % AHEAD;
+        if (it == 0) {
+          if (i > 0) now = pg;
+          if (i + AHEAD < n) pg = pages(i + AHEAD);
+        }
         const uint32_t ks = kv_s32(smk) + st * (2 * G::KV);
 #pragma unroll
         for (int z = 0; z < 2; z++) {        // K, then V
@@ -331,7 +339,7 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
           uint64_t* bar = z ? &vfull[st] : &kfull[st];
           if (lane == 0) pf_expect(bar, G::KV);
           for (int r = 0; r < PF_KT; r += p.box) {
-            const int page = __shfl_sync(0xffffffffu, now, r >> 4), row = (k0 + r) & ((1 << a.p.shift) - 1);
+            const int page = __shfl_sync(0xffffffffu, now, it * BT + (r >> 4)), row = (k0 + r) & ((1 << a.p.shift) - 1);
             if (lane == 0) {
               const int c1 = p.d_row == 1 ? row : (p.d_head == 1 ? kh : page), c2 = p.d_row == 2 ? row : (p.d_head == 2 ? kh : page),
                         c3 = p.d_row == 3 ? row : (p.d_head == 3 ? kh : page);
@@ -572,19 +580,20 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
         // by way of the (now idle) queries' rows, so that a warp writes whole rows together
         char* sr = smq + g * G::Q + r * 128;
 #pragma unroll
-        for (int e = 0; e < D; e += 32) {
-          unsigned o[32];
+        for (int e = 0; e < D; e += 64) {
+          unsigned o[64];
           if (n > 0) {
             pf_ld32(to + e, o);
+            pf_ld32(to + e + 32, o + 32);
             pf_wait_ld();
           } else {
 #pragma unroll
-            for (int k = 0; k < 32; k++) o[k] = 0u;
+            for (int k = 0; k < 64; k++) o[k] = 0u;
           }
 #pragma unroll
-          for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+          for (int k = 0; k < 64; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
+          for (int k = 0; k < 8; k++) {
             uint4 w;
             unsigned* x = &w.x;
 #pragma unroll
