@@ -41,6 +41,21 @@ PB_DEV void kv_locate(int n_seq, C count, F pick, int& total, int& b, int& first
     return;
   }
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  if (n_seq <= 32) {     // a lane per sequence, each warp for itself: no barrier
+    const int own = lane < n_seq ? count(lane) : 0;
+    int inc = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    total = __shfl_sync(0xffffffffu, inc, 31);
+    const int x = pick(total);
+    const unsigned at = __ballot_sync(0xffffffffu, x >= inc - own && x < inc);
+    b = __ffs((int)at) - 1;      // -1: none
+    first = __shfl_sync(0xffffffffu, inc - own, b & 31);
+    return;
+  }
   const int per = (n_seq + T - 1) / T, b0 = min(n_seq, t * per), b1 = min(n_seq, b0 + per);
   int own = 0;
   for (int i = b0; i < b1; i++) own += count(i);

@@ -244,6 +244,26 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(kv_s32(&tbase)), "n"(G::COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  if (threadIdx.x == 32) {             // (warp 1 has no other work)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mq) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
+    for (int i = 0; i < NST; i++) {
+      pf_init(&kfull[i], 1);
+      pf_init(&vfull[i], 1);
+    }
+    for (int g = 0; g < NG; g++) {
+      for (int i = 0; i < 2; i++) { pf_init(&sfull[g][i], 1); pf_init(&pready[g][i], 128); }
+      pf_init(&pvdone[g], 1);
+      pf_init(&ofin[g], 1);
+      pf_init(&done[g], 1);
+    }
+    for (int i = 0; i < 4; i++) pf_init(&lock[i], 1);
+    for (int i = 0; i < 3; i++) pf_init(&vfix[i], 1);
+    pf_init(&qfull, 1);
+    stop_f = 0;
+  }
+  __syncwarp();
 
   // ---- which rows: the last tiles of the line (the longest keys) first
   const int split = blockIdx.x % p.ns, kh = blockIdx.x / p.ns % a.p.n_kv, idx = blockIdx.x / p.ns / a.p.n_kv;
@@ -274,25 +294,21 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
   const int ng = ntok > p.tq ? 2 : 1;   // groups with rows
   const int* trow = a.p.table + (size_t)b * a.p.table_ld;
 
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < NST; i++) {
-      pf_init(&kfull[i], 1);
-      pf_init(&vfull[i], 1);
-      pf_init(&kempty[i], ng);
-      pf_init(&vempty[i], ng);
+  if (warp == 1) {
+    if (lane < NST) {
+      pf_init(&kempty[lane], ng);
+      pf_init(&vempty[lane], ng);
     }
-    for (int g = 0; g < NG; g++) {
-      for (int i = 0; i < 2; i++) { pf_init(&sfull[g][i], 1); pf_init(&pready[g][i], 128); }
-      pf_init(&pvdone[g], 1);
-      pf_init(&ofin[g], 1);
-      pf_init(&done[g], 1);
-    }
-    for (int i = 0; i < 4; i++) pf_init(&lock[i], 1);
-    for (int i = 0; i < 3; i++) pf_init(&vfix[i], 1);
-    pf_init(&qfull, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    stop_f = 0;
   }
+  // the pages of 8 tiles, 4 blocks of 16 rows each, a lane for each
+  constexpr int BT = PF_KT / 16, AHEAD = 32 / BT;
+  auto pages = [&](int i) {
+    const int j = pf_key(line, i0 + i + lane / BT) + lane % BT * 16;
+    const int e = i + lane / BT < n && j < line.end ? __ldg(trow + (j >> a.p.shift)) : -1;
+    return (unsigned)e < (unsigned)a.p.n_pages ? e : a.p.n_pages;   // the box behind the last page: zeros
+  };
+  int now = warp == 0 ? pages(0) : 0;
   pf_fence_before();
   __syncthreads();
   pf_fence_after();
@@ -301,13 +317,6 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
 
   if (warp == 0) {
     // ------------------------------------------------------------ copies
-    // the pages of 8 tiles, 4 blocks of 16 rows each, a lane for each; the next 8 tiles' 8 tiles ahead
-    constexpr int BT = PF_KT / 16, AHEAD = 32 / BT;
-    auto pages = [&](int i) {
-      const int j = pf_key(line, i0 + i + lane / BT) + lane % BT * 16;
-      const int e = i + lane / BT < n && j < line.end ? __ldg(trow + (j >> a.p.shift)) : -1;
-      return (unsigned)e < (unsigned)a.p.n_pages ? e : a.p.n_pages;   // the box behind the last page: zeros
-    };
     if (n > 0 && lane == 0) {
       // the queries: a box of tq tokens and 64 columns for each head (rows past the sequence's last
       // token are another's or zeros, and go nowhere)
@@ -318,7 +327,7 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
           for (int c = 0; c < D / 64; c++)
             pf_tma2(kv_s32(smq) + g * G::Q + c * QP + h * p.tq * 128, &mq, (kh * a.grp + h) * D + c * 64, row0 + g * p.tq, &qfull);
     }
-    int now = pages(0), pg = 0, st = 0, sf = 0;
+    int pg = 0, st = 0, sf = 0;
     unsigned epar = 1, fpar = 0;
     int fixes = 0;    // at most 3: where the sinks end, where the window begins, the last tile
     // a tile's V is looked at LAG tiles later: by then others are on their way
@@ -329,7 +338,7 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
         const int k0 = pf_key(line, i0 + i), it = i % AHEAD;
         if (it == 0) {
           if (i > 0) now = pg;
-          if (i + AHEAD < n) pg = pages(i + AHEAD);
+          if (i + AHEAD < n) pg = pages(i + AHEAD);   // (for 8 tiles on)
         }
         const uint32_t ks = kv_s32(smk) + st * (2 * G::KV);
 #pragma unroll
