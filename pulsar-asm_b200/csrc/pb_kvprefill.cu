@@ -17,7 +17,7 @@
 //    2^8; the output is rescaled in TMEM then, which is rare. The sum of a row
 //    stays with its thread. Any maximum that is near enough gives the same
 //    quotient.
-// Warp 0 brings K and V tiles by TMA (a box per page, or part of one, and 64
+// Warp 1 brings the queries, warp 0 K and V tiles, by TMA (a box per page, or part of one, and 64
 // columns, in the 128-byte swizzle the tensor cores read; a table entry that
 // names no page becomes a box outside the pool, which reads as zeros), warps 2
 // and 3 issue the two groups' matrix products, warps 4-7 and 8-11 are the two
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(kv_s32(&tbase)), "n"(G::COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  if (threadIdx.x == 32) {             // (warp 1 has no other work)
+  if (threadIdx.x == 32) {             // (warp 1: the barriers, then the queries)
     asm volatile("prefetch.tensormap [%0];" ::"l"(&mq) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&mk) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&mv) : "memory");
@@ -317,16 +317,6 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
 
   if (warp == 0) {
     // ------------------------------------------------------------ copies
-    if (n > 0 && lane == 0) {
-      // the queries: a box of tq tokens and 64 columns for each head (rows past the sequence's last
-      // token are another's or zeros, and go nowhere)
-      pf_expect(&qfull, ng * a.grp * p.tq * (D * 2));
-      for (int g = 0; g < ng; g++)
-        for (int h = 0; h < a.grp; h++)
-#pragma unroll
-          for (int c = 0; c < D / 64; c++)
-            pf_tma2(kv_s32(smq) + g * G::Q + c * QP + h * p.tq * 128, &mq, (kh * a.grp + h) * D + c * 64, row0 + g * p.tq, &qfull);
-    }
     int pg = 0, st = 0, sf = 0;
     unsigned epar = 1, fpar = 0;
     int fixes = 0;    // at most 3: where the sinks end, where the window begins, the last tile
@@ -382,6 +372,18 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
     if (*stop) {
       const unsigned long long t1 = pf_now();
       while (pf_now() - t1 < 1000000ull) {}
+    }
+  } else if (warp == 1) {
+    // the queries, beside the first keys: a box of tq tokens and 64 columns for each head (rows past the
+    // sequence's last token are another's or zeros, and go nowhere)
+    if (n > 0) {
+      const int per = a.grp * (D / 64);
+      if (lane == 0) pf_expect(&qfull, ng * per * (p.tq * 128));
+      __syncwarp();
+      for (int u = lane; u < ng * per; u += 32) {
+        const int g = u / per, h = u % per / (D / 64), c = u % (D / 64);
+        pf_tma2(kv_s32(smq) + g * G::Q + c * QP + h * p.tq * 128, &mq, (kh * a.grp + h) * D + c * 64, row0 + g * p.tq, &qfull);
+      }
     }
   } else if (warp == PF_MMA || warp == PF_MMA + 1) {
     // ---------------------------------------------------- matrix products
