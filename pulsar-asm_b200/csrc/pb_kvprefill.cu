@@ -27,9 +27,12 @@
 // 8192 tokens of 32/8 heads x 128 take 472 us (1164 TFLOP/s): tensor pipe and
 // exponentials each busy half the time (52 %), the steps of the two groups
 // meeting imperfectly. A ragged batch of 5 prompts to 4000 tokens with a
-// window of 256, 16/4 x 128: 82 us, a CTA's start (queries, first tiles, its
-// search: some 6 us) against the 5 or 6 tiles it works on. A chunk of 32
-// tokens against 4131 rows: 18 us, two launches and the join of the splits.
+// window of 256, 16/4 x 128: 74 us; of a CTA's 12 some 4 pass until its first
+// scores (search, first copies) and 2 at its end (the rows go out), beside 5
+// to 7 tiles of 1 us. A chunk of 32 tokens against 4131 rows: 17 us, two
+// launches and the join of the splits. (The queries by a warp of their own
+// took the ragged batch from 77.5 to 73.9 us; asking for the next CTA's
+// queries into L2 ahead of it gained nothing.)
 // All waits are bounded; a wait that gives up
 // records an error (pb_kv_status); copies and products in flight are waited
 // for and the TMEM is freed before the CTA ends.
@@ -224,8 +227,8 @@ PB_DEV int pf_key(const PfLine& s, int i) { return (i < s.nst ? i : i - s.nst + 
 
 // P2: the probabilities as two numbers of the cache's type, for an output with
 // more bits than that has; the second ones take the other half of the scores'
-// columns, and a second product with V (8192 tokens of 32/8 heads x 128: 596
-// against 459 us; the ragged batch with a window 89 against 82).
+// columns, and a second product with V (8192 tokens of 32/8 heads x 128: 608
+// against 459 us; the ragged batch with a window 80 against 74).
 template <int D, int CT, bool P2>
 __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mq,
              PfArgs p) {
