@@ -429,7 +429,8 @@ typedef struct {
 } pb_kv_evict_args;
 /* n_tok rows qkv [n_tok][ldx] (x_dtype bf16, fp16 or fp32; q heads | k heads |
  * v heads, anything behind them ignored: the gate values of a q|k|v|gate
- * projection): RMS norm of every query and key head (weights qnorm, knorm
+ * projection; rows may start at any element, on 16 bytes they are read
+ * faster): RMS norm of every query and key head (weights qnorm, knorm
  * fp32 [head_dim]; NULL: no norm), rotation of the pairs (i, i + head_dim/2),
  * i < half, by row pos[i] (NULL: slot[i]) of cos / sin (fp32 [n_rope][half];
  * half 0: none), the query heads to q [n_tok][ldq] (the cache's dtype), the K

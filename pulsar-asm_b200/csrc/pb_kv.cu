@@ -27,6 +27,7 @@ struct AppendArgs {
   const int* slot;
   const int* pos;          // null: the slot
   const float *qn, *kn, *cs, *sn;
+  int xa;                  // bytes that every row of x is aligned to: 16, 8, 4 or 2
   int n_tok, nh, half, n_rope, rows, parts, n_qk, n_groups;   // groups of query and key heads, and with those of value heads
   float eps;
 };
@@ -35,10 +36,30 @@ template <int XT>
 struct KvRaw {             // 8 values
   uint4 a, b;
 };
-template <int XT>
-PB_DEV void ap_load(KvRaw<XT>& r, const char* p) {
-  r.a = pb_ldg_stream(p);
-  if (XT == PB_DT_F32) r.b = pb_ldg_stream(p + 16);
+PB_DEV unsigned ap_ld16(const char* p) {
+  unsigned short r;
+  asm volatile("ld.global.nc.L1::no_allocate.u16 %0, [%1];" : "=h"(r) : "l"(p));
+  return r;
+}
+PB_DEV uint4 ap_ld(const char* p, int xa) {     // 16 bytes at less than 16-byte alignment
+  uint4 r;
+  if (xa == 8) {
+    const uint2 x = pb_ldg_stream64(p), y = pb_ldg_stream64(p + 8);
+    r = make_uint4(x.x, x.y, y.x, y.y);
+  } else if (xa == 4) {
+    r = make_uint4(pb_ldg_stream32(p), pb_ldg_stream32(p + 4), pb_ldg_stream32(p + 8), pb_ldg_stream32(p + 12));
+  } else {
+    r = make_uint4(ap_ld16(p) | ap_ld16(p + 2) << 16, ap_ld16(p + 4) | ap_ld16(p + 6) << 16,
+                   ap_ld16(p + 8) | ap_ld16(p + 10) << 16, ap_ld16(p + 12) | ap_ld16(p + 14) << 16);
+  }
+  return r;
+}
+// VEC: rows on 16 bytes. A projection with a value per head behind v (gates)
+// has other rows.
+template <int XT, bool VEC>
+PB_DEV void ap_load(KvRaw<XT>& r, const char* p, int xa) {
+  r.a = VEC ? pb_ldg_stream(p) : ap_ld(p, xa);
+  if (XT == PB_DT_F32) r.b = VEC ? pb_ldg_stream(p + 16) : ap_ld(p + 16, xa);
 }
 template <int XT>
 PB_DEV void ap_up(const KvRaw<XT>& r, float (&x)[8]) {
@@ -92,7 +113,7 @@ PB_DEV ap_f2 ap_mul2(ap_f2 a, ap_f2 b) {
 constexpr int AP_W = 8;    // warps per CTA
 constexpr int AP_U = 2;    // groups whose loads are in flight together
 
-template <int D, int XT, int CT>
+template <int D, int XT, int CT, bool VEC>
 __global__ void __launch_bounds__(32 * AP_W, XT == PB_DT_F32 ? 3 : 4) k_kv_append(AppendArgs a) {
   constexpr int L = D / 16, HPW = 32 / L, XB = XT == PB_DT_F32 ? 4 : 2;
   __shared__ __align__(16) float nw[2][D];   // the norms' weights, of queries and of keys
@@ -114,8 +135,8 @@ __global__ void __launch_bounds__(32 * AP_W, XT == PB_DT_F32 ? 3 : 4) k_kv_appen
   auto fetch = [&](int g, int u) {
     const int h = head(g);
     if (live(g, h)) {
-      ap_load<XT>(lo[u], x0 + (size_t)h * (D * XB));
-      ap_load<XT>(hi[u], x0 + (size_t)h * (D * XB) + D / 2 * XB);
+      ap_load<XT, VEC>(lo[u], x0 + (size_t)h * (D * XB), a.xa);
+      ap_load<XT, VEC>(hi[u], x0 + (size_t)h * (D * XB) + D / 2 * XB, a.xa);
     } else {
       lo[u].a = lo[u].b = hi[u].a = hi[u].b = make_uint4(0, 0, 0, 0);
     }
@@ -198,10 +219,15 @@ __global__ void __launch_bounds__(32 * AP_W, XT == PB_DT_F32 ? 3 : 4) k_kv_appen
   }
 }
 
+template <int D, int XT, int CT>
+void ap_launch_t(const AppendArgs& a, dim3 grid, cudaStream_t st) {
+  if (a.xa == 16) k_kv_append<D, XT, CT, true><<<grid, 32 * AP_W, 0, st>>>(a);
+  else k_kv_append<D, XT, CT, false><<<grid, 32 * AP_W, 0, st>>>(a);
+}
 template <int D, int XT>
 void ap_launch(const AppendArgs& a, int ct, dim3 grid, cudaStream_t st) {
-  if (ct == PB_DT_F16) k_kv_append<D, XT, PB_DT_F16><<<grid, 32 * AP_W, 0, st>>>(a);
-  else k_kv_append<D, XT, PB_DT_BF16><<<grid, 32 * AP_W, 0, st>>>(a);
+  if (ct == PB_DT_F16) ap_launch_t<D, XT, PB_DT_F16>(a, grid, st);
+  else ap_launch_t<D, XT, PB_DT_BF16>(a, grid, st);
 }
 
 // ------------------------------------------------------------------- evict
@@ -459,8 +485,10 @@ extern "C" int pb_kv_append(const pb_kv_pages* c, const pb_kv_append_args* g, vo
   const long long wide = (long long)(n_heads + 2 * c->n_kv) * D;
   const int xb = x_dtype == PB_DT_F32 ? 4 : 2;
   if (ldx < wide || ldq < (long long)n_heads * D) return pb_set_error(PB_EINVAL, "pb_kv_append: row strides %lld, %lld", ldx, ldq);
-  if (((reinterpret_cast<size_t>(g->qkv) | reinterpret_cast<size_t>(g->q) | (size_t)(ldx * xb) | (size_t)(ldq * 2)) & 15))
-    return pb_set_error(PB_EINVAL, "pb_kv_append: qkv and q rows must be 16-byte aligned");
+  const size_t xa = reinterpret_cast<size_t>(g->qkv) | (n_tok > 1 ? (size_t)(ldx * xb) : 0) | 16;
+  a.xa = (int)(xa & ~(xa - 1));
+  if (a.xa < xb || ((reinterpret_cast<size_t>(g->q) | (size_t)(ldq * 2)) & 15))
+    return pb_set_error(PB_EINVAL, "pb_kv_append: q rows must be 16-byte aligned, those of qkv aligned to its elements");
   if (kv_overlap(g->qkv, ((size_t)(n_tok - 1) * ldx + wide) * xb, g->q, ((size_t)(n_tok - 1) * ldq + (size_t)n_heads * D) * 2))
     return pb_set_error(PB_EINVAL, "pb_kv_append: q overlaps qkv");
   a.x = static_cast<const char*>(g->qkv);

@@ -159,6 +159,33 @@ def test_append(pb, cuda, nh, nkv, D, ps, dt, xt, half, layout, weights, pos, no
         assert np.array_equal(f64(c.w), W), "weights"
 
 
+@pytest.mark.parametrize("xt", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("nh,D,extra,skip", [(12, 64, 12, 0), (6, 64, 6, 0), (7, 128, 7, 0), (4, 128, 8, 1), (4, 64, 16, 4)])
+def test_append_rows_at_any_element(pb, cuda, nh, D, extra, skip, xt):
+    """rows with a value per head behind v, or from within a wider tensor, are not on 16 bytes: the same bits as from a
+    copy that is"""
+    torch = cuda
+    xt, nkv, n = getattr(torch, xt), nh if nh == 7 else 2, 37
+    wide = (nh + 2 * nkv) * D
+    g = torch.Generator().manual_seed(nh + extra)
+    big = (torch.randn((n, wide + extra + skip), generator=g) * 2).to(xt).cuda()
+    x = big[:, skip:]
+    ang = torch.arange(64).double()[:, None] * 1e4 ** (-torch.arange(D // 2).double() / (D // 2))
+    cos, sin = ang.cos().float().cuda(), ang.sin().float().cuda()
+    norm = (1 + 0.1 * torch.randn(D, generator=g)).cuda()
+    i = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    got = []
+    for rows in (x[:, :wide].clone().contiguous(), x):
+        c = Cache(pb, torch, [64], nkv, D, 16, torch.float16, seed=1)
+        q = torch.zeros((n, nh, D), dtype=torch.float16, device="cuda")
+        c.h.append(c.dev(), i([0] * n), i(list(range(5, 5 + n))), None, rows, q, q_norm=norm, k_norm=norm, cos=cos, sin=sin)
+        torch.cuda.synchronize()
+        got.append((q, c.k, c.v))
+    assert got[0][0].abs().max() > 1
+    for a, b in zip(*got):
+        assert np.array_equal(f64(a), f64(b), equal_nan=True)
+
+
 def test_append_refuses_what_the_pointers_do_not_show(pb, cuda):
     torch = cuda
     c = Cache(pb, torch, [40], 2, 64, 16, torch.float16)

@@ -94,8 +94,8 @@ def test_bad_tables_are_refused(pb, call, over):
 
 @pytest.mark.parametrize("over", [
     dict(x=None), dict(seq=None), dict(slot=None), dict(q=None), dict(x_dtype=3), dict(n_tok=-1), dict(nh=0), dict(half=-1),
-    dict(half=65), dict(cos=None), dict(sin=None), dict(n_rope=0), dict(ldx=48 * 128 - 8), dict(ldq=31 * 128), dict(x=P + 8),
-    dict(q=P + 2), dict(ldx=48 * 128 + 4), dict(ldq=32 * 128 + 1),
+    dict(half=65), dict(cos=None), dict(sin=None), dict(n_rope=0), dict(ldx=48 * 128 - 8), dict(ldq=31 * 128), dict(x=P + 1),
+    dict(q=P + 2), dict(q=P + 8), dict(ldq=32 * 128 + 4), dict(ldq=32 * 128 + 1),
     dict(q=P + (1 << 36) + 16),               # q inside qkv
 ])
 def test_append_refusals(pb, over):
