@@ -464,7 +464,9 @@ int pb_kv_status(void* stream);
  * weights: the lowest row first; a weight that is not above 0 counts as 0).
  * The kept rows move in order, with their weights, to rows 0.. of the pages
  * of dst_table (rows of dst_ld), which must share no page with the sequences'
- * own; new_len[b] = min(len[b], budget) (len itself, or apart from it). A sequence
+ * own. A row on no page (a freed one of a sliding window, say) is left out
+ * and takes no place: new_len[b] = the least of budget and the rows that lie
+ * on a page (written to len itself, or apart from it). A sequence
  * within the budget moves whole. The old pages are left as they are. Kept
  * rows stay rotated by their own positions, so later tokens go to slot
  * new_len.. with their true positions in pb_kv_append's pos.                 */

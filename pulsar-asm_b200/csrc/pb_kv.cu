@@ -235,7 +235,9 @@ void ap_launch(const AppendArgs& a, int ct, dim3 grid, cudaStream_t st) {
 // `sinks`, the last `recent`, and of the others the `need` of largest weight
 // (equal weights: the lowest row first), by a radix select on the weights'
 // bits (non-negative floats order as integers; anything not above zero counts
-// as zero), then lists them in order with ballots. One sequence of 1087 rows
+// as zero), then lists them in order with ballots. A row on no page is left
+// out, whichever it is: moved nowhere, it must not count as a row of the new
+// cache, where it would be seen. One sequence of 1087 rows
 // to 1024: 10.4 us with the gather; the passes' barriers bound it, not its few
 // bytes.
 struct EvictArgs {
@@ -245,7 +247,7 @@ struct EvictArgs {
   const int* dst;       // table of the fresh pages
   int dst_ld, max_len, budget, sinks, recent;
   int lcap;             // rows of a list: min(budget, max_len)
-  int* list;            // [sequence][kv head][lcap], or null: no sequence passes the budget
+  int* list;            // [sequence][kv head][lcap], -1 behind the last kept row; null: no sequence passes the budget
   int staged;           // rows whose keys fit in shared memory
   bool in_place;        // new_len is len
 };
@@ -253,9 +255,11 @@ struct EvictArgs {
 constexpr int EV_T = 1024;
 static_assert(EV_T == 32 * 32, "one lane of warp 0 scans each warp's sum");
 
+constexpr unsigned EV_GONE = 0xffffffffu;   // the key of a row on no page; no weight has it
+
 PB_DEV unsigned ev_key(const EvictArgs& a, const int* trow, int h, int j) {
   const int page = kv_page(a.p, trow, j);
-  if (page < 0) return 0u;
+  if (page < 0) return EV_GONE;
   const float w = a.p.w[((size_t)page * a.p.n_kv + h) * (1 << a.p.shift) + (j & ((1 << a.p.shift) - 1))];
   return w > 0.0f ? __float_as_uint(w) : 0u;
 }
@@ -264,33 +268,40 @@ __global__ void __launch_bounds__(EV_T) k_kv_select(EvictArgs a) {
   extern __shared__ unsigned keys[];
   __shared__ int hist[2048];
   __shared__ int wsum[EV_T / 32], wsum2[EV_T / 32];
-  __shared__ int s_bin, s_need;
+  __shared__ int s_bin, s_need, s_gone[2];   // (rows on no page: among those that compete, and the others)
   const int b = blockIdx.x / a.p.n_kv, h = blockIdx.x % a.p.n_kv;
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
   pb_grid_launch_dependents();
   const int len = kv_len(a.len[b], a.max_len);
-  if (len <= a.budget) {         // every row stays
-    if (a.in_place)
-      for (int j = t; j < len; j += EV_T) a.list[(size_t)blockIdx.x * a.lcap + j] = j;
-    return;
-  }
+  if (len <= a.budget) return;   // every row stays: no list
   const int* trow = a.p.table + (size_t)b * a.p.table_ld;
   const int lo = min(a.sinks, len), hi = max(lo, len - a.recent);   // [lo, hi) competes
-  int need = a.budget - (len - (hi - lo));                          // how many of it stay (>= 0: sinks + recent <= budget)
+  if (t < 2) s_gone[t] = 0;
+  __syncthreads();
+  for (int j = t << a.p.shift; j < len; j += EV_T << a.p.shift)
+    if (kv_page(a.p, trow, j) < 0) {
+      const int end = min(len, j + (1 << a.p.shift)), in = max(0, min(end, hi) - max(j, lo));
+      atomicAdd(&s_gone[0], in);
+      atomicAdd(&s_gone[1], end - j - in);
+    }
   const int m = min(hi, a.staged);
   for (int j = lo + t; j < m; j += EV_T) keys[j] = ev_key(a, trow, h, j);
   __syncthreads();
+  const bool gaps = s_gone[0] + s_gone[1] > 0;
+  const int kept = min(a.budget, len - s_gone[0] - s_gone[1]);
+  int need = kept - (len - (hi - lo) - s_gone[1]);   // how many of [lo, hi) stay (>= 0: sinks + recent <= budget)
+  const bool all = need == hi - lo - s_gone[0];
   auto key = [&](int j) { return j < a.staged ? keys[j] : ev_key(a, trow, h, j); };
 
   unsigned prefix = 0, mask = 0;
-  if (need > 0) {
+  if (need > 0 && !all) {
     for (int pass = 0; pass < 3; pass++) {
       const int sh = pass == 0 ? 20 : (pass == 1 ? 10 : 0), nb = pass == 0 ? 2048 : 1024;
       for (int i = t; i < nb; i += EV_T) hist[i] = 0;
       __syncthreads();
       for (int j = lo + t; j < hi; j += EV_T) {
         const unsigned k = key(j);
-        if ((k & mask) == prefix) atomicAdd(&hist[(k >> sh) & (nb - 1)], 1);
+        if (k != EV_GONE && (k & mask) == prefix) atomicAdd(&hist[(k >> sh) & (nb - 1)], 1);
       }
       __syncthreads();
       // the bin, counted from the top, in which the need-th largest key lies
@@ -328,20 +339,25 @@ __global__ void __launch_bounds__(EV_T) k_kv_select(EvictArgs a) {
       __syncthreads();
     }
   }
-  // kept: outside [lo, hi), a key above prefix, or one of the first `need`
-  // keys equal to it. (need == 0 here only when nothing of [lo, hi) stays.)
+  // kept, if on a page: outside [lo, hi), a key above prefix, or one of the
+  // first `need` keys equal to it; with `all`, every one. (need == 0 here only
+  // when nothing of [lo, hi) stays.)
   const bool none = need == 0;
+  auto keep = [&](int j, bool& gt, bool& eq) {
+    if (j < lo || j >= hi) {
+      gt = !gaps || kv_page(a.p, trow, j) >= 0;
+    } else if (!none) {
+      const unsigned k = key(j);
+      gt = k != EV_GONE && (all || k > prefix);
+      eq = !all && k == prefix;
+    }
+  };
   int* out = a.list + (size_t)blockIdx.x * a.lcap;
   const int seg = (len + EV_T - 1) / EV_T * 32, j0 = warp * seg, j1 = min(len, j0 + seg);
   int ngt = 0, neq = 0;
   for (int j = j0 + lane; j - lane < j1; j += 32) {
     bool gt = false, eq = false;
-    if (j < j1) {
-      const bool in = j >= lo && j < hi;
-      const unsigned k = in && !none ? key(j) : 0u;
-      gt = !in || (!none && k > prefix);
-      eq = in && !none && k == prefix;
-    }
+    if (j < j1) keep(j, gt, eq);
     ngt += __popc(__ballot_sync(0xffffffffu, gt));
     neq += __popc(__ballot_sync(0xffffffffu, eq));
   }
@@ -352,12 +368,7 @@ __global__ void __launch_bounds__(EV_T) k_kv_select(EvictArgs a) {
   const unsigned lt = (1u << lane) - 1u;
   for (int j = j0 + lane; j - lane < j1; j += 32) {
     bool gt = false, eq = false;
-    if (j < j1) {
-      const bool in = j >= lo && j < hi;
-      const unsigned k = in && !none ? key(j) : 0u;
-      gt = !in || (!none && k > prefix);
-      eq = in && !none && k == prefix;
-    }
+    if (j < j1) keep(j, gt, eq);
     const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
     const int e = peq + __popc(be & lt);
     const int d = pgt + __popc(bg & lt) + min(e, need);
@@ -365,59 +376,142 @@ __global__ void __launch_bounds__(EV_T) k_kv_select(EvictArgs a) {
     pgt += __popc(bg);
     peq += __popc(be);
   }
+  for (int d = kept + t; d < a.lcap; d += EV_T) out[d] = -1;
+}
+
+// rows of sequence row trow, of its first len, that lie on a page; for a whole CTA
+template <int T>
+PB_DEV int ev_named(const KvPool& p, const int* trow, int len) {
+  __shared__ int part[T / 32];
+  int n = 0;
+  for (int j = threadIdx.x << p.shift; j < len; j += T << p.shift)
+    if (kv_page(p, trow, j) >= 0) n += min(1 << p.shift, len - j);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = n;
+  __syncthreads();
+  n = 0;
+#pragma unroll
+  for (int w = 0; w < T / 32; w++) n += part[w];
+  return n;
 }
 
 // The kept rows to the fresh pages: D / 8 lanes per row, K and V and the
-// weight, EV_R rows per lane group with all their loads in flight. 16
+// weight, EV_R rows per lane group with all their loads in flight. A sequence
+// within the budget has no list (for 16 sequences of 2500 to 4352 rows, most
+// of them within 4096, lists of all rows cost 96 against 86 us): row i is row
+// i, unless a page before it is missing. That is looked up beside the rows'
+// loads, and only then the rows are found by counting. 16
 // sequences of 2500 to 4352 rows to 4096, 32/8 heads x 128: 86 us with the
 // select (17 of them, hardly beside the gather), 5.3 TB/s over the whole call.
 constexpr int EV_R = 4, EV_GT = 256;
 
+// rows c0 .. c0 + C - 1 of a sequence within the budget some of whose pages
+// are missing: the pages in order, EV_GT at a time, with the rows before each
 template <int D>
-__global__ void __launch_bounds__(EV_GT) k_kv_gather(EvictArgs a, int chunks) {
-  constexpr int LPH = D / 8, G = EV_GT / LPH;   // lane groups per CTA
+__device__ __noinline__ void ev_gather_named(const EvictArgs& a, int b, int h, int c0, int len) {
+  constexpr int LPH = D / 8, G = EV_GT / LPH, C = G * EV_R;
+  __shared__ int from_row[C], wsum[EV_GT / 32];
+  const int t = threadIdx.x, ps = 1 << a.p.shift;
+  const int* trow = a.p.table + (size_t)b * a.p.table_ld;
+  for (int i = t; i < C; i += EV_GT) from_row[i] = -1;
+  int base = 0;
+  for (int j0 = 0; j0 < len && base < c0 + C; j0 += EV_GT << a.p.shift) {
+    const int j = j0 + (t << a.p.shift), own = j < len && kv_page(a.p, trow, j) >= 0 ? min(ps, len - j) : 0;
+    int inc = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if ((t & 31) >= o) inc += v;
+    }
+    __syncthreads();
+    if ((t & 31) == 31) wsum[t >> 5] = inc;
+    __syncthreads();
+    int first = base + inc - own;
+    for (int x = 0; x < EV_GT / 32; x++) {
+      if (x < t >> 5) first += wsum[x];
+      base += wsum[x];
+    }
+    for (int i = max(first, c0); i < min(first + own, c0 + C); i++) from_row[i - c0] = j + i - first;
+  }
+  __syncthreads();
+  const int l = t % LPH;
+  for (int r = t / LPH; r < C; r += G) {
+    const int j = from_row[r], i = c0 + r;
+    if (j < 0) break;
+    const int sp = kv_page(a.p, trow, j), dp = kv_page(a.p, a.dst + (size_t)b * a.dst_ld, i);
+    if (dp < 0) continue;
+    const long long from = (long long)sp * a.p.ps + (long long)h * a.p.hs + (long long)(j & (ps - 1)) * a.p.rs + l * 16;
+    const long long to = (long long)dp * a.p.ps + (long long)h * a.p.hs + (long long)(i & (ps - 1)) * a.p.rs + l * 16;
+    *reinterpret_cast<uint4*>(a.p.k + to) = *reinterpret_cast<const uint4*>(a.p.k + from);
+    *reinterpret_cast<uint4*>(a.p.v + to) = *reinterpret_cast<const uint4*>(a.p.v + from);
+    if (l == 0)
+      a.p.w[((size_t)dp * a.p.n_kv + h) * ps + (i & (ps - 1))] = a.p.w[((size_t)sp * a.p.n_kv + h) * ps + (j & (ps - 1))];
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(EV_GT) k_kv_gather(const __grid_constant__ EvictArgs a, int chunks) {
+  constexpr int LPH = D / 8, G = EV_GT / LPH, C = G * EV_R;   // lane groups, rows per CTA
   const int bh = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
   const int b = bh / a.p.n_kv, h = bh % a.p.n_kv;
-  const int l = threadIdx.x % LPH, g = threadIdx.x / LPH;
-  const int len = kv_len(a.len[b], a.max_len), n = min(len, a.budget);
+  const int t = threadIdx.x, l = t % LPH, g = t / LPH, c0 = chunk * C;
+  const int len = kv_len(a.len[b], a.max_len), n = min(len, a.budget);   // (n: no more rows than that)
   const int ps = 1 << a.p.shift;
-  pb_grid_wait();      // the lists
-  // In place, CTAs that start later read this as len[b]: min(n, budget) = n,
-  // and nothing but n depends on it then (every sequence has a list. Otherwise
-  // those within the budget need none: 86 against 96 us for 16 sequences of
-  // 2500 to 4352 rows, most of them within 4096).
-  if (chunk == 0 && h == 0 && threadIdx.x == 0) a.new_len[b] = n;
   const int* trow = a.p.table + (size_t)b * a.p.table_ld;
   const int* drow = a.dst + (size_t)b * a.dst_ld;
-  const bool listed = a.in_place ? a.list != nullptr : len > a.budget;
+  const bool listed = len > a.budget;
   const int* list = a.list + ((size_t)b * a.p.n_kv + h) * a.lcap;
-  const int i0 = chunk * (G * EV_R) + g;
+  pb_grid_launch_dependents();
+  bool gone = false;
+  if (!listed)
+    for (int j = t << a.p.shift; j < min(n, c0 + C); j += EV_GT << a.p.shift) gone |= kv_page(a.p, trow, j) < 0;
+  pb_grid_wait();      // the lists
   uint4 kk[EV_R], vv[EV_R];
   float w[EV_R];
-  long long to[EV_R];
-  size_t wto[EV_R];
+  int to[EV_R];        // the fresh page, or -1
 #pragma unroll
   for (int r = 0; r < EV_R; r++) {
-    const int i = i0 + r * G;
+    const int i = c0 + g + r * G;
     to[r] = -1;
     if (i >= n) continue;
     const int j = listed ? list[i] : i;
+    if (j < 0) continue;
     const int sp = kv_page(a.p, trow, j), dp = kv_page(a.p, drow, i);
     if (sp < 0 || dp < 0) continue;
     const long long from = (long long)sp * a.p.ps + (long long)h * a.p.hs + (long long)(j & (ps - 1)) * a.p.rs + l * 16;
-    to[r] = (long long)dp * a.p.ps + (long long)h * a.p.hs + (long long)(i & (ps - 1)) * a.p.rs + l * 16;
-    wto[r] = ((size_t)dp * a.p.n_kv + h) * ps + (i & (ps - 1));
+    to[r] = dp;
     kk[r] = *reinterpret_cast<const uint4*>(a.p.k + from);
     vv[r] = *reinterpret_cast<const uint4*>(a.p.v + from);
     w[r] = a.p.w[((size_t)sp * a.p.n_kv + h) * ps + (j & (ps - 1))];
   }
+  if (!listed && __syncthreads_or(gone)) {
+    ev_gather_named<D>(a, b, h, c0, len);
+  } else {
 #pragma unroll
-  for (int r = 0; r < EV_R; r++) {
-    if (to[r] < 0) continue;
-    *reinterpret_cast<uint4*>(a.p.k + to[r]) = kk[r];
-    *reinterpret_cast<uint4*>(a.p.v + to[r]) = vv[r];
-    if (l == 0) a.p.w[wto[r]] = w[r];
+    for (int r = 0; r < EV_R; r++) {
+      if (to[r] < 0) continue;
+      const int row = (c0 + g + r * G) & (ps - 1);
+      const long long at = (long long)to[r] * a.p.ps + (long long)h * a.p.hs + (long long)row * a.p.rs + l * 16;
+      *reinterpret_cast<uint4*>(a.p.k + at) = kk[r];
+      *reinterpret_cast<uint4*>(a.p.v + at) = vv[r];
+      if (l == 0) a.p.w[((size_t)to[r] * a.p.n_kv + h) * ps + row] = w[r];
+    }
   }
+  if (chunk == 0 && h == 0 && !a.in_place) {
+    const int m = min(ev_named<EV_GT>(a.p, trow, len), a.budget);
+    if (t == 0) a.new_len[b] = m;
+  }
+}
+
+// The lengths where they replace the old ones, which every CTA of the gather
+// reads: a kernel of its own behind it.
+constexpr int EV_LT = 128;
+__global__ void __launch_bounds__(EV_LT) k_kv_lengths(EvictArgs a) {
+  const int b = blockIdx.x;
+  const int n = min(ev_named<EV_LT>(a.p, a.p.table + (size_t)b * a.p.table_ld, kv_len(a.len[b], a.max_len)), a.budget);
+  pb_grid_wait();
+  if (threadIdx.x == 0) a.new_len[b] = n;
 }
 
 }  // namespace
@@ -568,6 +662,8 @@ extern "C" int pb_kv_evict(const pb_kv_pages* c, const pb_kv_evict_args* g, void
   const long long blocks = (long long)n_seq * c->n_kv * chunks;
   if (blocks > INT_MAX) return pb_set_error(PB_EINVAL, "pb_kv_evict: %d sequences of %d rows", n_seq, cap);
   const bool pdl = max_len > budget;   // (behind the select)
-  return c->head_dim == 64 ? kv_launch(k_kv_gather<64>, (unsigned)blocks, EV_GT, 0, st, pdl, "k_kv_gather", a, chunks)
-                           : kv_launch(k_kv_gather<128>, (unsigned)blocks, EV_GT, 0, st, pdl, "k_kv_gather", a, chunks);
+  int rc = c->head_dim == 64 ? kv_launch(k_kv_gather<64>, (unsigned)blocks, EV_GT, 0, st, pdl, "k_kv_gather", a, chunks)
+                             : kv_launch(k_kv_gather<128>, (unsigned)blocks, EV_GT, 0, st, pdl, "k_kv_gather", a, chunks);
+  if (!rc && a.in_place) rc = kv_launch(k_kv_lengths, (unsigned)n_seq, EV_LT, 0, st, true, "k_kv_lengths", a);
+  return rc;
 }

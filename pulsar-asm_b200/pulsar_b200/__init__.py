@@ -543,7 +543,8 @@ class KVPages:
 
     def evict(self, table, length, dst_table, new_length, budget, sinks=0, recent=0, max_len=0, scratch=None, stream=None):
         """keep up to `budget` rows of each sequence and K/V head (the first `sinks`, the last `recent`, then the
-        largest weights), moved in order to the pages of dst_table; new_length (may be length) receives the lengths"""
+        largest weights), moved in order to the pages of dst_table; new_length (may be length) receives the lengths. Rows
+        on no page are left out."""
         if self._away():
             return self._on_device(self.evict, table, length, dst_table, new_length, budget, sinks, recent, max_len, scratch, stream)
         L = lib()

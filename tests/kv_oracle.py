@@ -89,3 +89,16 @@ def evict_rows(wgt, n, budget, sinks, recent):
     free = sorted(range(lo, hi), key=lambda j: (-wgt[j], j))
     gone = set(free[len(free) - (n - budget):])
     return [j for j in range(n) if j not in gone]
+
+
+def evict_rows_named(wgt, named, n, budget, sinks, recent):
+    """the same where some rows lie on no page (named: which do): those are left out, as if they were not there, but the
+    first and the last rows are counted by their place in the sequence"""
+    have = [j for j in range(n) if named[j]]
+    if len(have) <= budget:
+        return have
+    wgt = [float(x) if x > 0 else 0.0 for x in wgt]
+    lo, hi = min(sinks, n), max(min(sinks, n), n - recent)
+    free = sorted((j for j in have if lo <= j < hi), key=lambda j: (-wgt[j], j))
+    gone = set(free[len(free) - (len(have) - budget):])
+    return [j for j in have if j not in gone]

@@ -800,3 +800,63 @@ def test_prefill_of_many_sequences(pb, cuda):
     check(torch, f64(out), o, spread, slack, tiny, 20, c.dt, torch.float16, "prefill")
     (o, spread, slack, tiny), _ = oracle_rows(c, q1, lens, [1] * S, 64 ** -0.5, 0, 0)
     check(torch, f64(one), o, spread, slack, tiny, 20, c.dt, torch.float16, "decode")
+
+
+# --------------------------------------------------- rows that lie on no page
+EVICT_GONE = [  # nkv, D, ps, dtype, layout, lens, pages without a name, budget, sinks, recent, weights
+    (2, 128, 16, "bfloat16", "head", [300, 300, 170, 120, 90, 77, 310, 0],
+     [[0, 1, 2], [5, 9, 18], [2, 4, 10], [0, 3], range(6), [], [], []], 160, 5, 20, "random"),
+    (2, 64, 16, "float16", "row", [300, 300, 170, 120, 90, 77, 310, 0],
+     [[0, 1, 2], [5, 9, 18], [2, 4, 10], [0, 3], range(6), [], [], []], 160, 5, 20, "zeros"),
+    (1, 64, 32, "float16", "mixed", [300, 300, 170, 120, 90, 77], [[0], [4, 9], [2, 5], [0, 2], [0, 1, 2], []], 400, 3, 20, "random"),
+    (3, 128, 64, "float16", "head", [9000, 8700, 700], [[0, 1, 2, 50, 139], [], [10]], 8600, 64, 100, "random"),
+    (1, 64, 16, "bfloat16", "head", [5000, 4990], [[0, 260], range(0, 300, 2)], 4990, 0, 0, "random"),
+    (64, 128, 64, "float16", "head", [4300, 100], [[0, 40], [0]], 4096, 0, 8, "random"),
+]
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("nkv,D,ps,dt,layout,lens,gone,budget,sinks,recent,kind", EVICT_GONE)
+def test_evict_leaves_rows_without_a_page_out(pb, cuda, nkv, D, ps, dt, layout, lens, gone, budget, sinks, recent, kind, in_place):
+    """the fresh pages hold NaN and may be more than the kept rows need: every row of the new length is a row that was
+    seen before, and nothing behind it is written"""
+    torch = cuda
+    S = len(lens)
+    c = Cache(pb, torch, lens + [min(n, budget) for n in lens], nkv, D, ps, getattr(torch, dt), layout, True, seed=budget + D)
+    table, dst = c.table[:S].contiguous(), c.table[S:].contiguous()
+    for t in (c.k, c.v):
+        t[torch.unique(dst[dst >= 0]).long().cuda()] = float("nan")
+    for b in range(S):
+        for i, p in enumerate(gone[b]):
+            table[b, p] = (-1, c.n_pages, 10 ** 9)[i % 3]
+    if kind == "zeros":
+        c.w.zero_()
+    K, V, W = c.k.clone(), c.v.clone(), c.w.clone()
+    w = f64(c.w)
+    kept = []
+    for b, n in enumerate(lens):
+        pg, r, ok = KO.rows_of(table.numpy(), b, n, ps, c.n_pages)
+        for h in range(nkv):
+            at = KO.evict_rows_named(w[np.where(ok, pg, 0), h, r], ok, n, budget, sinks, recent)
+            to, tr, _ = KO.rows_of(dst.numpy(), b, len(at), ps, c.n_pages)
+            i = [torch.from_numpy(np.ascontiguousarray(x)).long().cuda() for x in (to, tr, pg[at], r[at])]
+            for t, o in ((K, c.k), (V, c.v), (W, c.w)):
+                t[i[0], h, i[1]] = o[i[2], h, i[3]]
+        kept.append(len(at))
+    length = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    new = length if in_place else torch.full((S,), -1, dtype=torch.int32, device="cuda")
+    c.h.evict(table.cuda(), length, dst.cuda(), new, budget, sinks=sinks, recent=recent,
+              scratch=torch.zeros(4 * S * nkv * budget, dtype=torch.uint8, device="cuda"))
+    torch.cuda.synchronize()
+    assert new.tolist() == kept
+    bits = lambda t: t.contiguous().view(torch.int32 if t.dtype == torch.float32 else torch.int16)
+    for got, want, what in ((c.k, K, "k"), (c.v, V, "v"), (c.w, W, "weights")):
+        assert torch.equal(bits(got), bits(want)), what
+    # the next step sees the kept rows alone
+    c.table = dst
+    q = torch.randn((S, 2 * nkv, D), generator=c.g).to(c.dt).cuda()
+    out = torch.empty_like(q)
+    c.h.decode(dst.cuda(), new, q, out)
+    torch.cuda.synchronize()
+    (o, spread, slack, tiny), _ = oracle_rows(c, q, kept, [1] * S, D ** -0.5, 0, 0)
+    check(torch, f64(out), o, spread, slack, tiny, max(kept), c.dt, c.dt, "decode behind it")

@@ -214,3 +214,15 @@ def test_oracle_evict_order():
     assert KO.evict_rows(w, 8, 5, 0, 0) == [1, 3, 4, 5, 6]
     assert KO.evict_rows(w, 8, 2, 1, 1) == [0, 7]
     assert KO.evict_rows([float("nan"), -3, 1, 0], 4, 2, 0, 0) == [0, 2]
+
+
+def test_oracle_evict_order_with_rows_on_no_page():
+    w, all_, n = [0, 5, 1, 5, 9, 2, 5, 0], [True] * 8, 8
+    for budget, sinks, recent in ((8, 1, 1), (4, 1, 1), (5, 0, 0), (2, 1, 1)):
+        assert KO.evict_rows_named(w, all_, n, budget, sinks, recent) == KO.evict_rows(w, n, budget, sinks, recent)
+    some = [False, True, True, False, True, True, True, True]
+    assert KO.evict_rows_named(w, some, n, 8, 1, 1) == [1, 2, 4, 5, 6, 7]      # within the budget: moved together
+    assert KO.evict_rows_named(w, some, n, 6, 1, 1) == [1, 2, 4, 5, 6, 7]
+    assert KO.evict_rows_named(w, some, n, 3, 1, 1) == [1, 4, 7]               # row 0 is not there to stay
+    assert KO.evict_rows_named(w, some, n, 4, 0, 3) == [4, 5, 6, 7]
+    assert KO.evict_rows_named(w, [False] * 8, n, 3, 1, 1) == []
