@@ -128,6 +128,7 @@ template <int D, int CT, int NT, bool P2>
 __global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs d) {
   typedef DcGeo<D> G;
   constexpr int KT = G::KT, TILE = G::TILE, NB = G::NB, NS = G::NS, CPR = D / 8, RS = 32 / CPR;
+  constexpr float UP = CT == PB_DT_F16 ? 15.0f : 0.0f;   // log2 of the probabilities' factor
   extern __shared__ __align__(128) char dsm[];
   const AttnKvArgs& a = d.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -316,11 +317,13 @@ __global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs
           }
         }
         // p in the cache's type for the matrix product (as exact as an output of that type: the
-        // roundings of many rows average out); their sum in fp32 from before that rounding
+        // roundings of many rows average out); their sum in fp32 from before that rounding. In
+        // fp16, times 2^15, in the sum as well: what lies below 2^-25 of the largest would be 0 there,
+        // and many such rows together may be all that an output has (a first row far above the rest).
         float p[4];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-          const float r = m[n][u] == -INFINITY ? 0.0f : m[n][u];
+          const float r = (m[n][u] == -INFINITY ? 0.0f : m[n][u]) - UP;
           p[u] = kv_ex2(s[n][u] - r);
           p[2 + u] = kv_ex2(s[n][2 + u] - r);
           l[n][u] += p[u] + p[2 + u];
@@ -364,7 +367,7 @@ __global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs
               row[k * 16 + g] = o[n][half * 4 + k][u];
               row[k * 16 + g + 8] = o[n][half * 4 + k][2 + u];
             }
-            if (g == 0) { mml[(warp * 8 + 2 * c + u) * 2] = m[n][u]; mml[(warp * 8 + 2 * c + u) * 2 + 1] = l[n][u]; }
+            if (g == 0) { mml[(warp * 8 + 2 * c + u) * 2] = m[n][u] - UP; mml[(warp * 8 + 2 * c + u) * 2 + 1] = l[n][u]; }
           }
           __syncthreads();
           {

@@ -860,3 +860,46 @@ def test_evict_leaves_rows_without_a_page_out(pb, cuda, nkv, D, ps, dt, layout, 
     torch.cuda.synchronize()
     (o, spread, slack, tiny), _ = oracle_rows(c, q, kept, [1] * S, D ** -0.5, 0, 0)
     check(torch, f64(out), o, spread, slack, tiny, max(kept), c.dt, c.dt, "decode behind it")
+
+
+# ------------------------------------- one row far above a long, even rest
+def far_below(pb, torch, n, nkv, D, dt, gap, first, noise, seed):
+    """row `first` of a cache of n rows scores `gap` above the others (q = 4 in dimension 0, scale 1) and has V = 0, so
+    that what the others leave is the whole output"""
+    c = Cache(pb, torch, [n], nkv, D, 64, dt, seed=seed)
+    pg, r, _ = KO.rows_of(c.table.numpy(), 0, n, 64, c.n_pages)
+    pg, r = torch.from_numpy(pg).long().cuda(), torch.from_numpy(r).cuda()
+    k = torch.zeros((n, nkv, D))
+    k[:, :, 0] = torch.randn((n, nkv), generator=c.g) * noise / 4
+    k[first, :, 0] = gap / 4
+    v = torch.ones((n, nkv, D))
+    v[:, :, 1::2] += 0.5 * torch.randn((n, nkv, D // 2), generator=c.g)
+    v[first] = 0
+    c.k[pg, :, r], c.v[pg, :, r] = k.to(dt).cuda(), v.to(dt).cuda()
+    return c
+
+
+FAR = [("float16", "float16"), ("float16", "bfloat16"), ("bfloat16", "bfloat16")]
+
+
+@pytest.mark.parametrize("dt,ot", FAR)
+@pytest.mark.parametrize("D,gap,first,noise", [(64, 16.0, 0, 0.0), (128, 17.5, 0, 0.0), (128, 18.0, 0, 0.3), (64, 18.0, 9000, 0.0),
+                                               (128, 20.0, 3, 0.3)])
+def test_decode_small_probabilities_are_kept(pb, cuda, D, gap, first, noise, dt, ot):
+    """The probabilities are relative to the largest, times 2^15 in fp16: half a step of what is not normal there is
+    2^-25 2^-15 of the largest, whatever the cache's length. One sequence, whose pieces have maxima of their own, and
+    many that share its pages, so that a CTA goes through a whole one."""
+    torch = cuda
+    dt, ot = getattr(torch, dt), getattr(torch, ot)
+    n = 20011
+    c = far_below(pb, torch, n, 2, D, dt, gap, first, noise, seed=D)
+    for S, nh in ((1, 24), (300, 2)):
+        q = torch.zeros((S, nh, D), dtype=dt, device="cuda")
+        q[:, :, 0] = 4.0
+        out = torch.empty((S, nh, D), dtype=ot, device="cuda")
+        length = torch.full((S,), n, dtype=torch.int32, device="cuda")
+        c.h.decode(c.dev().expand(S, -1).contiguous(), length, q, out, scale=1.0)
+        torch.cuda.synchronize()
+        (o, spread, slack, tiny), _ = oracle_rows(c, q[:1], [n], [1], 1.0, 0, 0)
+        for b in {0, S // 2, S - 1}:
+            check(torch, f64(out)[b:b + 1], o, spread, slack, tiny * 2.0 ** -15, n, dt, ot, (S, b))
