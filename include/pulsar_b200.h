@@ -360,8 +360,11 @@ int pb_tq_attention(int bits, const float* d_q, const uint32_t* d_kcode, const f
  * (pb_kv_append), attend with one new token per sequence (pb_kv_decode) or
  * with the last rows of each (pb_kv_prefill), and drop the rows of least
  * accumulated weight (pb_kv_evict). None has a counterpart in the reference,
- * whose caches are contiguous; their results are held to the formulas (fp32
- * sums, one rounding at the store), not to the reference's orders.
+ * whose caches are contiguous; their results are held to the formulas, not to
+ * the reference's orders: sums, norms and softmax statistics in fp32, one
+ * rounding at the store, and in the attention the probabilities rounded once
+ * to the cache's type (to two numbers of it where out has more bits) for the
+ * product with V.
  *  - head_dim 64 or 128; page_size 16, 32, 64, 128 or 256; dtype (of K, V and
  *    q) PB_DT_F16 or PB_DT_BF16; n_heads / n_kv a whole number up to 16.
  *  - Strides are in elements, the last dimension is contiguous, rows start on

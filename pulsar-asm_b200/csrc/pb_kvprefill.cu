@@ -16,7 +16,8 @@
 //  - the running maximum only moves when a row's scores pass it by more than
 //    2^8; the output is rescaled in TMEM then, which is rare. The sum of a row
 //    stays with its thread. Any maximum that is near enough gives the same
-//    quotient.
+//    quotient; so does a factor in the probabilities and their sum, which an
+//    fp16 cache has (2^7).
 // Warp 1 brings the queries, warp 0 K and V tiles, by TMA (a box per page, or part of one, and 64
 // columns, in the 128-byte swizzle the tensor cores read; a table entry that
 // names no page becomes a box outside the pool, which reads as zeros), warps 2
@@ -234,6 +235,11 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
              PfArgs p) {
   typedef PfGeo<D> G;
   constexpr int NST = G::NST, KP = PF_KT * 128, QP = 128 * 128;   // bytes of a 64-column panel of K or V, of Q
+  // log2: how far a score may pass the row's maximum before that moves, and the factor of the probabilities. In fp16,
+  // what lies below 2^-25 would be 0 in the product with V but not in the sum, and many such rows together may be all
+  // that an output has (a first row far above a long rest); so the two take all of the range above 1 and what is lost
+  // lies below 2^-32. (Moving at 2^4 with a factor of 2^11: 513 against 478 us for 8192 tokens of 32/8 heads x 128.)
+  constexpr float LAG = 8.0f, UP = CT == PB_DT_F16 ? 15.0f - LAG : 0.0f;
   extern __shared__ __align__(128) char psm_raw[];
   __shared__ uint64_t kfull[NST], kempty[NST], vfull[NST], vempty[NST], sfull[NG][2], pready[NG][2], pvdone[NG], ofin[NG], lock[4], qfull, vfix[3], done[NG];
   __shared__ uint32_t tbase;
@@ -323,10 +329,10 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
     int pg = 0, st = 0, sf = 0;
     unsigned epar = 1, fpar = 0;
     int fixes = 0;    // at most 3: where the sinks end, where the window begins, the last tile
-    // a tile's V is looked at LAG tiles later: by then others are on their way
+    // a tile's V is looked at LATER tiles on: by then others are on their way
     // (fewer than NST, so that issuing them has not waited for this one's product)
-    constexpr int LAG = 2;
-    for (int i = 0; i < n + LAG; i++) {
+    constexpr int LATER = 2;
+    for (int i = 0; i < n + LATER; i++) {
       if (i < n) {
         const int k0 = pf_key(line, i0 + i), it = i % AHEAD;
         if (it == 0) {
@@ -352,8 +358,8 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
         }
         if (++st == NST) { st = 0; epar ^= 1; }
       }
-      if (i >= LAG) {   // V rows behind what is seen
-        const int k0 = pf_key(line, i0 + i - LAG);
+      if (i >= LATER) {   // V rows behind what is seen
+        const int k0 = pf_key(line, i0 + i - LATER);
         if (pf_edge(line, k0)) {
           pf_wait(&vfull[sf], fpar, stop, 9);
           char* vs = smk + sf * (2 * G::KV) + G::KV;
@@ -489,7 +495,7 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
       }
     const bool gaps = __any_sync(0xffffffffu, gap);
     const pf_f2 sc2 = pf_pk(a.scale2, a.scale2);
-    const float over = 8.0f / a.scale2;
+    const float over = LAG / a.scale2;
     float thr = -INFINITY;                                     // m + over
     const int steps = g < ng ? n : 0;
     for (int i = 0; i < steps; i++) {
@@ -549,10 +555,10 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
           }
         }
       }
-      // p = 2^(scale2 s - ms), rounded to the cache's type, which the product
+      // p = 2^(scale2 s - ms + UP), rounded to the cache's type, which the product
       // with V needs (as exact as an output of that type); the sum takes the
       // unrounded ones
-      const pf_f2 nms = pf_pk(-ms, -ms);
+      const pf_f2 nms = pf_pk(UP - ms, UP - ms);
       pf_f2 y[2] = {0ull, 0ull};
 #pragma unroll
       for (int q = 0; q < 4; q++) {

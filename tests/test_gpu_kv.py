@@ -903,3 +903,26 @@ def test_decode_small_probabilities_are_kept(pb, cuda, D, gap, first, noise, dt,
         (o, spread, slack, tiny), _ = oracle_rows(c, q[:1], [n], [1], 1.0, 0, 0)
         for b in {0, S // 2, S - 1}:
             check(torch, f64(out)[b:b + 1], o, spread, slack, tiny * 2.0 ** -15, n, dt, ot, (S, b))
+
+
+@pytest.mark.parametrize("dt,ot", FAR)
+@pytest.mark.parametrize("D,gap,first,noise,chunk", [(64, 16.0, 0, 0.0, 16), (128, 17.5, 0, 0.0, 40), (128, 18.0, 0, 0.3, 5000),
+                                                     (64, 18.0, 9000, 0.0, 5000), (128, 20.0, 3, 0.3, 16)])
+def test_prefill_small_probabilities_are_kept(pb, cuda, D, gap, first, noise, chunk, dt, ot):
+    """as in decode, but times 2^7 at the least: the maximum that the probabilities are relative to may be 2^8 behind.
+    Few rows split over the SMs, and many rows with the whole line in each CTA."""
+    torch = cuda
+    dt, ot = getattr(torch, dt), getattr(torch, ot)
+    n, nh = 20011, 8
+    c = far_below(pb, torch, n, 2, D, dt, gap, first, noise, seed=D + 1)
+    q = torch.zeros((chunk, nh, D), dtype=dt, device="cuda")
+    q[:, :, 0] = 4.0
+    out = torch.empty((chunk, nh, D), dtype=ot, device="cuda")
+    c.h.prefill(c.dev(), torch.tensor([0, chunk], dtype=torch.int32, device="cuda"),
+                torch.tensor([n], dtype=torch.int32, device="cuda"), q, out, scale=1.0)
+    torch.cuda.synchronize()
+    c.h.status()
+    k, v, qq, got = f64(c.k), f64(c.v), f64(q), f64(out)
+    for i in sorted({0, chunk // 2, chunk - 2, chunk - 1}):
+        o, spread, slack, tiny, _ = KO.attend(qq[i], k, v, None, c.table.numpy(), 0, n - chunk + i, n, 1.0, 0, 0)
+        check(torch, got[i:i + 1], o[None], spread[None], slack[None], tiny[None] * 2.0 ** -7, n, dt, ot, i)
