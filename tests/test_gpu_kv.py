@@ -961,3 +961,37 @@ def test_prefill_time_does_not_depend_on_left_shared_memory(pb, cuda, nh, nkv, D
             first = out.clone() if first is None else first
             assert torch.equal(out, first)
     assert np.median(times[1]) < 1.1 * np.median(times[0]), [np.median(t) for t in times]
+
+
+# -------------------------------------------------- lines of many key tiles
+@pytest.mark.parametrize("nh,nkv,D,ps,dt,window", [(8, 2, 64, 16, "float16", 0), (8, 2, 128, 64, "bfloat16", 0),
+                                                   (6, 1, 64, 32, "bfloat16", 0), (5, 1, 128, 16, "float16", 1100),
+                                                   (16, 8, 64, 128, "float16", 1000)])
+def test_prefill_of_some_thousand_rows(pb, cuda, nh, nkv, D, ps, dt, window):
+    """prompts whose CTAs go through 25 to 50 key tiles each: every ring stage is used several times, pages are looked up
+    several times; not split over the keys"""
+    torch = cuda
+    dt = getattr(torch, dt)
+    lens, counts = [1500, 3100], [1500, 2500]
+    c = Cache(pb, torch, lens, nkv, D, ps, dt, seed=nh + ps)
+    rows = sum(counts)
+    q = torch.randn((rows, nh, D), generator=c.g).to(dt).cuda()
+    out = torch.full((rows, nh, D), 9.0, dtype=dt, device="cuda")
+    start = torch.tensor([0, 1500, 4000], dtype=torch.int32, device="cuda")
+    c.h.prefill(c.dev(), start, torch.tensor(lens, dtype=torch.int32, device="cuda"), q, out, window=window, sinks=5)
+    torch.cuda.synchronize()
+    c.h.status()
+    # in 64 bits, a whole head at a time
+    k, v, qq, got, r = f64(c.k), f64(c.v), f64(q), f64(out), 0
+    for b, (n, m) in enumerate(zip(lens, counts)):
+        pg, rr, _ = KO.rows_of(c.table.numpy(), b, n, ps, c.n_pages)
+        sees = np.stack([KO.seen(t, n, window, 5) for t in range(n - m, n)])
+        for h in range(nh):
+            kk, vv, x = k[pg, h // (nh // nkv), rr], v[pg, h // (nh // nkv), rr], qq[r:r + m, h]
+            s = np.where(sees, x @ kk.T * D ** -0.5, -np.inf)
+            e = np.exp(s - s.max(1, keepdims=True))
+            p = e / e.sum(1, keepdims=True)
+            slack = 2.0 ** -24 * ((D + 8) * np.where(sees, np.abs(x) @ np.abs(kk).T, 0).max(1) * D ** -0.5 + 16)
+            check(torch, got[r:r + m, h], p @ vv, p @ np.abs(vv), slack, sees @ np.abs(vv) / e.sum(1, keepdims=True), n, dt, dt,
+                  (b, h))
+        r += m
