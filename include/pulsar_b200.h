@@ -362,9 +362,9 @@ int pb_tq_attention(int bits, const float* d_q, const uint32_t* d_kcode, const f
  * accumulated weight (pb_kv_evict). None has a counterpart in the reference,
  * whose caches are contiguous; their results are held to the formulas, not to
  * the reference's orders: sums, norms and softmax statistics in fp32, one
- * rounding at the store, and in the attention the probabilities rounded once
- * to the cache's type (to two numbers of it where out has more bits) for the
- * product with V.
+ * rounding at the store. For the product with V the attention rounds the
+ * probabilities: pb_kv_decode to more bits than out has, pb_kv_prefill to the
+ * cache's type (two numbers of it where out has more bits).
  *  - head_dim 64 or 128; page_size 16, 32, 64, 128 or 256; dtype (of K, V and
  *    q) PB_DT_F16 or PB_DT_BF16; n_heads / n_kv a whole number up to 16.
  *  - Strides are in elements, the last dimension is contiguous, rows start on

@@ -121,9 +121,14 @@ PB_DEV void dc_store(const DcArgs& d, int b, int h, int e, const float4& x) {
   *reinterpret_cast<uint2*>(o) = w;
 }
 
-// P2: the probabilities as two numbers of the cache's type, for an output with
-// more bits than that has (fp16 from a bf16 cache: error against 64 bits 0.0002
-// instead of 0.0007 of the output for sequences of 2 and 3 rows; the same time).
+// P2: the probabilities as two numbers of the cache's type, the second what the
+// rounding of the first left, so that the output's own rounding is the largest
+// error: for every output but bf16 of an fp16 cache, which has that with one
+// (error against 64 bits of fp16 from bf16, 2 and 3 rows: 0.0002 instead of
+// 0.0007 of the output; of bf16 from bf16, long: 0.0016 instead of 0.0020).
+// Long caches take the same time (139.6 against 139.2 us), a window with sinks
+// 63.9 against 63.8; with 64 ragged sequences, whose fp16 cache and bf16
+// output do without, it would be 30.0 against 29.6.
 template <int D, int CT, int NT, bool P2>
 __global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs d) {
   typedef DcGeo<D> G;
@@ -316,8 +321,7 @@ __global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs
             for (int k = 0; k < D / 16; k++) { o[n][k][u] *= f; o[n][k][2 + u] *= f; }
           }
         }
-        // p in the cache's type for the matrix product (as exact as an output of that type: the
-        // roundings of many rows average out); their sum in fp32 from before that rounding. In
+        // p in the cache's type for the matrix product; their sum in fp32 from before that rounding. In
         // fp16, times 2^15, in the sum as well: what lies below 2^-25 of the largest would be 0 there,
         // and many such rows together may be all that an output has (a first row far above the rest).
         float p[4];
@@ -576,8 +580,8 @@ template <int D>
 int dc_run(const DcArgs& d, int ct, bool join, cudaStream_t st) {
   const bool two = d.a.grp > 8;
   int rc;
-  if (ct == PB_DT_F16) rc = two ? dc_launch<D, PB_DT_F16, 2, false>(d, st) : dc_launch<D, PB_DT_F16, 1, false>(d, st);
-  else if (d.out_bf16) rc = two ? dc_launch<D, PB_DT_BF16, 2, false>(d, st) : dc_launch<D, PB_DT_BF16, 1, false>(d, st);
+  if (ct == PB_DT_F16 && d.out_bf16) rc = two ? dc_launch<D, PB_DT_F16, 2, false>(d, st) : dc_launch<D, PB_DT_F16, 1, false>(d, st);
+  else if (ct == PB_DT_F16) rc = two ? dc_launch<D, PB_DT_F16, 2, true>(d, st) : dc_launch<D, PB_DT_F16, 1, true>(d, st);
   else rc = two ? dc_launch<D, PB_DT_BF16, 2, true>(d, st) : dc_launch<D, PB_DT_BF16, 1, true>(d, st);
   if (rc) return rc;
   // (a group's pieces: at most one per tile and per CTA)

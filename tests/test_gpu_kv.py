@@ -995,3 +995,22 @@ def test_prefill_of_some_thousand_rows(pb, cuda, nh, nkv, D, ps, dt, window):
             check(torch, got[r:r + m, h], p @ vv, p @ np.abs(vv), slack, sees @ np.abs(vv) / e.sum(1, keepdims=True), n, dt, dt,
                   (b, h))
         r += m
+
+
+@pytest.mark.parametrize("dt,ot,u", [("bfloat16", "bfloat16", 2.0 ** -16), ("float16", "float16", 2.0 ** -22),
+                                     ("bfloat16", "float16", 2.0 ** -16), ("float16", "bfloat16", 2.0 ** -11)])
+@pytest.mark.parametrize("nh,nkv,D", [(8, 2, 64), (16, 1, 128), (4, 4, 128)])
+def test_decode_rounds_at_the_store(pb, cuda, nh, nkv, D, dt, ot, u):
+    """the probabilities keep more bits than the output has, u (two numbers of the cache's type, each off by half a step
+    of what is left, or fp16 for bf16), so that the output's own rounding is the largest error"""
+    torch = cuda
+    dt, ot = getattr(torch, dt), getattr(torch, ot)
+    lens = [1, 2, 3, 17, 200, 70, 2600, 900]
+    c = Cache(pb, torch, lens, nkv, D, 32, dt, seed=D + nh)
+    S = len(lens)
+    q = (torch.randn((S, nh, D), generator=c.g) * 0.5).to(dt).cuda()
+    out = torch.empty((S, nh, D), dtype=ot, device="cuda")
+    c.h.decode(c.dev(), torch.tensor(lens, dtype=torch.int32, device="cuda"), q, out)
+    torch.cuda.synchronize()
+    (o, spread, slack, tiny), _ = oracle_rows(c, q, lens, [1] * S, D ** -0.5, 0, 0)
+    check(torch, f64(out), o, spread, slack, tiny * 2.0 ** -15, max(lens), dt, ot, "out", u=u)
