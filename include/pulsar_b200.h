@@ -459,8 +459,11 @@ int pb_kv_decode(const pb_kv_pages* c, const pb_kv_attention_args* a, void* stre
  * every sequence are left as they were.                                      */
 long long pb_kv_prefill_scratch(const pb_kv_pages* c, int n_seq, int max_len, int n_tok, int n_heads);
 int pb_kv_prefill(const pb_kv_pages* c, const pb_kv_attention_args* a, void* stream);
-/* synchronise `stream` and report a bounded wait inside the current device's
- * pb_kv_prefill kernels that gave up since the last report: PB_OK or PB_ECUDA */
+/* The waits inside pb_kv_prefill are bounded: one that lasts a second is given
+ * up, the output of that call is void, and only this call says so. It
+ * synchronises `stream` and reports the waits that pb_kv_prefill calls gave up
+ * on the current device since the last report, on any stream, once:
+ * PB_OK or PB_ECUDA. */
 int pb_kv_status(void* stream);
 /* per sequence and K/V head, keep the first `sinks` rows, the last `recent`
  * rows and, up to `budget` rows in all, those of the largest weight (equal

@@ -39,6 +39,7 @@
 // for and the TMEM is freed before the CTA ends.
 #include "pb_kvattn.cuh"
 #include <cuda.h>
+#include <mutex>
 
 namespace {
 
@@ -69,7 +70,11 @@ struct PfArgs {
   float2* ml;               // [split][row][head] maximum and sum
 };
 
-__device__ int kv_pf_err;
+// waits that gave up on this device, by their role (1 to 15). The counts only
+// grow: the host compares them with those that it reported last, so no record
+// is lost between a read and a reset.
+constexpr int PF_ROLES = 16;
+__device__ unsigned kv_pf_gave_up[PF_ROLES];
 
 PB_DEV void pf_init(uint64_t* b, unsigned c) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(kv_s32(b)), "r"(c) : "memory");
@@ -92,14 +97,14 @@ PB_DEV unsigned long long pf_now() {
 // raises the CTA's stop flag, at which every further wait returns at once. The
 // roles run on through their loops (all accesses stay in bounds), so copies
 // and products end and the TMEM is freed; the result is void.
-PB_DEV void pf_wait_slow(uint64_t* b, unsigned par, volatile int* stop, int role) {
+PB_DEV void pf_wait_slow(uint64_t* b, unsigned par, volatile int* stop, int role, unsigned long long limit = PF_WAIT_NS) {
   const unsigned long long t0 = pf_now();
   for (unsigned i = 1; !pf_try(b, par); i++) {
     if ((i & 63) == 0) {
       if (*stop) return;
-      if (pf_now() - t0 > PF_WAIT_NS) {
+      if (pf_now() - t0 > limit) {
         *stop = 1;
-        atomicCAS(&kv_pf_err, 0, role);
+        atomicAdd(&kv_pf_gave_up[role], 1u);
         return;
       }
     }
@@ -857,10 +862,41 @@ extern "C" int pb_kv_prefill(const pb_kv_pages* c, const pb_kv_attention_args* g
 }
 
 extern "C" int pb_kv_status(void* stream) {
+  static std::mutex mu;
+  static unsigned reported[64][PF_ROLES];
+  int dev = 0;
+  PB_TRY_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return pb_set_error(PB_ENOTSUP, "pb_kv_status: device %d", dev);
   PB_TRY_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
-  int e = 0;
-  const int zero = 0;
-  PB_TRY_CUDA(cudaMemcpyFromSymbol(&e, kv_pf_err, sizeof e));
-  if (e) PB_TRY_CUDA(cudaMemcpyToSymbol(kv_pf_err, &zero, sizeof zero));
-  return e ? pb_set_error(PB_ECUDA, "k_kv_prefill: a bounded wait gave up (role %d)", e) : PB_OK;
+  std::lock_guard<std::mutex> lk(mu);
+  unsigned now[PF_ROLES];
+  PB_TRY_CUDA(cudaMemcpyFromSymbolAsync(now, kv_pf_gave_up, sizeof now, 0, cudaMemcpyDeviceToHost, (cudaStream_t)stream));
+  PB_TRY_CUDA(cudaStreamSynchronize((cudaStream_t)stream));
+  int role = 0;
+  for (int i = 0; i < PF_ROLES; i++) {
+    if (now[i] != reported[dev][i]) role = i;
+    reported[dev][i] = now[i];
+  }
+  return role ? pb_set_error(PB_ECUDA, "k_kv_prefill: a bounded wait gave up (role %d)", role) : PB_OK;
+}
+
+namespace {
+// the prompt kernel's wait on a barrier that nothing arrives at: it gives up
+// after `limit` and records that; the next one then returns at once
+__global__ void k_test_kv_wait(unsigned long long limit) {
+  __shared__ uint64_t bar;
+  __shared__ int stop;
+  if (threadIdx.x == 0) {
+    pf_init(&bar, 1);
+    stop = 0;
+    pf_wait_slow(&bar, 0, &stop, 14, limit);
+    pf_wait_slow(&bar, 0, &stop, 15, limit);
+  }
+}
+}  // namespace
+// test hook (not part of the public ABI)
+extern "C" int pb_test_kv_wait(unsigned long long limit_ns, void* stream) {
+  k_test_kv_wait<<<1, 32, 0, (cudaStream_t)stream>>>(limit_ns);
+  PB_LAUNCHED("k_test_kv_wait");
+  return PB_OK;
 }

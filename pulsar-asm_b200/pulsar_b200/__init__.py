@@ -123,6 +123,7 @@ def lib():
     L.pb_time_step_kernel.argtypes = [vp, vp, i, i, C.POINTER(C.c_float), C.POINTER(C.c_double), vp]
     L.pb_test_expf.argtypes = [vp, vp, i, vp]
     L.pb_test_grid_wait.argtypes = [vp, C.c_uint, C.c_uint, vp, vp]
+    L.pb_test_kv_wait.argtypes = [C.c_ulonglong, vp]
     L.pb_layer_step_noalloc.argtypes = [vp, vp, i, i, vp, vp]
     L.pb_state_status.argtypes = [vp, vp]
     L.pb_prefill_chunk.argtypes = [vp, vp, vp, i, i, vp, vp, vp]
@@ -537,7 +538,8 @@ class KVPages:
             check(rc)
 
     def status(self, stream=None):
-        """synchronise and raise if a prefill kernel recorded a wait that gave up"""
+        """synchronise the stream and raise if a prefill call on the device, on any stream, has given up a wait since the
+        last report (its output is void then)"""
         with self._torch.cuda.device(self.device):
             check(lib().pb_kv_status(_stream(stream)))
 
@@ -604,6 +606,12 @@ def device_grid_wait(counter, target, limit, stream=None):
     check(lib().pb_test_grid_wait(_ptr(counter), target, limit, _ptr(status), _stream(stream)))
     torch.cuda.synchronize()
     return int(status.item())
+
+
+def device_kv_wait(limit_ns, stream=None):
+    """test hook: a bounded wait of the prompt attention kernel on a barrier
+    that nothing arrives at, which gives up after limit_ns."""
+    check(lib().pb_test_kv_wait(limit_ns, _stream(stream)))
 
 
 def compat_gemv(rows, cols, w, xq, y):

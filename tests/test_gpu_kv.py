@@ -1014,3 +1014,28 @@ def test_decode_rounds_at_the_store(pb, cuda, nh, nkv, D, dt, ot, u):
     torch.cuda.synchronize()
     (o, spread, slack, tiny), _ = oracle_rows(c, q, lens, [1] * S, D ** -0.5, 0, 0)
     check(torch, f64(out), o, spread, slack, tiny * 2.0 ** -15, max(lens), dt, ot, "out", u=u)
+
+
+def test_a_wait_that_gives_up_is_reported_once(pb, cuda):
+    """the prompt kernel's wait on a barrier that nothing arrives at, with a limit of 20 ms: recorded by whichever
+    stream, reported by the next status of any, once; the calls behind it run as before"""
+    torch = cuda
+    c = Cache(pb, torch, [200], 2, 64, 16, torch.float16, seed=2)
+    q = torch.randn((200, 4, 64), generator=c.g).half().cuda()
+    start, length = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 200], [200]))
+    want, out = torch.empty_like(q), torch.empty_like(q)
+    c.h.prefill(c.dev(), start, length, q, want)
+    c.h.status()
+    side = torch.cuda.Stream()
+    for k in range(3):
+        pb.device_kv_wait(20_000_000, side if k else None)
+        if k == 1:
+            pb.device_kv_wait(20_000_000)         # two records, one report
+        torch.cuda.synchronize()                      # (a status waits for its own stream alone)
+        with pytest.raises(pb.PBError, match=r"gave up \(role 14\)"):      # (15: the wait behind it, which returns at once)
+            c.h.status(None if k else side)
+        c.h.status()
+        c.h.status(side)
+    c.h.prefill(c.dev(), start, length, q, out)
+    c.h.status()
+    assert torch.equal(out, want)
