@@ -381,7 +381,12 @@ int pb_tq_attention(int bits, const float* d_q, const uint32_t* d_kcode, const f
  *    In pb_kv_prefill that goes for rows that no query of the chunk sees; a
  *    row that one query of a chunk sees is finite.
  *  - scratch: *_scratch bytes (0: none) of device memory, 16-byte aligned, with no contents kept between
- *    calls; calls that may run at the same time take different scratch.
+ *    calls; calls that may run at the same time take different scratch. The
+ *    *_scratch functions know no table, so their max_len is the bound itself,
+ *    above 0 (table_ld * page_size for a call whose max_len is 0); they return
+ *    -1 for what no call takes. The bytes grow with max_len, not with the
+ *    lengths: the weights of pb_kv_decode take n_seq * max_len floats for
+ *    each query head.
  * Everything is asynchronous on `stream`; tables, lengths and rows must stay
  * as they are until the call has run.                                        */
 typedef struct {

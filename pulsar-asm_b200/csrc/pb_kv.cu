@@ -621,7 +621,8 @@ extern "C" int pb_kv_append(const pb_kv_pages* c, const pb_kv_append_args* g, vo
 }
 
 extern "C" long long pb_kv_evict_scratch(const pb_kv_pages* c, int n_seq, int max_len, int budget) {
-  if (!c || n_seq < 0 || c->n_kv <= 0 || max_len < 0 || budget <= 0) return -1;
+  if (!c || n_seq < 0 || c->n_kv <= 0 || budget <= 0) return -1;
+  if (max_len <= 0) return n_seq == 0 && max_len == 0 ? 0 : -1;
   const long long cap = max_len > budget ? budget : 0;   // no list when nothing can pass the budget
   return (long long)n_seq * c->n_kv * cap * 4;
 }

@@ -602,7 +602,8 @@ int dc_run(const DcArgs& d, int ct, bool join, cudaStream_t st) {
 }  // namespace
 
 extern "C" long long pb_kv_decode_scratch(const pb_kv_pages* c, int n_seq, int max_len, int n_heads, int accumulate) {
-  if (!c || n_seq < 0 || max_len < 0 || n_heads <= 0 || c->n_kv <= 0 || (c->head_dim != 64 && c->head_dim != 128)) return -1;
+  if (!c || n_seq < 0 || n_heads <= 0 || c->n_kv <= 0 || (c->head_dim != 64 && c->head_dim != 128)) return -1;
+  if (max_len <= 0) return n_seq == 0 && max_len == 0 ? 0 : -1;
   const DcPlan p = dc_plan(c, n_seq, max_len, n_heads, accumulate);
   return 4 * (p.part + p.ml + p.lse + p.score);
 }

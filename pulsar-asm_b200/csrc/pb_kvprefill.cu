@@ -833,7 +833,8 @@ int pf_types(const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mq
 }  // namespace
 
 extern "C" long long pb_kv_prefill_scratch(const pb_kv_pages* c, int n_seq, int max_len, int n_tok, int n_heads) {
-  if (!c || n_seq < 0 || max_len < 0 || n_tok < 0 || n_heads <= 0 || c->n_kv <= 0 || n_heads / c->n_kv > 16) return -1;
+  if (!c || n_seq < 0 || n_tok < 0 || n_heads <= 0 || c->n_kv <= 0 || n_heads / c->n_kv > 16) return -1;
+  if (max_len <= 0) return n_seq == 0 && max_len == 0 ? 0 : -1;
   // (a window may need fewer splits: the whole cache's need covers both)
   const PfPlan p = pf_plan(c, n_seq, max_len, n_tok, n_heads, 0, 0);
   return 4 * (p.part + p.ml);

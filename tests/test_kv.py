@@ -226,3 +226,17 @@ def test_oracle_evict_order_with_rows_on_no_page():
     assert KO.evict_rows_named(w, some, n, 3, 1, 1) == [1, 4, 7]               # row 0 is not there to stay
     assert KO.evict_rows_named(w, some, n, 4, 0, 3) == [4, 5, 6, 7]
     assert KO.evict_rows_named(w, [False] * 8, n, 3, 1, 1) == []
+
+
+def test_scratch_sizes_need_the_bound(pb):
+    """0 is no bound of rows there (a call takes it as the table's rows, which these functions do not know): the size of
+    nothing would be refused by the call behind it"""
+    L, c = pb.lib(), C.byref(pool(pb))
+    sizes = (lambda s, m: L.pb_kv_decode_scratch(c, s, m, 32, 1), lambda s, m: L.pb_kv_decode_scratch(c, s, m, 32, 0),
+             lambda s, m: L.pb_kv_prefill_scratch(c, s, m, 9, 32), lambda s, m: L.pb_kv_evict_scratch(c, s, m, 200))
+    for size in sizes:
+        assert size(4, 0) == -1 and size(4, -1) == -1 and size(0, -5) == -1
+        assert size(0, 0) == 0
+        assert size(4, 320) >= 0
+    assert decode(pb, acc=1, bytes=sizes[0](4, 320) - 1) == EINVAL      # what max_len 0 stands for
+    assert evict(pb, bytes=sizes[3](4, 320) - 1) == EINVAL
