@@ -457,6 +457,8 @@ class KVPages:
         # (a negative max_len or count, which the call itself refuses, needs no scratch)
         need = self._need.get((fn.__name__, shape))
         if need is None:
+            if len(self._need) >= 512:      # ragged prompts bring ever new token counts
+                self._need.clear()
             need = self._need[fn.__name__, shape] = fn(self._r, *shape)
         return need
 

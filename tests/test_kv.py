@@ -240,3 +240,13 @@ def test_scratch_sizes_need_the_bound(pb):
         assert size(4, 320) >= 0
     assert decode(pb, acc=1, bytes=sizes[0](4, 320) - 1) == EINVAL      # what max_len 0 stands for
     assert evict(pb, bytes=sizes[3](4, 320) - 1) == EINVAL
+
+
+def test_python_keeps_few_scratch_sizes(pb):
+    """one entry per call shape, of which a server of ragged prompts has no end"""
+    h = object.__new__(pb.KVPages)          # (a real one needs CUDA tensors)
+    h._need, h._r = {}, C.byref(pool(pb))
+    fn = pb.lib().pb_kv_prefill_scratch
+    for n in range(5000):
+        assert h._bytes(fn, 4, 320, 1 + n % 3000, 32) == fn(h._r, 4, 320, 1 + n % 3000, 32)
+    assert len(h._need) <= 1024
