@@ -348,7 +348,7 @@ extern "C" int pb_qlow_pack(const void* codes, const void* scales, int bits, int
   pb_qlow* w = new pb_qlow();
   w->bits = bits; w->N = N; w->K = K;
   if (cudaMalloc(&w->codes, cb) != cudaSuccess || cudaMalloc(&w->scales, sb) != cudaSuccess ||
-      cudaMalloc(&w->err, sizeof(int)) != cudaSuccess || cudaMemset(w->err, 0, sizeof(int)) != cudaSuccess) {
+      cudaMalloc(&w->err, sizeof(int)) != cudaSuccess) {
     cudaGetLastError();
     cudaFree(w->codes);
     cudaFree(w->scales);
@@ -358,7 +358,10 @@ extern "C" int pb_qlow_pack(const void* codes, const void* scales, int bits, int
   }
   cudaStream_t st = (cudaStream_t)stream;
   const cudaMemcpyKind kind = src_on_device ? cudaMemcpyDeviceToDevice : cudaMemcpyHostToDevice;
-  if (cudaMemcpyAsync(w->codes, codes, cb, kind, st) != cudaSuccess ||
+  // (the error word on the same stream: on the default one its fill may run behind a first product on a stream that does
+  // not wait for that, and take its report away)
+  if (cudaMemsetAsync(w->err, 0, sizeof(int), st) != cudaSuccess ||
+      cudaMemcpyAsync(w->codes, codes, cb, kind, st) != cudaSuccess ||
       cudaMemcpyAsync(w->scales, scales, sb, kind, st) != cudaSuccess || cudaStreamSynchronize(st) != cudaSuccess) {
     cudaGetLastError();
     cudaFree(w->codes);
