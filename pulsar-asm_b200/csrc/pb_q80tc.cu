@@ -684,7 +684,9 @@ extern "C" int pb_q80_gemm(const pb_q8* w, int T, const int8_t* d_qx, const uint
       return pb_set_error(PB_ENOMEM, "pb_q80_gemm: scratch");
     }
     g_tc.cap[dev] = need;
+    // there before a kernel on a stream that does not wait for the default one
     PB_TRY_CUDA(cudaMemset(g_tc.p[dev], 0, 256));
+    PB_TRY_CUDA(cudaStreamSynchronize(nullptr));
   }
   int* err = reinterpret_cast<int*>(g_tc.p[dev]);
   int8_t* bq = reinterpret_cast<int8_t*>(g_tc.p[dev] + 256);
