@@ -442,7 +442,8 @@ typedef struct {
  * fp32 [head_dim]; NULL: no norm), rotation of the pairs (i, i + head_dim/2),
  * i < half, by row pos[i] (NULL: slot[i]) of cos / sin (fp32 [n_rope][half];
  * half 0: none), the query heads to q [n_tok][ldq] (the cache's dtype), the K
- * and V rows to row slot[i] of sequence seq[i], whose weight becomes 0. A row
+ * and V rows to row slot[i] of sequence seq[i], whose weight becomes 0 (only
+ * pb_kv_decode adds to it, so behind a prompt all weights are 0). A row
  * whose sequence, slot, page or position is out of range is padding: nothing
  * is written for it. Two rows of a call with the same sequence and slot leave
  * that cache row undefined. q must not overlap qkv. */

@@ -238,7 +238,7 @@ void ap_launch(const AppendArgs& a, int ct, dim3 grid, cudaStream_t st) {
 // as zero), then lists them in order with ballots. A row on no page is left
 // out, whichever it is: moved nowhere, it must not count as a row of the new
 // cache, where it would be seen. One sequence of 1087 rows
-// to 1024: 10.4 us with the gather; the passes' barriers bound it, not its few
+// to 1024: 10.7 us with the gather; the passes' barriers bound it, not its few
 // bytes.
 struct EvictArgs {
   KvPool p;
@@ -402,7 +402,7 @@ PB_DEV int ev_named(const KvPool& p, const int* trow, int len) {
 // of them within 4096, lists of all rows cost 96 against 86 us): row i is row
 // i, unless a page before it is missing. That is looked up beside the rows'
 // loads, and only then the rows are found by counting. 16
-// sequences of 2500 to 4352 rows to 4096, 32/8 heads x 128: 86 us with the
+// sequences of 2500 to 4352 rows to 4096, 32/8 heads x 128: 87 us with the
 // select (17 of them, hardly beside the gather), 5.3 TB/s over the whole call.
 constexpr int EV_R = 4, EV_GT = 256;
 
@@ -505,7 +505,8 @@ __global__ void __launch_bounds__(EV_GT) k_kv_gather(const __grid_constant__ Evi
 }
 
 // The lengths where they replace the old ones, which every CTA of the gather
-// reads: a kernel of its own behind it.
+// reads: a kernel of its own behind it. (Apart from them, the gather's first
+// CTA of each sequence writes them.)
 constexpr int EV_LT = 128;
 __global__ void __launch_bounds__(EV_LT) k_kv_lengths(EvictArgs a) {
   const int b = blockIdx.x;

@@ -19,8 +19,8 @@ namespace {
 //    pieces, one per CTA, whatever the lengths are; a sequence and head that a
 //    cut goes through is joined by a second, small kernel from the pieces'
 //    unnormalised sums, in the order of the line (the same bits every time).
-// Two sequences of 65537 and 131071 rows, 32/8 heads x 128 bf16: 141 us, 6.4
-// TB/s, the rate of a plain copy. 64 ragged ones of 16 to 2048 rows, 32/8 x
+// Two sequences of 65537 and 131071 rows, 32/8 heads x 128 bf16: 139 to 142 us,
+// 6.4 to 6.5 TB/s, the rate of a plain copy. 64 ragged ones of 16 to 2048 rows, 32/8 x
 // 64: 30 us, 4.5 TB/s; there each warp's chain of a tile's steps is what is
 // left (58 % of the DRAM's cycles, 32 % of the issue slots, tensor pipe 9 %).
 // One of 1029 rows: 6.7 us, the latency of two launches and one tile.
@@ -32,7 +32,7 @@ struct DcGeo {
   static constexpr int TILE = DC_W * KT;         // rows per tile
   static constexpr int NB = KT / 16;             // 16-row blocks: one page each
   static constexpr int NS = 2;                   // ring stages per warp: with 3 CTAs an SM faster than 3 stages and 2 CTAs
-                                                 // (64 ragged: 29.7 against 32.1 us, long: 138 against 146): a warp's step is
+                                                 // (64 ragged: 29.7 against 32.1 us, long: 138 against 146, at the time): a warp's step is
                                                  // a chain of some 3000 cycles, which other warps have to fill
   static constexpr int RING = DC_W * NS * 8192;
   static constexpr int OP = 64 + 4;              // padded row of the merge buffer: 64 columns at a time, so
@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(JN_T) k_kv_join(DcArgs d) {
 // line of tiles, in finer pieces: its few loads depend on one another, so it
 // takes many small CTAs (with one piece per CTA of the attention this kernel
 // took 46 us of a decode step of 16 sequences of 2048 to 4352 rows, 32/8
-// heads x 128; in 32 per SM it takes 12, cold, of the step's 52).
+// heads x 128; in 32 per SM it takes 12, cold, of the step's 51).
 template <int D>
 __global__ void __launch_bounds__(DcGeo<D>::TILE) k_kv_weight(DcArgs d) {
   constexpr int TILE = DcGeo<D>::TILE;

@@ -25,8 +25,9 @@
 // groups' softmax (a warp reads its quarter of the TMEM lanes). In a tile at
 // the end of what the queries see, V rows behind it are set to zero: they may
 // hold anything, and 0 times that must be 0.
-// 8192 tokens of 32/8 heads x 128 take 472 us (1164 TFLOP/s): tensor pipe and
-// exponentials each busy half the time (52 %), the steps of the two groups
+// 8192 tokens of 32/8 heads x 128 take 470 to 485 us, by the clock that the
+// power cap leaves (1160 TFLOP/s at 474): tensor pipe and
+// exponentials each busy half the time (56 %), the steps of the two groups
 // meeting imperfectly. A ragged batch of 5 prompts to 4000 tokens with a
 // window of 256, 16/4 x 128: 74 us; of a CTA's 12 some 4 pass until its first
 // scores (search, first copies) and 2 at its end (the rows go out), beside 5
@@ -233,8 +234,11 @@ PB_DEV int pf_key(const PfLine& s, int i) { return (i < s.nst ? i : i - s.nst + 
 
 // P2: the probabilities as two numbers of the cache's type, for an output with
 // more bits than that has; the second ones take the other half of the scores'
-// columns, and a second product with V (8192 tokens of 32/8 heads x 128: 608
-// against 459 us; the ragged batch with a window 80 against 74).
+// columns, and a second product with V (8192 tokens of 32/8 heads x 128: 615
+// against 505 us on one box; the ragged batch with a window 81 against 74).
+// Elsewhere one number has to do, and in an output of the same type its
+// rounding shows beside the output's own (bf16, ragged batch: error against 64
+// bits 0.0022 of the output, 0.0016 with two).
 template <int D, int CT, bool P2>
 __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mq,
              PfArgs p) {
@@ -564,8 +568,7 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
         }
       }
       // p = 2^(scale2 s - ms + UP), rounded to the cache's type, which the product
-      // with V needs (as exact as an output of that type); the sum takes the
-      // unrounded ones
+      // with V needs; the sum takes the unrounded ones
       const pf_f2 nms = pf_pk(UP - ms, UP - ms);
       pf_f2 y[2] = {0ull, 0ull};
 #pragma unroll
