@@ -133,7 +133,7 @@ template <int D, int CT, int NT, bool P2>
 __global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs d) {
   typedef DcGeo<D> G;
   constexpr int KT = G::KT, TILE = G::TILE, NB = G::NB, NS = G::NS, CPR = D / 8, RS = 32 / CPR;
-  constexpr float UP = CT == PB_DT_F16 ? 15.0f : 0.0f;   // log2 of the probabilities' factor
+  constexpr int UP = CT == PB_DT_F16 ? 15 : 0;      // log2 of the probabilities' factor
   extern __shared__ __align__(128) char dsm[];
   const AttnKvArgs& a = d.a;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs
         if (__any_sync(0xffffffffu, mx[0] > m[n][0] || mx[1] > m[n][1])) {
 #pragma unroll
           for (int u = 0; u < 2; u++) {
-            const float f = mx[u] > m[n][u] ? kv_ex2(m[n][u] - mx[u]) : 1.0f;
+            const float f = mx[u] > m[n][u] ? kv_ex2(kv_ref<UP>(m[n][u]) - kv_ref<UP>(mx[u])) : 1.0f;
             m[n][u] = mx[u];
             l[n][u] *= f;
 #pragma unroll
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs
         float p[4];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-          const float r = (m[n][u] == -INFINITY ? 0.0f : m[n][u]) - UP;
+          const float r = m[n][u] == -INFINITY ? 0.0f : kv_ref<UP>(m[n][u]);
           p[u] = kv_ex2(s[n][u] - r);
           p[2 + u] = kv_ex2(s[n][2 + u] - r);
           l[n][u] += p[u] + p[2 + u];
@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(32 * DC_W, NT == 1 ? 3 : 2) k_kv_decode(DcArgs
               row[k * 16 + g] = o[n][half * 4 + k][u];
               row[k * 16 + g + 8] = o[n][half * 4 + k][2 + u];
             }
-            if (g == 0) { mml[(warp * 8 + 2 * c + u) * 2] = m[n][u] - UP; mml[(warp * 8 + 2 * c + u) * 2 + 1] = l[n][u]; }
+            if (g == 0) { mml[(warp * 8 + 2 * c + u) * 2] = kv_ref<UP>(m[n][u]); mml[(warp * 8 + 2 * c + u) * 2 + 1] = l[n][u]; }
           }
           __syncthreads();
           {

@@ -26,6 +26,15 @@ PB_DEV float kv_ex2(float x) {
   return y;
 }
 
+// The probabilities of an fp16 cache carry a factor 2^UP, in the product with V
+// and in the sum: they are 2^(s - kv_ref(m)) under the maximum m. None where a
+// score's own step in fp32 (2^-4 and more) could bring them past fp16's range.
+// Factors between maxima go by kv_ref as well, so that they agree with it.
+template <int UP>
+PB_DEV float kv_ref(float m) {
+  return UP == 0 || !(fabsf(m) < 1048576.0f) ? m : m - (float)UP;
+}
+
 // Sequences laid end to end on a line, count(i) units each: the line's length
 // and, for the unit pick(length), its sequence and that sequence's first unit
 // (b = -1 when it lies past the line: the caller has no work then). A thread

@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
   // what lies below 2^-25 would be 0 in the product with V but not in the sum, and many such rows together may be all
   // that an output has (a first row far above a long rest); so the two take all of the range above 1 and what is lost
   // lies below 2^-32. (Moving at 2^4 with a factor of 2^11: 513 against 478 us for 8192 tokens of 32/8 heads x 128.)
-  constexpr float LAG = 8.0f, UP = CT == PB_DT_F16 ? 15.0f - LAG : 0.0f;
+  constexpr int LAG = 8, UP = CT == PB_DT_F16 ? 15 - LAG : 0;
   extern __shared__ __align__(128) char psm_raw[];
   __shared__ uint64_t kfull[NST], kempty[NST], vfull[NST], vempty[NST], sfull[NG][2], pready[NG][2], pvdone[NG], ofin[NG], lock[4], qfull, vfix[3], done[NG];
   __shared__ uint32_t tbase;
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
     // of the group: what all rows see, for tiles that need no masks
     const int ta = t0 + min(g * p.tq, ntok - 1), tb = t0 + min((g + 1) * p.tq - 1, ntok - 1);
     const int whi = a.window > 0 ? tb + 1 - a.window : 0;
-    float m = -INFINITY, ms = 0.0f, l = 0.0f;                  // maximum of the raw scores, the same scaled, sum
+    float m = -INFINITY, ms = 0.0f, l = 0.0f;                  // maximum of the raw scores, what is taken off the scaled ones, sum
     // does every 16-row block of the line have its page? (while the first tile is on its way)
     bool gap = false;
     if (g < ng)
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
       }
     const bool gaps = __any_sync(0xffffffffu, gap);
     const pf_f2 sc2 = pf_pk(a.scale2, a.scale2);
-    const float over = LAG / a.scale2;
+    const float over = (float)LAG / a.scale2;
     float thr = -INFINITY;                                     // m + over
     const int steps = g < ng ? n : 0;
     for (int i = 0; i < steps; i++) {
@@ -548,8 +548,9 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
       const bool over_it = live && !(mx <= thr);
       if (__any_sync(0xffffffffu, over_it)) {
         const bool move = mx > thr;
-        const float f = !move ? 1.0f : (m == -INFINITY ? 0.0f : kv_ex2((m - mx) * a.scale2));
-        if (move) { m = mx; ms = mx * a.scale2; thr = mx + over; }
+        const float now_ms = kv_ref<UP>(mx * a.scale2);
+        const float f = !move ? 1.0f : (m == -INFINITY ? 0.0f : kv_ex2(ms - now_ms));
+        if (move) { m = mx; ms = now_ms; thr = mx + over; }
         if (over_it && !(mx < INFINITY)) l = __int_as_float(0x7fffffff);
         l *= f;
         if (i > 0) {   // the output so far, which the product of tile i - 1 has completed
@@ -567,9 +568,9 @@ __global__ void __launch_bounds__(PfGeo<D>::T, 1) k_kv_prefill(const __grid_cons
           }
         }
       }
-      // p = 2^(scale2 s - ms + UP), rounded to the cache's type, which the product
+      // p = 2^(scale2 s - ms), rounded to the cache's type, which the product
       // with V needs; the sum takes the unrounded ones
-      const pf_f2 nms = pf_pk(UP - ms, UP - ms);
+      const pf_f2 nms = pf_pk(-ms, -ms);
       pf_f2 y[2] = {0ull, 0ull};
 #pragma unroll
       for (int q = 0; q < 4; q++) {

@@ -1039,3 +1039,36 @@ def test_a_wait_that_gives_up_is_reported_once(pb, cuda):
     c.h.prefill(c.dev(), start, length, q, out)
     c.h.status()
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dt,ot", FAR + [("bfloat16", "float16")])
+def test_scores_near_the_end_of_fp32_integers(pb, cuda, dt, ot):
+    """scores of 2^25, whose neighbours are 4 apart, in powers of two: a factor in the probabilities that is subtracted
+    from such a maximum would come out as another one and pass fp16's largest value. The scores themselves are exact
+    (products of powers of two, and 8): row 100 is 2^8 above row 0, everything else 2^24 below."""
+    torch = cuda
+    dt, ot = getattr(torch, dt), getattr(torch, ot)
+    D, n, nh, scale = 64, 300, 4, 0.6931471824645996      # 2^(scale log2(e) s) = 2^s in fp32
+    c = Cache(pb, torch, [n], 2, D, 32, dt, seed=3)
+    pg, r, _ = KO.rows_of(c.table.numpy(), 0, n, 32, c.n_pages)
+    pg, r = torch.from_numpy(pg).long().cuda(), torch.from_numpy(r).cuda()
+    k = torch.zeros((n, 2, D))
+    k[0, :, 0], k[100, :, 0], k[100, :, 1] = 8192.0, 8192.0, 8.0
+    k[1:100, :, 0], k[101:, :, 0] = 4096.0, 4096.0
+    c.k[pg, :, r] = k.to(dt).cuda()
+    q = torch.zeros((n, nh, D), dtype=dt, device="cuda")
+    q[:, :, 0], q[:, :, 1] = 4096.0, 1.0
+    v = f64(c.v[pg, :, r])                                 # [row][kv head][dim]
+    length = torch.tensor([n], dtype=torch.int32, device="cuda")
+    one, out = torch.empty((1, nh, D), dtype=ot, device="cuda"), torch.empty((n, nh, D), dtype=ot, device="cuda")
+    c.h.decode(c.dev(), length, q[-1:], one, scale=scale)
+    c.h.prefill(c.dev(), torch.tensor([0, n], dtype=torch.int32, device="cuda"), length, q, out, scale=scale)
+    chunk = torch.empty((2, nh, D), dtype=ot, device="cuda")
+    c.h.prefill(c.dev(), torch.tensor([0, 2], dtype=torch.int32, device="cuda"), length, q[-2:], chunk, scale=scale)
+    torch.cuda.synchronize()
+    for h in range(nh):
+        both = (256 * v[100, h // 2] + v[0, h // 2]) / 257
+        # a probability's rounding in the cache's type, the store's, and a few of fp32
+        tol = (U(torch, dt) + U(torch, ot) + 2.0 ** -20) * (256 * np.abs(v[100, h // 2]) + np.abs(v[0, h // 2])) / 257 + 2.0 ** -25
+        for got, want in ((one[0], both), (out[99], v[0, h // 2]), (out[100], both), (out[n - 1], both), (chunk[0], both), (chunk[1], both)):
+            assert (np.abs(f64(got)[h] - want) <= tol + (U(torch, ot) + 2.0 ** -20) * np.abs(want)).all(), h
