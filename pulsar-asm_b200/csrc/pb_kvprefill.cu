@@ -235,7 +235,7 @@ PB_DEV int pf_key(const PfLine& s, int i) { return (i < s.nst ? i : i - s.nst + 
 // P2: the probabilities as two numbers of the cache's type, for an output with
 // more bits than that has; the second ones take the other half of the scores'
 // columns, and a second product with V (8192 tokens of 32/8 heads x 128: 615
-// against 505 us on one box; the ragged batch with a window 81 against 74).
+// against 505 us on one GPU; the ragged batch with a window 81 against 74).
 // Elsewhere one number has to do, and in an output of the same type its
 // rounding shows beside the output's own (bf16, ragged batch: error against 64
 // bits 0.0022 of the output, 0.0016 with two).
